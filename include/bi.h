@@ -185,6 +185,119 @@ int bi_qgemm(const void* x, const void* w, const void* scales, const void* biase
              int64_t M, int64_t N, int64_t K, int group_size, int bits, int dtype,
              void* hip_stream);
 
+/*
+ * Block tables and slot maps of a serving step over a paged cache, from the
+ * requests' lengths. Request r holds context_lens[r] rows and brings
+ * new_lens[r] more (negative lengths count as 0); its row i is row
+ * i % page_size of page block_tables[r][i / page_size].
+ *
+ *   block_tables (R, W) int32, rows table_stride apart, updated in place: the
+ *                pages that the new rows begin are taken from free_pages in
+ *                the requests' order, from its front; -1 where the F free
+ *                pages do not reach. No other entry is written. Rows past
+ *                W * page_size have no page.
+ *   slots        (T) page * page_size + row of every new token, -1 for one
+ *                without a page and behind the last token
+ *   positions    (T) its row in the request, -1 behind the last token
+ *   query_start  (R + 1) first token of every request, and their number
+ *   seq_lens     (R) context_lens + new_lens
+ *   pages_used   (1) pages the new rows begin (more than F: not all were there)
+ *
+ * Where the new tokens are more than T, the first T have their slots written
+ * and all their pages; the sums must stay below 2^31.
+ */
+int bi_page_tables(int32_t* block_tables, const int32_t* context_lens, const int32_t* new_lens,
+                   const int32_t* free_pages, int32_t* slots, int32_t* positions,
+                   int32_t* query_start, int32_t* seq_lens, int32_t* pages_used,
+                   int64_t R, int64_t W, int64_t table_stride, int64_t F, int64_t T,
+                   int64_t page_size, void* hip_stream);
+
+/*
+ * Writes T tokens' keys and values into a paged cache: row slots[t] %
+ * page_size of page slots[t] / page_size takes k[t] and v[t]; a slot that is
+ * negative or not below num_pages * page_size writes nothing. Slots are
+ * distinct (of two tokens with one slot either may be kept, unit by unit).
+ *
+ *   k (T, Hkv, D), v (T, Hkv, V)     element strides strides[0..1], [2..3]
+ *   k_cache (num_pages, Hkv, page_size, D)   strides[4..6] (page, head, row)
+ *   v_cache (num_pages, Hkv, page_size, V)   strides[7..9]
+ *   the last dimension of each is contiguous
+ */
+int bi_paged_update(const void* k, const void* v, void* k_cache, void* v_cache,
+                    const int32_t* slots, int64_t T, int64_t Hkv, int64_t D, int64_t V,
+                    int64_t num_pages, int64_t page_size, const int64_t* strides, int dtype,
+                    void* hip_stream);
+
+/*
+ * Causal attention of new tokens over a paged cache that already holds their
+ * keys and values (bi_paged_update). Tokens query_start[r] ..
+ * query_start[r + 1] - 1 are the last ones of request r's seq_lens[r] rows:
+ * the last token sees every row, the one before it all but one. With window >
+ * 0 a token at position p sees rows j with p - window < j <= p, and the first
+ * sink_tokens rows (j < sink_tokens, j <= p); window 0 is none.
+ *
+ *   q            (T, H, D)    strides[0..1] (token, head)
+ *   k_cache      (num_pages, Hkv, page_size, D)  strides[2..4] (page, head, row)
+ *   v_cache      (num_pages, Hkv, page_size, V)  strides[5..7]
+ *                pointers and strides are multiples of 16 bytes
+ *   block_tables (R, W) int32, rows strides[8] apart. A row whose entry is not
+ *                a page of the cache, or lies past the table, is not seen.
+ *   query_start  (R + 1), seq_lens (R) int32
+ *   sinks        (H,) logits in `dtype`, or NULL: one more term of each
+ *                head's denominator
+ *   out          (T, H, V) contiguous; a token that no request owns, and one
+ *                that sees nothing, is 0
+ *   max_query, max_seq   bounds of the requests' new tokens and lengths that
+ *                the launch may rely on; a request beyond one of them gets NaN
+ *   workspace    at least bi_paged_attention_workspace bytes, 16-byte aligned,
+ *                or NULL: slower, with the same bits
+ *
+ * Arithmetic (bi_paged_attn.h): keys are taken by their position in the
+ * request, in segments of a fixed length whose results are folded in order,
+ * so that a token's bits depend on its own request's rows alone: not on other
+ * requests, on how many tokens are new, on the pages, on the workspace or on
+ * rows it does not see. bi_window_attention gives the same bits for the same
+ * rows in contiguous memory. (Not bi_sdpa's bits: its chains have no segments.)
+ * Rows that no token of a request sees never reach its output, whatever they
+ * hold; a NaN or infinity in a row that one token sees may reach the tokens
+ * of the same request that do not see it.
+ * Built for (D, V) in {(64, 64), (96, 96), (128, 128), (192, 128), (192, 192),
+ * (256, 256)}.
+ */
+int bi_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* block_tables, const int32_t* query_start,
+                       const int32_t* seq_lens, const void* sinks, void* out, int64_t T, int64_t R,
+                       int64_t H, int64_t Hkv, int64_t D, int64_t V, int64_t num_pages,
+                       int64_t page_size, int64_t W, const int64_t* strides, float scale,
+                       int64_t window, int64_t sink_tokens, int64_t max_query, int64_t max_seq,
+                       int dtype, void* workspace, int64_t workspace_bytes, void* hip_stream);
+
+/* Bytes with which bi_paged_attention runs fastest; 0 if it would use none. */
+int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D,
+                                     int64_t V, int64_t window, int64_t sink_tokens,
+                                     int64_t max_query, int64_t max_seq, int dtype);
+
+/*
+ * Causal attention with a sliding window and first tokens that stay visible,
+ * over contiguous keys: the rule, types, head dims and bits of
+ * bi_paged_attention for B requests of N rows each, the last qL of them new.
+ *
+ *   q (B, H, qL, D), k (B, Hkv, N, D), v (B, Hkv, N, V): element strides
+ *   strides[0..2], [3..5], [6..8] for all but the contiguous last dimension;
+ *   out (B, H, qL, V) contiguous. qL may be more than N: the first rows then
+ *   see nothing and are 0.
+ */
+int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks, void* out,
+                        int64_t B, int64_t H, int64_t Hkv, int64_t qL, int64_t N, int64_t D,
+                        int64_t V, const int64_t* strides, float scale, int64_t window,
+                        int64_t sink_tokens, int dtype, void* workspace, int64_t workspace_bytes,
+                        void* hip_stream);
+
+/* Bytes with which bi_window_attention runs fastest; 0 if it would use none. */
+int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t qL, int64_t N,
+                                      int64_t D, int64_t V, int64_t window, int64_t sink_tokens,
+                                      int dtype);
+
 #ifdef __cplusplus
 }
 #endif

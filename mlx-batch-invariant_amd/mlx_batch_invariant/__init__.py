@@ -25,6 +25,8 @@ import torch.nn.functional as F
 from ._attention import HEAD_DIMS, scaled_dot_product_attention, supported_head_dims
 from ._attention import _mask_args, _sdpa
 from ._gemm import TILE, addmm, geometries, linear, matmul
+from ._paged import (PAGED_HEAD_DIMS, PageTables, page_tables, paged_attention,
+                     paged_cache_update, window_attention)
 from ._quant import (QUANT_BITS, QuantizedLinear, dequantize, quantize, quantized_linear,
                      quantized_matmul)
 
@@ -39,6 +41,12 @@ __all__ = [
     "dequantize",
     "QuantizedLinear",
     "QUANT_BITS",
+    "page_tables",
+    "paged_cache_update",
+    "paged_attention",
+    "window_attention",
+    "PageTables",
+    "PAGED_HEAD_DIMS",
     "batch_invariant_mode",
     "is_enabled",
     "TILE",

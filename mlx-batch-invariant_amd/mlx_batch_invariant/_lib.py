@@ -41,6 +41,14 @@ SIGNATURES = {
     "bi_sdpa_ws": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64p, _c_vp, _c_vp,
                             _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                             _c_i64p, _c_float, _c_int, _c_i64, _c_int, _c_vp, _c_i64, _c_vp]),
+    "bi_page_tables": (_c_int, [_c_vp] * 9 + [_c_i64] * 6 + [_c_vp]),
+    "bi_paged_update": (_c_int, [_c_vp] * 5 + [_c_i64] * 6 + [_c_i64p, _c_int, _c_vp]),
+    "bi_paged_attention": (_c_int, [_c_vp] * 8 + [_c_i64] * 9 + [_c_i64p, _c_float]
+                           + [_c_i64] * 4 + [_c_int, _c_vp, _c_i64, _c_vp]),
+    "bi_paged_attention_workspace": (_c_i64, [_c_i64] * 10 + [_c_int]),
+    "bi_window_attention": (_c_int, [_c_vp] * 5 + [_c_i64] * 7 + [_c_i64p, _c_float]
+                            + [_c_i64] * 2 + [_c_int, _c_vp, _c_i64, _c_vp]),
+    "bi_window_attention_workspace": (_c_i64, [_c_i64] * 9 + [_c_int]),
     "bi_gemm_num_geometries": (_c_int, []),
     "bi_gemm_geometry_info": (_c_int, [_c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
                                        ctypes.POINTER(_c_int)]),

@@ -4,13 +4,14 @@ The reference's kernels are opaque to ``mx.compile``, which may reorder and
 fuse the graph around them but never inside (reference
 tests/test_invariance.py:595-640). The same holds here: while torch.compile
 traces, ``bi.*`` calls become the ops ``mlx_bi::gemm``, ``mlx_bi::qgemm`` and
-``mlx_bi::sdpa``, which the compiler treats as opaque nodes (their fake
-implementations give only output shapes) and which run the HIP kernels
-unchanged. Eager calls skip
-the dispatcher and launch directly.
+``mlx_bi::sdpa`` (and, for the paged cache, ``mlx_bi::page_tables``,
+``mlx_bi::paged_cache_update``, ``mlx_bi::paged_attention`` and
+``mlx_bi::window_attention``), which the compiler treats as opaque nodes (their
+fake implementations give only output shapes) and which run the HIP kernels
+unchanged. Eager calls skip the dispatcher and launch directly.
 """
 
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -55,3 +56,64 @@ def qgemm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.
 @qgemm.register_fake
 def _qgemm_fake(x, w, scales, biases, group_size, bits):
     return x.new_empty((*x.shape[:-1], w.shape[0]))
+
+
+@torch.library.custom_op("mlx_bi::page_tables", mutates_args=("block_tables",))
+def page_tables(block_tables: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
+                free_pages: torch.Tensor, page_size: int, num_tokens: int
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import _paged
+
+    # Outputs of a custom op may not share storage.
+    return tuple(t.clone() for t in _paged._page_tables_eager(
+        block_tables, context_lens, new_lens, free_pages, page_size, num_tokens))
+
+
+@page_tables.register_fake
+def _page_tables_fake(block_tables, context_lens, new_lens, free_pages, page_size, num_tokens):
+    n = context_lens.shape[0]
+    return tuple(context_lens.new_empty(s) for s in ((num_tokens,), (num_tokens,), (n + 1,), (n,),
+                                                     ()))
+
+
+@torch.library.custom_op("mlx_bi::paged_cache_update", mutates_args=("k_cache", "v_cache"))
+def paged_cache_update(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, slots: torch.Tensor) -> None:
+    from . import _paged
+
+    _paged._update_eager(k, v, k_cache, v_cache, slots)
+
+
+@paged_cache_update.register_fake
+def _paged_cache_update_fake(k, v, k_cache, v_cache, slots):
+    return None
+
+
+@torch.library.custom_op("mlx_bi::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_tables: torch.Tensor, query_start: torch.Tensor, seq_lens: torch.Tensor,
+                    max_query: int, max_seq: int, scale: float, window: int, sink_tokens: int,
+                    sinks: Optional[torch.Tensor]) -> torch.Tensor:
+    from . import _paged
+
+    return _paged._paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens,
+                               max_query, max_seq, scale, window, sink_tokens, sinks)
+
+
+@paged_attention.register_fake
+def _paged_attention_fake(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_query,
+                          max_seq, scale, window, sink_tokens, sinks):
+    return q.new_empty((q.shape[0], q.shape[1], v_cache.shape[3]))
+
+
+@torch.library.custom_op("mlx_bi::window_attention", mutates_args=())
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int,
+                     sink_tokens: int, sinks: Optional[torch.Tensor]) -> torch.Tensor:
+    from . import _paged
+
+    return _paged._window_eager(q, k, v, scale, window, sink_tokens, sinks)
+
+
+@window_attention.register_fake
+def _window_attention_fake(q, k, v, scale, window, sink_tokens, sinks):
+    return q.new_empty((q.shape[0], q.shape[1], q.shape[2], v.shape[-1]))
