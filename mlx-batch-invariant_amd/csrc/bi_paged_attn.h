@@ -1,5 +1,6 @@
 // Attention over a paged cache, or over contiguous keys with a window: launch
-// arguments and the visibility rule shared by its kernels.
+// arguments shared by the kernels (bi_paged_attn_kernel.h) and the C entry
+// points (bi_paged_attn.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -23,43 +24,33 @@ struct Args {
   int64_t kb, kh, kn;     // keys: page or request, head, row
   int64_t vb, vh, vn;
   int64_t table_stride;
-  int32_t R, H, Hkv, G, W, page, pages;
+  int32_t R, H, Hkv, G, W, page, page_shift, pages;  // page_shift < 0: not a power of two
   int32_t qL, N;          // contiguous
   int32_t T;              // tokens of a paged call
   int32_t window, first;  // window 0: none
   int32_t max_query, max_seq;
   float scale2;           // |scale| * log2(e)
-  uint32_t qneg;          // nonzero: negate the scores
+  uint32_t qsign;         // negative scale: the sign bits of a query dword
+  // The split route: partial results of (request, kv head, column, segment).
+  float* po;              // [V] each
+  float2* pml;            // base and sum
+  int32_t nseg, ccap;     // segments and columns kept per (request, kv head)
+  int32_t split_cols;     // requests of at most this many columns are split
+  int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
+  int32_t tiles;          // whole route: column tiles per kv head
 };
 
-// One request: its tokens t0 .. t0 + L - 1 sit at rows n - L .. n - 1.
-struct Request {
-  int64_t t0;
-  int32_t L, n;
-  bool beyond;  // past max_query or max_seq
+typedef void (*Kernel)(Args);
+struct Kernels {
+  Kernel split16, split32;  // 16 or 32 columns per workgroup
+  Kernel combine, whole;
+  int step;                 // keys per step; a segment is 4 steps
+  int whole_cols, whole_threads;
 };
 
-__device__ __forceinline__ Request request(const Args& p, int r) {
-  Request q;
-  if (p.qstart) {
-    int32_t a = p.qstart[r], b = p.qstart[r + 1];
-    a = a < 0 ? 0 : a > p.T ? p.T : a;
-    b = b < a ? a : b > p.T ? p.T : b;
-    q.t0 = a;
-    q.L = b - a;
-    q.n = p.seq[r] < 0 ? 0 : p.seq[r];
-    q.beyond = q.L > p.max_query || q.n > p.max_seq;
-  } else {
-    q.t0 = 0;
-    q.L = p.qL;
-    q.n = p.N;
-    q.beyond = false;
-  }
-  return q;
-}
-
-__device__ __forceinline__ bool sees(const Args& p, int32_t pos, int32_t key) {
-  return key <= pos && (p.window == 0 || key > pos - p.window || key < p.first);
-}
+#define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)
+#define BI_PAGED_DECLARE(D, V) Kernels kernels_d##D##_v##V(int dtype);
+BI_PAGED_DIM_PAIRS(BI_PAGED_DECLARE)
+#undef BI_PAGED_DECLARE
 
 }  // namespace bi_paged

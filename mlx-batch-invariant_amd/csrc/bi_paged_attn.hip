@@ -1,6 +1,6 @@
 // Attention over a paged cache and windowed attention over contiguous keys:
-// the C entry points and the kernels (contract in include/bi.h).
-#include <float.h>
+// the C entry points and the choice of route (contract in include/bi.h, kernels
+// in bi_paged_attn_kernel.h).
 #include <math.h>
 
 #include "bi_paged_attn.h"
@@ -9,108 +9,6 @@ namespace {
 
 using namespace bi_paged;
 
-template <typename T> __device__ __forceinline__ float up(T x) { return (float)x; }
-
-// One wave per (token, head): 64 keys at a time, a key per lane, then a value
-// dim per lane.
-template <typename T, int D, int V>
-__global__ void __launch_bounds__(64) attend_simple(Args p) {
-  const int lane = threadIdx.x;
-  const int h = blockIdx.y, kvh = h / p.G;
-  int r = 0, i = 0;
-  int64_t qoff, ooff;
-  Request rq;
-  constexpr int NV = (V + 63) / 64;
-  if (p.qstart) {
-    const int t = blockIdx.x;
-    qoff = t * p.qt + h * p.qh;
-    ooff = t * p.ot + h * p.oh;
-    bool owned = false;
-    for (r = 0; r < p.R; r++) {
-      rq = request(p, r);
-      if (t >= rq.t0 && t < rq.t0 + rq.L) {
-        owned = true;
-        break;
-      }
-    }
-    if (!owned) {
-      for (int j = 0; j < NV; j++)
-        if (lane + 64 * j < V) static_cast<T*>(p.out)[ooff + lane + 64 * j] = (T)0.f;
-      return;
-    }
-    i = (int)(t - rq.t0);
-  } else {
-    r = blockIdx.x / p.qL;
-    i = blockIdx.x % p.qL;
-    rq = request(p, r);
-    qoff = r * p.qb + i * p.qt + h * p.qh;
-    ooff = r * p.ob + i * p.ot + h * p.oh;
-  }
-  const T* q = static_cast<const T*>(p.q) + qoff;
-  T* out = static_cast<T*>(p.out) + ooff;
-  const int32_t pos = rq.n - rq.L + i;
-  float m = -INFINITY, l = 0.f, o[NV] = {};
-  if (p.sinks) {
-    m = up(static_cast<const T*>(p.sinks)[h]) * 1.4426950408889634f;
-    l = 1.f;
-  }
-  for (int32_t j0 = 0; j0 <= pos; j0 += 64) {
-    const int32_t j = j0 + lane;
-    bool use = sees(p, pos, j);
-    int64_t ko = 0, vo = 0;
-    if (use) {
-      if (p.qstart) {
-        const int32_t pg = j / p.page, row = j - pg * p.page;
-        const int32_t id = pg < p.W ? p.table[r * p.table_stride + pg] : -1;
-        use = id >= 0 && id < p.pages;
-        ko = id * p.kb + kvh * p.kh + row * p.kn;
-        vo = id * p.vb + kvh * p.vh + row * p.vn;
-      } else {
-        ko = r * p.kb + kvh * p.kh + j * p.kn;
-        vo = r * p.vb + kvh * p.vh + j * p.vn;
-      }
-    }
-    float s = -INFINITY;
-    if (use) {
-      const T* k = static_cast<const T*>(p.k) + ko;
-      float a = 0.f;
-      for (int d = 0; d < D; d++) a = fmaf(up(q[d]), up(k[d]), a);
-      s = (p.qneg ? -a : a) * p.scale2;
-    }
-    float bm = s;
-    for (int x = 1; x < 64; x <<= 1) bm = fmaxf(bm, __shfl_xor(bm, x));
-    const float mn = fmaxf(m, bm);
-    if (mn == -INFINITY) continue;
-    const float f = exp2f(m - mn);
-    const float w = use ? exp2f(s - mn) : 0.f;
-    float bs = w;
-    for (int x = 1; x < 64; x <<= 1) bs += __shfl_xor(bs, x);
-    l = l * f + bs;
-    m = mn;
-    for (int jv = 0; jv < NV; jv++) o[jv] *= f;
-    for (int x = 0; x < 64; x++) {
-      const float wx = __shfl(w, x);
-      const int64_t vx = __shfl(vo, x);
-      if (!__shfl((int)use, x)) continue;
-      const T* v = static_cast<const T*>(p.v) + vx;
-      for (int jv = 0; jv < NV; jv++)
-        if (lane + 64 * jv < V) o[jv] = fmaf(wx, up(v[lane + 64 * jv]), o[jv]);
-    }
-  }
-  for (int jv = 0; jv < NV; jv++)
-    if (lane + 64 * jv < V)
-      out[lane + 64 * jv] = rq.beyond ? (T)NAN : (T)(l == 0.f ? 0.f : o[jv] / l);
-}
-
-typedef void (*Kernel)(Args);
-template <int D, int V> Kernel kernel_of(int dtype) {
-  return dtype == BI_F32 ? attend_simple<float, D, V>
-         : dtype == BI_F16 ? attend_simple<_Float16, D, V>
-                           : attend_simple<__bf16, D, V>;
-}
-
-#define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)
-
 bool dims_built(int64_t D, int64_t V) {
 #define BI_CASE(d, v) if (D == d && V == v) return true;
   BI_PAGED_DIM_PAIRS(BI_CASE)
@@ -118,16 +16,87 @@ bool dims_built(int64_t D, int64_t V) {
   return false;
 }
 
-int launch(const char* who, const Args& p, int64_t D, int64_t V, int dtype, void* stream) {
-  Kernel fn = nullptr;
-#define BI_CASE(d, v) if (D == d && V == v) fn = kernel_of<d, v>(dtype);
+Kernels kernels(int64_t D, int64_t V, int dtype) {
+#define BI_CASE(d, v) if (D == d && V == v) return kernels_d##d##_v##v(dtype);
   BI_PAGED_DIM_PAIRS(BI_CASE)
 #undef BI_CASE
-  const int64_t rows = p.qstart ? p.T : (int64_t)p.R * p.qL;
-  hipLaunchKernelGGL(fn, dim3((unsigned)rows, (unsigned)p.H), dim3(64), 0,
-                     static_cast<hipStream_t>(stream), p);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? BI_OK : bi::launch_error(e, who);
+  return Kernels{};
+}
+
+// Tokens, lengths and windows past this are not computed with (positions
+// minus a window stay in 32 bits).
+constexpr int64_t kMost = (int64_t)1 << 30;
+
+// How a call is split: the columns up to which a request is (0: none), and the
+// memory of its partial results. `exact`: every request has max_query tokens.
+struct Plan {
+  int64_t split_cols, ccap, nseg, bytes;
+};
+Plan plan(int64_t R, int64_t G, int64_t Hkv, int64_t V, int64_t window, int64_t first,
+          int64_t max_query, int64_t max_seq, bool exact, const Kernels& k) {
+  Plan s = {0, 0, 0, 0};
+  const int64_t cols = max_query * G, seg = 4 * (int64_t)k.step;
+  if (R <= 0 || cols <= 0 || max_seq <= 0) return s;
+  s.split_cols = 32;
+  if (exact && cols > s.split_cols) return Plan{0, 0, 0, 0};
+  s.ccap = cols < s.split_cols ? cols : s.split_cols;
+  s.nseg = (max_seq + seg - 1) / seg;
+  if (window) {
+    // Tokens of a workgroup's columns, rows that they see between them.
+    const int64_t nc = s.ccap <= 16 ? 16 : 32;
+    const int64_t span = window + (nc - 1) / G + 1;
+    const int64_t n = (span + seg - 2) / seg + 1 + (first + seg - 1) / seg;
+    if (n < s.nseg) s.nseg = n;
+  }
+  s.bytes = R * Hkv * s.ccap * s.nseg * (V + 2) * (int64_t)sizeof(float);
+  if (s.bytes > (int64_t)1 << 31 || R * Hkv * s.nseg > INT32_MAX ||
+      R * Hkv * s.ccap > INT32_MAX) return Plan{0, 0, 0, 0};
+  return s;
+}
+
+int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, int64_t ws_bytes,
+           void* stream) {
+  const Kernels k = kernels(D, V, dtype);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t most = p.qstart ? p.max_query : p.qL;
+  Plan s = plan(p.R, p.G, p.Hkv, V, p.window, p.first, most, p.qstart ? p.max_seq : p.N,
+                !p.qstart, k);
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0};
+  hipError_t e;
+  if (s.split_cols) {
+    p.split_cols = (int32_t)s.split_cols;
+    p.ccap = (int32_t)s.ccap;
+    p.nseg = (int32_t)s.nseg;
+    p.po = static_cast<float*>(ws);
+    p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv * s.ccap * s.nseg * V);
+    const int nc = s.ccap <= 16 ? 16 : 32;
+    const dim3 grid((unsigned)(p.R * p.Hkv * s.nseg), (unsigned)((s.ccap + nc - 1) / nc));
+    hipLaunchKernelGGL(nc == 16 ? k.split16 : k.split32, grid, dim3(256), 0, st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+  }
+  const bool whole = most * p.G > s.split_cols;
+  p.fill_blocks = p.qstart ? 16 : 0;
+  if (s.split_cols) {
+    const int64_t cols = (int64_t)p.R * p.Hkv * s.ccap;
+    hipLaunchKernelGGL(k.combine, dim3((unsigned)((cols + 3) / 4 + p.fill_blocks)), dim3(256), 0,
+                       st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+    p.fill_blocks = 0;
+  }
+  if (whole || p.fill_blocks) {
+    // Column tiles: every request with tokens may end in a part of one.
+    const int64_t wc = k.whole_cols;
+    const int64_t reqs = p.T < p.R ? p.T : p.R;
+    int64_t tiles = p.qstart ? (int64_t)p.T * p.G / wc + reqs
+                             : (int64_t)p.R * (((int64_t)p.qL * p.G + wc - 1) / wc);
+    if (!whole) tiles = 0;
+    const int64_t blocks = tiles * p.Hkv + p.fill_blocks;
+    if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
+    if (blocks == 0) return BI_OK;
+    hipLaunchKernelGGL(k.whole, dim3((unsigned)blocks), dim3(k.whole_threads), 0, st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+  }
+  return BI_OK;
 }
 
 // The checks that both entry points share.
@@ -153,16 +122,17 @@ bool aligned16(const void* a, const void* b, const void* c, const int64_t* strid
   return true;
 }
 
-int32_t clamp32(int64_t x) { return x > INT32_MAX ? INT32_MAX : (int32_t)x; }
+int32_t clamp32(int64_t x) { return x > kMost ? (int32_t)kMost : (int32_t)x; }
 
-void common(Args& p, int64_t H, int64_t Hkv, float scale, int64_t window, int64_t sink_tokens) {
+void common(Args& p, int64_t H, int64_t Hkv, float scale, int64_t window, int64_t sink_tokens,
+            int dtype) {
   p.H = (int32_t)H;
   p.Hkv = (int32_t)Hkv;
   p.G = (int32_t)(H / Hkv);
   p.window = clamp32(window);
   p.first = clamp32(sink_tokens);
   p.scale2 = fabsf(scale) * 1.4426950408889634f;
-  p.qneg = scale < 0.f;
+  p.qsign = scale < 0.f ? (dtype == BI_F32 ? 0x80000000u : 0x80008000u) : 0u;
 }
 
 }  // namespace
@@ -180,7 +150,7 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
   int rc = check(who, H, Hkv, D, V, scale, window, sink_tokens, dtype);
   if (rc) return rc;
   if (T < 0 || R < 0 || num_pages < 0 || page_size <= 0 || W < 0 || max_query < 0 || max_seq < 0 ||
-      T > INT32_MAX || R > INT32_MAX || num_pages > INT32_MAX || page_size > INT32_MAX ||
+      T > kMost || T * H > INT32_MAX || R > kMost || num_pages > INT32_MAX || page_size > INT32_MAX ||
       W > INT32_MAX)
     return bi::fail(BI_EINVAL, "%s: bad sizes T=%lld R=%lld pages=%lld x %lld W=%lld", who,
                     (long long)T, (long long)R, (long long)num_pages, (long long)page_size,
@@ -194,7 +164,7 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
     return bi::fail(BI_EINVAL, "%s: q and caches must be 16-byte aligned, with strides of "
                     "multiples of 16 bytes", who);
   Args p = {};
-  common(p, H, Hkv, scale, window, sink_tokens);
+  common(p, H, Hkv, scale, window, sink_tokens, dtype);
   p.q = q;
   p.k = k_cache;
   p.v = v_cache;
@@ -215,14 +185,21 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
   p.T = (int32_t)T;
   p.max_query = clamp32(max_query);
   p.max_seq = clamp32(max_seq);
-  return launch(who, p, D, V, dtype, hip_stream);
+  p.page_shift = -1;
+  for (int i = 0; i < 31; i++)
+    if (page_size == (int64_t)1 << i) p.page_shift = i;
+  return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
 }
 
 extern "C" int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
                                                 int64_t D, int64_t V, int64_t window,
                                                 int64_t sink_tokens, int64_t max_query,
                                                 int64_t max_seq, int dtype) {
-  return 0;
+  if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || !bi::elem_size(dtype) ||
+      !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
+    return 0;
+  return plan(R, H / Hkv, Hkv, V, clamp32(window), clamp32(sink_tokens),
+              clamp32(max_query), clamp32(max_seq), false, kernels(D, V, dtype)).bytes;
 }
 
 extern "C" int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks,
@@ -233,8 +210,8 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
   const char* who = "bi_window_attention";
   int rc = check(who, H, Hkv, D, V, scale, window, sink_tokens, dtype);
   if (rc) return rc;
-  if (B < 0 || qL < 0 || N < 0 || N > INT32_MAX - 4096 || qL > INT32_MAX || B > INT32_MAX ||
-      B * qL > INT32_MAX)
+  if (B < 0 || qL < 0 || N < 0 || N > kMost || qL > kMost || B > kMost || B * qL > kMost ||
+      B * qL * H > INT32_MAX)
     return bi::fail(BI_EINVAL, "%s: bad sizes B=%lld qL=%lld N=%lld", who, (long long)B,
                     (long long)qL, (long long)N);
   if (B == 0 || qL == 0) return BI_OK;
@@ -244,7 +221,7 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
     return bi::fail(BI_EINVAL, "%s: q, k and v must be 16-byte aligned, with strides of multiples "
                     "of 16 bytes", who);
   Args p = {};
-  common(p, H, Hkv, scale, window, sink_tokens);
+  common(p, H, Hkv, scale, window, sink_tokens, dtype);
   p.q = q;
   p.k = k;
   p.v = v;
@@ -257,8 +234,7 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
   p.R = (int32_t)B;
   p.qL = (int32_t)qL;
   p.N = (int32_t)N;
-  p.max_query = p.max_seq = INT32_MAX;
-  return launch(who, p, D, V, dtype, hip_stream);
+  return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
 }
 
 extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t qL,

@@ -1,0 +1,4 @@
+// Paged and windowed attention for D = 192, V = 192 (bi_paged_attn_kernel.h).
+#include "bi_paged_attn_kernel.h"
+
+BI_PAGED_KERNELS(192, 192)
