@@ -240,5 +240,9 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
 extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t qL,
                                                  int64_t N, int64_t D, int64_t V, int64_t window,
                                                  int64_t sink_tokens, int dtype) {
-  return 0;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || qL <= 0 || N <= 0 || !bi::elem_size(dtype) ||
+      !dims_built(D, V) || qL > kMost || N > kMost || B > kMost || window < 0 || sink_tokens < 0)
+    return 0;
+  return plan(B, H / Hkv, Hkv, V, clamp32(window), clamp32(sink_tokens), qL, N, true,
+              kernels(D, V, dtype)).bytes;
 }

@@ -24,11 +24,12 @@
 //     unrounded p). f is a power of two, as every base is an integer.
 //   * Segments start from nothing and are folded in ascending order: with M'
 //     the larger base, O = fma(o, 2^(m - M'), O * 2^(M - M')), L alike.
-//   * The sink enters last: out = (O * e) / (L * e + 2^(sink2 - X)), X the
-//     larger of M and sink2, e = 2^(M - X); rounded once.
+//   * The sink enters last: out = (O * e) / (L * e + 2^(sink2 - X)) + 0.0, X the
+//     larger of M and sink2, e = 2^(M - X), the division by a product with the
+//     rounded inverse; rounded once to the type.
 // A step or segment that a column sees nothing of leaves it as it is, so which
 // of them a workgroup walks for its other columns changes no bits (a zero's
-// sign would: O + 0.0 before the division).
+// sign would: hence the + 0.0).
 //
 // Two routes, the same bits:
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment); its
@@ -118,8 +119,15 @@ __device__ __forceinline__ bool any_seen(const Args& p, int32_t lo, int32_t hi, 
 __device__ __forceinline__ bool all_seen(const Args& p, int32_t lo, int32_t hi, int32_t j, int size) {
   return j + size - 1 <= lo && (p.window == 0 || j > hi - p.window || j + size - 1 < p.first);
 }
-__device__ __forceinline__ bool sees(const Args& p, int32_t pos, int32_t key) {
-  return key <= pos && (p.window == 0 || key > pos - p.window || key < p.first);
+// Bits 0 .. d of 64 (none for d < 0).
+__device__ __forceinline__ uint64_t bits_to(int32_t d) {
+  return d < 0 ? 0ull : d >= 63 ? ~0ull : (2ull << d) - 1;
+}
+// Bit n: a token at `pos` sees row key0 + n, if it is mapped.
+__device__ __forceinline__ uint64_t seen_bits(const Args& p, int32_t pos, int32_t key0, uint64_t mapped) {
+  uint64_t b = bits_to(pos - key0);
+  if (p.window) b &= ~bits_to(pos - p.window - key0) | bits_to(p.first - 1 - key0);
+  return b & mapped;
 }
 
 // A row's page, or -1; contiguous keys: the request.
@@ -135,6 +143,14 @@ __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
   return p.page_shift >= 0 ? key & (p.page - 1) : (int32_t)((uint32_t)key % (uint32_t)p.page);
 }
 
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
+}
 // Loads that write LDS are not covered by a barrier's own waits.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -173,8 +189,9 @@ __device__ __forceinline__ void finish(float M, float L, float sink2, bool has, 
     den = __builtin_fmaf(L, e, __builtin_amdgcn_exp2f(sink2 - x));
   }
 }
-template <typename T> __device__ __forceinline__ T result(float O, float e, float den) {
-  return den == 0.f ? (T)0.f : (T)(__builtin_fmaf(O, e, 0.f) / den);
+__device__ __forceinline__ float inverse(float den) { return den == 0.f ? 0.f : 1.f / den; }
+template <typename T> __device__ __forceinline__ T result(float O, float e, float inv) {
+  return (T)__builtin_fmaf(O * e, inv, 0.f);
 }
 
 template <typename T, int D_, int V_>
@@ -207,6 +224,15 @@ struct Geo {
   }
   // Element i of a tile is row 8 (i / 4) + 4 half + i % 4.
   __device__ __forceinline__ static int row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
+  // Scores of unseen rows become -inf; `seen` is shifted by the half's 4 rows.
+  __device__ __forceinline__ static void hide(f32x16 (&s)[KT], uint64_t seen) {
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) {
+      const uint32_t w = (uint32_t)(seen >> (32 * kt));
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[kt][i] = w & (1u << row(i, 0)) ? s[kt][i] : -INFINITY;
+    }
+  }
   // p of a tile rounded to the type: unit u holds elements (16 / PU) u ...
   __device__ __forceinline__ static void pack(const f32x16& p, uint4 (&u)[PU]) {
     if constexpr (E == 2) {
@@ -397,17 +423,13 @@ __global__ void __launch_bounds__(256) split_kernel(Args p) {
       f32x16 c = {};
 #pragma unroll
       for (int t = 0; t < G::NQ; t++) c = G::score(kr[kt][t], q[t], c);
-      if (!full) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int o = kt * 32 + G::row(i, half);
-          c[i] = sees(p, pos, key0 + o) && ((mapped >> o) & 1) ? c[i] : -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, c[i]);
       s[kt] = c;
     }
+    if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, s[kt][i]);
     top = half_swap_max(top);
   }
   if (lane < NC) s_max[wave][lane] = top;
@@ -551,10 +573,11 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   float e, den;
   finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
          p.sinks != nullptr, e, den);
+  const float inv = inverse(den);
   T* out = out_at<T>(p, r, rq, tok, head);
 #pragma unroll
   for (int j = 0; j < NV; j++)
-    if (lane + 64 * j < V) out[lane + 64 * j] = result<T>(O[j], e, den);
+    if (lane + 64 * j < V) out[lane + 64 * j] = result<T>(O[j], e, inv);
 }
 
 // Whole route: NW waves of 32 columns each walk the steps that some column of
@@ -672,16 +695,17 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     if (lane == 0) s_map[j & 3] = m;
   };
   auto load_step = [&](int j, uint4* kd, uint4* vd) __attribute__((always_inline)) {
+    const int td = opaque(tid);
 #pragma unroll
     for (int i = 0; i < (KU + NT - 1) / NT; i++) {
-      const int at = i * NT + tid, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
+      const int at = i * NT + td, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
       if (KU % NT == 0 || at < KU)
         __builtin_amdgcn_global_load_lds((global_void*)(s_row[j & 1][0][row] + c * 16),
                                          (lds_void*)(kd + i * NT + wave * 64), 16, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < (VU + NT - 1) / NT; i++) {
-      const int at = i * NT + tid, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
+      const int at = i * NT + td, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
       if (VU % NT == 0 || at < VU)
         __builtin_amdgcn_global_load_lds((global_void*)(s_row[j & 1][1][row] + c * 16),
                                          (lds_void*)(vd + i * NT + wave * 64), 16, 0, 0);
@@ -703,6 +727,9 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   }
   auto step = [&](int j, const uint4* kd, const uint4* vd, uint4* kn, uint4* vn)
       __attribute__((always_inline)) {
+    // LDS addresses are computed anew each step: kept across steps they, for
+    // two buffers, take the registers that o and O need.
+    const int ln = opaque(lane), hf = ln >> 5;
     wait_loads();     // this wave's part of step j
     __syncthreads();  // everyone's, and everyone is done with the other buffers
     int32_t id = -1;
@@ -710,7 +737,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     if (j + 1 < steps) load_step(j + 1, kn, vn);
     const int32_t unit = w.unit(j), key0 = unit * S;
     if (any_seen(p, wlo, whi, key0, S)) {
-      const uint64_t mapped = s_map[j & 3];
+      const uint64_t mapped = uniform(s_map[j & 3]);
       const bool full = whole_tile && mapped == (S == 64 ? ~0ull : 0xFFFFFFFFull) &&
                         all_seen(p, wlo, whi, key0, S);
       f32x16 s[KT];
@@ -718,20 +745,12 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
 #pragma unroll
       for (int kt = 0; kt < KT; kt++) {
         f32x16 c = {};
-        const int row = kt * 32 + col, sw = G::kswz(row);
+        const int row = kt * 32 + (ln & 31), sw = G::kswz(row);
 #pragma unroll
-        for (int t = 0; t < G::NQ; t++) c = G::score(kd[row * G::CH + ((2 * t + half) ^ sw)], q[t], c);
+        for (int t = 0; t < G::NQ; t++) c = G::score(kd[row * G::CH + ((2 * t + hf) ^ sw)], q[t], c);
         s[kt] = c;
       }
-      if (!full) {
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int n = kt * 32 + G::row(i, half);
-            s[kt][i] = sees(p, pos, key0 + n) && ((mapped >> n) & 1) ? s[kt][i] : -INFINITY;
-          }
-      }
+      if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
 #pragma unroll
       for (int kt = 0; kt < KT; kt++)
 #pragma unroll
@@ -765,7 +784,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
 #pragma unroll
       for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) G::accumulate(vd, kt * 32, dt, lane, pu[kt], o[dt]);
+        for (int kt = 0; kt < KT; kt++) G::accumulate(vd, kt * 32, dt, ln, pu[kt], o[dt]);
     }
     // The segment's end: fold it.
     if (j + 1 == steps || w.unit(j + 1) / 4 != unit / 4) {
@@ -800,6 +819,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   float e, den;
   finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
          p.sinks != nullptr, e, den);
+  const float inv = inverse(den);
   T* out = out_at<T>(p, r, rq, tok, head);
 #pragma unroll
   for (int dt = 0; dt < DT; dt++)
@@ -808,7 +828,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
       typedef T T4 __attribute__((ext_vector_type(4)));
       T4 y;
 #pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, den);
+      for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, inv);
       *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half) = y;
     }
 }
