@@ -31,7 +31,7 @@ struct Args {
   int32_t max_query, max_seq;
   float scale2;           // |scale| * log2(e)
   uint32_t qsign;         // negative scale: the sign bits of a query dword
-  // The split route: partial results of (request, kv head, column, segment).
+  // The split route: partial results of (request, kv head, segment, column).
   float* po;              // [V] each
   float2* pml;            // base and sum
   int32_t nseg, ccap;     // segments and columns kept per (request, kv head)
@@ -40,11 +40,13 @@ struct Args {
   int32_t tiles;          // whole route: column tiles per kv head
 };
 
+constexpr int kSegSteps = 8;  // steps to a segment
+
 typedef void (*Kernel)(Args);
 struct Kernels {
   Kernel split16, split32;  // 16 or 32 columns per workgroup
   Kernel combine, whole;
-  int step;                 // keys per step; a segment is 4 steps
+  int step;                 // rows per step
   int whole_cols, whole_threads;
 };
 

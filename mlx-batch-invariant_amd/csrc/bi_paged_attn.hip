@@ -35,17 +35,18 @@ struct Plan {
 Plan plan(int64_t R, int64_t G, int64_t Hkv, int64_t V, int64_t window, int64_t first,
           int64_t max_query, int64_t max_seq, bool exact, const Kernels& k) {
   Plan s = {0, 0, 0, 0};
-  const int64_t cols = max_query * G, seg = 4 * (int64_t)k.step;
+  const int64_t cols = max_query * G;
   if (R <= 0 || cols <= 0 || max_seq <= 0) return s;
   s.split_cols = 32;
   if (exact && cols > s.split_cols) return Plan{0, 0, 0, 0};
   s.ccap = cols < s.split_cols ? cols : s.split_cols;
-  s.nseg = (max_seq + seg - 1) / seg;
+  const int64_t part = (int64_t)kSegSteps * k.step;
+  s.nseg = (max_seq + part - 1) / part;
   if (window) {
     // Tokens of a workgroup's columns, rows that they see between them.
     const int64_t nc = s.ccap <= 16 ? 16 : 32;
     const int64_t span = window + (nc - 1) / G + 1;
-    const int64_t n = (span + seg - 2) / seg + 1 + (first + seg - 1) / seg;
+    const int64_t n = (span + part - 2) / part + 1 + (first + part - 1) / part;
     if (n < s.nseg) s.nseg = n;
   }
   s.bytes = R * Hkv * s.ccap * s.nseg * (V + 2) * (int64_t)sizeof(float);

@@ -10,7 +10,7 @@
 //
 // Fixed arithmetic of a column (what makes its bits independent of the call):
 //   * Rows are taken by their position in the request: steps of kStep rows (64
-//     where a row of keys and of values is at most 256 bytes, else 32), four
+//     where a row of keys and of values is at most 256 bytes, else 32), eight
 //     steps to a segment.
 //   * raw_j is a chain of 32x32 matrix products over the head dim from +0.0:
 //     of 16 dims for 16-bit types, of 2 for fp32; 16-byte chunks 2t and 2t + 1
@@ -32,13 +32,14 @@
 // sign would: hence the + 0.0).
 //
 // Two routes, the same bits:
-//   * split: a workgroup per (request, kv head, up to 32 columns, segment); its
-//     four waves take a step each, so a segment's keys and values are all in
-//     flight at once, and a second kernel folds the segments. For few columns,
-//     where what bounds it is reading the cache.
+//   * split: a workgroup per (request, kv head, up to 32 columns, segment),
+//     whose four waves take a step each at a time; a second kernel folds the
+//     segments. For few columns, where what bounds it is reading the cache.
 //   * whole: a workgroup per 128 columns walks all their steps, 32 columns per
 //     wave, keys and values through two LDS buffers. For chunks of a prompt,
 //     where the matrix products and the exponentials bound it.
+// A segment is long enough that writing its results costs little beside
+// reading it, and short enough that one long sequence fills the GPU.
 #pragma once
 
 #include <float.h>
@@ -59,7 +60,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-typedef __attribute__((address_space(1))) const void global_void;
 
 constexpr float kNone = -FLT_MAX;  // the base of a column that has seen nothing
 
@@ -97,6 +97,11 @@ struct Walk {
   int32_t a, b, e;
   __device__ __forceinline__ int count() const { return a + (e - b); }
   __device__ __forceinline__ int unit(int i) const { return i < a ? i : b + (i - a); }
+  // How many of them are before unit u.
+  __device__ __forceinline__ int below(int u) const {
+    const int late = (u < e ? u : e) - b;
+    return (u < a ? u : a) + (late > 0 ? late : 0);
+  }
 };
 __device__ __forceinline__ Walk walk(const Args& p, int32_t lo, int32_t hi, int size) {
   Walk w;
@@ -130,13 +135,20 @@ __device__ __forceinline__ uint64_t seen_bits(const Args& p, int32_t pos, int32_
   return b & mapped;
 }
 
-// A row's page, or -1; contiguous keys: the request.
-__device__ __forceinline__ int32_t page_of(const Args& p, int r, int32_t key) {
-  if (!p.qstart) return r;
-  const int32_t pg = p.page_shift >= 0 ? key >> p.page_shift : (int32_t)((uint32_t)key / (uint32_t)p.page);
-  if (pg >= p.W) return -1;
-  const int32_t id = p.table[r * p.table_stride + pg];
-  return id < p.pages ? id : -1;
+// A row's table entry as it stands (loaded without a branch, so that nothing
+// waits for it before it is used), and what it says: the row's page, the
+// request for contiguous keys, -1 for none.
+__device__ __forceinline__ int32_t table_column(const Args& p, int32_t key) {
+  return p.page_shift >= 0 ? key >> p.page_shift : (int32_t)((uint32_t)key / (uint32_t)p.page);
+}
+__device__ __forceinline__ int32_t entry_of(const Args& p, int r, int32_t key) {
+  if (!p.qstart || p.W == 0) return r;
+  const int32_t c = table_column(p, key);
+  return p.table[r * p.table_stride + (c < 0 ? 0 : c < p.W ? c : p.W - 1)];
+}
+__device__ __forceinline__ int32_t page_of(const Args& p, int32_t entry, int32_t key) {
+  if (!p.qstart) return entry;
+  return table_column(p, key) < p.W && entry < p.pages ? entry : -1;
 }
 __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
   if (!p.qstart) return key;
@@ -147,12 +159,46 @@ __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+// Runs `use(n, operand)` for n = 0 .. N - 1 with the operands `read(n)` from LDS
+// four products ahead. (Left to itself the compiler reads each operand right
+// before its product, which then waits out the LDS latency.)
+template <int N, typename Read, typename Use>
+__device__ __forceinline__ void feed(const Read& read, const Use& use) {
+  static_assert(N % 4 == 0, "groups of four");
+  uint4 x[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[0][i] = read(i);
+#pragma unroll
+  for (int n = 0; n < N; n += 4) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (n + 4 < N)
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[(n / 4 + 1) & 1][i] = read(n + 4 + i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) use(n + i, x[(n / 4) & 1][i]);
+  }
+}
 __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32) |
          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 }
-// Loads that write LDS are not covered by a barrier's own waits.
+// 16 bytes from each lane's address to LDS at `to` + 16 * lane (`to` uniform),
+// in flight until wait_loads(). As asm, since beside the builtin, which the
+// compiler counts as an access of both memories, it waits for all LDS reads
+// and all loads wherever it waits for one. It has no result that could be
+// taken before it is there; the caller waits and meets a barrier before it
+// reads the LDS. (M0, which nothing else here uses, holds the LDS address.)
+__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(at), "v"(from) : "memory");
+}
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// LDS written before is visible to the workgroup after; loads stay in flight.
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 __device__ __forceinline__ float half_swap_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -199,13 +245,16 @@ struct Geo {
   static constexpr int D = D_, V = V_;
   static constexpr int E = sizeof(T);
   static constexpr int kStep = (D > V ? D : V) * E <= 256 ? 64 : 32;
-  static constexpr int kSeg = 4 * kStep;
+  static constexpr int kSeg = kSegSteps * kStep;
   static constexpr int KT = kStep / 32;       // score tiles per step
   static constexpr int CH = D * E / 16;       // 16-byte chunks per key row
   static constexpr int VCH = V * E / 16;      // per value row
+  static constexpr int MCH = CH > VCH ? CH : VCH;
   static constexpr int NQ = CH / 2;           // chunks per lane half
   static constexpr int PU = E;                // 16-byte units of p per tile and lane
   static constexpr int DT = V / 32;           // tiles of output dims
+  // Split workgroups per CU: 64 KB of values (4 steps) and their p twice fit its LDS.
+  static constexpr int kSplitPerCu = 4 * kStep * MCH > 4096 ? 1 : 2;
 
   // The lane's chunk pair t of keys and query: one product (fp32: four).
   __device__ __forceinline__ static f32x16 score(uint4 k, uint4 q, f32x16 c) {
@@ -282,53 +331,56 @@ struct Geo {
     else return (r >> 2) & 3;
   }
 
-  // o += values of rows `row0` + 0 .. 31 (LDS `v`) times p, output dims 32 dt ...
-  __device__ __forceinline__ static void accumulate(const uint4* v, int row0, int dt, int lane,
-                                                    const uint4 (&pu)[PU], f32x16& o) {
+  // The values' operand of product u of a tile: LDS rows row0 + 0 .. 31, those
+  // of p's unit u, output dims 32 dt ...
+  __device__ __forceinline__ static uint4 value(const uint4* v, int row0, int u, int dt, int lane) {
     const int half = lane >> 5;
     if constexpr (E == 2) {
       const int g = lane >> 4, i = lane & 15;
       const int rr = i >> 2, piece = i & 3;
       const int c = dt * 4 + (g & 1) * 2 + (piece >> 1);
+      i16x4 a[2];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        i16x4 a[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int r = row0 + 16 * u + 8 * x + 4 * half + rr;
-          const char* at = reinterpret_cast<const char*>(v + r * VCH + (c ^ vswz(r))) + 8 * (piece & 1);
-          a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
-        }
-        const uint2 lo = __builtin_bit_cast(uint2, a[0]), hi = __builtin_bit_cast(uint2, a[1]);
-        o = score(make_uint4(lo.x, lo.y, hi.x, hi.y), pu[u], o);
+      for (int x = 0; x < 2; x++) {
+        const int r = row0 + 16 * u + 8 * x + 4 * half + rr;
+        const char* at = reinterpret_cast<const char*>(v + r * VCH + (c ^ vswz(r))) + 8 * (piece & 1);
+        a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
       }
+      const uint2 lo = __builtin_bit_cast(uint2, a[0]), hi = __builtin_bit_cast(uint2, a[1]);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
     } else {
+      uint32_t a[4];
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        float a[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          a[e] = reinterpret_cast<const float*>(v + (row0 + 8 * u + 4 * half + e) * VCH)[32 * dt + (lane & 31)];
-        o = score(make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]),
-                             __float_as_uint(a[3])), pu[u], o);
-      }
+      for (int e = 0; e < 4; e++)
+        a[e] = reinterpret_cast<const uint32_t*>(v + (row0 + 8 * u + 4 * half + e) * VCH)[32 * dt + (lane & 31)];
+      return make_uint4(a[0], a[1], a[2], a[3]);
     }
   }
 };
 
+// A load from device memory. (From a generic pointer, such as one kept in LDS,
+// it would be a flat load, which counts as an LDS access too and makes every
+// later wait one for all loads.)
 __device__ __forceinline__ uint4 ld16(const void* p) {
-  return __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4*>(p));
+  typedef __attribute__((address_space(1))) const u32x4 gvec;
+  return __builtin_bit_cast(uint4, *(gvec*)p);
 }
 
-// A column's query as products' operand: chunks 2t + half.
+__device__ __forceinline__ void st16(uint4* p, uint4 v) {
+  *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, v);
+}
+
+// A column's query as the products' operand: chunks 2t + half.
 template <typename G>
-__device__ __forceinline__ void load_query(const Args& p, const char* q, bool valid, int half,
-                                           uint4 (&out)[G::NQ]) {
+__device__ __forceinline__ void load_query(const char* q, int half, uint4 (&out)[G::NQ]) {
 #pragma unroll
-  for (int t = 0; t < G::NQ; t++) {
-    uint4 x = valid ? ld16(q + (2 * t + half) * 16) : make_uint4(0, 0, 0, 0);
-    out[t] = make_uint4(x.x ^ p.qsign, x.y ^ p.qsign, x.z ^ p.qsign, x.w ^ p.qsign);
-  }
+  for (int t = 0; t < G::NQ; t++) out[t] = ld16(q + (2 * t + half) * 16);
+}
+template <typename G>
+__device__ __forceinline__ void sign_query(const Args& p, uint4 (&q)[G::NQ]) {
+#pragma unroll
+  for (int t = 0; t < G::NQ; t++)
+    q[t] = make_uint4(q[t].x ^ p.qsign, q[t].y ^ p.qsign, q[t].z ^ p.qsign, q[t].w ^ p.qsign);
 }
 template <typename T>
 __device__ __forceinline__ const char* query_at(const Args& p, int r, const Request& rq, int i, int head) {
@@ -341,24 +393,29 @@ __device__ __forceinline__ T* out_at(const Args& p, int r, const Request& rq, in
   return static_cast<T*>(p.out) + off + head * p.oh;
 }
 
-// Split route: partial result of NC columns over one segment; wave w takes
-// step w of the segment.
+// Split route: a segment's (m, l, o) of NC columns, four steps to a pass, one
+// per wave. What bounds it is reading the cache, which it does 64 KB at a
+// time: a step's values are on their way while its scores are computed, the
+// next pass's keys while the values are used, both through the same registers
+// (the table's entries are loaded two passes ahead). Reading 2 GB in 1 KB
+// loads, 16 a wave in flight on two such workgroups per CU, reaches 6.0-6.4
+// TB/s on this card, and 32 a wave only 4.7.
 template <typename T, int D, int V, int NC>
-__global__ void __launch_bounds__(256) split_kernel(Args p) {
+__global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel(Args p) {
   using G = Geo<T, D, V>;
   constexpr int S = G::kStep, KT = G::KT, PU = G::PU;
-  __shared__ uint4 s_v[G::kSeg * G::VCH];
+  __shared__ uint4 s_kv[4 * S * G::MCH];  // a step per wave: its keys, then its values
   __shared__ uint4 s_p[4 * KT * PU * 2 * NC];
-  __shared__ const char* s_row[2][G::kSeg];
+  __shared__ const char* s_row[2][4 * S];
   __shared__ float s_max[4][NC];
   __shared__ float s_sum[4][2 * NC];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, half = lane >> 5;
+  const int col = lane & 31, half = lane >> 5, cn = col & (NC - 1);
   int x = blockIdx.x;
   const int kvh = x % p.Hkv;
   x /= p.Hkv;
-  const int si = x % p.nseg;
+  const int part = x % p.nseg;
   const int r = x / p.nseg;
   const Request rq = request(p, r);
   const int ncol = rq.L * p.G;
@@ -366,82 +423,120 @@ __global__ void __launch_bounds__(256) split_kernel(Args p) {
   if (rq.beyond || ncol > p.split_cols || c0 >= ncol) return;
   const int clast = (c0 + NC < ncol ? c0 + NC : ncol) - 1;
   const int32_t lo = rq.n - rq.L + c0 / p.G, hi = rq.n - rq.L + clast / p.G;
+  // The segment's passes (4 steps each) that some column sees.
   const Walk w = walk(p, lo, hi, G::kSeg);
-  if (si >= w.count()) return;  // at most p.nseg of them
-  const int32_t seg0 = w.unit(si) * G::kSeg;
-  const int32_t key0 = seg0 + wave * S;
-  const bool live = any_seen(p, lo, hi, key0, S);
+  if (part >= w.count()) return;  // at most p.nseg of them
+  constexpr int PS = 4 * S, PN = G::kSeg / PS;
+  int s0 = w.unit(part) * PN, s1 = s0 + PN;
+  while (!any_seen(p, lo, hi, s0 * PS, PS)) s0++;
+  while (!any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
 
-  // Column.
+  // Column; one without a token takes the first one's query and sees nothing.
   const int cc = c0 + col;
   const bool cv = col < NC && cc < ncol;
-  const int tok = cv ? cc / p.G : 0, head = kvh * p.G + (cv ? cc - tok * p.G : 0);
+  const int cq = cv ? cc : c0;
+  const int tok = cq / p.G, head = kvh * p.G + (cq - tok * p.G);
   const int32_t pos = cv ? rq.n - rq.L + tok : -1;
+  const char* kh = static_cast<const char*>(p.k) + kvh * p.kh * (int64_t)sizeof(T);
+  const char* vh = static_cast<const char*>(p.v) + kvh * p.vh * (int64_t)sizeof(T);
 
-  uint64_t mapped = 0;
-  uint4 kr[KT][G::NQ], q[G::NQ];
-  if (live) {
-    const int32_t key = key0 + lane;
-    const char *ka = reinterpret_cast<const char*>(g_zero_row), *va = ka;
-    bool ok = lane < S && any_seen(p, lo, hi, key, 1);
-    const int32_t id = ok ? page_of(p, r, key) : -1;
-    ok = id >= 0;
-    if (ok) {
-      const int64_t row = row_of(p, key);
-      ka = static_cast<const char*>(p.k) + (id * p.kb + kvh * p.kh + row * p.kn) * (int64_t)sizeof(T);
-      va = static_cast<const char*>(p.v) + (id * p.vb + kvh * p.vh + row * p.vn) * (int64_t)sizeof(T);
+  // Row addresses of the wave's step of a segment; a row that no column sees,
+  // or that has no page, is a row of zeros. Without branches, so that the
+  // loads in flight are counted exactly.
+  auto key_of = [&](int si) __attribute__((always_inline)) { return si * PS + wave * S; };
+  auto entry_for = [&](int si) __attribute__((always_inline)) -> int32_t {
+    return entry_of(p, r, key_of(si) + (lane & (S - 1)));
+  };
+  auto put_rows = [&](int si, int32_t entry) __attribute__((always_inline)) -> uint64_t {
+    const int32_t key = key_of(si) + (lane & (S - 1));
+    const int32_t id = si < s1 && any_seen(p, lo, hi, key, 1) ? page_of(p, entry, key) : -1;
+    const int64_t row = row_of(p, key);
+    const char* zero = reinterpret_cast<const char*>(g_zero_row);
+    const char* ka = kh + (id * p.kb + row * p.kn) * (int64_t)sizeof(T);
+    const char* va = vh + (id * p.vb + row * p.vn) * (int64_t)sizeof(T);
+    s_row[0][wave * S + (lane & (S - 1))] = id >= 0 ? ka : zero;
+    s_row[1][wave * S + (lane & (S - 1))] = id >= 0 ? va : zero;
+    __builtin_amdgcn_wave_barrier();
+    return __builtin_amdgcn_ballot_w64(id >= 0);
+  };
+  // Rows are loaded whole, consecutive lanes taking consecutive chunks. Lane
+  // numbers go by way of opaque(): addresses are computed where they are used,
+  // not kept across segments in registers that the loads need.
+  constexpr int KL = S * G::CH / 64, VL = S * G::VCH / 64;
+  uint4 x16[KL > VL ? KL : VL], q[G::NQ];
+  auto load_keys = [&]() __attribute__((always_inline)) {
+    const int ln = opaque(lane);
+#pragma unroll
+    for (int j = 0; j < KL; j++) {
+      const int at = j * 64 + ln, row = at / G::CH;
+      x16[j] = ld16(s_row[0][wave * S + row] + (at - row * G::CH) * 16);
     }
-    mapped = __builtin_amdgcn_ballot_w64(ok);
-    if (lane < S) {
-      s_row[0][wave * S + lane] = ka;
-      s_row[1][wave * S + lane] = va;
+  };
+  auto load_values = [&]() __attribute__((always_inline)) {
+    const int ln = opaque(lane);
+#pragma unroll
+    for (int j = 0; j < VL; j++) {
+      const int at = j * 64 + ln, row = at / G::VCH;
+      x16[j] = ld16(s_row[1][wave * S + row] + (at - row * G::VCH) * 16);
     }
-    load_query<G>(p, query_at<T>(p, r, rq, tok, head), cv, half, q);
+  };
+
+  const int32_t entry0 = entry_for(s0);
+  int32_t entry = entry_for(s0 + 1);
+  load_query<G>(query_at<T>(p, r, rq, tok, head), half, q);
+  uint64_t mapped = put_rows(s0, entry0);
+  load_keys();
+  sign_query<G>(p, q);
+
+  constexpr int TW = (G::DT + 3) / 4;  // tiles of output dims per wave
+  float m = kNone, l = 0.f;
+  f32x16 o[TW];
+#pragma unroll
+  for (int i = 0; i < TW; i++) o[i] = f32x16{};
+  for (int si = s0; si < s1; si++) {
+    const int32_t pass0 = si * PS, key0 = pass0 + wave * S;
+    const int32_t entry2 = entry_for(si + 2);
+    // Scores of the wave's step and their largest.
+    // The keys change from rows to
+    // the products' operands by way of the LDS where the wave's values go next.
+    f32x16 s[KT];
+    float top = -INFINITY;
+    const int lk = opaque(lane);
+#pragma unroll
+    for (int j = 0; j < KL; j++) {
+      const int at = j * 64 + lk, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
+      st16(s_kv + wave * S * G::MCH + row * G::CH + c, x16[j]);
+    }
+    load_values();
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
-      const char* ra = s_row[0][wave * S + kt * 32 + col];
-#pragma unroll
-      for (int t = 0; t < G::NQ; t++) kr[kt][t] = ld16(ra + (2 * t + half) * 16);
-    }
-#pragma unroll
-    for (int j = 0; j < S * G::VCH / 64; j++) {
-      const int at = j * 64 + lane, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
-      const char* ra = s_row[1][wave * S + row];
-      __builtin_amdgcn_global_load_lds((global_void*)(ra + c * 16),
-                                       (lds_void*)(s_v + wave * S * G::VCH + j * 64), 16, 0, 0);
-    }
-  }
-
-  // Scores of the wave's step and their largest.
-  f32x16 s[KT];
-  float top = -INFINITY;
-  if (live) {
-    const bool full = mapped == (S == 64 ? ~0ull : 0xFFFFFFFFull) && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
       f32x16 c = {};
+      const int row = kt * 32 + (lk & 31), sw = G::kswz(row);
 #pragma unroll
-      for (int t = 0; t < G::NQ; t++) c = G::score(kr[kt][t], q[t], c);
+      for (int t = 0; t < G::NQ; t++)
+        c = G::score(s_kv[wave * S * G::MCH + row * G::CH + ((2 * t + (lk >> 5)) ^ sw)], q[t], c);
       s[kt] = c;
     }
+    const bool full = mapped == ~0ull && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
     if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
 #pragma unroll
     for (int kt = 0; kt < KT; kt++)
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, s[kt][i]);
     top = half_swap_max(top);
-  }
-  if (lane < NC) s_max[wave][lane] = top;
-  __syncthreads();
+    if (lane < NC) s_max[wave][lane] = top;
+    barrier();
 
-  // The bases of the segment's steps; this wave's p.
-  const int cn = col & (NC - 1);
-  float base[4], m = kNone;
+    // The bases of the pass's steps; this wave's p.
+    float base[4], f[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) base[i] = m = next_base(m, s_max[i][cn], p.scale2);
-  float psum = 0.f;
-  if (live) {
+    for (int i = 0; i < 4; i++) {
+      base[i] = next_base(m, s_max[i][cn], p.scale2);
+      f[i] = pow2(m - base[i]);
+      m = base[i];
+    }
+    float psum = 0.f;
     const float mw = wave == 0 ? base[0] : wave == 1 ? base[1] : wave == 2 ? base[2] : base[3];
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
@@ -456,48 +551,57 @@ __global__ void __launch_bounds__(256) split_kernel(Args p) {
 #pragma unroll
         for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = u[j];
     }
-  }
-  if (col < NC) s_sum[wave][half * NC + col] = psum;
-  wait_loads();
-  __syncthreads();
-
-  // The wave's tiles of output dims over the segment's steps.
-  const int64_t slot = (((int64_t)r * p.Hkv + kvh) * p.ccap + cc) * p.nseg + si;
-  if (wave == 0) {
-    float l = 0.f;
-    m = kNone;
+    if (col < NC) s_sum[wave][half * NC + col] = psum;
+    const int ln = opaque(lane);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      l = __builtin_fmaf(l, pow2(m - base[i]), s_sum[i][half * NC + cn]);
-      m = base[i];
+    for (int j = 0; j < VL; j++) {
+      const int at = j * 64 + ln, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
+      st16(s_kv + wave * S * G::MCH + row * G::VCH + c, x16[j]);
     }
-    l = half_swap_sum(l);
-    if (cv && half == 0) p.pml[slot] = make_float2(m, l);
-  }
-  for (int dt = wave; dt < G::DT; dt += 4) {
-    f32x16 o = {};
-    m = kNone;
+    mapped = put_rows(si + 1, entry);
+    entry = entry2;
+    load_keys();
+    barrier();
+
+    // The sum, and the wave's tiles of output dims over the pass's steps.
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (!any_seen(p, lo, hi, seg0 + i * S, S)) continue;
-      const float f = pow2(m - base[i]);
-      m = base[i];
+    for (int i = 0; i < 4; i++) l = __builtin_fmaf(l, f[i], s_sum[i][half * NC + cn]);
 #pragma unroll
-      for (int e = 0; e < 16; e++) o[e] *= f;
+    for (int x = 0; x < TW; x++) {
+      const int dt = wave + 4 * x;
+      if (dt >= G::DT) break;
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++) {
-        uint4 u[PU];
+      for (int i = 0; i < 4; i++) {
+        if (!any_seen(p, lo, hi, pass0 + i * S, S)) continue;
+        if (__builtin_amdgcn_ballot_w64(f[i] != 1.f) != 0)
 #pragma unroll
-        for (int j = 0; j < PU; j++) u[j] = s_p[((i * KT + kt) * PU + j) * 2 * NC + half * NC + cn];
-        G::accumulate(s_v, i * S + kt * 32, dt, lane, u, o);
+          for (int e = 0; e < 16; e++) o[x][e] *= f[i];
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+          uint4 u[PU];
+#pragma unroll
+          for (int j = 0; j < PU; j++) u[j] = s_p[((i * KT + kt) * PU + j) * 2 * NC + (ln >> 5) * NC + (ln & (NC - 1))];
+#pragma unroll
+          for (int j = 0; j < PU; j++)
+            o[x] = G::score(G::value(s_kv + i * S * G::MCH, kt * 32, j, dt, ln), u[j], o[x]);
+        }
       }
     }
-    if (cv) {
-      float* to = p.po + slot * V + 32 * dt;
+    barrier();  // everyone is done with the values and p
+  }
+
+  l = half_swap_sum(l);
+  if (!cv) return;
+  const int64_t slot = (((int64_t)r * p.Hkv + kvh) * p.nseg + part) * p.ccap + cc;
+  if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
 #pragma unroll
-      for (int b = 0; b < 4; b++)
-        *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) = f32x4{o[4 * b], o[4 * b + 1], o[4 * b + 2], o[4 * b + 3]};
-    }
+  for (int x = 0; x < TW; x++) {
+    if (wave + 4 * x >= G::DT) break;
+    float* to = p.po + slot * V + 32 * (wave + 4 * x);
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+      *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
+          f32x4{o[x][4 * b], o[x][4 * b + 1], o[x][4 * b + 2], o[x][4 * b + 3]};
   }
 }
 
@@ -529,7 +633,7 @@ __device__ void fill(const Args& p, int block) {
 template <typename T, int D, int V>
 __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   using G = Geo<T, D, V>;
-  constexpr int NV = (V + 63) / 64;
+  constexpr int NV = (V + 127) / 128;
   if ((int)blockIdx.x < p.fill_blocks) {
     fill<T, V>(p, blockIdx.x);
     return;
@@ -549,25 +653,32 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
   const int n = w.count() < p.nseg ? w.count() : p.nseg;
   const int tok = cc / p.G, head = kvh * p.G + cc - tok * p.G;
-  const int64_t slot = (((int64_t)r * p.Hkv + kvh) * p.ccap + cc) * p.nseg;
-  float M = kNone, L = 0.f, O[NV] = {};
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float o[8][NV];
-    float2 ml[8];
+  const int64_t slot = ((int64_t)r * p.Hkv + kvh) * p.nseg * p.ccap + cc;  // segments ccap apart
+  // Dims 2 lane, 2 lane + 1 and those 128 further; 16 segments' loads in flight.
+  constexpr int NB = 16;
+  float M = kNone, L = 0.f;
+  f32x2 O[NV] = {};
+  for (int i0 = 0; i0 < n; i0 += NB) {
+    f32x2 o[NB][NV];
+    float2 ml[NB];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < NB; i++) {
       const bool in = i0 + i < n;
-      ml[i] = in ? p.pml[slot + i0 + i] : make_float2(kNone, 0.f);
+      ml[i] = in ? p.pml[slot + (int64_t)(i0 + i) * p.ccap] : make_float2(kNone, 0.f);
 #pragma unroll
       for (int j = 0; j < NV; j++)
-        o[i][j] = in && lane + 64 * j < V ? p.po[(slot + i0 + i) * V + lane + 64 * j] : 0.f;
+        o[i][j] = in && 2 * lane + 128 * j < V
+                      ? *reinterpret_cast<const f32x2*>(p.po + (slot + (int64_t)(i0 + i) * p.ccap) * V + 2 * lane + 128 * j)
+                      : f32x2{0.f, 0.f};
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < NB; i++) {
       float fa, fb;
       fold_base(M, L, ml[i].x, ml[i].y, fa, fb);
 #pragma unroll
-      for (int j = 0; j < NV; j++) O[j] = __builtin_fmaf(o[i][j], fb, O[j] * fa);
+      for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) O[j][k] = __builtin_fmaf(o[i][j][k], fb, O[j][k] * fa);
     }
   }
   float e, den;
@@ -577,7 +688,11 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   T* out = out_at<T>(p, r, rq, tok, head);
 #pragma unroll
   for (int j = 0; j < NV; j++)
-    if (lane + 64 * j < V) out[lane + 64 * j] = result<T>(O[j], e, inv);
+    if (2 * lane + 128 * j < V) {
+      typedef T T2 __attribute__((ext_vector_type(2)));
+      *reinterpret_cast<T2*>(out + 2 * lane + 128 * j) =
+          T2{result<T>(O[j][0], e, inv), result<T>(O[j][1], e, inv)};
+    }
 }
 
 // Whole route: NW waves of 32 columns each walk the steps that some column of
@@ -591,6 +706,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   __shared__ const char* s_row[2][2][S];
   __shared__ uint64_t s_map[4];
   __shared__ int s_scan[NW + 3];
+  __shared__ float s_ml[2][NT];  // each lane's own M and L
 
   if ((int)blockIdx.x < p.fill_blocks) {
     fill<T, V>(p, blockIdx.x);
@@ -661,11 +777,12 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
 
   const int cc = cw + col;
   const bool cv = cc < ncol;
-  const int tok = cv ? cc / p.G : 0, head = kvh * p.G + (cv ? cc - tok * p.G : 0);
+  const int tok = cv ? cc / p.G : 0;
   const int32_t pos = cv ? p0 + tok : -1;
   const bool whole_tile = cw + 32 <= ncol;
   uint4 q[G::NQ];
-  load_query<G>(p, query_at<T>(p, r, rq, tok, head), cv, half, q);
+  load_query<G>(query_at<T>(p, r, rq, tok, kvh * p.G + (cv ? cc - tok * p.G : 0)), half, q);
+  sign_query<G>(p, q);
 
   const Walk w = walk(p, lo, hi, S);
   const int steps = w.count();
@@ -674,16 +791,16 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
 
   // Row addresses of a step, by the first wave: the page's number is loaded a
   // step before they are written, which is a step before they are used.
-  auto page_for = [&](int j) __attribute__((always_inline)) -> int32_t {
-    if (j >= steps || lane >= S) return -1;
-    const int32_t key = w.unit(j) * S + lane;
-    return any_seen(p, lo, hi, key, 1) ? page_of(p, r, key) : -1;
+  auto entry_for = [&](int j) __attribute__((always_inline)) -> int32_t {
+    return entry_of(p, r, w.unit(j) * S + lane);
   };
-  auto put_rows = [&](int j, int32_t id) __attribute__((always_inline)) {
+  auto put_rows = [&](int j, int32_t entry) __attribute__((always_inline)) {
     if (j >= steps) return;
+    const int32_t key = w.unit(j) * S + lane;
+    const int32_t id = lane < S && any_seen(p, lo, hi, key, 1) ? page_of(p, entry, key) : -1;
     const char *ka = reinterpret_cast<const char*>(g_zero_row), *va = ka;
     if (id >= 0) {
-      const int64_t row = row_of(p, w.unit(j) * S + lane);
+      const int64_t row = row_of(p, key);
       ka = kh + (id * p.kb + row * p.kn) * (int64_t)sizeof(T);
       va = vh + (id * p.vb + row * p.vn) * (int64_t)sizeof(T);
     }
@@ -700,27 +817,30 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     for (int i = 0; i < (KU + NT - 1) / NT; i++) {
       const int at = i * NT + td, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
       if (KU % NT == 0 || at < KU)
-        __builtin_amdgcn_global_load_lds((global_void*)(s_row[j & 1][0][row] + c * 16),
-                                         (lds_void*)(kd + i * NT + wave * 64), 16, 0, 0);
+        load_to_lds(s_row[j & 1][0][row] + c * 16, kd + i * NT + wave * 64);
     }
 #pragma unroll
     for (int i = 0; i < (VU + NT - 1) / NT; i++) {
       const int at = i * NT + td, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
       if (VU % NT == 0 || at < VU)
-        __builtin_amdgcn_global_load_lds((global_void*)(s_row[j & 1][1][row] + c * 16),
-                                         (lds_void*)(vd + i * NT + wave * 64), 16, 0, 0);
+        load_to_lds(s_row[j & 1][1][row] + c * 16, vd + i * NT + wave * 64);
     }
   };
 
-  float M = kNone, L = 0.f, m = kNone, l = 0.f;
+  // The segment's o and the result's O are in registers, the result's base and
+  // sum, which are touched once in 8 steps, in LDS. (O in scratch memory cost
+  // 490 us of 1060 over 8192 keys: what the waves keep there exceeds the L2.)
+  float m = kNone, l = 0.f;
   f32x16 O[DT], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) O[dt] = f32x16{}, o[dt] = f32x16{};
+  s_ml[0][tid] = kNone;
+  s_ml[1][tid] = 0.f;
 
   if (steps > 0) {
     if (wave == 0) {
-      put_rows(0, page_for(0));
-      put_rows(1, page_for(1));
+      put_rows(0, entry_for(0));
+      put_rows(1, entry_for(1));
     }
     __syncthreads();
     load_step(0, s_k0, s_v0);
@@ -730,10 +850,10 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     // LDS addresses are computed anew each step: kept across steps they, for
     // two buffers, take the registers that o and O need.
     const int ln = opaque(lane), hf = ln >> 5;
-    wait_loads();     // this wave's part of step j
-    __syncthreads();  // everyone's, and everyone is done with the other buffers
+    wait_loads();  // this wave's part of step j
+    barrier();     // everyone's, and everyone is done with the other buffers
     int32_t id = -1;
-    if (wave == 0) id = page_for(j + 2);
+    if (wave == 0) id = entry_for(j + 2);
     if (j + 1 < steps) load_step(j + 1, kn, vn);
     const int32_t unit = w.unit(j), key0 = unit * S;
     if (any_seen(p, wlo, whi, key0, S)) {
@@ -743,14 +863,16 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
       f32x16 s[KT];
       float top = -INFINITY;
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++) {
-        f32x16 c = {};
-        const int row = kt * 32 + (ln & 31), sw = G::kswz(row);
-#pragma unroll
-        for (int t = 0; t < G::NQ; t++) c = G::score(kd[row * G::CH + ((2 * t + hf) ^ sw)], q[t], c);
-        s[kt] = c;
-      }
-      if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
+      for (int kt = 0; kt < KT; kt++) s[kt] = f32x16{};
+      feed<KT * G::NQ>(
+          [&](int n) __attribute__((always_inline)) {
+            const int row = n % KT * 32 + (ln & 31), t = n / KT;
+            return kd[row * G::CH + ((2 * t + hf) ^ G::kswz(row))];
+          },
+          [&](int n, uint4 k) __attribute__((always_inline)) {
+            s[n % KT] = G::score(k, q[n / KT], s[n % KT]);
+          });
+      if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * hf));
 #pragma unroll
       for (int kt = 0; kt < KT; kt++)
 #pragma unroll
@@ -781,29 +903,29 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
         G::pack(e, pu[kt]);
       }
       l = __builtin_fmaf(l, f, psum);
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) G::accumulate(vd, kt * 32, dt, ln, pu[kt], o[dt]);
+      // Products of one output tile are a chain: those of the others go between.
+      feed<DT * KT * PU>(
+          [&](int n) __attribute__((always_inline)) {
+            return G::value(vd, n / DT / PU * 32, n / DT % PU, n % DT, ln);
+          },
+          [&](int n, uint4 v) __attribute__((always_inline)) {
+            o[n % DT] = G::score(v, pu[n / DT / PU][n / DT % PU], o[n % DT]);
+          });
     }
     // The segment's end: fold it.
-    if (j + 1 == steps || w.unit(j + 1) / 4 != unit / 4) {
+    if (j + 1 == steps || w.unit(j + 1) / kSegSteps != unit / kSegSteps) {
       if (__builtin_amdgcn_ballot_w64(m != kNone) != 0) {
-        float fa, fb;
+        const int td = opaque(tid);
+        float M = s_ml[0][td], L = s_ml[1][td], fa, fb;
         fold_base(M, L, m, half_swap_sum(l), fa, fb);
-        if (__builtin_amdgcn_ballot_w64(fa != 1.f || fb != 1.f) == 0) {
+        s_ml[0][td] = M;
+        s_ml[1][td] = L;
 #pragma unroll
-          for (int dt = 0; dt < DT; dt++)
+        for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) O[dt][i] += o[dt][i];
-        } else {
-#pragma unroll
-          for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) O[dt][i] = __builtin_fmaf(o[dt][i], fb, O[dt][i] * fa);
+          for (int i = 0; i < 16; i++) O[dt][i] = __builtin_fmaf(o[dt][i], fb, O[dt][i] * fa);
+          o[dt] = f32x16{};
         }
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) o[dt] = f32x16{};
         m = kNone;
         l = 0.f;
       }
@@ -815,22 +937,27 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     if (j + 1 < steps) step(j + 1, s_k1, s_v1, s_k0, s_v0);
   }
 
-  if (!cv) return;
+  // The column anew (kept, it would take registers that the loop needs).
+  const int lane2 = opaque(lane), cc2 = cw + (lane2 & 31), half2 = lane2 >> 5;
+  if (cc2 >= ncol) return;
+  const int tok2 = cc2 / p.G, head = kvh * p.G + cc2 - tok2 * p.G;
+  const float M = s_ml[0][wave * 64 + lane2], L = s_ml[1][wave * 64 + lane2];
   float e, den;
   finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
          p.sinks != nullptr, e, den);
   const float inv = inverse(den);
-  T* out = out_at<T>(p, r, rq, tok, head);
+  T* out = out_at<T>(p, r, rq, tok2, head);
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++)
+  for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
     for (int b = 0; b < 4; b++) {
       typedef T T4 __attribute__((ext_vector_type(4)));
       T4 y;
 #pragma unroll
       for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, inv);
-      *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half) = y;
+      *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half2) = y;
     }
+  }
 }
 
 template <typename T, int D, int V>
