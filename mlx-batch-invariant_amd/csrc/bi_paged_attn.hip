@@ -132,7 +132,8 @@ void common(Args& p, int64_t H, int64_t Hkv, float scale, int64_t window, int64_
   p.G = (int32_t)(H / Hkv);
   p.window = clamp32(window);
   p.first = clamp32(sink_tokens);
-  p.scale2 = fabsf(scale) * 1.4426950408889634f;
+  // Not 0, with which an unseen row's -inf would not stay one.
+  p.scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.2e-38f);
   p.qsign = scale < 0.f ? (dtype == BI_F32 ? 0x80000000u : 0x80008000u) : 0u;
 }
 

@@ -16,8 +16,8 @@
 //     of 16 dims for 16-bit types, of 2 for fp32; 16-byte chunks 2t and 2t + 1
 //     of the rows enter product t (fp32: products 4t .. 4t + 3).
 //   * Within a segment the running base m moves at a step whose largest seen
-//     score M exceeds m + 8, to the multiple of 8 nearest M. p_j =
-//     2^(fma(raw_j, a, -m)), 0 for an unseen row; l = l * f + (the step's sum,
+//     score M exceeds m + 6, to the next multiple of 4 from M on. p_j =
+//     2^(fma(raw_j, a, -m)), 0 for an unseen row (whose raw_j is -inf); l = l * f + (the step's sum,
 //     in a fixed tree per lane half); o = o * f, then o += v . p by 32x32
 //     products over the step's rows in ascending order, p rounded once to the
 //     type (the products of bf16 and f16 take such operands; l sums the
@@ -44,6 +44,8 @@
 
 #include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "bi_paged_attn.h"
 
@@ -202,7 +204,7 @@ __device__ __forceinline__ void barrier() {
 
 __device__ __forceinline__ float half_swap_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float half_swap_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -212,10 +214,13 @@ __device__ __forceinline__ float half_swap_sum(float x) {
 __device__ __forceinline__ float pow2(float e) {
   return __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(e, -300.f));
 }
-// The base after a step whose largest seen raw score is `top` (-inf: none seen).
+// The base after a step whose largest seen raw score is `top` (-inf: none seen):
+// p is at most 2^kRise, and above 2^-4 for the largest score of a segment's
+// first step (f16 holds p to 2^-25).
+constexpr float kRise = 6.f, kMostSum = 64.f;
 __device__ __forceinline__ float next_base(float m, float top, float a) {
   const float s = top * a;
-  return top > -INFINITY && s > m + 8.f ? rintf(s * 0.125f) * 8.f : m;
+  return top > -INFINITY && s > m + kRise ? ceilf(s * 0.25f) * 4.f : m;
 }
 // Folds a segment's (m, l) into the running (M, L); fa and fb scale O and o.
 __device__ __forceinline__ void fold_base(float& M, float& L, float m, float l, float& fa, float& fb) {
@@ -273,6 +278,26 @@ struct Geo {
   }
   // Element i of a tile is row 8 (i / 4) + 4 half + i % 4.
   __device__ __forceinline__ static int row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
+  // Row 32 kt + r's chunk 2 t + half. (Where a row's chunks are a power of two,
+  // 2t only flips bits of the place at t = 0.)
+  __device__ __forceinline__ static uint4 key_chunk(const uint4* k, int kt, int r, int t, int half) {
+    const char* at = reinterpret_cast<const char*>(k + 32 * kt * CH);
+    if constexpr ((CH & (CH - 1)) == 0) at += ((r * CH + (half ^ kswz(r))) * 16) ^ (32 * t);
+    else at += (r * CH + ((2 * t + half) ^ kswz(r))) * 16;
+    return __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4*>(at));
+  }
+  // The largest score. (As the IEEE maximum, of which there is an instruction of
+  // three operands; fmaxf would first quiet both of its own. A NaN score makes
+  // its column NaN in any case.)
+  __device__ __forceinline__ static float top(const f32x16 (&s)[KT]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2)
+        m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, s[kt][i]), s[kt][i + 1]);
+    return half_swap_max(m);
+  }
   // Scores of unseen rows become -inf; `seen` is shifted by the half's 4 rows.
   __device__ __forceinline__ static void hide(f32x16 (&s)[KT], uint64_t seen) {
 #pragma unroll
@@ -500,7 +525,6 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
     // The keys change from rows to
     // the products' operands by way of the LDS where the wave's values go next.
     f32x16 s[KT];
-    float top = -INFINITY;
     const int lk = opaque(lane);
 #pragma unroll
     for (int j = 0; j < KL; j++) {
@@ -512,19 +536,14 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
       f32x16 c = {};
-      const int row = kt * 32 + (lk & 31), sw = G::kswz(row);
 #pragma unroll
       for (int t = 0; t < G::NQ; t++)
-        c = G::score(s_kv[wave * S * G::MCH + row * G::CH + ((2 * t + (lk >> 5)) ^ sw)], q[t], c);
+        c = G::score(G::key_chunk(s_kv + wave * S * G::MCH, kt, lk & 31, t, lk >> 5), q[t], c);
       s[kt] = c;
     }
     const bool full = mapped == ~0ull && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
     if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, s[kt][i]);
-    top = half_swap_max(top);
+    const float top = G::top(s);
     if (lane < NC) s_max[wave][lane] = top;
     barrier();
 
@@ -543,7 +562,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
       f32x16 e;
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        e[i] = s[kt][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -mw));
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -mw));
       psum = kt == 0 ? G::sum(e) : psum + G::sum(e);
       uint4 u[PU];
       G::pack(e, u);
@@ -811,26 +830,29 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     }
     if (lane == 0) s_map[j & 3] = m;
   };
-  auto load_step = [&](int j, uint4* kd, uint4* vd) __attribute__((always_inline)) {
+  auto load_rows = [&](const char* const* rows, auto ch, auto swizzle, uint4* to)
+      __attribute__((always_inline)) {
+    constexpr int C = decltype(ch)::value, U = S * C;
     const int td = opaque(tid);
 #pragma unroll
-    for (int i = 0; i < (KU + NT - 1) / NT; i++) {
-      const int at = i * NT + td, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
-      if (KU % NT == 0 || at < KU)
-        load_to_lds(s_row[j & 1][0][row] + c * 16, kd + i * NT + wave * 64);
+    for (int i = 0; i < (U + NT - 1) / NT; i++) {
+      // Of chunk i NT + td of the step.
+      const int row = NT % C == 0 ? i * (NT / C) + td / C : (i * NT + td) / C;
+      const int c = NT % C == 0 ? td % C : (i * NT + td) % C;
+      if (U % NT == 0 || i * NT + td < U)
+        load_to_lds(rows[row] + (c ^ swizzle(row)) * 16, to + i * NT + wave * 64);
     }
-#pragma unroll
-    for (int i = 0; i < (VU + NT - 1) / NT; i++) {
-      const int at = i * NT + td, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
-      if (VU % NT == 0 || at < VU)
-        load_to_lds(s_row[j & 1][1][row] + c * 16, vd + i * NT + wave * 64);
-    }
+  };
+  auto load_step = [&](int j, uint4* kd, uint4* vd) __attribute__((always_inline)) {
+    load_rows(s_row[j & 1][0], std::integral_constant<int, G::CH>(), G::kswz, kd);
+    load_rows(s_row[j & 1][1], std::integral_constant<int, G::VCH>(), G::vswz, vd);
   };
 
   // The segment's o and the result's O are in registers, the result's base and
   // sum, which are touched once in 8 steps, in LDS. (O in scratch memory cost
   // 490 us of 1060 over 8192 keys: what the waves keep there exceeds the L2.)
   float m = kNone, l = 0.f;
+  bool fresh = true;  // the segment has no step yet
   f32x16 O[DT], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) O[dt] = f32x16{}, o[dt] = f32x16{};
@@ -861,48 +883,52 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
       const bool full = whole_tile && mapped == (S == 64 ? ~0ull : 0xFFFFFFFFull) &&
                         all_seen(p, wlo, whi, key0, S);
       f32x16 s[KT];
-      float top = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < KT; kt++) s[kt] = f32x16{};
       feed<KT * G::NQ>(
           [&](int n) __attribute__((always_inline)) {
-            const int row = n % KT * 32 + (ln & 31), t = n / KT;
-            return kd[row * G::CH + ((2 * t + hf) ^ G::kswz(row))];
+            return G::key_chunk(kd, n % KT, ln & 31, n / KT, hf);
           },
           [&](int n, uint4 k) __attribute__((always_inline)) {
             s[n % KT] = G::score(k, q[n / KT], s[n % KT]);
           });
-      if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * hf));
-#pragma unroll
-      for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) top = fmaxf(top, s[kt][i]);
-      top = half_swap_max(top);
-      const float mn = next_base(m, top, p.scale2);
-      const float f = pow2(m - mn);
-      if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) o[dt][i] *= f;
-        m = mn;
+      if (!full) {
+        const int ps = opaque(pos);  // keeps the bits' computation in this branch
+        G::hide(s, seen_bits(p, ps, key0, mapped) >> (4 * hf));
       }
+      // A lane's sum of at most 2^kRise holds no p above it, so the base does
+      // not move; else, and at a segment's first step, the largest score
+      // decides.
       uint4 pu[KT][PU];
-      float psum = 0.f;
+      float psum;
+      bool look = fresh;
+      for (;;) {
+        if (look) {
+          const float mn = next_base(m, G::top(s), p.scale2);
+          if (!fresh && __builtin_amdgcn_ballot_w64(mn != m) != 0) {
+            const float f = pow2(m - mn);
+            l *= f;  // exact, as in the sum's fma(l, f, .)
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++) {
-        f32x16 e;
+            for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -m));
-        if (!full) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) e[i] = s[kt][i] == -INFINITY ? 0.f : e[i];
+              for (int i = 0; i < 16; i++) o[dt][i] *= f;
+          }
+          m = mn;
         }
-        psum = kt == 0 ? G::sum(e) : psum + G::sum(e);
-        G::pack(e, pu[kt]);
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+          f32x16 e;
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -m));
+          psum = kt == 0 ? G::sum(e) : psum + G::sum(e);
+          G::pack(e, pu[kt]);
+        }
+        if (look || __builtin_amdgcn_ballot_w64(psum > kMostSum) == 0) break;
+        look = true;
       }
-      l = __builtin_fmaf(l, f, psum);
+      l += psum;
+      fresh = false;
       // Products of one output tile are a chain: those of the others go between.
       feed<DT * KT * PU>(
           [&](int n) __attribute__((always_inline)) {
@@ -914,20 +940,26 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     }
     // The segment's end: fold it.
     if (j + 1 == steps || w.unit(j + 1) / kSegSteps != unit / kSegSteps) {
-      if (__builtin_amdgcn_ballot_w64(m != kNone) != 0) {
+      if (!fresh) {
         const int td = opaque(tid);
         float M = s_ml[0][td], L = s_ml[1][td], fa, fb;
         fold_base(M, L, m, half_swap_sum(l), fa, fb);
         s_ml[0][td] = M;
         s_ml[1][td] = L;
+        if (__builtin_amdgcn_ballot_w64(fa != 1.f) != 0)
+#pragma unroll
+          for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) O[dt][i] *= fa;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
-          for (int i = 0; i < 16; i++) O[dt][i] = __builtin_fmaf(o[dt][i], fb, O[dt][i] * fa);
+          for (int i = 0; i < 16; i++) O[dt][i] = __builtin_fmaf(o[dt][i], fb, O[dt][i]);
           o[dt] = f32x16{};
         }
         m = kNone;
         l = 0.f;
+        fresh = true;
       }
     }
     if (wave == 0) put_rows(j + 2, id);
