@@ -2,6 +2,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
+
 #include <hip/hip_runtime_api.h>
 
 #include "bi_internal.h"
@@ -23,6 +25,20 @@ int fail(int code, const char* fmt, ...) {
 int launch_error(int hip_error, const char* what) {
   return fail(BI_ELAUNCH, "%s: HIP error %d (%s)", what, hip_error,
               hipGetErrorString(static_cast<hipError_t>(hip_error)));
+}
+
+int device_cus() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n <= 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        n <= 0)
+      n = 256;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 }  // namespace bi

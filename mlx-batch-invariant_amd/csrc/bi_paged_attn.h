@@ -37,7 +37,6 @@ struct Args {
   int32_t nseg, ccap;     // segments and columns kept per (request, kv head)
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
-  int32_t tiles;          // whole route: column tiles per kv head
 };
 
 constexpr int kSegSteps = 8;  // steps to a segment
@@ -45,9 +44,9 @@ constexpr int kSegSteps = 8;  // steps to a segment
 typedef void (*Kernel)(Args);
 struct Kernels {
   Kernel split16, split32;  // 16 or 32 columns per workgroup
-  Kernel combine, whole;
+  Kernel combine;
+  Kernel whole4, whole8;    // 4 or 8 waves of 32 columns per workgroup
   int step;                 // rows per step
-  int whole_cols, whole_threads;
 };
 
 #define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)

@@ -85,16 +85,21 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.fill_blocks = 0;
   }
   if (whole || p.fill_blocks) {
+    // Eight waves share their keys' and values' loads and addresses where that
+    // leaves a workgroup for every compute unit (4096 tokens over 8192 keys 517
+    // -> 496 us); with fewer, four of them fill more (two chunks of 511 tokens
+    // beside 30 decodes 161 us, 175 with eight).
+    const int64_t cols = p.qstart ? (int64_t)p.T * p.G : (int64_t)p.R * p.qL * p.G;
+    const int waves = cols / 256 * p.Hkv >= bi::device_cus() ? 8 : 4;
+    const int64_t wc = 32 * waves;
     // Column tiles: every request with tokens may end in a part of one.
-    const int64_t wc = k.whole_cols;
-    const int64_t reqs = p.T < p.R ? p.T : p.R;
-    int64_t tiles = p.qstart ? (int64_t)p.T * p.G / wc + reqs
+    int64_t tiles = p.qstart ? cols / wc + (p.T < p.R ? p.T : p.R)
                              : (int64_t)p.R * (((int64_t)p.qL * p.G + wc - 1) / wc);
     if (!whole) tiles = 0;
     const int64_t blocks = tiles * p.Hkv + p.fill_blocks;
     if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
     if (blocks == 0) return BI_OK;
-    hipLaunchKernelGGL(k.whole, dim3((unsigned)blocks), dim3(k.whole_threads), 0, st, p);
+    hipLaunchKernelGGL(waves == 8 ? k.whole8 : k.whole4, dim3((unsigned)blocks), dim3(64 * waves), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   return BI_OK;

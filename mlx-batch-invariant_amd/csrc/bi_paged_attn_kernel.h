@@ -17,11 +17,11 @@
 //     of the rows enter product t (fp32: products 4t .. 4t + 3).
 //   * Within a segment the running base m moves at a step whose largest seen
 //     score M exceeds m + 6, to the next multiple of 4 from M on. p_j =
-//     2^(fma(raw_j, a, -m)), 0 for an unseen row (whose raw_j is -inf); l = l * f + (the step's sum,
-//     in a fixed tree per lane half); o = o * f, then o += v . p by 32x32
+//     2^(fma(raw_j, a, -m)), 0 for an unseen row (whose raw_j is -inf); l = l * f + (the step's sum of
+//     p, in a fixed order per lane half); o = o * f, then o += v . p by 32x32
 //     products over the step's rows in ascending order, p rounded once to the
-//     type (the products of bf16 and f16 take such operands; l sums the
-//     unrounded p). f is a power of two, as every base is an integer.
+//     type (the products of bf16 and f16 take such operands), and l sums what
+//     was rounded. f is a power of two, as every base is an integer.
 //   * Segments start from nothing and are folded in ascending order: with M'
 //     the larger base, O = fma(o, 2^(m - M'), O * 2^(M - M')), L alike.
 //   * The sink enters last: out = (O * e) / (L * e + 2^(sink2 - X)) + 0.0, X the
@@ -35,7 +35,7 @@
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment),
 //     whose four waves take a step each at a time; a second kernel folds the
 //     segments. For few columns, where what bounds it is reading the cache.
-//   * whole: a workgroup per 128 columns walks all their steps, 32 columns per
+//   * whole: a workgroup per 128 or 256 columns walks all their steps, 32 columns per
 //     wave, keys and values through two LDS buffers. For chunks of a prompt,
 //     where the matrix products and the exponentials bound it.
 // A segment is long enough that writing its results costs little beside
@@ -59,6 +59,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
@@ -332,11 +333,32 @@ struct Geo {
                           __float_as_uint(p[4 * j + 2]), __float_as_uint(p[4 * j + 3]));
     }
   }
-  __device__ __forceinline__ static float sum(const f32x16& p) {
-    float s[8];
+  // A lane's sum of the step's p as they were rounded, so that what is divided
+  // by is what was multiplied with: a chain per unit, units in pairs.
+  __device__ __forceinline__ static float sum(const uint4 (&u)[KT][PU]) {
+    float s[KT * PU];
 #pragma unroll
-    for (int i = 0; i < 8; i++) s[i] = p[2 * i] + p[2 * i + 1];
-    return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    for (int i = 0; i < KT * PU; i++) {
+      const uint4 x = u[i / PU][i % PU];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      s[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if constexpr (__is_same(T, __bf16))
+          s[i] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[j]),
+                                                 __builtin_bit_cast(bf16x2, 0x3F803F80u), s[i], false);
+        else if constexpr (__is_same(T, _Float16))
+          s[i] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w[j]),
+                                        __builtin_bit_cast(f16x2, 0x3C003C00u), s[i], false);
+        else
+          s[i] = j == 0 ? __uint_as_float(w[0]) : s[i] + __uint_as_float(w[j]);
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < KT * PU; d *= 2)
+#pragma unroll
+      for (int i = 0; i + d < KT * PU; i += 2 * d) s[i] += s[i + d];
+    return s[0];
   }
 
   // Values in LDS: row r's chunk c at chunk c ^ vswz(r). A transposing read
@@ -555,21 +577,20 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
       f[i] = pow2(m - base[i]);
       m = base[i];
     }
-    float psum = 0.f;
     const float mw = wave == 0 ? base[0] : wave == 1 ? base[1] : wave == 2 ? base[2] : base[3];
+    uint4 pu[KT][PU];
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
       f32x16 e;
 #pragma unroll
       for (int i = 0; i < 16; i++)
         e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -mw));
-      psum = kt == 0 ? G::sum(e) : psum + G::sum(e);
-      uint4 u[PU];
-      G::pack(e, u);
+      G::pack(e, pu[kt]);
       if (col < NC)
 #pragma unroll
-        for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = u[j];
+        for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = pu[kt][j];
     }
+    const float psum = G::sum(pu);
     if (col < NC) s_sum[wave][half * NC + col] = psum;
     const int ln = opaque(lane);
 #pragma unroll
@@ -834,14 +855,18 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
       __attribute__((always_inline)) {
     constexpr int C = decltype(ch)::value, U = S * C;
     const int td = opaque(tid);
+    // Chunk i NT + td of the step; all addresses before the first load.
+    constexpr int N = (U + NT - 1) / NT;
+    const char* from[N];
 #pragma unroll
-    for (int i = 0; i < (U + NT - 1) / NT; i++) {
-      // Of chunk i NT + td of the step.
+    for (int i = 0; i < N; i++) {
       const int row = NT % C == 0 ? i * (NT / C) + td / C : (i * NT + td) / C;
       const int c = NT % C == 0 ? td % C : (i * NT + td) % C;
-      if (U % NT == 0 || i * NT + td < U)
-        load_to_lds(rows[row] + (c ^ swizzle(row)) * 16, to + i * NT + wave * 64);
+      from[i] = rows[U % NT == 0 || i * NT + td < U ? row : 0] + (c ^ swizzle(row)) * 16;
     }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (U % NT == 0 || i * NT + td < U) load_to_lds(from[i], to + i * NT + wave * 64);
   };
   auto load_step = [&](int j, uint4* kd, uint4* vd) __attribute__((always_inline)) {
     load_rows(s_row[j & 1][0], std::integral_constant<int, G::CH>(), G::kswz, kd);
@@ -921,9 +946,9 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
 #pragma unroll
           for (int i = 0; i < 16; i++)
             e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -m));
-          psum = kt == 0 ? G::sum(e) : psum + G::sum(e);
           G::pack(e, pu[kt]);
         }
+        psum = G::sum(pu);
         if (look || __builtin_amdgcn_ballot_w64(psum > kMostSum) == 0) break;
         look = true;
       }
@@ -998,10 +1023,9 @@ Kernels kernels_of() {
   k.split16 = split_kernel<T, D, V, 16>;
   k.split32 = split_kernel<T, D, V, 32>;
   k.combine = combine_kernel<T, D, V>;
-  k.whole = whole_kernel<T, D, V, 4>;
   k.step = Geo<T, D, V>::kStep;
-  k.whole_cols = 128;
-  k.whole_threads = 256;
+  k.whole4 = whole_kernel<T, D, V, 4>;
+  k.whole8 = whole_kernel<T, D, V, 8>;
   return k;
 }
 

@@ -33,7 +33,6 @@
 //     out = L == 0 ? o : o / L (reference :124-141), one rounding to T.
 #include <hip/hip_runtime.h>
 #include <float.h>
-#include <atomic>
 #include <stdint.h>
 
 #include <type_traits>
@@ -296,20 +295,7 @@ __global__ void __launch_bounds__(kThreads) sdpa_kernel(SdpaArgs p) {
   }
 }
 
-// Compute units of the current device, read once per device.
-int device_cus() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  int n = cached[dev].load(std::memory_order_relaxed);
-  if (n <= 0) {
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        n <= 0)
-      n = 256;
-    cached[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
+using bi::device_cus;
 
 // ---------------------------------------------------------------- fp32 shapes
 // Shape s of the fp32 kernel groups GC = 2^s query heads per workgroup

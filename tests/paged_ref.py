@@ -73,10 +73,14 @@ def rows(q, k, v, n, window, first, scale, sinks, seen=None):
         # (2); a weight's numerator and denominator by that each. The sums over
         # n keys cost n roundings each, numerator and denominator; the weights
         # are rounded once to the type (f16: below 2^-14 by 2^-25 against a
-        # denominator of at least 2^-4), the result once more.
+        # denominator of at least 2^-4), the result once more. The rounded
+        # weights p (1 + e), |e| <= u, stand in numerator and denominator alike:
+        # sum p (1 + e) v / sum p (1 + e) is off by sum w e (v - out) / (1 + e'),
+        # at most u (sum w |v| + |out|) to first order, so |out| counts u once
+        # for this and once for the result's own rounding.
         delta = (D + 5) * f32 * mag + 2 * f32
         part = u + 2 * delta + 2 * n * f32
-        tol[:, h] = u * out[:, h].abs() + 1.01 * part[:, None] * (w @ vh.abs()) + 1e-30
+        tol[:, h] = 2.02 * u * out[:, h].abs() + 1.01 * part[:, None] * (w @ vh.abs()) + 1e-30
         if dtype == torch.float16:
             big = torch.where(see.any(0)[:, None], vh.abs(), 0.0).amax()
             tol[:, h] += n * 2.0 ** -21 * big + 2.0 ** -25  # the result's own half step
