@@ -24,6 +24,7 @@ hold its keys, and for paged and contiguous keys alike. The kernels
 
 import collections
 import ctypes
+import functools
 import math
 
 import torch
@@ -37,15 +38,27 @@ PageTables = collections.namedtuple(
     "PageTables", ("block_tables", "slots", "positions", "query_start", "seq_lens", "pages_used"))
 
 
-def _on_one_gpu(what, *tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda" or any(t.device != dev for t in tensors[1:]):
-        raise ValueError("%s runs on the GPU; all operands must be on one cuda device, got %s"
-                         % (what, sorted({str(t.device) for t in tensors})))
+_I32 = torch.int32
+_I64x9 = ctypes.c_int64 * 9
+_I64x10 = ctypes.c_int64 * 10
 
 
-def _int32(name, t, shape):
-    if t.dtype != torch.int32:
+def _on_one_gpu(what, dev, tensors):
+    if dev.type == "cuda":
+        for t in tensors:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return
+    raise ValueError("%s runs on the GPU; all operands must be on one cuda device, got %s"
+                     % (what, sorted({str(t.device) for t in tensors if t is not None} | {str(dev)})))
+
+
+def _int32(name, t, *shape):
+    """Checks for int32 and a shape; None in it: any length."""
+    if t.dtype is _I32 and (t.shape == shape or shape == (None,) and t.ndim == 1):
+        return
+    if t.dtype != _I32:
         raise ValueError("%s must be int32, got %s" % (name, t.dtype))
     if t.ndim != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
         raise ValueError("%s must have shape (%s), got %s"
@@ -54,11 +67,14 @@ def _int32(name, t, shape):
 
 
 def _table(t):
-    """(R, W) table with contiguous rows and their distance."""
-    _int32("block_tables", t, (None, None))
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    """Distance of the (R, W) table's rows, which are contiguous."""
+    if t.dtype is not _I32 or t.ndim != 2:
+        _int32("block_tables", t, None, None)
+    W = t.shape[1]
+    row, one = t.stride()
+    if W > 1 and one != 1:
         raise ValueError("block_tables must have contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return row if t.shape[0] > 1 else W
 
 
 def _call(device, what, fn, *args):
@@ -96,10 +112,10 @@ def page_tables(block_tables, context_lens, new_lens, free_pages, page_size, num
     ``num_tokens`` is the length of the step's token tensors: the sum of
     ``new_lens``, or more for a padded step.
     """
-    R = context_lens.shape[0] if context_lens.ndim else 0
-    _int32("context_lens", context_lens, (None,))
-    _int32("new_lens", new_lens, (R,))
-    _int32("free_pages", free_pages, (None,))
+    _int32("context_lens", context_lens, None)
+    R = context_lens.shape[0]
+    _int32("new_lens", new_lens, R)
+    _int32("free_pages", free_pages, None)
     _table(block_tables)
     if block_tables.shape[0] != R:
         raise ValueError("block_tables must have %d rows, got %d" % (R, block_tables.shape[0]))
@@ -116,32 +132,38 @@ def page_tables(block_tables, context_lens, new_lens, free_pages, page_size, num
 
 
 def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_size, num_tokens):
-    _on_one_gpu("page_tables", block_tables, context_lens, new_lens, free_pages)
-    R, W, T = context_lens.shape[0], block_tables.shape[1], int(num_tokens)
-    # One allocation: slots, positions, query_start, seq_lens, pages_used.
-    buf = torch.empty(2 * T + 2 * R + 2, dtype=torch.int32, device=context_lens.device)
-    slots, positions, start, seq, used = buf.split((T, T, R + 1, R, 1))
+    dev = context_lens.device
+    _on_one_gpu("page_tables", dev, (block_tables, new_lens, free_pages))
+    (R, W), T = block_tables.shape, int(num_tokens)
+    # One allocation for all outputs.
+    buf = torch.empty(2 * T + 2 * R + 2, dtype=_I32, device=dev)
+    slots, positions, start, seq, used = buf.split_with_sizes((T, T, R + 1, R, 1))
     context_lens, new_lens = context_lens.contiguous(), new_lens.contiguous()
     free_pages = free_pages.contiguous()
-    L = _lib.lib()
-    _call(buf.device, "bi_page_tables", L.bi_page_tables, _at(block_tables), _at(context_lens),
-          _at(new_lens), _at(free_pages), _at(slots), _at(positions), _at(start), _at(seq),
-          _at(used), R, W, _table(block_tables), free_pages.shape[0], T, int(page_size))
+    at = buf.data_ptr()
+    _call(dev, "bi_page_tables", _lib.lib().bi_page_tables, block_tables.data_ptr(),
+          context_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), at, at + 4 * T,
+          at + 8 * T, at + 8 * T + 4 * R + 4, at + 8 * T + 8 * R + 4, R, W, _table(block_tables),
+          free_pages.shape[0], T, int(page_size))
     return slots, positions, start, seq, used.view(())
 
 
 def _cache_shapes(k_cache, v_cache):
-    if k_cache.ndim != 4 or v_cache.ndim != 4 or k_cache.shape[:3] != v_cache.shape[:3]:
+    """The caches' strides (page, head, row, 1), after their checks."""
+    ks, vs = k_cache.shape, v_cache.shape
+    if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3]:
         raise ValueError("caches must be (num_pages, Hkv, page_size, head dim), got %s and %s"
-                         % (tuple(k_cache.shape), tuple(v_cache.shape)))
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+                         % (tuple(ks), tuple(vs)))
+    kst, vst = k_cache.stride(), v_cache.stride()
+    if kst[3] != 1 or vst[3] != 1:
         raise ValueError("the caches' last dimension must be contiguous")
     if k_cache.dtype != v_cache.dtype or k_cache.dtype not in _lib.DTYPE_CODES:
         raise ValueError("caches must share a dtype of float32, float16 or bfloat16, got %s and %s"
                          % (k_cache.dtype, v_cache.dtype))
-    if k_cache.shape[0] * k_cache.shape[2] >= 2 ** 31:
+    if ks[0] * ks[2] >= 2 ** 31:
         raise ValueError("a cache holds fewer than 2**31 rows per head, got %d pages of %d"
-                         % (k_cache.shape[0], k_cache.shape[2]))
+                         % (ks[0], ks[2]))
+    return kst, vst
 
 
 def paged_cache_update(k, v, k_cache, v_cache, slots):
@@ -163,7 +185,7 @@ def paged_cache_update(k, v, k_cache, v_cache, slots):
     if not k.dtype == v.dtype == k_cache.dtype:
         raise ValueError("k and v must share the caches' dtype %s, got %s and %s"
                          % (k_cache.dtype, k.dtype, v.dtype))
-    _int32("slots", slots, (k.shape[0],))
+    _int32("slots", slots, k.shape[0])
     if torch.compiler.is_compiling():
         from . import _ops  # noqa: F401  (registers the ops)
 
@@ -173,19 +195,22 @@ def paged_cache_update(k, v, k_cache, v_cache, slots):
 
 
 def _update_eager(k, v, k_cache, v_cache, slots):
-    _on_one_gpu("paged_cache_update", k_cache, v_cache, k, v, slots)
+    dev = k.device
+    _on_one_gpu("paged_cache_update", dev, (v, k_cache, v_cache, slots))
     if k.stride(2) != 1:
         k = k.contiguous()
     if v.stride(2) != 1:
         v = v.contiguous()
-    slots = slots.contiguous()
-    st = _lib.i64_array(k.stride()[:2] + v.stride()[:2] + k_cache.stride()[:3]
-                        + v_cache.stride()[:3])
     T, Hkv, D = k.shape
-    if T and k_cache.numel() and v_cache.numel():
-        _call(k.device, "bi_paged_update", _lib.lib().bi_paged_update, _at(k), _at(v),
-              _at(k_cache), _at(v_cache), _at(slots), T, Hkv, D, v.shape[2], k_cache.shape[0],
-              k_cache.shape[2], st, _lib.DTYPE_CODES[k.dtype])
+    P, _, page, V = v_cache.shape
+    if not (T and P and Hkv and page and D and V):
+        return
+    slots = slots.contiguous()
+    kc, vc = k_cache.stride(), v_cache.stride()
+    st = _I64x10(*k.stride()[:2], *v.stride()[:2], *kc[:3], *vc[:3])
+    _call(dev, "bi_paged_update", _lib.lib().bi_paged_update, k.data_ptr(), v.data_ptr(),
+          k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), T, Hkv, D, V, P, page, st,
+          _lib.DTYPE_CODES[k.dtype])
 
 
 def _attention_options(q, D, V, H, Hkv, scale, window, sink_tokens, sinks):
@@ -236,10 +261,10 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     P, Hkv, page, Dk = k_cache.shape
     if D != Dk:
         raise ValueError("q has head dimension %d, the cache %d" % (D, Dk))
-    R = block_tables.shape[0] if block_tables.ndim else 0
     _table(block_tables)
-    _int32("query_start", query_start, (R + 1,))
-    _int32("seq_lens", seq_lens, (R,))
+    R = block_tables.shape[0]
+    _int32("query_start", query_start, R + 1)
+    _int32("seq_lens", seq_lens, R)
     scale, window, sinks = _attention_options(q, D, v_cache.shape[3], H, Hkv, scale, window,
                                               sink_tokens, sinks)
     max_query = T if max_query is None else max_query
@@ -257,9 +282,14 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     return _paged_eager(*args)
 
 
-def _aligned(t):
-    ce = 16 // t.element_size()
-    return t.data_ptr() % 16 == 0 and all(s % ce == 0 for s in t.stride()[:-1])
+@functools.lru_cache(maxsize=1024)
+def _paged_bytes(device, *sizes):
+    return _lib.lib().bi_paged_attention_workspace(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_bytes(device, *sizes):
+    return _lib.lib().bi_window_attention_workspace(*sizes)
 
 
 def _workspace(need, device):
@@ -276,28 +306,31 @@ def _workspace(need, device):
 
 def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_query, max_seq,
                  scale, window, sink_tokens, sinks):
-    _on_one_gpu("paged_attention", *[t for t in (q, k_cache, v_cache, block_tables, query_start,
-                                                 seq_lens, sinks) if t is not None])
-    if not (_aligned(k_cache) and _aligned(v_cache)):
+    dev = q.device
+    _on_one_gpu("paged_attention", dev, (k_cache, v_cache, block_tables, query_start, seq_lens,
+                                         sinks))
+    kp, kh, kn, _ = k_cache.stride()
+    vp, vh, vn, _ = v_cache.stride()
+    ka, va = k_cache.data_ptr(), v_cache.data_ptr()
+    if (kp | kh | kn | vp | vh | vn) * q.element_size() % 16 or (ka | va) % 16:
         raise ValueError("the caches must be 16-byte aligned, with strides of multiples of 16 bytes")
     T, H, D = q.shape
-    P, Hkv, page, _ = k_cache.shape
+    P, Hkv, page, V = v_cache.shape
     R, W = block_tables.shape
-    V = v_cache.shape[3]
-    out = torch.empty((T, H, V), dtype=q.dtype, device=q.device)
+    out = torch.empty((T, H, V), dtype=q.dtype, device=dev)
     if not T:
         return out
     q = _kernel_view(q)
     query_start, seq_lens = query_start.contiguous(), seq_lens.contiguous()
-    st = _lib.i64_array(q.stride()[:2] + k_cache.stride()[:3] + v_cache.stride()[:3]
-                        + (_table(block_tables),))
-    L, dt = _lib.lib(), _lib.DTYPE_CODES[q.dtype]
-    ws = _workspace(L.bi_paged_attention_workspace(T, R, H, Hkv, D, V, window, sink_tokens,
-                                                   max_query, max_seq, dt), q.device)
-    _call(q.device, "bi_paged_attention", L.bi_paged_attention, _at(q), _at(k_cache),
-          _at(v_cache), _at(block_tables), _at(query_start), _at(seq_lens), _at(sinks), _at(out),
-          T, R, H, Hkv, D, V, P, page, W, st, scale, window, sink_tokens, max_query, max_seq, dt,
-          _at(ws), 0 if ws is None else ws.numel())
+    qt, qh, _ = q.stride()
+    st = _I64x9(qt, qh, kp, kh, kn, vp, vh, vn, _table(block_tables))
+    dt = _lib.DTYPE_CODES[q.dtype]
+    need = _paged_bytes(dev, T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt)
+    ws = _workspace(need, dev)
+    _call(dev, "bi_paged_attention", _lib.lib().bi_paged_attention, q.data_ptr(), ka, va,
+          block_tables.data_ptr(), query_start.data_ptr(), seq_lens.data_ptr(), _at(sinks),
+          out.data_ptr(), T, R, H, Hkv, D, V, P, page, W, st, scale, window, sink_tokens,
+          max_query, max_seq, dt, _at(ws), 0 if ws is None else need)
     return out
 
 
@@ -328,18 +361,19 @@ def window_attention(q, k, v, window, *, sink_tokens=0, scale=None, sinks=None):
 
 
 def _window_eager(q, k, v, scale, window, sink_tokens, sinks):
-    _on_one_gpu("window_attention", *[t for t in (q, k, v, sinks) if t is not None])
+    dev = q.device
+    _on_one_gpu("window_attention", dev, (k, v, sinks))
     B, H, qL, D = q.shape
-    Hkv, N, V = k.shape[1], k.shape[2], v.shape[3]
-    out = torch.empty((B, H, qL, V), dtype=q.dtype, device=q.device)
-    if not out.numel():
+    _, Hkv, N, V = v.shape
+    out = torch.empty((B, H, qL, V), dtype=q.dtype, device=dev)
+    if not (B and qL):
         return out
     q, k, v = _kernel_view(q), _kernel_view(k), _kernel_view(v)
-    st = _lib.i64_array(q.stride()[:3] + k.stride()[:3] + v.stride()[:3])
-    L, dt = _lib.lib(), _lib.DTYPE_CODES[q.dtype]
-    ws = _workspace(L.bi_window_attention_workspace(B, H, Hkv, qL, N, D, V, window, sink_tokens,
-                                                    dt), q.device)
-    _call(q.device, "bi_window_attention", L.bi_window_attention, _at(q), _at(k), _at(v),
-          _at(sinks), _at(out), B, H, Hkv, qL, N, D, V, st, scale, window, sink_tokens, dt,
-          _at(ws), 0 if ws is None else ws.numel())
+    st = _I64x9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    dt = _lib.DTYPE_CODES[q.dtype]
+    need = _window_bytes(dev, B, H, Hkv, qL, N, D, V, window, sink_tokens, dt)
+    ws = _workspace(need, dev)
+    _call(dev, "bi_window_attention", _lib.lib().bi_window_attention, q.data_ptr(), k.data_ptr(),
+          v.data_ptr(), _at(sinks), out.data_ptr(), B, H, Hkv, qL, N, D, V, st, scale, window,
+          sink_tokens, dt, _at(ws), 0 if ws is None else need)
     return out
