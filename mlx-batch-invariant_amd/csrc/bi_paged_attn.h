@@ -10,6 +10,20 @@
 
 namespace bi_paged {
 
+// Division of numbers below 2^31 by a launch's constant: a high product, an
+// addition and a shift.
+struct Div {
+  uint32_t d, mul, shift;
+};
+inline Div make_div(int64_t d) {
+  uint32_t s = 0;
+  while (((int64_t)1 << s) < d) s++;
+  return Div{(uint32_t)d, (uint32_t)(((((uint64_t)1 << s) - (uint64_t)d) << 32) / (uint64_t)d + 1), s};
+}
+__device__ __forceinline__ int32_t operator/(int32_t x, const Div& v) {
+  return (int32_t)((__umulhi((uint32_t)x, v.mul) + (uint32_t)x) >> v.shift);
+}
+
 struct Args {
   const void* q;
   const void* k;
@@ -24,7 +38,8 @@ struct Args {
   int64_t kb, kh, kn;     // keys: page or request, head, row
   int64_t vb, vh, vn;
   int64_t table_stride;
-  int32_t R, H, Hkv, G, W, page, page_shift, pages;  // page_shift < 0: not a power of two
+  int32_t R, H, W, pages;
+  Div Hkv, G, page;       // G: query heads of a kv head
   int32_t qL, N;          // contiguous
   int32_t T;              // tokens of a paged call
   int32_t window, first;  // window 0: none
@@ -34,19 +49,18 @@ struct Args {
   // The split route: partial results of (request, kv head, segment, column).
   float* po;              // [V] each
   float2* pml;            // base and sum
-  int32_t nseg, ccap;     // segments and columns kept per (request, kv head)
+  Div nseg, ccap;         // segments and columns kept per (request, kv head)
+  int32_t nc;             // columns per workgroup, 16 or 32
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
 };
-
-constexpr int kSegSteps = 8;  // steps to a segment
 
 typedef void (*Kernel)(Args);
 struct Kernels {
   Kernel split16, split32;  // 16 or 32 columns per workgroup
   Kernel combine;
   Kernel whole4, whole8;    // 4 or 8 waves of 32 columns per workgroup
-  int step;                 // rows per step
+  int seg;                  // rows per segment
 };
 
 #define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)

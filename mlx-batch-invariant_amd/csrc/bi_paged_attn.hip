@@ -30,28 +30,30 @@ constexpr int64_t kMost = (int64_t)1 << 30;
 // How a call is split: the columns up to which a request is (0: none), and the
 // memory of its partial results. `exact`: every request has max_query tokens.
 struct Plan {
-  int64_t split_cols, ccap, nseg, bytes;
+  int64_t split_cols, ccap, nc, nseg, bytes;
 };
 Plan plan(int64_t R, int64_t G, int64_t Hkv, int64_t V, int64_t window, int64_t first,
           int64_t max_query, int64_t max_seq, bool exact, const Kernels& k) {
-  Plan s = {0, 0, 0, 0};
+  Plan s = {0, 0, 0, 0, 0};
   const int64_t cols = max_query * G;
   if (R <= 0 || cols <= 0 || max_seq <= 0) return s;
   s.split_cols = 32;
-  if (exact && cols > s.split_cols) return Plan{0, 0, 0, 0};
+  if (exact && cols > s.split_cols) return Plan{0, 0, 0, 0, 0};
   s.ccap = cols < s.split_cols ? cols : s.split_cols;
-  const int64_t part = (int64_t)kSegSteps * k.step;
+  // Beside requests of more columns those of few are mostly single tokens: then
+  // two workgroups of 16 columns, of which such a request needs one.
+  s.nc = s.ccap > 16 && cols <= s.split_cols ? 32 : 16;
+  const int64_t part = k.seg;
   s.nseg = (max_seq + part - 1) / part;
   if (window) {
     // Tokens of a workgroup's columns, rows that they see between them.
-    const int64_t nc = s.ccap <= 16 ? 16 : 32;
-    const int64_t span = window + (nc - 1) / G + 1;
+    const int64_t span = window + (s.nc - 1) / G + 1;
     const int64_t n = (span + part - 2) / part + 1 + (first + part - 1) / part;
     if (n < s.nseg) s.nseg = n;
   }
   s.bytes = R * Hkv * s.ccap * s.nseg * (V + 2) * (int64_t)sizeof(float);
   if (s.bytes > (int64_t)1 << 31 || R * Hkv * s.nseg > INT32_MAX ||
-      R * Hkv * s.ccap > INT32_MAX) return Plan{0, 0, 0, 0};
+      R * Hkv * s.ccap > INT32_MAX) return Plan{0, 0, 0, 0, 0};
   return s;
 }
 
@@ -60,25 +62,25 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   const Kernels k = kernels(D, V, dtype);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t most = p.qstart ? p.max_query : p.qL;
-  Plan s = plan(p.R, p.G, p.Hkv, V, p.window, p.first, most, p.qstart ? p.max_seq : p.N,
+  Plan s = plan(p.R, p.G.d, p.Hkv.d, V, p.window, p.first, most, p.qstart ? p.max_seq : p.N,
                 !p.qstart, k);
-  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0};
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0};
   hipError_t e;
   if (s.split_cols) {
     p.split_cols = (int32_t)s.split_cols;
-    p.ccap = (int32_t)s.ccap;
-    p.nseg = (int32_t)s.nseg;
+    p.ccap = make_div(s.ccap);
+    p.nseg = make_div(s.nseg);
+    p.nc = (int32_t)s.nc;
     p.po = static_cast<float*>(ws);
-    p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv * s.ccap * s.nseg * V);
-    const int nc = s.ccap <= 16 ? 16 : 32;
-    const dim3 grid((unsigned)(p.R * p.Hkv * s.nseg), (unsigned)((s.ccap + nc - 1) / nc));
-    hipLaunchKernelGGL(nc == 16 ? k.split16 : k.split32, grid, dim3(256), 0, st, p);
+    p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv.d * s.ccap * s.nseg * V);
+    const dim3 grid((unsigned)(p.R * p.Hkv.d * s.nseg), (unsigned)((s.ccap + s.nc - 1) / s.nc));
+    hipLaunchKernelGGL(s.nc == 16 ? k.split16 : k.split32, grid, dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
-  const bool whole = most * p.G > s.split_cols;
+  const bool whole = most * p.G.d > s.split_cols;
   p.fill_blocks = p.qstart ? 16 : 0;
   if (s.split_cols) {
-    const int64_t cols = (int64_t)p.R * p.Hkv * s.ccap;
+    const int64_t cols = (int64_t)p.R * p.Hkv.d * s.ccap;
     hipLaunchKernelGGL(k.combine, dim3((unsigned)((cols + 3) / 4 + p.fill_blocks)), dim3(256), 0,
                        st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
@@ -89,14 +91,14 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     // leaves a workgroup for every compute unit (4096 tokens over 8192 keys 517
     // -> 496 us); with fewer, four of them fill more (two chunks of 511 tokens
     // beside 30 decodes 161 us, 175 with eight).
-    const int64_t cols = p.qstart ? (int64_t)p.T * p.G : (int64_t)p.R * p.qL * p.G;
-    const int waves = cols / 256 * p.Hkv >= bi::device_cus() ? 8 : 4;
+    const int64_t cols = p.qstart ? (int64_t)p.T * p.G.d : (int64_t)p.R * p.qL * p.G.d;
+    const int waves = cols / 256 * p.Hkv.d >= bi::device_cus() ? 8 : 4;
     const int64_t wc = 32 * waves;
     // Column tiles: every request with tokens may end in a part of one.
     int64_t tiles = p.qstart ? cols / wc + (p.T < p.R ? p.T : p.R)
-                             : (int64_t)p.R * (((int64_t)p.qL * p.G + wc - 1) / wc);
+                             : (int64_t)p.R * (((int64_t)p.qL * p.G.d + wc - 1) / wc);
     if (!whole) tiles = 0;
-    const int64_t blocks = tiles * p.Hkv + p.fill_blocks;
+    const int64_t blocks = tiles * p.Hkv.d + p.fill_blocks;
     if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
     if (blocks == 0) return BI_OK;
     hipLaunchKernelGGL(waves == 8 ? k.whole8 : k.whole4, dim3((unsigned)blocks), dim3(64 * waves), 0, st, p);
@@ -133,8 +135,8 @@ int32_t clamp32(int64_t x) { return x > kMost ? (int32_t)kMost : (int32_t)x; }
 void common(Args& p, int64_t H, int64_t Hkv, float scale, int64_t window, int64_t sink_tokens,
             int dtype) {
   p.H = (int32_t)H;
-  p.Hkv = (int32_t)Hkv;
-  p.G = (int32_t)(H / Hkv);
+  p.Hkv = make_div(Hkv);
+  p.G = make_div(H / Hkv);
   p.window = clamp32(window);
   p.first = clamp32(sink_tokens);
   // Not 0, with which an unseen row's -inf would not stay one.
@@ -187,14 +189,11 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
   p.table_stride = strides[8];
   p.R = (int32_t)R;
   p.W = (int32_t)W;
-  p.page = (int32_t)page_size;
   p.pages = (int32_t)num_pages;
   p.T = (int32_t)T;
   p.max_query = clamp32(max_query);
   p.max_seq = clamp32(max_seq);
-  p.page_shift = -1;
-  for (int i = 0; i < 31; i++)
-    if (page_size == (int64_t)1 << i) p.page_shift = i;
+  p.page = make_div(page_size);
   return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
 }
 

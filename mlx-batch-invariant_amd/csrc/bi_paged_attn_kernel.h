@@ -11,7 +11,7 @@
 // Fixed arithmetic of a column (what makes its bits independent of the call):
 //   * Rows are taken by their position in the request: steps of kStep rows (64
 //     where a row of keys and of values is at most 256 bytes, else 32), eight
-//     steps to a segment.
+//     steps (fp32: four) to a segment.
 //   * raw_j is a chain of 32x32 matrix products over the head dim from +0.0:
 //     of 16 dims for 16-bit types, of 2 for fp32; 16-byte chunks 2t and 2t + 1
 //     of the rows enter product t (fp32: products 4t .. 4t + 3).
@@ -142,12 +142,12 @@ __device__ __forceinline__ uint64_t seen_bits(const Args& p, int32_t pos, int32_
 // waits for it before it is used), and what it says: the row's page, the
 // request for contiguous keys, -1 for none.
 __device__ __forceinline__ int32_t table_column(const Args& p, int32_t key) {
-  return p.page_shift >= 0 ? key >> p.page_shift : (int32_t)((uint32_t)key / (uint32_t)p.page);
+  return (key < 0 ? 0 : key) / p.page;
 }
 __device__ __forceinline__ int32_t entry_of(const Args& p, int r, int32_t key) {
   if (!p.qstart || p.W == 0) return r;
   const int32_t c = table_column(p, key);
-  return p.table[r * p.table_stride + (c < 0 ? 0 : c < p.W ? c : p.W - 1)];
+  return p.table[r * p.table_stride + (c < p.W ? c : p.W - 1)];
 }
 __device__ __forceinline__ int32_t page_of(const Args& p, int32_t entry, int32_t key) {
   if (!p.qstart) return entry;
@@ -155,8 +155,9 @@ __device__ __forceinline__ int32_t page_of(const Args& p, int32_t entry, int32_t
 }
 __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
   if (!p.qstart) return key;
-  return p.page_shift >= 0 ? key & (p.page - 1) : (int32_t)((uint32_t)key % (uint32_t)p.page);
+  return key - key / p.page * (int32_t)p.page.d;
 }
+
 
 __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+v"(x));
@@ -251,6 +252,9 @@ struct Geo {
   static constexpr int D = D_, V = V_;
   static constexpr int E = sizeof(T);
   static constexpr int kStep = (D > V ? D : V) * E <= 256 ? 64 : 32;
+  // Steps to a segment; half as many for fp32, whose rows and products take
+  // twice as long and more.
+  static constexpr int kSegSteps = E == 2 ? 8 : 4;
   static constexpr int kSeg = kSegSteps * kStep;
   static constexpr int KT = kStep / 32;       // score tiles per step
   static constexpr int CH = D * E / 16;       // 16-byte chunks per key row
@@ -459,13 +463,19 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5, cn = col & (NC - 1);
-  int x = blockIdx.x;
-  const int kvh = x % p.Hkv;
-  x /= p.Hkv;
-  const int part = x % p.nseg;
-  const int r = x / p.nseg;
+  // Workgroup -> kv head, segment of the walk, request.
+  const int x = blockIdx.x, xs = x / p.Hkv, kvh = x - xs * (int)p.Hkv.d;
+  const int r = xs / p.nseg, part = xs - r * (int)p.nseg.d;
+  // Without a window the walk's entries are the segments themselves, and the
+  // table's entries can be on their way before the request is known.
+  constexpr int PS = 4 * S, PN = G::kSeg / PS;
+  int32_t entry0 = 0, entry = 0;
+  if (!p.window) {
+    entry0 = entry_of(p, r, part * G::kSeg + wave * S + (lane & (S - 1)));
+    entry = entry_of(p, r, part * G::kSeg + PS + wave * S + (lane & (S - 1)));
+  }
   const Request rq = request(p, r);
-  const int ncol = rq.L * p.G;
+  const int ncol = rq.L * (int)p.G.d;
   const int c0 = blockIdx.y * NC;
   if (rq.beyond || ncol > p.split_cols || c0 >= ncol) return;
   const int clast = (c0 + NC < ncol ? c0 + NC : ncol) - 1;
@@ -473,7 +483,6 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   // The segment's passes (4 steps each) that some column sees.
   const Walk w = walk(p, lo, hi, G::kSeg);
   if (part >= w.count()) return;  // at most p.nseg of them
-  constexpr int PS = 4 * S, PN = G::kSeg / PS;
   int s0 = w.unit(part) * PN, s1 = s0 + PN;
   while (!any_seen(p, lo, hi, s0 * PS, PS)) s0++;
   while (!any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
@@ -482,7 +491,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   const int cc = c0 + col;
   const bool cv = col < NC && cc < ncol;
   const int cq = cv ? cc : c0;
-  const int tok = cq / p.G, head = kvh * p.G + (cq - tok * p.G);
+  const int tok = cq / p.G, head = kvh * (int)p.G.d + (cq - tok * (int)p.G.d);
   const int32_t pos = cv ? rq.n - rq.L + tok : -1;
   const char* kh = static_cast<const char*>(p.k) + kvh * p.kh * (int64_t)sizeof(T);
   const char* vh = static_cast<const char*>(p.v) + kvh * p.vh * (int64_t)sizeof(T);
@@ -528,8 +537,10 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
     }
   };
 
-  const int32_t entry0 = entry_for(s0);
-  int32_t entry = entry_for(s0 + 1);
+  if (p.window) {
+    entry0 = entry_for(s0);
+    entry = entry_for(s0 + 1);
+  }
   load_query<G>(query_at<T>(p, r, rq, tok, head), half, q);
   uint64_t mapped = put_rows(s0, entry0);
   load_keys();
@@ -632,7 +643,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 
   l = half_swap_sum(l);
   if (!cv) return;
-  const int64_t slot = (((int64_t)r * p.Hkv + kvh) * p.nseg + part) * p.ccap + cc;
+  const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + cc;
   if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
 #pragma unroll
   for (int x = 0; x < TW; x++) {
@@ -679,40 +690,44 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
     return;
   }
   const int lane = threadIdx.x & 63;
-  int64_t x = ((int64_t)blockIdx.x - p.fill_blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int cc = (int)(x % p.ccap);
-  x /= p.ccap;
-  const int kvh = (int)(x % p.Hkv), r = (int)(x / p.Hkv);
+  const int x = (blockIdx.x - p.fill_blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int xh = x / p.ccap, cc = x - xh * (int)p.ccap.d;
+  const int r = xh / p.Hkv, kvh = xh - r * (int)p.Hkv.d;
   if (r >= p.R) return;
-  const Request rq = request(p, r);
-  const int ncol = rq.L * p.G;
-  if (rq.beyond || ncol > p.split_cols || cc >= ncol) return;
-  // The columns that shared a workgroup, and with them its segments.
-  const int NC = p.ccap <= 16 ? 16 : 32;
-  const int c0 = cc / NC * NC, clast = (c0 + NC < ncol ? c0 + NC : ncol) - 1;
-  const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
-  const int n = w.count() < p.nseg ? w.count() : p.nseg;
-  const int tok = cc / p.G, head = kvh * p.G + cc - tok * p.G;
-  const int64_t slot = ((int64_t)r * p.Hkv + kvh) * p.nseg * p.ccap + cc;  // segments ccap apart
-  // Dims 2 lane, 2 lane + 1 and those 128 further; 16 segments' loads in flight.
-  constexpr int NB = 16;
-  float M = kNone, L = 0.f;
-  f32x2 O[NV] = {};
-  for (int i0 = 0; i0 < n; i0 += NB) {
-    f32x2 o[NB][NV];
-    float2 ml[NB];
+  // Dims 2 lane, 2 lane + 1 and those 128 further; 8 segments' loads in flight,
+  // the first of them before the request is known (their memory is there in
+  // any case).
+  constexpr int NB = 8;
+  const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
+  f32x2 o[NB][NV];
+  float2 ml[NB];
+  auto load = [&](int i0, int n) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const bool in = i0 + i < n;
-      ml[i] = in ? p.pml[slot + (int64_t)(i0 + i) * p.ccap] : make_float2(kNone, 0.f);
+      const int64_t at = slot + (int64_t)(in ? i0 + i : 0) * p.ccap.d;
+      ml[i] = p.pml[at];
 #pragma unroll
       for (int j = 0; j < NV; j++)
-        o[i][j] = in && 2 * lane + 128 * j < V
-                      ? *reinterpret_cast<const f32x2*>(p.po + (slot + (int64_t)(i0 + i) * p.ccap) * V + 2 * lane + 128 * j)
-                      : f32x2{0.f, 0.f};
+        o[i][j] = *reinterpret_cast<const f32x2*>(p.po + at * V + (2 * lane + 128 * j < V ? 2 * lane + 128 * j : 0));
     }
+  };
+  load(0, p.nseg.d);
+  const Request rq = request(p, r);
+  const int ncol = rq.L * (int)p.G.d;
+  if (rq.beyond || ncol > p.split_cols || cc >= ncol) return;
+  // The columns that shared a workgroup, and with them its segments.
+  const int c0 = cc & -p.nc, clast = (c0 + p.nc < ncol ? c0 + p.nc : ncol) - 1;
+  const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
+  const int n = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
+  const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
+  float M = kNone, L = 0.f;
+  f32x2 O[NV] = {};
+  for (int i0 = 0; i0 < n; i0 += NB) {
+    if (i0) load(i0, n);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
+      if (i0 + i >= n) break;
       float fa, fb;
       fold_base(M, L, ml[i].x, ml[i].y, fa, fb);
 #pragma unroll
@@ -759,10 +774,10 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   // with 8 kv heads each XCD's L2 holds one of them), request, column tile;
   // a request's last tiles, which see the most rows, start first.
   const int x = blockIdx.x - p.fill_blocks;
-  const int kvh = x % p.Hkv;
   int tile = x / p.Hkv, r = 0;
+  const int kvh = x - tile * (int)p.Hkv.d;
   if (!p.qstart) {
-    const int per = (p.qL * p.G + COLS - 1) / COLS;
+    const int per = (p.qL * (int)p.G.d + COLS - 1) / COLS;
     r = tile / per;
     tile = per - 1 - (tile - r * per);
   } else {
@@ -771,7 +786,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
       int n = 0;
       if (r0 + tid < p.R) {
         const Request rq = request(p, r0 + tid);
-        const int ncol = rq.L * p.G;
+        const int ncol = rq.L * (int)p.G.d;
         n = rq.beyond || ncol <= p.split_cols ? 0 : (ncol + COLS - 1) / COLS;
       }
       int sum = n;
@@ -806,7 +821,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   r = __builtin_amdgcn_readfirstlane(r);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Request rq = request(p, r);
-  const int ncol = rq.L * p.G;
+  const int ncol = rq.L * (int)p.G.d;
   const int c0 = tile * COLS, cw = c0 + 32 * wave;
   const int clast = (c0 + COLS < ncol ? c0 + COLS : ncol) - 1;
   const int32_t p0 = rq.n - rq.L;
@@ -821,7 +836,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   const int32_t pos = cv ? p0 + tok : -1;
   const bool whole_tile = cw + 32 <= ncol;
   uint4 q[G::NQ];
-  load_query<G>(query_at<T>(p, r, rq, tok, kvh * p.G + (cv ? cc - tok * p.G : 0)), half, q);
+  load_query<G>(query_at<T>(p, r, rq, tok, kvh * (int)p.G.d + (cv ? cc - tok * (int)p.G.d : 0)), half, q);
   sign_query<G>(p, q);
 
   const Walk w = walk(p, lo, hi, S);
@@ -874,7 +889,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   };
 
   // The segment's o and the result's O are in registers, the result's base and
-  // sum, which are touched once in 8 steps, in LDS. (O in scratch memory cost
+  // sum, which are touched once a segment, in LDS. (O in scratch memory cost
   // 490 us of 1060 over 8192 keys: what the waves keep there exceeds the L2.)
   float m = kNone, l = 0.f;
   bool fresh = true;  // the segment has no step yet
@@ -964,7 +979,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
           });
     }
     // The segment's end: fold it.
-    if (j + 1 == steps || w.unit(j + 1) / kSegSteps != unit / kSegSteps) {
+    if (j + 1 == steps || w.unit(j + 1) / G::kSegSteps != unit / G::kSegSteps) {
       if (!fresh) {
         const int td = opaque(tid);
         float M = s_ml[0][td], L = s_ml[1][td], fa, fb;
@@ -997,7 +1012,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   // The column anew (kept, it would take registers that the loop needs).
   const int lane2 = opaque(lane), cc2 = cw + (lane2 & 31), half2 = lane2 >> 5;
   if (cc2 >= ncol) return;
-  const int tok2 = cc2 / p.G, head = kvh * p.G + cc2 - tok2 * p.G;
+  const int tok2 = cc2 / p.G, head = kvh * (int)p.G.d + cc2 - tok2 * (int)p.G.d;
   const float M = s_ml[0][wave * 64 + lane2], L = s_ml[1][wave * 64 + lane2];
   float e, den;
   finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
@@ -1023,7 +1038,7 @@ Kernels kernels_of() {
   k.split16 = split_kernel<T, D, V, 16>;
   k.split32 = split_kernel<T, D, V, 32>;
   k.combine = combine_kernel<T, D, V>;
-  k.step = Geo<T, D, V>::kStep;
+  k.seg = Geo<T, D, V>::kSeg;
   k.whole4 = whole_kernel<T, D, V, 4>;
   k.whole8 = whole_kernel<T, D, V, 8>;
   return k;
