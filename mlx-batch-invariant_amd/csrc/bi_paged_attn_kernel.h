@@ -694,25 +694,6 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   const int xh = x / p.ccap, cc = x - xh * (int)p.ccap.d;
   const int r = xh / p.Hkv, kvh = xh - r * (int)p.Hkv.d;
   if (r >= p.R) return;
-  // Dims 2 lane, 2 lane + 1 and those 128 further; 8 segments' loads in flight,
-  // the first of them before the request is known (their memory is there in
-  // any case).
-  constexpr int NB = 8;
-  const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
-  f32x2 o[NB][NV];
-  float2 ml[NB];
-  auto load = [&](int i0, int n) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-      const bool in = i0 + i < n;
-      const int64_t at = slot + (int64_t)(in ? i0 + i : 0) * p.ccap.d;
-      ml[i] = p.pml[at];
-#pragma unroll
-      for (int j = 0; j < NV; j++)
-        o[i][j] = *reinterpret_cast<const f32x2*>(p.po + at * V + (2 * lane + 128 * j < V ? 2 * lane + 128 * j : 0));
-    }
-  };
-  load(0, p.nseg.d);
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
   if (rq.beyond || ncol > p.split_cols || cc >= ncol) return;
@@ -721,13 +702,27 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
   const int n = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
   const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
+  const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
+  // Dims 2 lane, 2 lane + 1 and those 128 further; 16 segments' loads in flight.
+  constexpr int NB = 16;
   float M = kNone, L = 0.f;
   f32x2 O[NV] = {};
   for (int i0 = 0; i0 < n; i0 += NB) {
-    if (i0) load(i0, n);
+    f32x2 o[NB][NV];
+    float2 ml[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      if (i0 + i >= n) break;
+      const bool in = i0 + i < n;
+      const int64_t at = slot + (int64_t)(i0 + i) * p.ccap.d;
+      ml[i] = in ? p.pml[at] : make_float2(kNone, 0.f);
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        o[i][j] = in && 2 * lane + 128 * j < V
+                      ? *reinterpret_cast<const f32x2*>(p.po + at * V + 2 * lane + 128 * j)
+                      : f32x2{0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
       float fa, fb;
       fold_base(M, L, ml[i].x, ml[i].y, fa, fb);
 #pragma unroll
