@@ -59,7 +59,10 @@ typedef void (*Kernel)(Args);
 struct Kernels {
   Kernel split16, split32;  // 16 or 32 columns per workgroup
   Kernel combine;
-  Kernel whole4, whole8;    // 4 or 8 waves of 32 columns per workgroup
+  // 4 or 8 waves of 32 columns per workgroup, one to a CU, or 4 waves two to a
+  // CU (the last two where the registers allow two waves per SIMD, else NULL).
+  Kernel whole4, whole8, whole4_pair;
+  int whole4_threads;       // its loading waves among them
   int seg;                  // rows per segment
 };
 

@@ -90,10 +90,13 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     // Eight waves share their keys' and values' loads and addresses where that
     // leaves a workgroup for every compute unit (4096 tokens over 8192 keys 517
     // -> 496 us); with fewer, four of them fill more (two chunks of 511 tokens
-    // beside 30 decodes 161 us, 175 with eight).
+    // beside 30 decodes 161 us, 175 with eight), two to a compute unit where
+    // there are more than these.
     const int64_t cols = p.qstart ? (int64_t)p.T * p.G.d : (int64_t)p.R * p.qL * p.G.d;
-    const int waves = cols / 256 * p.Hkv.d >= bi::device_cus() ? 8 : 4;
-    const int64_t wc = 32 * waves;
+    const int cus = bi::device_cus();
+    const bool eight = k.whole8 && cols / 256 * p.Hkv.d >= cus;
+    const bool pair = !eight && k.whole4_pair && cols / 128 * p.Hkv.d > cus;
+    const int64_t wc = eight ? 256 : 128;
     // Column tiles: every request with tokens may end in a part of one.
     int64_t tiles = p.qstart ? cols / wc + (p.T < p.R ? p.T : p.R)
                              : (int64_t)p.R * (((int64_t)p.qL * p.G.d + wc - 1) / wc);
@@ -101,7 +104,8 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     const int64_t blocks = tiles * p.Hkv.d + p.fill_blocks;
     if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
     if (blocks == 0) return BI_OK;
-    hipLaunchKernelGGL(waves == 8 ? k.whole8 : k.whole4, dim3((unsigned)blocks), dim3(64 * waves), 0, st, p);
+    hipLaunchKernelGGL(eight ? k.whole8 : pair ? k.whole4_pair : k.whole4, dim3((unsigned)blocks),
+                       dim3(eight ? 512 : pair ? 256 : k.whole4_threads), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   return BI_OK;

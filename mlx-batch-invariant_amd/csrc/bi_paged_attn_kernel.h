@@ -145,12 +145,12 @@ __device__ __forceinline__ int32_t table_column(const Args& p, int32_t key) {
   return (key < 0 ? 0 : key) / p.page;
 }
 __device__ __forceinline__ int32_t entry_of(const Args& p, int r, int32_t key) {
-  if (!p.qstart || p.W == 0) return r;
+  if (!p.qstart || p.W == 0) return 0;
   const int32_t c = table_column(p, key);
   return p.table[r * p.table_stride + (c < p.W ? c : p.W - 1)];
 }
-__device__ __forceinline__ int32_t page_of(const Args& p, int32_t entry, int32_t key) {
-  if (!p.qstart) return entry;
+__device__ __forceinline__ int32_t page_of(const Args& p, int r, int32_t entry, int32_t key) {
+  if (!p.qstart) return r;
   return table_column(p, key) < p.W && entry < p.pages ? entry : -1;
 }
 __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
@@ -187,16 +187,24 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32) |
          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 }
-// 16 bytes from each lane's address to LDS at `to` + 16 * lane (`to` uniform),
+// 16 or 4 bytes from each lane's address to LDS at `to` + 16 or 4 * lane (`to` uniform),
 // in flight until wait_loads(). As asm, since beside the builtin, which the
 // compiler counts as an access of both memories, it waits for all LDS reads
 // and all loads wherever it waits for one. It has no result that could be
 // taken before it is there; the caller waits and meets a barrier before it
 // reads the LDS. (M0, which nothing else here uses, holds the LDS address.)
-__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* from, void* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(at), "v"(from) : "memory");
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(at), "v"(from) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(at), "v"(from) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads_but() {  // all but the N youngest
+  static_assert(N <= 63, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // LDS written before is visible to the workgroup after; loads stay in flight.
@@ -263,6 +271,11 @@ struct Geo {
   static constexpr int NQ = CH / 2;           // chunks per lane half
   static constexpr int PU = E;                // 16-byte units of p per tile and lane
   static constexpr int DT = V / 32;           // tiles of output dims
+  // Whole route: two waves per SIMD (256 registers each) hold o, O, the query
+  // and a step's scores; LDS buffers that fit a CU with one workgroup.
+  static constexpr bool kTwoWaves = V + 4 * NQ <= 192;
+  static constexpr int kStepBytes = kStep * (CH + VCH) * 16;
+  static constexpr int kDeep = kStepBytes <= 32768 ? 4 : 3;
   // Split workgroups per CU: 64 KB of values (4 steps) and their p twice fit its LDS.
   static constexpr int kSplitPerCu = 4 * kStep * MCH > 4096 ? 1 : 2;
 
@@ -505,7 +518,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   };
   auto put_rows = [&](int si, int32_t entry) __attribute__((always_inline)) -> uint64_t {
     const int32_t key = key_of(si) + (lane & (S - 1));
-    const int32_t id = si < s1 && any_seen(p, lo, hi, key, 1) ? page_of(p, entry, key) : -1;
+    const int32_t id = si < s1 && any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry, key) : -1;
     const int64_t row = row_of(p, key);
     const char* zero = reinterpret_cast<const char*>(g_zero_row);
     const char* ka = kh + (id * p.kb + row * p.kn) * (int64_t)sizeof(T);
@@ -746,17 +759,28 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
 }
 
 // Whole route: NW waves of 32 columns each walk the steps that some column of
-// the workgroup sees, two LDS buffers ahead of each other.
-template <typename T, int D, int V, int NW>
-__global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_kernel(Args p) {
+// the workgroup sees. Keys and values go through a ring of NB LDS buffers, NB -
+// 1 steps ahead of their use, by loads that LW waves more do nothing but issue
+// (LW = 0: the NW waves themselves). A wave spends about 150 cycles on issuing
+// a load that writes LDS, 8 a step: with another wave on its SIMD that is
+// hidden, alone it is a quarter of the step (512 tokens over 8192 keys 244 us,
+// XXX with loading waves).
+template <typename T, int D, int V, int NW, int LW, int NB>
+__global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 : 1))
+    whole_kernel(Args p) {
   using G = Geo<T, D, V>;
-  constexpr int S = G::kStep, KT = G::KT, PU = G::PU, DT = G::DT, NT = 64 * NW, COLS = 32 * NW;
-  constexpr int KU = S * G::CH, VU = S * G::VCH;
-  __shared__ uint4 s_k0[KU], s_k1[KU], s_v0[VU], s_v1[VU];
-  __shared__ const char* s_row[2][2][S];
-  __shared__ uint64_t s_map[4];
-  __shared__ int s_scan[NW + 3];
-  __shared__ float s_ml[2][NT];  // each lane's own M and L
+  constexpr int S = G::kStep, KT = G::KT, PU = G::PU, DT = G::DT, COLS = 32 * NW;
+  constexpr int KU = S * G::CH, VU = S * G::VCH, AHEAD = NB - 1;
+  constexpr int NT = 64 * (LW ? LW : NW);  // threads that load
+  // Loads per wave and step: its share of the keys and of the values.
+  constexpr int LPS = (KU + NT - 1) / NT + (VU + NT - 1) / NT;
+  __shared__ uint4 s_kv[NB * (KU + VU)];
+  __shared__ uint4 s_dump[KU % NT || VU % NT ? 64 : 1];  // of waves that have no share
+  __shared__ const char* s_row[NB][2][S];
+  __shared__ int32_t s_entry[8][64];
+  __shared__ uint64_t s_map[8];
+  __shared__ int s_scan[NW + LW + 3];
+  __shared__ float s_ml[2][64 * NW];  // each lane's own M and L
 
   if ((int)blockIdx.x < p.fill_blocks) {
     fill<T, V>(p, blockIdx.x);
@@ -777,7 +801,7 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     tile = per - 1 - (tile - r * per);
   } else {
     int before = 0, found = -1;
-    for (int r0 = 0; r0 < p.R; r0 += NT) {
+    for (int r0 = 0; r0 < p.R; r0 += 64 * (NW + LW)) {
       int n = 0;
       if (r0 + tid < p.R) {
         const Request rq = request(p, r0 + tid);
@@ -791,27 +815,27 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
         if (lane >= d) sum += y;
       }
       if (lane == 63) s_scan[wave] = sum;
-      if (tid == 0) s_scan[NW] = -1;
+      if (tid == 0) s_scan[NW + LW] = -1;
       __syncthreads();
       int all = 0;
 #pragma unroll
-      for (int i = 0; i < NW; i++) {
+      for (int i = 0; i < NW + LW; i++) {
         if (i < wave) sum += s_scan[i];
         all += s_scan[i];
       }
       if (tile >= before + sum - n && tile < before + sum) {
-        s_scan[NW] = r0 + tid;
-        s_scan[NW + 1] = n - 1 - (tile - (before + sum - n));
+        s_scan[NW + LW] = r0 + tid;
+        s_scan[NW + LW + 1] = n - 1 - (tile - (before + sum - n));
       }
       __syncthreads();
-      found = s_scan[NW];
+      found = s_scan[NW + LW];
       if (found >= 0) break;
       before += all;
       __syncthreads();
     }
     if (found < 0) return;
     r = found;
-    tile = s_scan[NW + 1];
+    tile = s_scan[NW + LW + 1];
   }
   r = __builtin_amdgcn_readfirstlane(r);
   tile = __builtin_amdgcn_readfirstlane(tile);
@@ -824,6 +848,9 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   // The wave's own columns; a wave without one only loads.
   const int wlast = cw + 31 < ncol ? cw + 31 : ncol - 1;
   const int32_t wlo = cw < ncol ? p0 + cw / p.G : INT32_MAX / 2, whi = cw < ncol ? p0 + wlast / p.G : -1;
+
+  const bool loads = LW == 0 || wave >= NW;
+  const int lw = LW ? wave - NW : wave;  // which of the loading waves
 
   const int cc = cw + col;
   const bool cv = cc < ncol;
@@ -839,32 +866,33 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   const char* kh = static_cast<const char*>(p.k) + kvh * p.kh * (int64_t)sizeof(T);
   const char* vh = static_cast<const char*>(p.v) + kvh * p.vh * (int64_t)sizeof(T);
 
-  // Row addresses of a step, by the first wave: the page's number is loaded a
-  // step before they are written, which is a step before they are used.
-  auto entry_for = [&](int j) __attribute__((always_inline)) -> int32_t {
-    return entry_of(p, r, w.unit(j) * S + lane);
+  // A step's way into LDS: the table's entries of its rows, NB + AHEAD steps
+  // before, and from them the rows' addresses, NB steps before, both by the
+  // first loading wave; then keys and values, AHEAD steps before. A wave issues
+  // the same number of loads every step, so that it can wait by their count.
+  auto load_entries = [&](int j) __attribute__((always_inline)) {
+    const int32_t* at = reinterpret_cast<const int32_t*>(g_zero_row);
+    if (p.qstart && p.W > 0) {
+      const int32_t c = table_column(p, w.unit(j) * S + (opaque(lane) & (S - 1)));
+      at = p.table + r * p.table_stride + (c < p.W ? c : p.W - 1);
+    }
+    load_to_lds<4>(at, s_entry[j & 7]);
   };
   auto put_rows = [&](int j, int32_t entry) __attribute__((always_inline)) {
     if (j >= steps) return;
-    const int32_t key = w.unit(j) * S + lane;
-    const int32_t id = lane < S && any_seen(p, lo, hi, key, 1) ? page_of(p, entry, key) : -1;
-    const char *ka = reinterpret_cast<const char*>(g_zero_row), *va = ka;
-    if (id >= 0) {
-      const int64_t row = row_of(p, key);
-      ka = kh + (id * p.kb + row * p.kn) * (int64_t)sizeof(T);
-      va = vh + (id * p.vb + row * p.vn) * (int64_t)sizeof(T);
-    }
-    const uint64_t m = __builtin_amdgcn_ballot_w64(id >= 0);
-    if (lane < S) {
-      s_row[j & 1][0][lane] = ka;
-      s_row[j & 1][1][lane] = va;
-    }
-    if (lane == 0) s_map[j & 3] = m;
+    const int ln = opaque(lane) & (S - 1);
+    const int32_t key = w.unit(j) * S + ln;
+    const int32_t id = any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry, key) : -1;
+    const int64_t row = row_of(p, key);
+    const char* zero = reinterpret_cast<const char*>(g_zero_row);
+    s_row[j % NB][0][ln] = id >= 0 ? kh + (id * p.kb + row * p.kn) * (int64_t)sizeof(T) : zero;
+    s_row[j % NB][1][ln] = id >= 0 ? vh + (id * p.vb + row * p.vn) * (int64_t)sizeof(T) : zero;
+    s_map[j & 7] = __builtin_amdgcn_ballot_w64(id >= 0);  // S = 32: both halves alike
   };
   auto load_rows = [&](const char* const* rows, auto ch, auto swizzle, uint4* to)
       __attribute__((always_inline)) {
     constexpr int C = decltype(ch)::value, U = S * C;
-    const int td = opaque(tid);
+    const int td = opaque(64 * lw + lane);
     // Chunk i NT + td of the step; all addresses before the first load.
     constexpr int N = (U + NT - 1) / NT;
     const char* from[N];
@@ -876,11 +904,12 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
     }
 #pragma unroll
     for (int i = 0; i < N; i++)
-      if (U % NT == 0 || i * NT + td < U) load_to_lds(from[i], to + i * NT + wave * 64);
+      load_to_lds<16>(from[i], U % NT == 0 || i * NT + lw * 64 < U ? to + i * NT + lw * 64 : s_dump);
   };
-  auto load_step = [&](int j, uint4* kd, uint4* vd) __attribute__((always_inline)) {
-    load_rows(s_row[j & 1][0], std::integral_constant<int, G::CH>(), G::kswz, kd);
-    load_rows(s_row[j & 1][1], std::integral_constant<int, G::VCH>(), G::vswz, vd);
+  auto load_step = [&](int j) __attribute__((always_inline)) {
+    uint4* to = s_kv + j % NB * (KU + VU);
+    load_rows(s_row[j % NB][0], std::integral_constant<int, G::CH>(), G::kswz, to);
+    load_rows(s_row[j % NB][1], std::integral_constant<int, G::VCH>(), G::vswz, to + KU);
   };
 
   // The segment's o and the result's O are in registers, the result's base and
@@ -891,32 +920,57 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
   f32x16 O[DT], o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; dt++) O[dt] = f32x16{}, o[dt] = f32x16{};
-  s_ml[0][tid] = kNone;
-  s_ml[1][tid] = 0.f;
-
-  if (steps > 0) {
-    if (wave == 0) {
-      put_rows(0, entry_for(0));
-      put_rows(1, entry_for(1));
-    }
-    __syncthreads();
-    load_step(0, s_k0, s_v0);
+  if (wave < NW) {
+    s_ml[0][tid] = kNone;
+    s_ml[1][tid] = 0.f;
   }
-  auto step = [&](int j, const uint4* kd, const uint4* vd, uint4* kn, uint4* vn)
-      __attribute__((always_inline)) {
-    // LDS addresses are computed anew each step: kept across steps they, for
-    // two buffers, take the registers that o and O need.
+
+  // Loads of step j, and for the first wave the entries of the step whose
+  // addresses are written when step j is waited for.
+  auto start_step = [&](int j) __attribute__((always_inline)) {
+    if (j >= steps) return;
+    if (lw == 0) load_entries(j + NB);
+    load_step(j);
+  };
+  // This wave's part of step j: all but the loads of the AHEAD - 1 later ones.
+  auto await_step = [&](int j) __attribute__((always_inline)) {
+    if (j + AHEAD > steps) wait_loads();
+    else if (lw == 0) wait_loads_but<(AHEAD - 1) * (LPS + 1)>();
+    else wait_loads_but<(AHEAD - 1) * LPS>();
+  };
+  if (loads && lw == 0) {
+    int32_t entry[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) entry[i] = entry_of(p, r, w.unit(i) * S + (lane & (S - 1)));
+#pragma unroll
+    for (int i = 0; i < NB; i++) put_rows(i, entry[i]);
+  }
+  __syncthreads();
+  if (loads)
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) start_step(i);
+  if constexpr (LW != 0)
+    if (loads) {
+      for (int j = 0; j < steps; j++) {
+        await_step(j);
+        barrier();
+        start_step(j + AHEAD);
+        if (lw == 0) put_rows(j + NB, s_entry[(j + NB) & 7][opaque(lane)]);
+      }
+      return;
+    }
+  for (int j = 0; j < steps; j++) {
+    // LDS addresses are computed anew each step: kept across steps they take
+    // the registers that o and O need.
     const int ln = opaque(lane), hf = ln >> 5;
-    wait_loads();  // this wave's part of step j
-    barrier();     // everyone's, and everyone is done with the other buffers
-    int32_t id = -1;
-    if (wave == 0) id = entry_for(j + 2);
-    if (j + 1 < steps) load_step(j + 1, kn, vn);
+    if constexpr (LW == 0) await_step(j);
+    barrier();  // step j is there, and everyone is done with step j - 1's buffer
+    if constexpr (LW == 0) start_step(j + AHEAD);
+    const uint4 *kd = s_kv + j % NB * (KU + VU), *vd = kd + KU;
     const int32_t unit = w.unit(j), key0 = unit * S;
     if (any_seen(p, wlo, whi, key0, S)) {
-      const uint64_t mapped = uniform(s_map[j & 3]);
-      const bool full = whole_tile && mapped == (S == 64 ? ~0ull : 0xFFFFFFFFull) &&
-                        all_seen(p, wlo, whi, key0, S);
+      const uint64_t mapped = uniform(s_map[j & 7]);
+      const bool full = whole_tile && mapped == ~0ull && all_seen(p, wlo, whi, key0, S);
       f32x16 s[KT];
 #pragma unroll
       for (int kt = 0; kt < KT; kt++) s[kt] = f32x16{};
@@ -997,11 +1051,8 @@ __global__ void __launch_bounds__(64 * NW, (D > 128 || V > 128) ? 1 : 2) whole_k
         fresh = true;
       }
     }
-    if (wave == 0) put_rows(j + 2, id);
-  };
-  for (int j = 0; j < steps; j += 2) {
-    step(j, s_k0, s_v0, s_k1, s_v1);
-    if (j + 1 < steps) step(j + 1, s_k1, s_v1, s_k0, s_v0);
+    if constexpr (LW == 0)
+      if (lw == 0) put_rows(j + NB, s_entry[(j + NB) & 7][opaque(lane)]);
   }
 
   // The column anew (kept, it would take registers that the loop needs).
@@ -1034,8 +1085,16 @@ Kernels kernels_of() {
   k.split32 = split_kernel<T, D, V, 32>;
   k.combine = combine_kernel<T, D, V>;
   k.seg = Geo<T, D, V>::kSeg;
-  k.whole4 = whole_kernel<T, D, V, 4>;
-  k.whole8 = whole_kernel<T, D, V, 8>;
+  using G = Geo<T, D, V>;
+  if constexpr (G::kTwoWaves) {
+    k.whole4 = whole_kernel<T, D, V, 4, 4, G::kDeep>;
+    k.whole4_pair = whole_kernel<T, D, V, 4, 0, 2>;
+    k.whole8 = whole_kernel<T, D, V, 8, 0, 2>;
+  } else {
+    k.whole4 = whole_kernel<T, D, V, 4, 0, 2>;
+    k.whole4_pair = k.whole8 = nullptr;
+  }
+  k.whole4_threads = G::kTwoWaves ? 512 : 256;
   return k;
 }
 
