@@ -7,16 +7,16 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "bi_div.h"
 #include "bi_internal.h"
 
 namespace {
 
+using bi::Div;
+
 constexpr int kThreads = 256;
-constexpr int kWave = 64;
-constexpr int kReqs = 4;                       // requests per thread and tile of the scan
-constexpr int kTile = kThreads * kReqs;        // requests per tile
-constexpr int kTokens = 4;                     // tokens per thread
-constexpr int kTokenTile = kThreads * kTokens;  // tokens per workgroup
+constexpr int kReqs = 4;                 // requests per thread and tile of the scan
+constexpr int kTile = kThreads * kReqs;  // requests per tile
 
 struct TablesArgs {
   int32_t* table;
@@ -29,132 +29,122 @@ struct TablesArgs {
   int32_t* seq;
   int32_t* used;
   int64_t R, W, F, T, table_stride;
-  int32_t page;
+  Div page;
 };
 
-__device__ __forceinline__ int64_t pages_of(int64_t rows, int32_t page, int64_t W) {
-  const int64_t n = (int64_t)(((uint64_t)rows + (uint32_t)page - 1) / (uint32_t)page);
+// Pages of the first `rows` rows, at most W.
+__device__ __forceinline__ uint32_t pages_of(uint32_t rows, const Div& page, uint32_t W) {
+  const uint32_t n = rows ? (int32_t)(rows - 1) / page + 1 : 0;
   return n < W ? n : W;
 }
-
-// Inclusive sums over the workgroup, 64-bit: over a wave by shuffles, over the
-// waves through LDS. Returns this thread's exclusive sum; `total` the whole.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t s = x;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t y = __shfl_up(s, d);
-    if (lane >= d) s += y;
-  }
-  if (lane == 63) part[wave] = s;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / kWave; w++) {
-    if (w < wave) before += part[w];
-    total += part[w];
-  }
-  __syncthreads();
-  return before + s - x;
+// A request's cached rows and all its rows (at most 2^31 - 1).
+__device__ __forceinline__ void lengths(int32_t ctx, int32_t fresh, uint32_t& c, uint32_t& n) {
+  c = ctx > 0 ? ctx : 0;
+  n = c + (fresh > 0 ? fresh : 0);
+  n = n < 0x7FFFFFFFu ? n : 0x7FFFFFFFu;
 }
 
 // One launch, no communication between workgroups: each takes a range of
-// tokens and computes the sums over the requests for itself (R loads from the
-// caches; with a few hundred requests one pass of the scan), so nothing waits
-// on another workgroup. A new page's table entry is written by the thread of
-// the page's first token, which is always a new token, straight from the free
-// list: no thread reads an entry that this launch writes.
+// tokens, one per thread, and computes the sums over the requests for itself
+// (one load of each length; 1024 requests are one pass of the scan), so
+// nothing waits on another workgroup: what bounds it is the chain of a launch,
+// two loads, the scan and a search. A new page's table entry is written by the
+// thread of the page's first token, which is always a new token, straight from
+// the free list: no thread reads an entry that this launch writes. Sums of
+// tokens (low) and pages (high) are scanned together; every index that depends
+// on them is checked, whatever the lengths hold.
 __global__ void __launch_bounds__(kThreads) page_tables_kernel(TablesArgs p) {
-  __shared__ int64_t s_start[kTile];  // first token of a request
-  __shared__ int64_t s_page[kTile];   // first place in the free list
-  __shared__ int64_t s_part[kThreads / kWave];
-  const int tid = threadIdx.x;
-  const int64_t stride = (int64_t)gridDim.x * kTokenTile;
-  int64_t t_base = 0, g_base = 0;  // tokens and pages of the requests before the tile
+  __shared__ uint32_t s_start[kTile];  // first token of a request
+  __shared__ uint32_t s_page[kTile];   // first place in the free list
+  __shared__ int32_t s_ctx[kTile];
+  __shared__ uint64_t s_part[kThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t W = (uint32_t)p.W, first = blockIdx.x * kThreads, stride = gridDim.x * kThreads;
+  uint64_t before = 0;  // of the tiles so far
   for (int64_t r0 = 0; r0 < p.R; r0 += kTile) {
-    int64_t n[kReqs], take[kReqs], sn = 0, st = 0;
-    int32_t c[kReqs];
-#pragma unroll
-    for (int i = 0; i < kReqs; i++) {
-      const int64_t r = r0 + tid * kReqs + i;
-      c[i] = 0;
-      n[i] = 0;
-      if (r < p.R) {
-        c[i] = p.ctx[r] > 0 ? p.ctx[r] : 0;
-        n[i] = p.fresh[r] > 0 ? p.fresh[r] : 0;
-      }
-      take[i] = pages_of(c[i] + n[i], p.page, p.W) - pages_of(c[i], p.page, p.W);
-      sn += n[i];
-      st += take[i];
-    }
-    int64_t tn, tt;
-    int64_t an = t_base + block_scan(sn, s_part, tn);
-    int64_t at = g_base + block_scan(st, s_part, tt);
     const int count = (int)(p.R - r0 < kTile ? p.R - r0 : kTile);
+    uint32_t c[kReqs], n[kReqs];
+    uint64_t own[kReqs], sum = 0;
 #pragma unroll
     for (int i = 0; i < kReqs; i++) {
-      const int64_t r = r0 + tid * kReqs + i;
-      s_start[tid * kReqs + i] = an;
-      s_page[tid * kReqs + i] = at;
-      if (r < p.R && blockIdx.x == 0) {
-        p.qstart[r] = (int32_t)an;
-        p.seq[r] = (int32_t)(c[i] + n[i]);
+      const int k = tid * kReqs + i;
+      lengths(k < count ? p.ctx[r0 + k] : 0, k < count ? p.fresh[r0 + k] : 0, c[i], n[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kReqs; i++) {
+      own[i] = (uint64_t)(pages_of(n[i], p.page, W) - pages_of(c[i], p.page, W)) << 32 | (n[i] - c[i]);
+      sum += own[i];
+    }
+    uint64_t upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    if (lane == 63) s_part[wave] = upto;
+    __syncthreads();
+    uint64_t at = before + upto - sum;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) {
+      if (w < wave) at += s_part[w];
+      before += s_part[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kReqs; i++) {
+      const int k = tid * kReqs + i;
+      s_start[k] = (uint32_t)at;
+      s_page[k] = (uint32_t)(at >> 32);
+      s_ctx[k] = (int32_t)c[i];
+      if (k < count && blockIdx.x == 0) {
+        p.qstart[r0 + k] = (int32_t)at;
+        p.seq[r0 + k] = (int32_t)n[i];
       }
-      an += n[i];
-      at += take[i];
+      at += own[i];
     }
     __syncthreads();
-    // The tile's tokens t_base .. t_base + tn - 1 that this workgroup owns.
-    const int64_t end = t_base + tn;
-    for (int64_t b = (int64_t)blockIdx.x * kTokenTile; b < end; b += stride) {
-      if (b + kTokenTile <= t_base) continue;
-#pragma unroll
-      for (int i = 0; i < kTokens; i++) {
-        const int64_t t = b + i * kThreads + tid;
-        if (t < t_base || t >= end) continue;
-        int lo = 0, hi = count - 1;  // the last request that starts at or before t
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (s_start[mid] <= t) lo = mid;
-          else hi = mid - 1;
-        }
-        const int64_t r = r0 + lo;
-        const int32_t ctx = p.ctx[r] > 0 ? p.ctx[r] : 0;
-        const int64_t pos = ctx + (t - s_start[lo]);
-        const int64_t pg = pos / p.page, row = pos - pg * p.page;
-        int32_t id = -1;
-        if (pg < p.W) {
-          const int64_t have = pages_of(ctx, p.page, p.W);
-          if (pg < have) {
-            id = p.table[r * p.table_stride + pg];
-          } else {
-            const int64_t f = s_page[lo] + pg - have;
-            if (f < p.F) id = p.pool[f];
-            if (row == 0) p.table[r * p.table_stride + pg] = id;
-          }
-        }
-        if (t < p.T) {
-          p.slots[t] = id < 0 ? -1 : (int32_t)((int64_t)id * p.page + row);
-          p.positions[t] = (int32_t)pos;
+    // The tile's tokens that this workgroup owns.
+    const uint32_t t0 = s_start[0], t1 = (uint32_t)before;
+    const uint32_t skip = t0 > first ? (t0 - first) / stride : 0;
+    for (uint64_t b = first + (uint64_t)skip * stride; b < t1; b += stride) {
+      const uint32_t t = (uint32_t)b + tid;
+      if (t < t0 || t >= t1) continue;
+      int lo = 0, hi = count - 1;  // the last request that starts at or before t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_start[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const uint32_t ctx = s_ctx[lo], pos = ctx + (t - s_start[lo]);
+      int32_t id = -1;
+      uint32_t row = 0;
+      if (pos < 0x7FFFFFFFu) {
+        const uint32_t pg = (int32_t)pos / p.page, have = pages_of(ctx, p.page, W);
+        row = pos - pg * p.page.d;
+        int32_t* entry = p.table + (r0 + lo) * p.table_stride + pg;
+        if (pg < have) {
+          id = *entry;
+        } else if (pg < W) {
+          const uint32_t f = s_page[lo] + pg - have;
+          if (f < (uint32_t)p.F) id = p.pool[f];
+          if (row == 0) *entry = id;
         }
       }
+      if (t < p.T) {
+        p.slots[t] = id < 0 ? -1 : (int32_t)((uint32_t)id * p.page.d + row);
+        p.positions[t] = (int32_t)pos;
+      }
     }
-    t_base = end;
-    g_base += tt;
     __syncthreads();
   }
   // Places behind the last request's tokens.
-  for (int64_t b = (int64_t)blockIdx.x * kTokenTile; b < p.T; b += stride)
-#pragma unroll
-    for (int i = 0; i < kTokens; i++) {
-      const int64_t t = b + i * kThreads + tid;
-      if (t >= t_base && t < p.T) p.slots[t] = p.positions[t] = -1;
-    }
+  const uint32_t end = (uint32_t)before;
+  for (uint64_t b = first; b < (uint64_t)p.T; b += stride) {
+    const uint64_t t = b + tid;
+    if (t >= end && t < (uint64_t)p.T) p.slots[t] = p.positions[t] = -1;
+  }
   if (blockIdx.x == 0 && tid == 0) {
-    p.qstart[p.R] = (int32_t)t_base;
-    *p.used = (int32_t)g_base;
+    p.qstart[p.R] = (int32_t)end;
+    *p.used = (int32_t)(before >> 32);
   }
 }
 
@@ -164,45 +154,32 @@ struct UpdateArgs {
   const int32_t* slots;
   int64_t ss[2][2];     // source byte strides: token, head
   int64_t ds[2][3];     // cache byte strides: page, head, row
-  int64_t T, slots_end;  // slots below num_pages * page_size
-  int32_t page, heads;
-  int32_t units[2];     // copies of U bytes per row
-  int32_t per_token;    // heads * (units[0] + units[1])
+  int32_t T, slots_end;  // slots below num_pages * page_size
+  int32_t keys, per_token;  // units of a token's keys; of keys and values
+  Div page, wide;       // wide: threads side by side on a token
+  Div units[2];         // copies of U bytes per row
 };
 
-// A copy: thread x of a token moves one U-sized unit of one head's key or
-// value row. kRows tokens per thread keep several loads in flight.
-constexpr int kRows = 4;
+// A copy: a thread moves one U-sized unit of one head's key or value row of one
+// token. (What bounds it is how many loads are in flight as the launch ramps
+// up: 8161 tokens of 4 KB took 16.6 us, 25 with two tokens a thread and 26.5
+// with four; a plain copy of as many bytes 11.1.)
 template <typename U>
 __global__ void __launch_bounds__(kThreads) paged_update_kernel(UpdateArgs p) {
-  const int wide = p.per_token < kThreads ? p.per_token : kThreads;  // units side by side
-  const int each = kThreads / wide;                                 // tokens side by side
-  const int sub = threadIdx.x / wide;
-  const int x = blockIdx.y * wide + threadIdx.x % wide;
-  if (sub >= each || x >= p.per_token) return;
-  const int keys = p.heads * p.units[0];
-  const int kv = x >= keys;
-  const int y = kv ? x - keys : x;
-  const int head = y / p.units[kv], unit = y - head * p.units[kv];
-  const char* src = p.src[kv] + head * p.ss[kv][1] + (int64_t)unit * sizeof(U);
-  char* dst = p.dst[kv] + head * p.ds[kv][1] + (int64_t)unit * sizeof(U);
-  const int64_t step = (int64_t)gridDim.x * each * kRows;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kRows) * each + sub; t0 < p.T; t0 += step) {
-    U u[kRows];
-    int32_t slot[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-      const int64_t t = t0 + i * each;
-      slot[i] = t < p.T ? p.slots[t] : -1;
-      if (t < p.T) u[i] = *reinterpret_cast<const U*>(src + t * p.ss[kv][0]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-      if (slot[i] < 0 || slot[i] >= p.slots_end) continue;
-      const int32_t pg = slot[i] / p.page, row = slot[i] - pg * p.page;
-      *reinterpret_cast<U*>(dst + pg * p.ds[kv][0] + row * p.ds[kv][2]) = u[i];
-    }
-  }
+  const int sub = (int)threadIdx.x / p.wide;
+  const int at = threadIdx.x - sub * (int)p.wide.d;
+  const int x = blockIdx.y * p.wide.d + at;
+  const int64_t t = (int64_t)blockIdx.x * (kThreads / p.wide.d) + sub;
+  if (sub >= (int)(kThreads / p.wide.d) || x >= p.per_token || t >= p.T) return;
+  const int32_t slot = p.slots[t];
+  const int kv = x >= p.keys;
+  const int y = kv ? x - p.keys : x;
+  const int head = y / p.units[kv];
+  const int64_t unit = (y - head * (int)p.units[kv].d) * (int64_t)sizeof(U);
+  const U u = *reinterpret_cast<const U*>(p.src[kv] + t * p.ss[kv][0] + head * p.ss[kv][1] + unit);
+  if (slot < 0 || slot >= p.slots_end) return;
+  const int32_t pg = slot / p.page, row = slot - pg * (int)p.page.d;
+  *reinterpret_cast<U*>(p.dst[kv] + pg * p.ds[kv][0] + head * p.ds[kv][1] + row * p.ds[kv][2] + unit) = u;
 }
 
 }  // namespace
@@ -223,8 +200,8 @@ extern "C" int bi_page_tables(int32_t* block_tables, const int32_t* context_lens
       (R > 0 && W > 0 && !block_tables) || (F > 0 && !free_pages) || (T > 0 && (!slots || !positions)))
     return bi::fail(BI_EINVAL, "bi_page_tables: null pointer");
   TablesArgs p = {block_tables, context_lens, new_lens, free_pages, slots, positions, query_start,
-                  seq_lens, pages_used, R, W, F, T, table_stride, (int32_t)page_size};
-  int64_t blocks = (T + kTokenTile - 1) / kTokenTile;
+                  seq_lens, pages_used, R, W, F, T, table_stride, bi::make_div(page_size)};
+  int64_t blocks = (T + kThreads - 1) / kThreads;
   if (blocks < 1) blocks = 1;
   if (blocks > 1024) blocks = 1024;
   hipLaunchKernelGGL(page_tables_kernel, dim3((unsigned)blocks), dim3(kThreads), 0,
@@ -260,10 +237,9 @@ extern "C" int bi_paged_update(const void* k, const void* v, void* k_cache, void
     for (int j = 0; j < 2; j++) p.ss[i][j] = strides[2 * i + j] * esz;
     for (int j = 0; j < 3; j++) p.ds[i][j] = strides[4 + 3 * i + j] * esz;
   }
-  p.T = T;
-  p.slots_end = num_pages * page_size;
-  p.page = (int32_t)page_size;
-  p.heads = (int32_t)Hkv;
+  p.T = (int32_t)T;
+  p.slots_end = (int32_t)(num_pages * page_size);
+  p.page = bi::make_div(page_size);
   // The widest unit that every row's address and length is a multiple of.
   uint64_t bits = (uint64_t)(D * esz) | (uint64_t)(V * esz) | (uintptr_t)k | (uintptr_t)v |
                   (uintptr_t)k_cache | (uintptr_t)v_cache;
@@ -273,13 +249,13 @@ extern "C" int bi_paged_update(const void* k, const void* v, void* k_cache, void
   }
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
   if (unit < esz) return bi::fail(BI_EINVAL, "bi_paged_update: pointers not aligned to elements");
-  p.units[0] = (int32_t)(D * esz / unit);
-  p.units[1] = (int32_t)(V * esz / unit);
-  p.per_token = p.heads * (p.units[0] + p.units[1]);
+  p.units[0] = bi::make_div(D * esz / unit);
+  p.units[1] = bi::make_div(V * esz / unit);
+  p.keys = (int32_t)(Hkv * p.units[0].d);
+  p.per_token = (int32_t)(p.keys + Hkv * p.units[1].d);
   const int64_t wide = p.per_token < kThreads ? p.per_token : kThreads;
-  const int64_t each = kThreads / wide, gy = (p.per_token + wide - 1) / wide;
-  int64_t gx = (T + each * kRows - 1) / (each * kRows);
-  if (gx > 65536) gx = 65536;
+  p.wide = bi::make_div(wide);
+  const int64_t each = kThreads / wide, gx = (T + each - 1) / each, gy = (p.per_token + wide - 1) / wide;
   if (gy > 65535) return bi::fail(BI_EINVAL, "bi_paged_update: rows too wide");
   const dim3 grid((unsigned)gx, (unsigned)gy);
   const hipStream_t s = static_cast<hipStream_t>(hip_stream);
