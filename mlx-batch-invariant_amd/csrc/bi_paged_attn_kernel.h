@@ -429,6 +429,11 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
   typedef __attribute__((address_space(1))) const u32x4 gvec;
   return __builtin_bit_cast(uint4, *(gvec*)p);
 }
+// One whose line is not wanted again.
+__device__ __forceinline__ uint4 ld16_once(const void* p) {
+  typedef __attribute__((address_space(1))) const u32x4 gvec;
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((gvec*)p));
+}
 
 __device__ __forceinline__ void st16(uint4* p, uint4 v) {
   *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, v);
@@ -461,9 +466,11 @@ __device__ __forceinline__ T* out_at(const Args& p, int r, const Request& rq, in
 // per wave. What bounds it is reading the cache, which it does 64 KB at a
 // time: a step's values are on their way while its scores are computed, the
 // next pass's keys while the values are used, both through the same registers
-// (the table's entries are loaded two passes ahead). Reading 2 GB in 1 KB
-// loads, 16 a wave in flight on two such workgroups per CU, reaches 6.0-6.4
-// TB/s on this card, and 32 a wave only 4.7.
+// (the table's entries are loaded two passes ahead). The same loads without
+// any computation read 64 requests of 8191 rows in pages of 16 in 350 us (6.1
+// TB/s); this kernel and its fold take 390, 410 with loads that keep their
+// lines in the caches. (32 loads a wave in flight, keys and values together,
+// were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
 template <typename T, int D, int V, int NC>
 __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel(Args p) {
   using G = Geo<T, D, V>;
@@ -538,7 +545,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 #pragma unroll
     for (int j = 0; j < KL; j++) {
       const int at = j * 64 + ln, row = at / G::CH;
-      x16[j] = ld16(s_row[0][wave * S + row] + (at - row * G::CH) * 16);
+      x16[j] = ld16_once(s_row[0][wave * S + row] + (at - row * G::CH) * 16);
     }
   };
   auto load_values = [&]() __attribute__((always_inline)) {
@@ -546,7 +553,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 #pragma unroll
     for (int j = 0; j < VL; j++) {
       const int at = j * 64 + ln, row = at / G::VCH;
-      x16[j] = ld16(s_row[1][wave * S + row] + (at - row * G::VCH) * 16);
+      x16[j] = ld16_once(s_row[1][wave * S + row] + (at - row * G::VCH) * 16);
     }
   };
 
@@ -764,7 +771,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
 // (LW = 0: the NW waves themselves). A wave spends about 150 cycles on issuing
 // a load that writes LDS, 8 a step: with another wave on its SIMD that is
 // hidden, alone it is a quarter of the step (512 tokens over 8192 keys 244 us,
-// XXX with loading waves).
+// 173 with loading waves; 1024 over 5120 167 and 125).
 template <typename T, int D, int V, int NW, int LW, int NB>
 __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 : 1))
     whole_kernel(Args p) {
