@@ -40,6 +40,7 @@ struct Args {
   float* po;              // [V] each
   float2* pml;            // base and sum
   Div nseg, ccap;         // segments and columns kept per (request, kv head)
+  Div reqs;               // R
   int32_t nc;             // columns per workgroup, 16 or 32
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes

@@ -70,6 +70,7 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.split_cols = (int32_t)s.split_cols;
     p.ccap = make_div(s.ccap);
     p.nseg = make_div(s.nseg);
+    p.reqs = make_div(p.R);
     p.nc = (int32_t)s.nc;
     p.po = static_cast<float*>(ws);
     p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv.d * s.ccap * s.nseg * V);

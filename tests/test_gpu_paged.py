@@ -300,6 +300,48 @@ def test_bits_do_not_depend_on_the_call(cuda, dtype, D, H, Hkv, window, first):
         t += k
 
 
+@pytest.mark.parametrize("D, V", [(64, 64), (96, 96), (128, 128), (192, 128), (192, 192), (256, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_bits_of_every_launch(cuda, dtype, D, V):
+    """A prompt long enough for workgroups of eight waves, one for two
+    workgroups per compute unit, a chunk with loading waves and single tokens:
+    the same rows, the same bits, over paged and contiguous keys."""
+    H, Hkv, n, window = 32, 8, 2200, 190
+    g = torch.Generator(device=cuda).manual_seed(D + V)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
+    q, k, v = rn(1, H, n, D), rn(1, Hkv, n, D), rn(1, Hkv, n, V)
+    base = bi.window_attention(q, k, v, window, sink_tokens=3)
+    for lo, hi in ((0, 1100), (1100, 2200), (700, 1000), (2195, 2200), (2000, 2001), (0, 1)):
+        y = bi.window_attention(q[:, :, lo:hi], k[:, :, :hi], v[:, :, :hi], window, sink_tokens=3)
+        assert same(y, base[:, :, lo:hi]), (lo, hi)
+    page = 64
+    table = torch.randperm(-(-n // page), generator=g, device=cuda).to(torch.int32)[None]
+    kc, vc = rn(table.shape[1], Hkv, page, D), rn(table.shape[1], Hkv, page, V)
+    i = torch.arange(n, device=cuda)
+    slots = (table[0, i // page] * page + i % page).to(torch.int32)
+    bi.paged_cache_update(k[0].transpose(0, 1), v[0].transpose(0, 1), kc, vc, slots)
+    qt = q[0].transpose(0, 1)
+    for lo, hi in ((0, 2200), (900, 2000), (1500, 1800)):
+        lens = torch.tensor([hi], dtype=torch.int32, device=cuda)
+        y = bi.paged_attention(qt[lo:hi], kc, vc, table, ref.starts([hi - lo], cuda), lens,
+                               window=window, sink_tokens=3)
+        assert same(y, base[0, :, lo:hi].transpose(0, 1).contiguous()), (lo, hi)
+
+
+def test_prompt_against_64_bits(cuda):
+    """Rows of a prompt of the size that takes eight waves per workgroup."""
+    H, Hkv, n, D = 32, 8, 2200, 128
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(n, H, D, generator=g).to(BF16)
+    k = torch.randn(n, Hkv, D, generator=g).to(BF16)
+    v = torch.randn(n, Hkv, D, generator=g).to(BF16)
+    dev = lambda t: t.to(cuda).transpose(0, 1)[None]
+    got = bi.window_attention(dev(q), dev(k), dev(v), None)[0].transpose(0, 1)
+    for lo, hi in ((0, 70), (1000, 1040), (2150, 2200)):
+        want, tol = ref.rows(q[lo:hi], k[:hi], v[:hi], hi, 0, 0, D ** -0.5, None)
+        check(got[lo:hi], want, tol, "rows %d" % lo)
+
+
 def _without_workspace(monkeypatch):
     monkeypatch.setattr(_paged, "_workspace", lambda need, device: None)
 
