@@ -166,20 +166,21 @@ struct UpdateArgs {
 // with four; a plain copy of as many bytes 11.1.)
 template <typename U>
 __global__ void __launch_bounds__(kThreads) paged_update_kernel(UpdateArgs p) {
+  const int each = kThreads / p.wide.d;  // tokens side by side
   const int sub = (int)threadIdx.x / p.wide;
-  const int at = threadIdx.x - sub * (int)p.wide.d;
-  const int x = blockIdx.y * p.wide.d + at;
-  const int64_t t = (int64_t)blockIdx.x * (kThreads / p.wide.d) + sub;
-  if (sub >= (int)(kThreads / p.wide.d) || x >= p.per_token || t >= p.T) return;
-  const int32_t slot = p.slots[t];
+  const int x = blockIdx.y * p.wide.d + (threadIdx.x - sub * (int)p.wide.d);
+  if (sub >= each || x >= p.per_token) return;
   const int kv = x >= p.keys;
   const int y = kv ? x - p.keys : x;
   const int head = y / p.units[kv];
   const int64_t unit = (y - head * (int)p.units[kv].d) * (int64_t)sizeof(U);
-  const U u = *reinterpret_cast<const U*>(p.src[kv] + t * p.ss[kv][0] + head * p.ss[kv][1] + unit);
-  if (slot < 0 || slot >= p.slots_end) return;
-  const int32_t pg = slot / p.page, row = slot - pg * (int)p.page.d;
-  *reinterpret_cast<U*>(p.dst[kv] + pg * p.ds[kv][0] + head * p.ds[kv][1] + row * p.ds[kv][2] + unit) = u;
+  for (int64_t t = (int64_t)blockIdx.x * each + sub; t < p.T; t += (int64_t)gridDim.x * each) {
+    const int32_t slot = p.slots[t];
+    const U u = *reinterpret_cast<const U*>(p.src[kv] + t * p.ss[kv][0] + head * p.ss[kv][1] + unit);
+    if (slot < 0 || slot >= p.slots_end) continue;
+    const int32_t pg = slot / p.page, row = slot - pg * (int)p.page.d;
+    *reinterpret_cast<U*>(p.dst[kv] + pg * p.ds[kv][0] + head * p.ds[kv][1] + row * p.ds[kv][2] + unit) = u;
+  }
 }
 
 }  // namespace
@@ -255,7 +256,8 @@ extern "C" int bi_paged_update(const void* k, const void* v, void* k_cache, void
   p.per_token = (int32_t)(p.keys + Hkv * p.units[1].d);
   const int64_t wide = p.per_token < kThreads ? p.per_token : kThreads;
   p.wide = bi::make_div(wide);
-  const int64_t each = kThreads / wide, gx = (T + each - 1) / each, gy = (p.per_token + wide - 1) / wide;
+  const int64_t each = kThreads / wide, gy = (p.per_token + wide - 1) / wide;
+  const int64_t tokens = (T + each - 1) / each, gx = tokens < 1 << 22 ? tokens : 1 << 22;
   if (gy > 65535) return bi::fail(BI_EINVAL, "bi_paged_update: rows too wide");
   const dim3 grid((unsigned)gx, (unsigned)gy);
   const hipStream_t s = static_cast<hipStream_t>(hip_stream);

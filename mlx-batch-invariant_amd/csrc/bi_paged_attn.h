@@ -42,6 +42,9 @@ struct Args {
   Div nseg, ccap;         // segments and columns kept per (request, kv head)
   Div reqs;               // R
   int32_t nc;             // columns per workgroup, 16 or 32
+  Div ctiles;             // workgroups of them
+  Div slots;              // R * nseg
+  int32_t once;           // keys and values are read by one of these only
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
 };

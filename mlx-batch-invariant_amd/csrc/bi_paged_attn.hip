@@ -25,36 +25,90 @@ Kernels kernels(int64_t D, int64_t V, int dtype) {
 
 // Tokens, lengths and windows past this are not computed with (positions
 // minus a window stay in 32 bits).
-constexpr int64_t kMost = (int64_t)1 << 30;
+constexpr int64_t kMost = (int64_t)1 << 29;
 
-// How a call is split: the columns up to which a request is (0: none), and the
-// memory of its partial results. `exact`: every request has max_query tokens.
+// A call as the host knows it; `exact`: every request has max_query tokens.
+struct Call {
+  int64_t R, tokens, G, Hkv, D, V, window, first, max_query, max_seq;
+  bool exact, f32;
+};
+
+// How a call is split: the columns up to which a request is (0: none), columns
+// kept per request and kv head, columns per workgroup, segments, and the bytes
+// of the partial results.
 struct Plan {
   int64_t split_cols, ccap, nc, nseg, bytes;
 };
-Plan plan(int64_t R, int64_t G, int64_t Hkv, int64_t V, int64_t window, int64_t first,
-          int64_t max_query, int64_t max_seq, bool exact, const Kernels& k) {
-  Plan s = {0, 0, 0, 0, 0};
-  const int64_t cols = max_query * G;
-  if (R <= 0 || cols <= 0 || max_seq <= 0) return s;
-  s.split_cols = 32;
-  if (exact && cols > s.split_cols) return Plan{0, 0, 0, 0, 0};
-  s.ccap = cols < s.split_cols ? cols : s.split_cols;
+
+// A plan that splits requests of up to `most` columns.
+Plan split_up_to(const Call& c, int64_t most, int64_t seg) {
+  Plan s;
+  const int64_t cols = c.max_query * c.G;
+  s.split_cols = most;
+  s.ccap = cols < most ? cols : most;
   // Beside requests of more columns those of few are mostly single tokens: then
-  // two workgroups of 16 columns, of which such a request needs one.
-  s.nc = s.ccap > 16 && cols <= s.split_cols ? 32 : 16;
-  const int64_t part = k.seg;
-  s.nseg = (max_seq + part - 1) / part;
-  if (window) {
+  // workgroups of 16 columns, of which such a request needs one.
+  s.nc = s.ccap > 16 && (cols <= most || c.G > 16) ? 32 : 16;
+  s.nseg = (c.max_seq + seg - 1) / seg;
+  if (c.window) {
     // Tokens of a workgroup's columns, rows that they see between them.
-    const int64_t span = window + (s.nc - 1) / G + 1;
-    const int64_t n = (span + part - 2) / part + 1 + (first + part - 1) / part;
+    const int64_t span = c.window + (s.nc - 1) / c.G + 1;
+    const int64_t n = (span + seg - 2) / seg + 1 + (c.first + seg - 1) / seg;
     if (n < s.nseg) s.nseg = n;
   }
-  s.bytes = R * Hkv * s.ccap * s.nseg * (V + 2) * (int64_t)sizeof(float);
-  if (s.bytes > (int64_t)1 << 31 || R * Hkv * s.nseg > INT32_MAX ||
-      R * Hkv * s.ccap > INT32_MAX) return Plan{0, 0, 0, 0, 0};
+  s.bytes = c.R * c.Hkv * s.ccap * s.nseg * (c.V + 2) * (int64_t)sizeof(float);
   return s;
+}
+int64_t split_grid(const Call& c, const Plan& s) {
+  return c.R * c.Hkv * s.nseg * ((s.ccap + s.nc - 1) / s.nc);
+}
+bool fits(const Call& c, const Plan& s) {
+  return s.bytes <= (int64_t)1 << 32 && split_grid(c, s) <= 1 << 23 && c.R * c.Hkv * s.ccap <= 1 << 24;
+}
+
+// Requests are split where that is estimated to take less time than to walk
+// them whole; beside chunks of more than 1024 columns those of single tokens
+// and a few (32 columns) are. Microseconds, from times of D = V = 128: a whole
+// workgroup 6 and 0.0195 a row it walks (fp32 five times that), one per compute
+// unit; a split one 5.5 and as much for a full segment, one or two per compute
+// unit; reading the cache once at 5 TB/s (whole: 3.6); the partial results' way through
+// memory and back at 4 TB/s; a launch 2, two 8. (Over 8192 rows 16 tokens
+// 161 us whole, 20.8 split, 64 166 and 58, 128 167 and 107, 256 169 and 202;
+// 64 requests of one token and 100 rows 20.1 whole, 17.4 split, one of 300 rows
+// 13.7 and 15.8.)
+Plan plan(const Call& c, const Kernels& k) {
+  const Plan none = {0, 0, 0, 0, 0};
+  const int64_t cols = c.max_query * c.G;
+  if (c.R <= 0 || cols <= 0 || c.max_seq <= 0) return none;
+  const int64_t few = c.G > 32 ? c.G : 32;
+  const double cus = bi::device_cus(), wide = (double)(c.D + c.V) / 256.0 * (c.f32 ? 2.0 : 1.0);
+  const double H = (double)(c.G * c.Hkv);
+  double rows = (double)c.max_seq;
+  if (c.window && (double)(c.window + c.first) < rows) rows = (double)(c.window + c.first);
+  const double full = rows < (double)k.seg ? rows / (double)k.seg : 1.0;
+  const double tiles = ((double)c.tokens * c.G / 128.0 + c.R) * c.Hkv / cus;
+  const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * (c.f32 ? 4.0 : 2.0) / 5e6;
+  double whole = (tiles > 1.0 ? tiles : 1.0) * (6.0 + rows * 0.0195 * wide * (c.f32 ? 2.5 : 1.0));
+  whole = 2.0 + (whole > 1.4 * read ? whole : 1.4 * read);
+  auto split = [&](const Plan& s) {
+    const double busy = ((double)c.tokens * c.G / s.nc + c.R) * c.Hkv * s.nseg;
+    const double grid = (double)split_grid(c, s);
+    double rounds = (grid < busy ? grid : busy) / ((s.nc == 16 && wide <= 1.0 ? 2.0 : 1.0) * cus);
+    if (rounds < 1.0) rounds = 1.0;
+    const double walk = rounds * (5.5 + 5.5 * full * (wide > 1.0 ? wide : 1.0));
+    const double idle = grid > busy ? (grid - busy) / (2.0 * cus) * 1.5 : 0.0;
+    return 8.0 + (walk > read ? walk : read) + (double)c.tokens * H * s.nseg * (c.V + 2) * 8.0 / 4e6 + idle;
+  };
+  if (cols <= few || cols <= 1024) {
+    const Plan s = split_up_to(c, cols > few ? cols : few, k.seg);
+    if (fits(c, s) && split(s) < whole) return s;
+    if (cols <= few && whole <= split(s)) return none;
+  }
+  if (c.exact) return none;
+  // Beside whole chunks; where the results would take too much, single tokens.
+  Plan s = split_up_to(c, few, k.seg);
+  if (!fits(c, s)) s = split_up_to(c, c.G, k.seg);
+  return fits(c, s) ? s : none;
 }
 
 int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, int64_t ws_bytes,
@@ -62,8 +116,9 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   const Kernels k = kernels(D, V, dtype);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t most = p.qstart ? p.max_query : p.qL;
-  Plan s = plan(p.R, p.G.d, p.Hkv.d, V, p.window, p.first, most, p.qstart ? p.max_seq : p.N,
-                !p.qstart, k);
+  const Call c = {p.R, p.qstart ? p.T : (int64_t)p.R * p.qL, p.G.d, p.Hkv.d, D, V, p.window, p.first,
+                  most, p.qstart ? p.max_seq : p.N, !p.qstart, dtype == BI_F32};
+  Plan s = plan(c, k);
   if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0};
   hipError_t e;
   if (s.split_cols) {
@@ -74,8 +129,13 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.nc = (int32_t)s.nc;
     p.po = static_cast<float*>(ws);
     p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv.d * s.ccap * s.nseg * V);
-    const dim3 grid((unsigned)(p.R * p.Hkv.d * s.nseg), (unsigned)((s.ccap + s.nc - 1) / s.nc));
-    hipLaunchKernelGGL(s.nc == 16 ? k.split16 : k.split32, grid, dim3(256), 0, st, p);
+    const int64_t ctiles = (s.ccap + s.nc - 1) / s.nc;
+    p.ctiles = make_div(ctiles);
+    p.slots = make_div(p.R * s.nseg);
+    // (Beside larger requests split ones mostly have one column tile.)
+    p.once = ctiles == 1 || most * p.G.d > s.split_cols;
+    hipLaunchKernelGGL(s.nc == 16 ? k.split16 : k.split32, dim3((unsigned)split_grid(c, s)), dim3(256),
+                       0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   const bool whole = most * p.G.d > s.split_cols;
@@ -209,8 +269,9 @@ extern "C" int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H,
   if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || !bi::elem_size(dtype) ||
       !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
     return 0;
-  return plan(R, H / Hkv, Hkv, V, clamp32(window), clamp32(sink_tokens),
-              clamp32(max_query), clamp32(max_seq), false, kernels(D, V, dtype)).bytes;
+  const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
+                  clamp32(max_seq), false, dtype == BI_F32};
+  return plan(c, kernels(D, V, dtype)).bytes;
 }
 
 extern "C" int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks,
@@ -254,6 +315,7 @@ extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t H
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || qL <= 0 || N <= 0 || !bi::elem_size(dtype) ||
       !dims_built(D, V) || qL > kMost || N > kMost || B > kMost || window < 0 || sink_tokens < 0)
     return 0;
-  return plan(B, H / Hkv, Hkv, V, clamp32(window), clamp32(sink_tokens), qL, N, true,
-              kernels(D, V, dtype)).bytes;
+  const Call c = {B, B * qL, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), qL, N, true,
+                  dtype == BI_F32};
+  return plan(c, kernels(D, V, dtype)).bytes;
 }

@@ -483,11 +483,18 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5, cn = col & (NC - 1);
-  // Workgroup -> kv head, segment of the walk, request. Request by request;
-  // under a window, where every request has the same few segments and the
-  // first and the last are cut, segment by segment (16 requests that see 1024
-  // rows 24.1 -> 21.4 us; 64 of 1000 to 8191 rows 271 -> 279).
-  const int x = blockIdx.x, xs = x / p.Hkv, kvh = x - xs * (int)p.Hkv.d;
+  // Workgroup -> kv head, columns, segment of the walk, request. A segment's
+  // column tiles are next to each other, with 8 kv heads on one XCD: they read
+  // the same rows; but one after the other where most requests have only the
+  // first (beside chunks: 30 of 32 requests, 70 us the other way, 47 so).
+  // Request by request; under a window, where every request has the same few
+  // segments and the first and the last are cut, segment by segment (16
+  // requests that see 1024 rows 24.1 -> 21.4 us; 64 of 1000 to 8191 rows 271
+  // -> 279).
+  const int x = blockIdx.x, xc = x / p.Hkv, kvh = x - xc * (int)p.Hkv.d;
+  const int xq = xc / (p.once ? p.slots : p.ctiles);
+  const int xr = xc - xq * (int)(p.once ? p.slots : p.ctiles).d;
+  const int xs = p.once ? xr : xq, c0 = (p.once ? xq : xr) * NC;
   const int outer = xs / (p.window ? p.reqs : p.nseg);
   const int inner = xs - outer * (int)(p.window ? p.reqs : p.nseg).d;
   const int r = p.window ? inner : outer, part = p.window ? outer : inner;
@@ -501,7 +508,6 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   }
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
-  const int c0 = blockIdx.y * NC;
   if (rq.beyond || ncol > p.split_cols || c0 >= ncol) return;
   const int clast = (c0 + NC < ncol ? c0 + NC : ncol) - 1;
   const int32_t lo = rq.n - rq.L + c0 / p.G, hi = rq.n - rq.L + clast / p.G;
@@ -545,21 +551,22 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   // not kept across segments in registers that the loads need.
   constexpr int KL = S * G::CH / 64, VL = S * G::VCH / 64;
   uint4 x16[KL > VL ? KL : VL], q[G::NQ];
-  auto load_keys = [&]() __attribute__((always_inline)) {
+  auto load_rows = [&](const char* const* rows, auto chunks, auto load) __attribute__((always_inline)) {
+    constexpr int C = decltype(chunks)::value;
     const int ln = opaque(lane);
 #pragma unroll
-    for (int j = 0; j < KL; j++) {
-      const int at = j * 64 + ln, row = at / G::CH;
-      x16[j] = ld16_once(s_row[0][wave * S + row] + (at - row * G::CH) * 16);
+    for (int j = 0; j < S * C / 64; j++) {
+      const int at = j * 64 + ln, row = at / C;
+      x16[j] = load(rows[wave * S + row] + (at - row * C) * 16);
     }
   };
+  auto load_keys = [&]() __attribute__((always_inline)) {
+    if (p.once) load_rows(s_row[0], std::integral_constant<int, G::CH>(), ld16_once);
+    else load_rows(s_row[0], std::integral_constant<int, G::CH>(), ld16);
+  };
   auto load_values = [&]() __attribute__((always_inline)) {
-    const int ln = opaque(lane);
-#pragma unroll
-    for (int j = 0; j < VL; j++) {
-      const int at = j * 64 + ln, row = at / G::VCH;
-      x16[j] = ld16_once(s_row[1][wave * S + row] + (at - row * G::VCH) * 16);
-    }
+    if (p.once) load_rows(s_row[1], std::integral_constant<int, G::VCH>(), ld16_once);
+    else load_rows(s_row[1], std::integral_constant<int, G::VCH>(), ld16);
   };
 
   if (p.window) {
