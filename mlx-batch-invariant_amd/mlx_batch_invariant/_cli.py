@@ -3,8 +3,8 @@
 Mirrors reference mlx_batch_invariant/_cli.py:17-161 (the linear batch sweep,
 the attention query-length sweep, the stock negative control and the exit
 codes), on torch + the HIP kernels, and adds the axes this build promises:
-every row position of a batch, context growth with masked keys past 4096, and
-HIP graph capture. Exit status 1 on any variance or if stock torch.matmul
+every row position of a batch, context growth with masked keys past 4096, HIP
+graph capture, and a paged cache (chunks, batches, pages, contiguous keys). Exit status 1 on any variance or if stock torch.matmul
 comes out invariant everywhere (then the sweep proves nothing); 2 on usage.
 """
 
@@ -12,7 +12,7 @@ import argparse
 import platform
 import sys
 
-from . import __version__, scaled_dot_product_attention
+from . import __version__, paged_attention, scaled_dot_product_attention, window_attention
 from ._gemm import linear
 
 _DTYPES = ("bfloat16", "float16", "float32")
@@ -115,6 +115,50 @@ def _graph_case(dtype, gen, device):
     return bad
 
 
+def _paged_case(dtype, gen, device, H, Hkv, D, n, L, window=None, first=0):
+    """The last L tokens of a request of n rows over a paged cache: token by
+    token, in chunks, beside another request, over pages of another size and
+    over contiguous keys, against all of them at once."""
+    import torch
+
+    k = _rn((n, Hkv, D), dtype, gen, device)
+    v = _rn((n, Hkv, D), dtype, gen, device)
+    q = _rn((L, H, D), dtype, gen, device)
+    kw = dict(window=window, sink_tokens=first)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+
+    def paged(page):
+        pages = -(-n // page)
+        order = torch.randperm(pages, generator=gen).to(device)
+        i = torch.arange(n, device=device)
+        caches = []
+        for x in (k, v):
+            pool = torch.zeros((pages, page, Hkv, D), dtype=dtype, device=device)
+            pool[order[i // page], i % page] = x
+            caches.append(pool.transpose(1, 2))
+        return caches, order.to(torch.int32)[None]
+
+    (kc, vc), table = paged(16)
+    run = lambda a, b: paged_attention(q[a:b], kc, vc, table, i32([0, b - a]), i32([n - L + b]), **kw)
+    base, bad = run(0, L), []
+    same = lambda x, y: torch.equal(_bits(x), _bits(y))
+    for step in (1, 7, 64):
+        if not all(same(run(a, min(a + step, L)), base[a:a + step]) for a in range(0, L, step)):
+            bad.append("chunks of %d" % step)
+    both = paged_attention(torch.cat([q[-3:], q]), kc, vc, torch.cat([table, table]),
+                           i32([0, 3, 3 + L]), i32([n, n]), **kw)
+    if not same(both[3:], base) or not same(both[:3], base[-3:]):
+        bad.append("batch")
+    (k2, v2), t2 = paged(48)
+    if not same(paged_attention(q, k2, v2, t2, i32([0, L]), i32([n]), **kw), base):
+        bad.append("pages")
+    y = window_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None],
+                         window, sink_tokens=first)
+    if not same(y[0].transpose(0, 1), base):
+        bad.append("contiguous")
+    return bad
+
+
 def _stock_matmul_variant(batches, gen, device):
     """Stock torch.matmul must be batch-variant somewhere (reference
     _cli.py:121-128 checks fp32 4096x4096; hipBLASLt picks kernels per shape,
@@ -180,6 +224,14 @@ def verify(argv=None):
             fails += bool(bad)
             print("  %-9s sdpa     H=%d/%-2d N=%-6d %s"
                   % (name, H, Hkv, N, "ok" if not bad else "VARIANT at qL %s" % bad))
+        pages = [(8, 8, 128, 700, 130, None, 0)] if args.quick else [
+            (8, 8, 128, 700, 130, None, 0), (32, 8, 128, 1500, 300, 400, 4), (16, 4, 64, 900, 200, None, 0)]
+        for H, Hkv, D, n, L, window, first in pages:
+            bad = _paged_case(dtype, gen, device, H, Hkv, D, n, L, window, first)
+            fails += bool(bad)
+            print("  %-9s paged    H=%d/%-2d N=%-6d %s%s"
+                  % (name, H, Hkv, n, "ok" if not bad else "VARIANT over %s" % ", ".join(bad),
+                     "" if window is None else " (window %d)" % window))
         if not args.quick:
             bad = _context_case(dtype, gen, device)
             fails += bool(bad)
