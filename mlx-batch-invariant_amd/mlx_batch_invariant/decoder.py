@@ -12,6 +12,12 @@ residual adds are stock torch, which computes them per row with a fixed
 reduction (tests/test_gpu_stock_ops.py guards that). Weights are random:
 there is no checkpoint. They are drawn on the device from torch's seeded
 generator, so the same seed gives the same model.
+
+:class:`PagedCache` and :func:`serve_step` run the same model over a paged cache,
+request by request and chunk by chunk (bi.page_tables, bi.paged_cache_update,
+bi.paged_attention); :func:`generate` decodes greedily on top of them. Under
+``batch_invariant_mode`` a request's logits have the same bits whatever is
+served beside it and however its prompt is cut into chunks.
 """
 
 import math
@@ -121,3 +127,105 @@ def determinism(model, length=512, batches=(2, 4, 8), seed=0, invariant=True):
     ids = prompts(c, max(batches), length, seed=seed, device=device)
     base = logits_bits(model, ids[:1], invariant)
     return {B: int((logits_bits(model, ids[:B], invariant) != base).sum()) for B in batches}
+
+
+class PagedCache:
+    """Keys and values of up to `requests` requests of up to `max_len` tokens in
+    pages shared by all, one pool per layer; one table for all layers. The
+    lengths are kept on the host too, which sizes every step without asking the
+    GPU."""
+
+    def __init__(self, config, requests, max_len, page_size=64, num_pages=None, device="cuda",
+                 dtype=torch.bfloat16):
+        c = config
+        width = -(-max_len // page_size)
+        self.num_pages = requests * width if num_pages is None else num_pages
+        self.page_size, self.max_len = page_size, max_len
+        shape = (c.layers, self.num_pages, c.kv_heads, page_size, c.head_dim)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.tables = torch.full((requests, width), -1, dtype=torch.int32, device=device)
+        self.free = torch.arange(self.num_pages, dtype=torch.int32, device=device)
+        self.used = 0
+        self.lens = [0] * requests
+
+    def begin(self, new):
+        """Takes the pages of a step that brings new[r] tokens of request r;
+        returns its bi.PageTables and (most new tokens, longest request)."""
+        from . import page_tables
+
+        if len(new) != len(self.lens) or min(new) < 0:
+            raise ValueError("expected %d token counts, got %s" % (len(self.lens), list(new)))
+        after = [a + b for a, b in zip(self.lens, new)]
+        if max(after) > self.max_len:
+            raise ValueError("a request of %d tokens exceeds max_len %d" % (max(after), self.max_len))
+        pages = lambda n: -(-n // self.page_size)
+        need = sum(pages(b) - pages(a) for a, b in zip(self.lens, after))
+        if self.used + need > self.num_pages:
+            raise RuntimeError("%d pages needed, %d of %d free"
+                               % (need, self.num_pages - self.used, self.num_pages))
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=self.tables.device)
+        t = page_tables(self.tables, i32(self.lens), i32(new), self.free[self.used:],
+                        self.page_size, sum(new))
+        self.used += need
+        self.lens = after
+        return t, max(new), max(after)
+
+
+def serve_step(model, cache, ids, new):
+    """One step over `cache`: ids (sum of new,) are the new tokens, new[r] of
+    request r, one request behind the other. Returns the logits of every
+    request's last token, (requests, vocab); those of a request without a new
+    token are its neighbour's and mean nothing."""
+    from . import paged_attention, paged_cache_update
+
+    c = model.c
+    t, most, longest = cache.begin(new)
+    x = model.embed(ids)
+    T = x.shape[0]
+    for i, blk in enumerate(model.blocks):
+        y = blk.n1(x)
+        k = blk.k(y).view(T, c.kv_heads, c.head_dim)
+        v = blk.v(y).view(T, c.kv_heads, c.head_dim)
+        paged_cache_update(k, v, cache.k[i], cache.v[i], t.slots)
+        a = paged_attention(blk.q(y).view(T, c.heads, c.head_dim), cache.k[i], cache.v[i],
+                            t.block_tables, t.query_start, t.seq_lens, max_query=most,
+                            max_seq=longest)
+        x = x + blk.o(a.reshape(T, c.heads * c.head_dim))
+        y = blk.n2(x)
+        x = x + blk.down(F.silu(blk.gate(y)) * blk.up(y))
+    last = (t.query_start[1:] - 1).clamp(min=0).long()
+    return model.head(model.norm(x[last]))
+
+
+def generate(model, prompts, steps, chunk=None, page_size=64, logits=None):
+    """Greedy continuation of `prompts` (1-d id tensors of any lengths) by
+    `steps` tokens each, (len(prompts), steps). Prompts enter in chunks of up to
+    `chunk` tokens (all of a prompt by default), all requests in one batch. A
+    list passed as `logits` receives every decoded token's (requests, vocab)."""
+    if not prompts or min(p.shape[0] for p in prompts) < 1 or steps < 1:
+        raise ValueError("expected prompts of one token or more and steps >= 1")
+    if chunk is not None and chunk < 1:
+        raise ValueError("chunk must be >= 1, got %d" % chunk)
+    device = next(model.parameters()).device
+    dtype = model.head.weight.dtype
+    left = [p.to(device) for p in prompts]
+    cache = PagedCache(model.c, len(left), max(p.shape[0] for p in left) + steps, page_size,
+                       device=device, dtype=dtype)
+    first = [None] * len(left)
+    with torch.no_grad():
+        while any(p.shape[0] for p in left):
+            part = [p if chunk is None else p[:chunk] for p in left]
+            y = serve_step(model, cache, torch.cat(part), [p.shape[0] for p in part])
+            for r, p in enumerate(part):
+                left[r] = left[r][p.shape[0]:]
+                if p.shape[0] and not left[r].shape[0]:
+                    first[r] = y[r]
+        y, out = torch.stack(first), []
+        for s in range(steps):
+            if logits is not None:
+                logits.append(y)
+            out.append(y.argmax(-1))
+            if s + 1 < steps:
+                y = serve_step(model, cache, out[-1], [1] * len(left))
+    return torch.stack(out, 1)

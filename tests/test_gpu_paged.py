@@ -597,3 +597,30 @@ def test_workspace_too_small_is_done_without(cuda):
                                   1 / math.sqrt(D), 0, 0, 1, n, _lib.BF16, wp, wb,
                                   torch.cuda.current_stream().cuda_stream)
         assert rc == 0 and same(out, base)
+
+
+def test_decoder_over_a_paged_cache(cuda):
+    """The synthetic decoder served over a paged cache: a request's logits have
+    the same bits alone, in a batch of other lengths and with its prompt in
+    chunks, and they are those of the contiguous model within the rounding of
+    its activations."""
+    from mlx_batch_invariant import decoder
+
+    c = decoder.DecoderConfig(hidden=512, inter=768, heads=8, kv_heads=2, head_dim=64, layers=2,
+                              vocab=1000)
+    m = decoder.build(c, device=cuda, seed=1)
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(0, c.vocab, (n,), generator=g) for n in (77, 5, 300, 1)]
+    with bi.batch_invariant_mode():
+        alone, both, cut = [], [], []
+        ids = decoder.generate(m, prompts[2:3], 6, logits=alone)
+        ids_b = decoder.generate(m, prompts, 6, logits=both)
+        ids_c = decoder.generate(m, prompts, 6, chunk=64, page_size=16, logits=cut)
+        with torch.no_grad():
+            full = m(prompts[2][None].to(cuda))
+    assert torch.equal(ids[0], ids_b[2]) and torch.equal(ids_b, ids_c)
+    for a, b, x in zip(alone, both, cut):
+        assert same(a[0], b[2]) and same(b, x)
+    # Two layers of bf16 activations, each rounded to 2^-8 some ten times.
+    err = (alone[0].double() - full.double()).abs().max() / full.double().abs().max()
+    assert float(err) < 2 * 10 * 2.0 ** -8

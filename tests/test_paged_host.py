@@ -178,3 +178,25 @@ def test_compiled_shapes():
         y = op.window_attention(torch.empty(2, 8, 3, 192), torch.empty(2, 2, 9, 192),
                                 torch.empty(2, 2, 9, 128), 0.1, 4, 0, None)
         assert y.shape == (2, 8, 3, 128)
+
+
+def test_decoder_cache_refusals():
+    """The decoder's cache checks a step on the host before any launch."""
+    from mlx_batch_invariant import decoder
+
+    c = decoder.DecoderConfig(hidden=64, inter=96, heads=2, kv_heads=1, head_dim=64, layers=1, vocab=50)
+    cache = decoder.PagedCache(c, 2, 100, page_size=16, num_pages=5, device="cpu")
+    assert cache.tables.shape == (2, 7) and cache.k.shape == (1, 5, 1, 16, 64)
+    with pytest.raises(ValueError, match="token counts"):
+        cache.begin([1])
+    with pytest.raises(ValueError, match="token counts"):
+        cache.begin([1, -1])
+    with pytest.raises(ValueError, match="max_len"):
+        cache.begin([101, 0])
+    with pytest.raises(RuntimeError, match="pages"):
+        cache.begin([90, 1])
+    assert cache.used == 0 and cache.lens == [0, 0]
+    for prompts, steps, chunk in (([], 1, None), ([torch.zeros(0).long()], 1, None),
+                                  ([torch.zeros(2).long()], 0, None), ([torch.zeros(2).long()], 1, 0)):
+        with pytest.raises(ValueError):
+            decoder.generate(None, prompts, steps, chunk)
