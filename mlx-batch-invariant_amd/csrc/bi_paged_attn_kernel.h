@@ -227,7 +227,10 @@ __device__ __forceinline__ float pow2(float e) {
 // The base after a step whose largest seen raw score is `top` (-inf: none seen):
 // p is at most 2^kRise, and above 2^-4 for the largest score of a segment's
 // first step (f16 holds p to 2^-25).
-constexpr float kRise = 6.f, kMostSum = 64.f;
+// A sum of rounded p up to kMostSum holds none of a score above the base +
+// kRise, whose p is 64 and rounds to no less than 63.75 in any type, with the
+// exponential's own error.
+constexpr float kRise = 6.f, kMostSum = 63.f;
 __device__ __forceinline__ float next_base(float m, float top, float a) {
   const float s = top * a;
   return top > -INFINITY && s > m + kRise ? ceilf(s * 0.25f) * 4.f : m;
@@ -1004,9 +1007,8 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
         const int ps = opaque(pos);  // keeps the bits' computation in this branch
         G::hide(s, seen_bits(p, ps, key0, mapped) >> (4 * hf));
       }
-      // A lane's sum of at most 2^kRise holds no p above it, so the base does
-      // not move; else, and at a segment's first step, the largest score
-      // decides.
+      // A lane's sum of at most kMostSum holds no score that moves the base;
+      // else, and at a segment's first step, the largest score decides.
       uint4 pu[KT][PU];
       float psum;
       bool look = fresh;

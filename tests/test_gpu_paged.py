@@ -624,3 +624,22 @@ def test_decoder_over_a_paged_cache(cuda):
     # Two layers of bf16 activations, each rounded to 2^-8 some ten times.
     err = (alone[0].double() - full.double()).abs().max() / full.double().abs().max()
     assert float(err) < 2 * 10 * 2.0 ** -8
+
+
+def test_bits_where_the_base_just_moves(cuda):
+    """A score just over the base's limit whose 2^x rounds to the limit itself,
+    alone in its step: the chunk's kernel has to see it as the single token's
+    does. (What shows it: f16 weights of 2^-18.5 under the one base, 0 under the
+    other, on values of 30000.)"""
+    n = 2000
+    k = torch.zeros(1, 1, n, 64, dtype=F16, device=cuda)
+    v = torch.zeros_like(k)
+    k[..., 65:128, 0] = -30.0
+    k[..., 64, 0], k[..., 64, 1] = 6.0, 0.0003
+    k[..., 128:512, 0] = -18.5
+    v[..., 128:512, :] = 30000.0
+    q = torch.zeros(1, 1, n, 64, dtype=F16, device=cuda)
+    q[..., :2] = 1.0
+    chunk = bi.window_attention(q, k, v, None, scale=math.log(2.0))
+    one = bi.window_attention(q[:, :, -1:], k, v, None, scale=math.log(2.0))
+    assert same(chunk[:, :, -1:], one)
