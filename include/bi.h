@@ -252,7 +252,7 @@ int bi_paged_update(const void* k, const void* v, void* k_cache, void* v_cache,
  *   workspace    at least bi_paged_attention_workspace bytes, 16-byte aligned,
  *                or NULL: slower, with the same bits
  *
- * Arithmetic (bi_paged_attn.h): keys are taken by their position in the
+ * Arithmetic (bi_paged_attn_kernel.h): keys are taken by their position in the
  * request, in segments of a fixed length whose results are folded in order,
  * so that a token's bits depend on its own request's rows alone: not on other
  * requests, on how many tokens are new, on the pages, on the workspace or on

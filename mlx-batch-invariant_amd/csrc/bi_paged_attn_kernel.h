@@ -17,8 +17,8 @@
 //     of the rows enter product t (fp32: products 4t .. 4t + 3).
 //   * Within a segment the running base m moves at a step whose largest seen
 //     score M exceeds m + 6, to the next multiple of 4 from M on. p_j =
-//     2^(fma(raw_j, a, -m)), 0 for an unseen row (whose raw_j is -inf); l = l * f + (the step's sum of
-//     p, in a fixed order per lane half); o = o * f, then o += v . p by 32x32
+//     2^(fma(raw_j, a, -m)), 0 for an unseen row (whose raw_j is -inf); l =
+//     l * f + (the step's sum of p, in a fixed order per lane half); o = o * f, then o += v . p by 32x32
 //     products over the step's rows in ascending order, p rounded once to the
 //     type (the products of bf16 and f16 take such operands), and l sums what
 //     was rounded. f is a power of two, as every base is an integer.
@@ -35,9 +35,10 @@
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment),
 //     whose four waves take a step each at a time; a second kernel folds the
 //     segments. For few columns, where what bounds it is reading the cache.
-//   * whole: a workgroup per 128 or 256 columns walks all their steps, 32 columns per
-//     wave, keys and values through two LDS buffers. For chunks of a prompt,
-//     where the matrix products and the exponentials bound it.
+//   * whole: a workgroup per 128 or 256 columns walks all their steps, 32
+//     columns per wave, keys and values through a ring of LDS buffers. For
+//     chunks of a prompt, where the matrix products and the exponentials bound
+//     it.
 // A segment is long enough that writing its results costs little beside
 // reading it, and short enough that one long sequence fills the GPU.
 #pragma once
@@ -589,8 +590,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   for (int si = s0; si < s1; si++) {
     const int32_t pass0 = si * PS, key0 = pass0 + wave * S;
     const int32_t entry2 = entry_for(si + 2);
-    // Scores of the wave's step and their largest.
-    // The keys change from rows to
+    // Scores of the wave's step and their largest. The keys change from rows to
     // the products' operands by way of the LDS where the wave's values go next.
     f32x16 s[KT];
     const int lk = opaque(lane);
@@ -786,7 +786,10 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
 // (LW = 0: the NW waves themselves). A wave spends about 150 cycles on issuing
 // a load that writes LDS, 8 a step: with another wave on its SIMD that is
 // hidden, alone it is a quarter of the step (512 tokens over 8192 keys 244 us,
-// 173 with loading waves; 1024 over 5120 167 and 125).
+// 173 with loading waves; 1024 over 5120 167 and 125). (Four more computing
+// waves on every second segment of the same columns, whose results go through
+// LDS, took 185: matrix products and exponentials do not overlap on a SIMD, and
+// one wave already fills it.)
 template <typename T, int D, int V, int NW, int LW, int NB>
 __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 : 1))
     whole_kernel(Args p) {
