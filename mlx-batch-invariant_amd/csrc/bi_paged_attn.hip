@@ -126,6 +126,7 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   if (s.split_cols) {
     p.split_cols = (int32_t)s.split_cols;
     p.ccap = make_div(s.ccap);
+    p.cstep = make_div(most * p.G.d > s.split_cols && p.G.d < s.ccap ? (int64_t)p.G.d : s.ccap);
     p.nseg = make_div(s.nseg);
     p.reqs = make_div(p.R);
     p.nc = (int32_t)s.nc;
@@ -143,7 +144,7 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   const bool whole = most * p.G.d > s.split_cols;
   p.fill_blocks = p.qstart ? 16 : 0;
   if (s.split_cols) {
-    const int64_t cols = (int64_t)p.R * p.Hkv.d * s.ccap;
+    const int64_t cols = (int64_t)p.R * p.Hkv.d * p.cstep.d;
     hipLaunchKernelGGL(k.combine, dim3((unsigned)((cols + 3) / 4 + p.fill_blocks)), dim3(256), 0,
                        st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);

@@ -715,7 +715,9 @@ __device__ void fill(const Args& p, int block) {
   }
 }
 
-// Split route: folds a column's segments; one wave per column.
+// Split route: folds a column's segments; one wave per column. Beside chunks a
+// wave takes every G-th column of a request, most of which have no more (30
+// single tokens beside two chunks 4.8 us, 10.0 with a wave per column).
 template <typename T, int D, int V>
 __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   using G = Geo<T, D, V>;
@@ -726,58 +728,65 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   }
   const int lane = threadIdx.x & 63;
   const int x = (blockIdx.x - p.fill_blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int xh = x / p.ccap, cc = x - xh * (int)p.ccap.d;
+  const int xh = x / p.cstep;
   const int r = xh / p.Hkv, kvh = xh - r * (int)p.Hkv.d;
   if (r >= p.R) return;
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
-  if (rq.beyond || ncol > p.split_cols || cc >= ncol) return;
-  // The columns that shared a workgroup, and with them its segments.
-  const int c0 = cc & -p.nc, clast = (c0 + p.nc < ncol ? c0 + p.nc : ncol) - 1;
-  const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
-  const int n = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
-  const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
-  const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
-  // Dims 2 lane, 2 lane + 1 and those 128 further; 16 segments' loads in flight.
-  constexpr int NB = 16;
-  float M = kNone, L = 0.f;
-  f32x2 O[NV] = {};
-  for (int i0 = 0; i0 < n; i0 += NB) {
-    f32x2 o[NB][NV];
-    float2 ml[NB];
+  if (rq.beyond || ncol > p.split_cols) return;
+  auto fold = [&](int cc) __attribute__((always_inline)) {
+    // The columns that shared a workgroup, and with them its segments.
+    const int c0 = cc & -p.nc, clast = (c0 + p.nc < ncol ? c0 + p.nc : ncol) - 1;
+    const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
+    const int n = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
+    const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
+    const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
+    // Dims 2 lane, 2 lane + 1 and those 128 further; 16 segments' loads in flight.
+    constexpr int NB = 16;
+    float M = kNone, L = 0.f;
+    f32x2 O[NV] = {};
+    for (int i0 = 0; i0 < n; i0 += NB) {
+      f32x2 o[NB][NV];
+      float2 ml[NB];
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-      const bool in = i0 + i < n;
-      const int64_t at = slot + (int64_t)(i0 + i) * p.ccap.d;
-      ml[i] = in ? p.pml[at] : make_float2(kNone, 0.f);
+      for (int i = 0; i < NB; i++) {
+        const bool in = i0 + i < n;
+        const int64_t at = slot + (int64_t)(i0 + i) * p.ccap.d;
+        ml[i] = in ? p.pml[at] : make_float2(kNone, 0.f);
 #pragma unroll
-      for (int j = 0; j < NV; j++)
-        o[i][j] = in && 2 * lane + 128 * j < V
-                      ? *reinterpret_cast<const f32x2*>(p.po + at * V + 2 * lane + 128 * j)
-                      : f32x2{0.f, 0.f};
+        for (int j = 0; j < NV; j++)
+          o[i][j] = in && 2 * lane + 128 * j < V
+                        ? *reinterpret_cast<const f32x2*>(p.po + at * V + 2 * lane + 128 * j)
+                        : f32x2{0.f, 0.f};
+      }
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        float fa, fb;
+        fold_base(M, L, ml[i].x, ml[i].y, fa, fb);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) O[j][k] = __builtin_fmaf(o[i][j][k], fb, O[j][k] * fa);
+      }
     }
+    float e, den;
+    finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
+           p.sinks != nullptr, e, den);
+    const float inv = inverse(den);
+    T* out = out_at<T>(p, r, rq, tok, head);
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-      float fa, fb;
-      fold_base(M, L, ml[i].x, ml[i].y, fa, fb);
-#pragma unroll
-      for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) O[j][k] = __builtin_fmaf(o[i][j][k], fb, O[j][k] * fa);
-    }
-  }
-  float e, den;
-  finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
-         p.sinks != nullptr, e, den);
-  const float inv = inverse(den);
-  T* out = out_at<T>(p, r, rq, tok, head);
-#pragma unroll
-  for (int j = 0; j < NV; j++)
-    if (2 * lane + 128 * j < V) {
-      typedef T T2 __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<T2*>(out + 2 * lane + 128 * j) =
-          T2{result<T>(O[j][0], e, inv), result<T>(O[j][1], e, inv)};
-    }
+    for (int j = 0; j < NV; j++)
+      if (2 * lane + 128 * j < V) {
+        typedef T T2 __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<T2*>(out + 2 * lane + 128 * j) =
+            T2{result<T>(O[j][0], e, inv), result<T>(O[j][1], e, inv)};
+      }
+  };
+  // (The first one apart: as the loop's body alone it took 1 us more.)
+  int cc = x - xh * (int)p.cstep.d;
+  if (cc >= ncol) return;
+  fold(cc);
+  while ((cc += p.cstep.d) < ncol) fold(cc);
 }
 
 // Whole route: NW waves of 32 columns each walk the steps that some column of

@@ -116,7 +116,7 @@ def page_tables(block_tables, context_lens, new_lens, free_pages, page_size, num
     R = context_lens.shape[0]
     _int32("new_lens", new_lens, R)
     _int32("free_pages", free_pages, None)
-    _table(block_tables)
+    row = _table(block_tables)
     if block_tables.shape[0] != R:
         raise ValueError("block_tables must have %d rows, got %d" % (R, block_tables.shape[0]))
     if page_size < 1 or num_tokens < 0:
@@ -128,10 +128,11 @@ def page_tables(block_tables, context_lens, new_lens, free_pages, page_size, num
         return PageTables(block_tables, *torch.ops.mlx_bi.page_tables(
             block_tables, context_lens, new_lens, free_pages, int(page_size), num_tokens))
     return PageTables(block_tables, *_page_tables_eager(block_tables, context_lens, new_lens,
-                                                        free_pages, page_size, num_tokens))
+                                                        free_pages, page_size, num_tokens, row))
 
 
-def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_size, num_tokens):
+def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_size, num_tokens,
+                       row=None):
     dev = context_lens.device
     _on_one_gpu("page_tables", dev, (block_tables, new_lens, free_pages))
     (R, W), T = block_tables.shape, int(num_tokens)
@@ -143,7 +144,8 @@ def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_si
     at = buf.data_ptr()
     _call(dev, "bi_page_tables", _lib.lib().bi_page_tables, block_tables.data_ptr(),
           context_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), at, at + 4 * T,
-          at + 8 * T, at + 8 * T + 4 * R + 4, at + 8 * T + 8 * R + 4, R, W, _table(block_tables),
+          at + 8 * T, at + 8 * T + 4 * R + 4, at + 8 * T + 8 * R + 4, R, W,
+          _table(block_tables) if row is None else row,
           free_pages.shape[0], T, int(page_size))
     return slots, positions, start, seq, used.view(())
 

@@ -643,3 +643,27 @@ def test_bits_where_the_base_just_moves(cuda):
     chunk = bi.window_attention(q, k, v, None, scale=math.log(2.0))
     one = bi.window_attention(q[:, :, -1:], k, v, None, scale=math.log(2.0))
     assert same(chunk[:, :, -1:], one)
+
+
+@pytest.mark.parametrize("G", [1, 3, 4, 40])
+def test_few_tokens_beside_a_chunk(cuda, G):
+    """Requests of one token and of a few beside a chunk: each has the bits that
+    it has alone."""
+    D, page, Hkv = 64, 16, 2
+    g = torch.Generator(device=cuda).manual_seed(G)
+    lens, news = [900, 1300, 5, 700, 2100], [1, 5, 5, 8, 1100 if G < 40 else 40]
+    W = -(-max(lens) // page)
+    table = torch.randperm(W * len(lens), generator=g, device=cuda).to(torch.int32).view(len(lens), W)
+    kc = torch.randn(W * len(lens), Hkv, page, D, generator=g, device=cuda).to(BF16)
+    vc = torch.randn(W * len(lens), Hkv, page, D, generator=g, device=cuda).to(BF16)
+    q = torch.randn(sum(news), Hkv * G, D, generator=g, device=cuda).to(BF16)
+    start = [0]
+    for n in news:
+        start.append(start[-1] + n)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)
+    both = bi.paged_attention(q, kc, vc, table, i32(start), i32(lens), max_query=max(news),
+                              max_seq=max(lens))
+    for r, n in enumerate(news):
+        a, b = start[r], start[r + 1]
+        one = bi.paged_attention(q[a:b], kc, vc, table[r:r + 1], i32([0, n]), i32([lens[r]]))
+        assert same(both[a:b], one), r
