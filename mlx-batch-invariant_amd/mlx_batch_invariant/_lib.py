@@ -122,6 +122,9 @@ def check(rc, what):
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# Without torch.cuda.current_device's check that the GPU is initialised: a
+# tensor on it is there already.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def launch_stream(device):
@@ -133,7 +136,7 @@ def launch_stream(device):
     (default) stream always means the current device to HIP.
     """
     idx = device.index
-    cur = torch.cuda.current_device()
+    cur = _current_device()
     if idx is None:
         idx = cur
     if _raw_stream is not None:

@@ -199,17 +199,22 @@ def paged_cache_update(k, v, k_cache, v_cache, slots):
 def _update_eager(k, v, k_cache, v_cache, slots):
     dev = k.device
     _on_one_gpu("paged_cache_update", dev, (v, k_cache, v_cache, slots))
-    if k.stride(2) != 1:
-        k = k.contiguous()
-    if v.stride(2) != 1:
-        v = v.contiguous()
     T, Hkv, D = k.shape
     P, _, page, V = v_cache.shape
     if not (T and P and Hkv and page and D and V):
         return
+    kt, kh, one = k.stride()
+    if one != 1:
+        k = k.contiguous()
+        kt, kh, _ = k.stride()
+    vt, vh, one = v.stride()
+    if one != 1:
+        v = v.contiguous()
+        vt, vh, _ = v.stride()
     slots = slots.contiguous()
-    kc, vc = k_cache.stride(), v_cache.stride()
-    st = _I64x10(*k.stride()[:2], *v.stride()[:2], *kc[:3], *vc[:3])
+    kp, kg, kr, _ = k_cache.stride()
+    vp, vg, vr, _ = v_cache.stride()
+    st = _I64x10(kt, kh, vt, vh, kp, kg, kr, vp, vg, vr)
     _call(dev, "bi_paged_update", _lib.lib().bi_paged_update, k.data_ptr(), v.data_ptr(),
           k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), T, Hkv, D, V, P, page, st,
           _lib.DTYPE_CODES[k.dtype])
