@@ -152,13 +152,21 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   }
   if (whole || p.fill_blocks) {
     // Eight waves share their keys' and values' loads and addresses where that
-    // leaves a workgroup for every compute unit (4096 tokens over 8192 keys 517
-    // -> 496 us); with fewer, four of them fill more (two chunks of 511 tokens
-    // beside 30 decodes 161 us, 175 with eight), two to a compute unit where
-    // there are more than these.
+    // leaves a workgroup for every compute unit and the walk is long (4096
+    // tokens over 8192 keys 476 us, 510 with two workgroups of four; 4096 alone
+    // 174 and 189). Over a short one a second workgroup, which starts while the
+    // first works, gains more: 2048 tokens alone 76 us with eight, 71 with
+    // twice four; 8192 under a window of 64 73 and 63, of 512 135 and 131, of
+    // 1024 197 and 201. With fewer columns four waves fill more (two chunks of
+    // 511 tokens beside 30 decodes 161 us, 175 with eight), two workgroups to a
+    // compute unit where there are more than these.
     const int64_t cols = p.qstart ? (int64_t)p.T * p.G.d : (int64_t)p.R * p.qL * p.G.d;
     const int cus = bi::device_cus();
-    const bool eight = k.whole8 && cols / 256 * p.Hkv.d >= cus;
+    // Rows that a tile walks, on average: 64 tokens see 63 more than the window.
+    const int64_t longest = p.qstart ? p.max_seq : p.N;
+    const int64_t seen = (int64_t)p.window + p.first + 63, causal = longest - most / 2;
+    const bool far = (p.window && seen < causal ? seen : causal) > 1024;
+    const bool eight = k.whole8 && far && cols / 256 * p.Hkv.d >= cus;
     const bool pair = !eight && k.whole4_pair && cols / 128 * p.Hkv.d > cus;
     const int64_t wc = eight ? 256 : 128;
     // Column tiles: every request with tokens may end in a part of one.

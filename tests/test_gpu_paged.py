@@ -302,11 +302,13 @@ def test_bits_do_not_depend_on_the_call(cuda, dtype, D, H, Hkv, window, first):
 
 @pytest.mark.parametrize("D, V", [(64, 64), (96, 96), (128, 128), (192, 128), (192, 192), (256, 256)])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-def test_bits_of_every_launch(cuda, dtype, D, V):
-    """A prompt long enough for workgroups of eight waves, one for two
-    workgroups per compute unit, a chunk with loading waves and single tokens:
-    the same rows, the same bits, over paged and contiguous keys."""
-    H, Hkv, n, window = 32, 8, 2200, 190
+@pytest.mark.parametrize("window", [190, 1100])
+def test_bits_of_every_launch(cuda, dtype, D, V, window):
+    """A prompt and, under the longer window, a walk long enough for workgroups
+    of eight waves, one for two workgroups per compute unit, a chunk with
+    loading waves and single tokens: the same rows, the same bits, over paged
+    and contiguous keys."""
+    H, Hkv, n = 32, 8, 2200
     g = torch.Generator(device=cuda).manual_seed(D + V)
     rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
     q, k, v = rn(1, H, n, D), rn(1, Hkv, n, D), rn(1, Hkv, n, V)
