@@ -40,6 +40,7 @@ struct Args {
   float* po;              // [V] each
   float2* pml;            // base and sum
   Div nseg, ccap;         // segments and columns kept per (request, kv head)
+  Div gseg;               // workgroups for a request's segments, which each takes in turn
   Div cstep;              // columns between those that a wave folds
   Div reqs;               // R
   int32_t nc;             // columns per workgroup, 16 or 32

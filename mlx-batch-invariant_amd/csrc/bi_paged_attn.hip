@@ -34,11 +34,18 @@ struct Call {
 };
 
 // How a call is split: the columns up to which a request is (0: none), columns
-// kept per request and kv head, columns per workgroup, segments, and the bytes
-// of the partial results.
+// kept per request and kv head, columns per workgroup, segments, workgroups for
+// these, and the bytes of the partial results.
 struct Plan {
-  int64_t split_cols, ccap, nc, nseg, bytes;
+  int64_t split_cols, ccap, nc, nseg, gseg, bytes;
 };
+
+// Column tiles of all requests that can have a token (one of each request is
+// not full).
+int64_t full_tiles(const Call& c, const Plan& s) {
+  const int64_t all = c.R * ((s.ccap + s.nc - 1) / s.nc), full = c.tokens * c.G / s.nc + c.R;
+  return all < full ? all : full;
+}
 
 // A plan that splits requests of up to `most` columns.
 Plan split_up_to(const Call& c, int64_t most, int64_t seg) {
@@ -56,28 +63,34 @@ Plan split_up_to(const Call& c, int64_t most, int64_t seg) {
     const int64_t n = (span + seg - 2) / seg + 1 + (c.first + seg - 1) / seg;
     if (n < s.nseg) s.nseg = n;
   }
+  // Places for a request's segments: 8192 workgroups in all, not counting
+  // columns that no token has.
+  const int64_t places = 8192 / (c.Hkv * full_tiles(c, s));
+  s.gseg = places < 1 ? 1 : places < s.nseg ? places : s.nseg;
   s.bytes = c.R * c.Hkv * s.ccap * s.nseg * (c.V + 2) * (int64_t)sizeof(float);
   return s;
 }
 int64_t split_grid(const Call& c, const Plan& s) {
-  return c.R * c.Hkv * s.nseg * ((s.ccap + s.nc - 1) / s.nc);
+  return c.R * c.Hkv * s.gseg * ((s.ccap + s.nc - 1) / s.nc);
 }
 bool fits(const Call& c, const Plan& s) {
   return s.bytes <= (int64_t)1 << 32 && split_grid(c, s) <= 1 << 23 && c.R * c.Hkv * s.ccap <= 1 << 24;
 }
 
 // Requests are split where that is estimated to take less time than to walk
-// them whole; beside chunks of more than 1024 columns those of single tokens
-// and a few (32 columns) are. Microseconds, from times of D = V = 128: a whole
-// workgroup 6 and 0.0195 a row it walks (fp32 five times that), one per compute
-// unit; a split one 5.5 and as much for a full segment, one or two per compute
-// unit; reading the cache once at 5 TB/s (whole: 3.6); the partial results' way through
-// memory and back at 4 TB/s; a launch 2, two 8. (Over 8192 rows 16 tokens
-// 161 us whole, 20.8 split, 64 166 and 58, 128 167 and 107, 256 169 and 202;
-// 64 requests of one token and 100 rows 20.1 whole, 17.4 split, one of 300 rows
-// 13.7 and 15.8.)
+// them whole; beside chunks of more than 1024 columns, and where the bounds are
+// far above the average request, those of single tokens and a few (32 columns)
+// are. Microseconds, from times of D = V = 128: a whole workgroup 6 and 0.0195
+// a row it walks (fp32 five times that), one per compute unit; a split one 5.5
+// and as much for a full segment, one or two per compute unit, an empty one
+// 3.3; reading the cache once at 5 TB/s (whole: 3.6); the partial results' way
+// through memory and back at 4 TB/s; a launch 2, two 8. (Over 8192 rows 16
+// tokens 161 us whole, 20.8 split, 64 166 and 58, 128 167 and 107, 256 169 and
+// 202; 64 requests of 16 tokens 379 and 853; 64 requests of one token and 100
+// rows 20.1 whole, 17.4 split, one of 300 rows 13.7 and 15.8. 64 single tokens
+// under a bound of 64 229, with all these columns split 1030.)
 Plan plan(const Call& c, const Kernels& k) {
-  const Plan none = {0, 0, 0, 0, 0};
+  const Plan none = {0, 0, 0, 0, 0, 0};
   const int64_t cols = c.max_query * c.G;
   if (c.R <= 0 || cols <= 0 || c.max_seq <= 0) return none;
   const int64_t few = c.G > 32 ? c.G : 32;
@@ -91,15 +104,17 @@ Plan plan(const Call& c, const Kernels& k) {
   double whole = (tiles > 1.0 ? tiles : 1.0) * (6.0 + rows * 0.0195 * wide * (c.f32 ? 2.5 : 1.0));
   whole = 2.0 + (whole > 1.4 * read ? whole : 1.4 * read);
   auto split = [&](const Plan& s) {
-    const double busy = ((double)c.tokens * c.G / s.nc + c.R) * c.Hkv * s.nseg;
-    const double grid = (double)split_grid(c, s);
-    double rounds = (grid < busy ? grid : busy) / ((s.nc == 16 && wide <= 1.0 ? 2.0 : 1.0) * cus);
+    const double busy = (double)full_tiles(c, s) * c.Hkv;
+    const double slots = (s.nc == 16 && wide <= 1.0 ? 2.0 : 1.0) * cus;
+    double rounds = busy * s.nseg / slots;
     if (rounds < 1.0) rounds = 1.0;
     const double walk = rounds * (5.5 + 5.5 * full * (wide > 1.0 ? wide : 1.0));
-    const double idle = grid > busy ? (grid - busy) / (2.0 * cus) * 1.5 : 0.0;
+    const double idle = ((double)split_grid(c, s) - busy * s.gseg) / slots * 3.3;
     return 8.0 + (walk > read ? walk : read) + (double)c.tokens * H * s.nseg * (c.V + 2) * 8.0 / 4e6 + idle;
   };
-  if (cols <= few || cols <= 1024) {
+  // Bounds far above the average request: most have a few columns.
+  const bool loose = cols > few && c.tokens * c.G <= c.R * (few / 2);
+  if (cols <= few || (cols <= 1024 && !loose)) {
     const Plan s = split_up_to(c, cols > few ? cols : few, k.seg);
     if (fits(c, s) && split(s) < whole) return s;
     if (cols <= few && whole <= split(s)) return none;
@@ -121,7 +136,7 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   const Call c = {p.R, p.qstart ? p.T : (int64_t)p.R * p.qL, p.G.d, p.Hkv.d, D, V, p.window, p.first,
                   most, p.qstart ? p.max_seq : p.N, !p.qstart, dtype == BI_F32};
   Plan s = plan(c, k);
-  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0};
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0, 0};
   hipError_t e;
   if (s.split_cols) {
     p.split_cols = (int32_t)s.split_cols;
@@ -134,7 +149,8 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.pml = reinterpret_cast<float2*>(p.po + (int64_t)p.R * p.Hkv.d * s.ccap * s.nseg * V);
     const int64_t ctiles = (s.ccap + s.nc - 1) / s.nc;
     p.ctiles = make_div(ctiles);
-    p.slots = make_div(p.R * s.nseg);
+    p.gseg = make_div(s.gseg);
+    p.slots = make_div(p.R * s.gseg);
     // (Beside larger requests split ones mostly have one column tile.)
     p.once = ctiles == 1 || most * p.G.d > s.split_cols;
     hipLaunchKernelGGL(s.nc == 16 ? k.split16 : k.split32, dim3((unsigned)split_grid(c, s)), dim3(256),

@@ -499,16 +499,16 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   const int xq = xc / (p.once ? p.slots : p.ctiles);
   const int xr = xc - xq * (int)(p.once ? p.slots : p.ctiles).d;
   const int xs = p.once ? xr : xq, c0 = (p.once ? xq : xr) * NC;
-  const int outer = xs / (p.window ? p.reqs : p.nseg);
-  const int inner = xs - outer * (int)(p.window ? p.reqs : p.nseg).d;
-  const int r = p.window ? inner : outer, part = p.window ? outer : inner;
+  const int outer = xs / (p.window ? p.reqs : p.gseg);
+  const int inner = xs - outer * (int)(p.window ? p.reqs : p.gseg).d;
+  const int r = p.window ? inner : outer, part0 = p.window ? outer : inner;
   // Without a window the walk's entries are the segments themselves, and the
   // table's entries can be on their way before the request is known.
   constexpr int PS = 4 * S, PN = G::kSeg / PS;
   int32_t entry0 = 0, entry = 0;
   if (!p.window) {
-    entry0 = entry_of(p, r, part * G::kSeg + wave * S + (lane & (S - 1)));
-    entry = entry_of(p, r, part * G::kSeg + PS + wave * S + (lane & (S - 1)));
+    entry0 = entry_of(p, r, part0 * G::kSeg + wave * S + (lane & (S - 1)));
+    entry = entry_of(p, r, part0 * G::kSeg + PS + wave * S + (lane & (S - 1)));
   }
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
@@ -517,10 +517,8 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   const int32_t lo = rq.n - rq.L + c0 / p.G, hi = rq.n - rq.L + clast / p.G;
   // The segment's passes (4 steps each) that some column sees.
   const Walk w = walk(p, lo, hi, G::kSeg);
-  if (part >= w.count()) return;  // at most p.nseg of them
-  int s0 = w.unit(part) * PN, s1 = s0 + PN;
-  while (!any_seen(p, lo, hi, s0 * PS, PS)) s0++;
-  while (!any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
+  const int parts = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
+  if (part0 >= parts) return;
 
   // Column; one without a token takes the first one's query and sees nothing.
   const int cc = c0 + col;
@@ -531,6 +529,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
   const char* kh = static_cast<const char*>(p.k) + kvh * p.kh * (int64_t)sizeof(T);
   const char* vh = static_cast<const char*>(p.v) + kvh * p.vh * (int64_t)sizeof(T);
 
+  int part = part0, s0, s1;
   // Row addresses of the wave's step of a segment; a row that no column sees,
   // or that has no page, is a row of zeros. Without branches, so that the
   // loads in flight are counted exactly.
@@ -573,122 +572,131 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel
     else load_rows(s_row[1], std::integral_constant<int, G::VCH>(), ld16);
   };
 
-  if (p.window) {
-    entry0 = entry_for(s0);
-    entry = entry_for(s0 + 1);
-  }
-  load_query<G>(query_at<T>(p, r, rq, tok, head), half, q);
-  uint64_t mapped = put_rows(s0, entry0);
-  load_keys();
-  sign_query<G>(p, q);
-
-  constexpr int TW = (G::DT + 3) / 4;  // tiles of output dims per wave
-  float m = kNone, l = 0.f;
-  f32x16 o[TW];
-#pragma unroll
-  for (int i = 0; i < TW; i++) o[i] = f32x16{};
-  for (int si = s0; si < s1; si++) {
-    const int32_t pass0 = si * PS, key0 = pass0 + wave * S;
-    const int32_t entry2 = entry_for(si + 2);
-    // Scores of the wave's step and their largest. The keys change from rows to
-    // the products' operands by way of the LDS where the wave's values go next.
-    f32x16 s[KT];
-    const int lk = opaque(lane);
-#pragma unroll
-    for (int j = 0; j < KL; j++) {
-      const int at = j * 64 + lk, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
-      st16(s_kv + wave * S * G::MCH + row * G::CH + c, x16[j]);
+  // The grid has p.gseg places for a request's segments: a few are enough
+  // where there are many workgroups, and empty ones are not free (64 requests
+  // of 250 rows under a bound of 65536 65 us, 128 with a place for each).
+  do {
+    s0 = w.unit(part) * PN, s1 = s0 + PN;
+    while (!any_seen(p, lo, hi, s0 * PS, PS)) s0++;
+    while (!any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
+    if (p.window || part != part0) {
+      entry0 = entry_for(s0);
+      entry = entry_for(s0 + 1);
     }
-    load_values();
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-      f32x16 c = {};
-#pragma unroll
-      for (int t = 0; t < G::NQ; t++)
-        c = G::score(G::key_chunk(s_kv + wave * S * G::MCH, kt, lk & 31, t, lk >> 5), q[t], c);
-      s[kt] = c;
-    }
-    const bool full = mapped == ~0ull && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
-    if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
-    const float top = G::top(s);
-    if (lane < NC) s_max[wave][lane] = top;
-    barrier();
-
-    // The bases of the pass's steps; this wave's p.
-    float base[4], f[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      base[i] = next_base(m, s_max[i][cn], p.scale2);
-      f[i] = pow2(m - base[i]);
-      m = base[i];
-    }
-    const float mw = wave == 0 ? base[0] : wave == 1 ? base[1] : wave == 2 ? base[2] : base[3];
-    uint4 pu[KT][PU];
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-      f32x16 e;
-#pragma unroll
-      for (int i = 0; i < 16; i++)
-        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -mw));
-      G::pack(e, pu[kt]);
-      if (col < NC)
-#pragma unroll
-        for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = pu[kt][j];
-    }
-    const float psum = G::sum(pu);
-    if (col < NC) s_sum[wave][half * NC + col] = psum;
-    const int ln = opaque(lane);
-#pragma unroll
-    for (int j = 0; j < VL; j++) {
-      const int at = j * 64 + ln, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
-      st16(s_kv + wave * S * G::MCH + row * G::VCH + c, x16[j]);
-    }
-    mapped = put_rows(si + 1, entry);
-    entry = entry2;
+    load_query<G>(query_at<T>(p, r, rq, tok, head), half, q);
+    uint64_t mapped = put_rows(s0, entry0);
     load_keys();
-    barrier();
+    sign_query<G>(p, q);
 
-    // The sum, and the wave's tiles of output dims over the pass's steps.
+    constexpr int TW = (G::DT + 3) / 4;  // tiles of output dims per wave
+    float m = kNone, l = 0.f;
+    f32x16 o[TW];
 #pragma unroll
-    for (int i = 0; i < 4; i++) l = __builtin_fmaf(l, f[i], s_sum[i][half * NC + cn]);
+    for (int i = 0; i < TW; i++) o[i] = f32x16{};
+    for (int si = s0; si < s1; si++) {
+      const int32_t pass0 = si * PS, key0 = pass0 + wave * S;
+      const int32_t entry2 = entry_for(si + 2);
+      // Scores of the wave's step and their largest. The keys change from rows to
+      // the products' operands by way of the LDS where the wave's values go next.
+      f32x16 s[KT];
+      const int lk = opaque(lane);
 #pragma unroll
-    for (int x = 0; x < TW; x++) {
-      const int dt = wave + 4 * x;
-      if (dt >= G::DT) break;
+      for (int j = 0; j < KL; j++) {
+        const int at = j * 64 + lk, row = at / G::CH, c = (at - row * G::CH) ^ G::kswz(row);
+        st16(s_kv + wave * S * G::MCH + row * G::CH + c, x16[j]);
+      }
+      load_values();
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++) {
+        f32x16 c = {};
+#pragma unroll
+        for (int t = 0; t < G::NQ; t++)
+          c = G::score(G::key_chunk(s_kv + wave * S * G::MCH, kt, lk & 31, t, lk >> 5), q[t], c);
+        s[kt] = c;
+      }
+      const bool full = mapped == ~0ull && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
+      if (!full) G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
+      const float top = G::top(s);
+      if (lane < NC) s_max[wave][lane] = top;
+      barrier();
+
+      // The bases of the pass's steps; this wave's p.
+      float base[4], f[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if (!any_seen(p, lo, hi, pass0 + i * S, S)) continue;
-        if (__builtin_amdgcn_ballot_w64(f[i] != 1.f) != 0)
+        base[i] = next_base(m, s_max[i][cn], p.scale2);
+        f[i] = pow2(m - base[i]);
+        m = base[i];
+      }
+      const float mw = wave == 0 ? base[0] : wave == 1 ? base[1] : wave == 2 ? base[2] : base[3];
+      uint4 pu[KT][PU];
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[x][e] *= f[i];
+      for (int kt = 0; kt < KT; kt++) {
+        f32x16 e;
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-          uint4 u[PU];
+        for (int i = 0; i < 16; i++)
+          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -mw));
+        G::pack(e, pu[kt]);
+        if (col < NC)
 #pragma unroll
-          for (int j = 0; j < PU; j++) u[j] = s_p[((i * KT + kt) * PU + j) * 2 * NC + (ln >> 5) * NC + (ln & (NC - 1))];
+          for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = pu[kt][j];
+      }
+      const float psum = G::sum(pu);
+      if (col < NC) s_sum[wave][half * NC + col] = psum;
+      const int ln = opaque(lane);
 #pragma unroll
-          for (int j = 0; j < PU; j++)
-            o[x] = G::score(G::value(s_kv + i * S * G::MCH, kt * 32, j, dt, ln), u[j], o[x]);
+      for (int j = 0; j < VL; j++) {
+        const int at = j * 64 + ln, row = at / G::VCH, c = (at - row * G::VCH) ^ G::vswz(row);
+        st16(s_kv + wave * S * G::MCH + row * G::VCH + c, x16[j]);
+      }
+      mapped = put_rows(si + 1, entry);
+      entry = entry2;
+      load_keys();
+      barrier();
+
+      // The sum, and the wave's tiles of output dims over the pass's steps.
+#pragma unroll
+      for (int i = 0; i < 4; i++) l = __builtin_fmaf(l, f[i], s_sum[i][half * NC + cn]);
+#pragma unroll
+      for (int x = 0; x < TW; x++) {
+        const int dt = wave + 4 * x;
+        if (dt >= G::DT) break;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if (!any_seen(p, lo, hi, pass0 + i * S, S)) continue;
+          if (__builtin_amdgcn_ballot_w64(f[i] != 1.f) != 0)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[x][e] *= f[i];
+#pragma unroll
+          for (int kt = 0; kt < KT; kt++) {
+            uint4 u[PU];
+#pragma unroll
+            for (int j = 0; j < PU; j++) u[j] = s_p[((i * KT + kt) * PU + j) * 2 * NC + (ln >> 5) * NC + (ln & (NC - 1))];
+#pragma unroll
+            for (int j = 0; j < PU; j++)
+              o[x] = G::score(G::value(s_kv + i * S * G::MCH, kt * 32, j, dt, ln), u[j], o[x]);
+          }
         }
       }
+      barrier();  // everyone is done with the values and p
     }
-    barrier();  // everyone is done with the values and p
-  }
 
-  l = half_swap_sum(l);
-  if (!cv) return;
-  const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + cc;
-  if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
+    l = half_swap_sum(l);
+    if (cv) {
+      const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + cc;
+      if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
 #pragma unroll
-  for (int x = 0; x < TW; x++) {
-    if (wave + 4 * x >= G::DT) break;
-    float* to = p.po + slot * V + 32 * (wave + 4 * x);
+      for (int x = 0; x < TW; x++) {
+        if (wave + 4 * x >= G::DT) break;
+        float* to = p.po + slot * V + 32 * (wave + 4 * x);
 #pragma unroll
-    for (int b = 0; b < 4; b++)
-      *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
-          f32x4{o[x][4 * b], o[x][4 * b + 1], o[x][4 * b + 2], o[x][4 * b + 3]};
-  }
+        for (int b = 0; b < 4; b++)
+          *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
+              f32x4{o[x][4 * b], o[x][4 * b + 1], o[x][4 * b + 2], o[x][4 * b + 3]};
+      }
+    }
+  } while ((part += p.gseg.d) < parts);
 }
 
 // Tokens that no kernel computes: 0 where no request owns them, NaN where the

@@ -669,3 +669,26 @@ def test_few_tokens_beside_a_chunk(cuda, G):
         a, b = start[r], start[r + 1]
         one = bi.paged_attention(q[a:b], kc, vc, table[r:r + 1], i32([0, n]), i32([lens[r]]))
         assert same(both[a:b], one), r
+
+
+@pytest.mark.parametrize("window", [None, 40000])
+def test_many_segments_of_many_requests(cuda, window):
+    """More segments than the launch has places for: a workgroup takes several.
+    The bits are those of the long request alone, which has a place for each."""
+    D, page, Hkv, R, n = 64, 256, 2, 60, 60000
+    g = torch.Generator(device=cuda).manual_seed(3)
+    W = -(-n // page)
+    table = torch.full((R, W), -1, dtype=torch.int32, device=cuda)
+    table[17] = torch.randperm(W, generator=g, device=cuda).to(torch.int32)
+    table[:17, 0] = table[18:, 0] = 5
+    kc = torch.randn(W, Hkv, page, D, generator=g, device=cuda).to(BF16)
+    vc = torch.randn(W, Hkv, page, D, generator=g, device=cuda).to(BF16)
+    q = torch.randn(R, 2 * Hkv, D, generator=g, device=cuda).to(BF16)
+    lens = torch.randint(0, 200, (R,), generator=g, device=cuda, dtype=torch.int32)
+    lens[17] = n
+    kw = dict(window=window, sink_tokens=700)
+    both = bi.paged_attention(q, kc, vc, table, ref.starts([1] * R, cuda), lens, max_query=1, **kw)
+    for r in (17, 3, 59):
+        one = bi.paged_attention(q[r:r + 1], kc, vc, table[r:r + 1], ref.starts([1], cuda),
+                                 lens[r:r + 1].clone(), **kw)
+        assert same(both[r:r + 1], one), r
