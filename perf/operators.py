@@ -26,18 +26,13 @@ BYTES = {"bf16": 2, "f16": 2, "f32": 4}
 HEADS = ((32, 8), (32, 8), (16, 8), (8, 8), (32, 4))
 
 
-_package = None
-
-
 def _bi():
-    """The package of the tree that is the working folder."""
-    global _package
-    if _package is None:
-        sys.path.insert(0, os.path.abspath("mlx-batch-invariant_amd"))
-        import mlx_batch_invariant
+    path = os.path.abspath("mlx-batch-invariant_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import mlx_batch_invariant
 
-        _package = mlx_batch_invariant
-    return _package
+    return mlx_batch_invariant
 
 
 # -------------------------------------------------------------------- cases
