@@ -43,14 +43,17 @@ DEVICE_FLAGS = [
     "-Wno-unused-command-line-argument",
 ]
 
-# The quantized GEMM and the MFMA attention work on MFMA results with VALU
+# The quantized GEMM and the attention kernels work on MFMA results with VALU
 # arithmetic (group folds; softmax and rescaling); with the results in
 # accumulation registers every such step would copy them out and back. This
-# keeps MFMA operands and results in VGPRs.
+# keeps MFMA operands and results in VGPRs. (Paged attention of V = 192 and 256,
+# whose accumulators exceed 256 registers, copied up to 256 of them twice a step
+# without it, and 32-bit V = 256 kept 70 in scratch memory; with it only what a
+# step does not use waits in accumulation registers.)
 EXTRA_FLAGS = {
     "bi_qgemm_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "bi_qgemm_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-    **{u: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for u in SDPA_MFMA_UNITS},
+    **{u: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for u in SDPA_MFMA_UNITS + PAGED_UNITS},
 }
 
 
