@@ -180,6 +180,8 @@ def serve_step(model, cache, ids, new):
     from . import paged_attention, paged_cache_update
 
     c = model.c
+    if ids.ndim != 1 or ids.shape[0] != sum(new) or not ids.shape[0]:
+        raise ValueError("expected %d ids, one or more, got %s" % (sum(new), tuple(ids.shape)))
     t, most, longest = cache.begin(new)
     x = model.embed(ids)
     T = x.shape[0]
