@@ -171,6 +171,16 @@ class PagedCache:
         self.lens = after
         return t, max(new), max(after)
 
+    def release(self, request):
+        """Ends a request: its pages are free again and its row, empty, is
+        another's. Steps that were launched before still read what was there
+        (the pages change hands in the stream's order)."""
+        n = -(-self.lens[request] // self.page_size)
+        self.free[self.used - n:self.used] = self.tables[request, :n]
+        self.tables[request] = -1
+        self.used -= n
+        self.lens[request] = 0
+
 
 def serve_step(model, cache, ids, new):
     """One step over `cache`: ids (sum of new,) are the new tokens, new[r] of
