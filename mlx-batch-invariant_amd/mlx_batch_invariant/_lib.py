@@ -127,16 +127,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _after_fork():
-    """A forked child has its parent's tensors but no GPU: there the check comes
-    first again, with torch's own error."""
-    global _current_device
-    _current_device = torch.cuda.current_device
-
-
-os.register_at_fork(after_in_child=_after_fork)
-
-
 def launch_stream(device):
     """(stream handle as int, needs_device_switch) for a launch on `device`.
 
