@@ -122,8 +122,8 @@ def check(rc, what):
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-# Without torch.cuda.current_device's check that the GPU is initialised: a
-# tensor on it is there already.
+# torch.cuda.current_device without its steps in Python. (The check that the GPU
+# is initialised is in the call itself, a forked child's error too.)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
