@@ -197,7 +197,8 @@ int bi_qgemm(const void* x, const void* w, const void* scales, const void* biase
  *                pages do not reach. No other entry is written. Rows past
  *                W * page_size have no page.
  *   slots        (T) page * page_size + row of every new token, -1 for one
- *                without a page and behind the last token
+ *                without a page (or one so far out that this passes 31 bits)
+ *                and behind the last token
  *   positions    (T) its row in the request, -1 behind the last token
  *   query_start  (R + 1) first token of every request, and their number
  *   seq_lens     (R) context_lens + new_lens

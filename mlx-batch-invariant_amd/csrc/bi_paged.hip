@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(TablesArgs p) {
         }
       }
       if (t < p.T) {
-        p.slots[t] = id < 0 ? -1 : (int32_t)((uint32_t)id * p.page.d + row);
+        // (An entry that is no page of any cache has no slot, rather than another's.)
+        const uint64_t slot = (uint64_t)(uint32_t)id * p.page.d + row;
+        p.slots[t] = id < 0 || slot > INT32_MAX ? -1 : (int32_t)slot;
         p.positions[t] = (int32_t)pos;
       }
     }
