@@ -45,7 +45,7 @@ struct Args {
   Div reqs;               // R
   int32_t nc;             // columns per workgroup, 16 or 32
   Div ctiles;             // workgroups of them
-  Div slots;              // R * nseg
+  Div slots;              // R * gseg
   int32_t once;           // keys and values are read by one of these only
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
@@ -59,7 +59,12 @@ struct Kernels {
   // CU (the last two where the registers allow two waves per SIMD, else NULL).
   Kernel whole4, whole8, whole4_pair;
   int whole4_threads;       // its loading waves among them
-  int seg;                  // rows per segment
+  int seg, pass;            // rows per segment and per pass of the split route (four steps)
+  // For the choice of route, in microseconds: what a row costs a whole
+  // workgroup, and a full segment the split ones of 16 and 32 columns that a
+  // CU runs together, per_cu of them.
+  double row_us, seg16_us, seg32_us;
+  int per_cu16, per_cu32;
 };
 
 #define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)

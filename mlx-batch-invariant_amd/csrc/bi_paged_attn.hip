@@ -78,43 +78,68 @@ bool fits(const Call& c, const Plan& s) {
 }
 
 // Requests are split where that is estimated to take less time than to walk
-// them whole; beside chunks of more than 1024 columns, and where the bounds are
+// them whole; beside chunks of more than 2048 columns, and where the bounds are
 // far above the average request, those of single tokens and a few (32 columns)
-// are. Microseconds, from times of D = V = 128: a whole workgroup 6 and 0.0195
-// a row it walks (fp32 five times that), one per compute unit; a split one 5.5
-// and as much for a full segment, one or two per compute unit, an empty one
-// 3.3; reading the cache once at 5 TB/s (whole: 3.6); the partial results' way
-// through memory and back at 4 TB/s; a launch 2, two 8. (Over 8192 rows 16
-// tokens 161 us whole, 20.8 split, 64 166 and 58, 128 167 and 107, 256 169 and
-// 202; 64 requests of 16 tokens 379 and 853; 64 requests of one token and 100
-// rows 20.1 whole, 17.4 split, one of 300 rows 13.7 and 15.8. 64 single tokens
-// under a bound of 64 229, with all these columns split 1030.)
+// are. Microseconds, from times of every head dim and type (prices of a row and
+// of a segment: Geo in bi_paged_attn_kernel.h): a whole workgroup 7.5 and the
+// rows it walks, one per compute unit at a time; the split ones that a compute
+// unit runs together as much as a full segment costs, half of it for a segment
+// and half by its passes of four steps (0.85 of it for one alone where two fit;
+// 0.4 of a round more, as the last is rarely full), an empty one 3.3; reading
+// the cache once at 5 TB/s; the partial results' way through memory and back at
+// 4 TB/s; a launch 2, two with their chain 10. Tokens of a chunk see all but
+// half of the chunk's rows on average. (whole / split, 32/8 heads: bf16, D = V =
+// 128, over 8192 rows 16 tokens 157 / 21.5, 64 162 / 59, 128 164 / 107, 256 163
+// / 199; 64 requests of one token and 300 rows 31.8 / 27.8, 32 of 16 and 1024
+// 33.3 / 70.6; 16 under a window of 1024 33.9 / 23.0, of 512 21.5 / 19.5, 64 of
+// 512 43.1 / 44.0. 64/64, 128 tokens over 8192 rows 125 / 55; 256/256, 256 513 /
+// 344, 512 513 / 659. fp32, 128/128, 64 requests of 2048 rows 570 / 284, 256
+// tokens over 4096 rows 559 / 368, 512 559 / 670; 256/256, 1000 tokens of a
+// prompt, 8/8 heads 331 / 124. Of 822 sizes timed both ways it picks the one
+// that takes 8 % more or worse four times, 29 % at most. 64 single tokens under a
+// bound of 64 229, with all these columns split 1030.)
 Plan plan(const Call& c, const Kernels& k) {
   const Plan none = {0, 0, 0, 0, 0, 0};
   const int64_t cols = c.max_query * c.G;
   if (c.R <= 0 || cols <= 0 || c.max_seq <= 0) return none;
   const int64_t few = c.G > 32 ? c.G : 32;
-  const double cus = bi::device_cus(), wide = (double)(c.D + c.V) / 256.0 * (c.f32 ? 2.0 : 1.0);
-  const double H = (double)(c.G * c.Hkv);
-  double rows = (double)c.max_seq;
-  if (c.window && (double)(c.window + c.first) < rows) rows = (double)(c.window + c.first);
-  const double full = rows < (double)k.seg ? rows / (double)k.seg : 1.0;
-  const double tiles = ((double)c.tokens * c.G / 128.0 + c.R) * c.Hkv / cus;
+  const double cus = bi::device_cus(), H = (double)(c.G * c.Hkv), seq = (double)c.max_seq;
+  // Rows that a token sees at most; `cut`: under a window.
+  const double wide = (double)(c.window + c.first);
+  const bool cut = c.window && wide < seq;
+  const double rows = cut ? wide : seq;
+  const double chunk = (double)(c.max_query < c.max_seq ? c.max_query : c.max_seq);
   const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * (c.f32 ? 4.0 : 2.0) / 5e6;
-  double whole = (tiles > 1.0 ? tiles : 1.0) * (6.0 + rows * 0.0195 * wide * (c.f32 ? 2.5 : 1.0));
-  whole = 2.0 + (whole > 1.4 * read ? whole : 1.4 * read);
+  const double all = (double)c.R * ((cols + 127) / 128), full = (double)c.tokens * c.G / 128.0 + c.R;
+  const double tiles = (all < full ? all : full) * c.Hkv / cus;
+  const double walked = (cut ? rows + 128.0 / c.G + 64.0 : rows) * k.row_us;
+  const double first = 7.5 + walked, most = tiles * (7.5 + walked * (cut ? 1.0 : 1.0 - 0.5 * chunk / seq));
+  double whole = first > most ? first : most;
+  whole = 2.0 + (whole > 1.1 * read ? whole : 1.1 * read);
   auto split = [&](const Plan& s) {
-    const double busy = (double)full_tiles(c, s) * c.Hkv;
-    const double slots = (s.nc == 16 && wide <= 1.0 ? 2.0 : 1.0) * cus;
-    double rounds = busy * s.nseg / slots;
-    if (rounds < 1.0) rounds = 1.0;
-    const double walk = rounds * (5.5 + 5.5 * full * (wide > 1.0 ? wide : 1.0));
-    const double idle = ((double)split_grid(c, s) - busy * s.gseg) / slots * 3.3;
-    return 8.0 + (walk > read ? walk : read) + (double)c.tokens * H * s.nseg * (c.V + 2) * 8.0 / 4e6 + idle;
+    const double busy = (double)full_tiles(c, s) * c.Hkv, n = (double)s.nseg;
+    const int per_cu = s.nc == 16 ? k.per_cu16 : k.per_cu32;
+    const double slots = per_cu * cus, seg = s.nc == 16 ? k.seg16_us : k.seg32_us;
+    // Segments and passes of a column tile, on average under a window, which
+    // begins and ends inside of them.
+    const double span = rows + (double)s.nc / c.G - 1.0, more = c.first ? 2.0 : 1.0;
+    double segs = cut ? span / k.seg + more : n, passes = cut ? span / k.pass + more : ceil(seq / k.pass);
+    const double in = (double)(k.seg / k.pass);
+    if (segs > n) segs = n;
+    if (passes > n * in) passes = n * in;
+    const double later = seq > k.seg ? 1.0 - k.seg / seq : 0.0, mean = cut ? 1.0 : 1.0 - 0.5 * chunk / seq * later;
+    const double rounds = busy * 0.5 * (segs + passes / in) / slots * mean;
+    const double part = rows < k.seg ? rows / k.seg : 1.0;
+    const double alone = (0.5 + 0.5 * part) * (per_cu == 2 ? 0.85 : 1.0);
+    double walk = rounds + (rounds < 1.0 ? 0.4 * rounds : 0.4);
+    walk = (walk > alone ? walk : alone) * seg;
+    const double idle = ((double)split_grid(c, s) - busy * s.gseg * mean) / slots * 3.3;
+    return 10.0 + (walk > 0.9 * read ? walk : 0.9 * read) +
+           (double)c.tokens * H * segs * (c.V + 2) * 8.0 / 4e6 + idle;
   };
   // Bounds far above the average request: most have a few columns.
   const bool loose = cols > few && c.tokens * c.G <= c.R * (few / 2);
-  if (cols <= few || (cols <= 1024 && !loose)) {
+  if (cols <= few || (cols <= 2048 && !loose)) {
     const Plan s = split_up_to(c, cols > few ? cols : few, k.seg);
     if (fits(c, s) && split(s) < whole) return s;
     if (cols <= few && whole <= split(s)) return none;

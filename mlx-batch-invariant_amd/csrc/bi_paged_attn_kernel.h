@@ -280,8 +280,32 @@ struct Geo {
   static constexpr bool kTwoWaves = V + 4 * NQ <= 192;
   static constexpr int kStepBytes = kStep * (CH + VCH) * 16;
   static constexpr int kDeep = kStepBytes <= 32768 ? 4 : 3;
-  // Split workgroups per CU: 64 KB of values (4 steps) and their p twice fit its LDS.
-  static constexpr int kSplitPerCu = 4 * kStep * MCH > 4096 ? 1 : 2;
+  // Split workgroups of NC columns per CU: two where its 160 KB of LDS hold their
+  // values (4 steps), p, row addresses, largest scores and sums twice.
+  static constexpr int split_per_cu(int NC) {
+    return 4 * kStep * MCH * 16 + 4 * KT * PU * 2 * NC * 16 + 2 * 4 * kStep * 8 + 4 * 3 * NC * 4 <= 81920 ? 2 : 1;
+  }
+  // Times for the choice of route, microseconds, fitted to both routes of every
+  // head dim at two head layouts and 19 sizes (one to 64 requests of one to
+  // 2048 tokens over 300 to 8192 rows). A row of a whole workgroup's walk: over
+  // 8192 rows 16-bit 15.3, 18.6, 20.0, 31.7, 53.2 and 62.5 ns for 64/64, 96/96,
+  // 128/128, 192/128, 192/192 and 256/256, fp32 (4096 rows) 68, 108, 136, 195,
+  // 248 and 317: the products and, for 16 bits, the exponentials, more where
+  // steps are of 32 rows, and twice that where one wave per SIMD has nothing
+  // beside it.
+  static constexpr double row_us() {
+    return 1e-3 * (E == 4 ? 0.53 * (D + V) * (kTwoWaves ? 1.0 : 1.17)
+                   : kTwoWaves ? (10.8 + 0.0345 * (D + V)) * (kStep == 64 ? 1.0 : 1.45)
+                               : 26.0 + 0.071 * (D + V));
+  }
+  // A full segment's workgroups that a CU runs together, by the segment's size
+  // (64 to 256 KB): 16-bit 10.8, 12.5, 11.8, 13.2, 16.2 and 20.3 us for the same
+  // head dims at 32 columns, fp32 12.2, 14.3, 11.5, 14.1, 17.7 and 22.5, with
+  // what their results cost.
+  static constexpr double seg_us(int NC) {
+    const double kb = kSeg * (D + V) * E / 1024.0;
+    return E == 4 ? (3.0 + 0.06 * kb) * (split_per_cu(NC) == 2 ? 1.3 : 1.0) : 5.5 + 0.023 * kb;
+  }
 
   // The lane's chunk pair t of keys and query: one product (fp32: four).
   __device__ __forceinline__ static f32x16 score(uint4 k, uint4 q, f32x16 c) {
@@ -476,7 +500,7 @@ __device__ __forceinline__ T* out_at(const Args& p, int r, const Request& rq, in
 // lines in the caches. (32 loads a wave in flight, keys and values together,
 // were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
 template <typename T, int D, int V, int NC>
-__global__ void __launch_bounds__(256, (Geo<T, D, V>::kSplitPerCu)) split_kernel(Args p) {
+__global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_kernel(Args p) {
   using G = Geo<T, D, V>;
   constexpr int S = G::kStep, KT = G::KT, PU = G::PU;
   __shared__ uint4 s_kv[4 * S * G::MCH];  // a step per wave: its keys, then its values
@@ -1125,8 +1149,11 @@ Kernels kernels_of() {
   k.split16 = split_kernel<T, D, V, 16>;
   k.split32 = split_kernel<T, D, V, 32>;
   k.combine = combine_kernel<T, D, V>;
-  k.seg = Geo<T, D, V>::kSeg;
   using G = Geo<T, D, V>;
+  k.seg = G::kSeg, k.pass = 4 * G::kStep;
+  k.row_us = G::row_us();
+  k.seg16_us = G::seg_us(16), k.seg32_us = G::seg_us(32);
+  k.per_cu16 = G::split_per_cu(16), k.per_cu32 = G::split_per_cu(32);
   if constexpr (G::kTwoWaves) {
     k.whole4 = whole_kernel<T, D, V, 4, 4, G::kDeep>;
     k.whole4_pair = whole_kernel<T, D, V, 4, 0, 2>;
