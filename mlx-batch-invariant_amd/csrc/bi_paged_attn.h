@@ -54,6 +54,7 @@ struct Args {
 typedef void (*Kernel)(Args);
 struct Kernels {
   Kernel split16, split32;  // 16 or 32 columns per workgroup
+  Kernel split16_one, split32_one;  // where no request has more than one token
   Kernel combine;
   // 4 or 8 waves of 32 columns per workgroup, one to a CU, or 4 waves two to a
   // CU (the last two where the registers allow two waves per SIMD, else NULL).

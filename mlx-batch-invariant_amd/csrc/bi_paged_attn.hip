@@ -178,8 +178,9 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.slots = make_div(p.R * s.gseg);
     // (Beside larger requests split ones mostly have one column tile.)
     p.once = ctiles == 1 || most * p.G.d > s.split_cols;
-    hipLaunchKernelGGL(s.nc == 16 ? k.split16 : k.split32, dim3((unsigned)split_grid(c, s)), dim3(256),
-                       0, st, p);
+    const Kernel split = most > 1 ? (s.nc == 16 ? k.split16 : k.split32)
+                                  : (s.nc == 16 ? k.split16_one : k.split32_one);
+    hipLaunchKernelGGL(split, dim3((unsigned)split_grid(c, s)), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   const bool whole = most * p.G.d > s.split_cols;

@@ -30,6 +30,13 @@
 // A step or segment that a column sees nothing of leaves it as it is, so which
 // of them a workgroup walks for its other columns changes no bits (a zero's
 // sign would: hence the + 0.0).
+// A value row that only some of a workgroup's tokens see is loaded, and p = 0
+// times an infinity or NaN in it would be NaN for the others. The values of the
+// steps that not all tokens see whole (a prompt's diagonal, a window's ends) are
+// looked at as they pass; where one of them is infinite or NaN, the workgroup
+// computes its tokens once more one by one (token_segment). The look costs 4096
+// tokens over 8192 rows 420 -> 425 us, prompts of 8192 tokens under a window of
+// 1024 190 -> 193, of 64 62.7 -> 65.7.
 //
 // Two routes, the same bits:
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment),
@@ -406,6 +413,14 @@ struct Geo {
     return s[0];
   }
 
+  // Sums of these over any elements have a bit of kOdd set if one of them is an
+  // infinity or NaN.
+  static constexpr uint32_t kExp = E == 4 ? 0x7F800000u : __is_same(T, __bf16) ? 0x7F807F80u : 0x7C007C00u;
+  static constexpr uint32_t kOne = E == 4 ? 0x00800000u : __is_same(T, __bf16) ? 0x00800080u : 0x04000400u;
+  static constexpr uint32_t kOdd = E == 4 ? 0x80000000u : 0x80008000u;
+  __device__ __forceinline__ static uint32_t odd(uint4 x) {
+    return ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
+  }
   // Values in LDS: row r's chunk c at chunk c ^ vswz(r). A transposing read
   // takes 4 consecutive rows, 64 bytes each, per pass (32 lanes of 8 bytes);
   // the exchange puts these in different quarters of the 64 banks. (Rows of
@@ -490,6 +505,119 @@ __device__ __forceinline__ T* out_at(const Args& p, int r, const Request& rq, in
   return static_cast<T*>(p.out) + off + head * p.oh;
 }
 
+// The lane's number, not taken from a register that the caller would keep for it.
+__device__ __forceinline__ int lane_anew() {
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, opaque(0)));
+}
+// Column c's (m, l of its lane half, o of the dims 32 dt ..) over one segment, by
+// one wave whose lanes hold the columns of one token: the arithmetic of the
+// kernels below with zeros for every row that the token does not see, for
+// tokens beside others that see a row of values with an infinity or NaN. (Slow
+// and rare: it keeps little in registers.) `lds`: 32 rows of values.
+template <typename T, int D, int V>
+__device__ __forceinline__ f32x16 token_segment(const Args& p, int r, const Request& rq, int kvh, int c, int dt,
+                                                int segment, uint4* lds, float& m, float& l) {
+  using G = Geo<T, D, V>;
+  constexpr int S = G::kStep, KT = G::KT, PU = G::PU;
+  const int lane = lane_anew(), half = lane >> 5;
+  const int token = c / p.G;
+  const int32_t pos = rq.n - rq.L + token;
+  const char* q = query_at<T>(p, r, rq, token, kvh * (int)p.G.d + c - token * (int)p.G.d);
+  auto row_at = [&](const void* base, int64_t page, int64_t head, int64_t row, int32_t key)
+      __attribute__((always_inline)) -> const char* {
+    const int32_t id = any_seen(p, pos, pos, key, 1) ? page_of(p, r, entry_of(p, r, key), key) : -1;
+    const char* at = static_cast<const char*>(base) +
+                     (kvh * head + id * page + row_of(p, key) * row) * (int64_t)sizeof(T);
+    return id >= 0 ? at : reinterpret_cast<const char*>(g_zero_row);
+  };
+  m = kNone, l = 0.f;
+  f32x16 o = {};
+#pragma unroll 1
+  for (int32_t key0 = segment * G::kSeg; key0 < (segment + 1) * G::kSeg; key0 += S) {
+    if (!any_seen(p, pos, pos, key0, S)) continue;
+    f32x16 s[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) {
+      const char* k = row_at(p.k, p.kb, p.kh, p.kn, key0 + 32 * kt + (lane & 31));
+      s[kt] = f32x16{};
+#pragma unroll 1
+      for (int t = 0; t < G::NQ; t++) {
+        uint4 x = ld16(q + (2 * t + half) * 16);
+        x = make_uint4(x.x ^ p.qsign, x.y ^ p.qsign, x.z ^ p.qsign, x.w ^ p.qsign);
+        s[kt] = G::score(ld16(k + (2 * t + half) * 16), x, s[kt]);
+      }
+    }
+    const int32_t key = key0 + (lane & (S - 1));
+    const uint64_t mapped = __builtin_amdgcn_ballot_w64(page_of(p, r, entry_of(p, r, key), key) >= 0);
+    G::hide(s, seen_bits(p, pos, key0, mapped) >> (4 * half));
+    const float base = next_base(m, G::top(s), p.scale2), f = pow2(m - base);
+    m = base;
+    uint4 pu[KT][PU];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) {
+      f32x16 e;
+#pragma unroll
+      for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], p.scale2, -m));
+      G::pack(e, pu[kt]);
+    }
+    l = __builtin_fmaf(l, f, G::sum(pu));
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[i] *= f;
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) {
+#pragma unroll 1
+      for (int at = lane; at < 32 * G::VCH; at += 64) {
+        const int row = at / G::VCH, chunk = at - row * G::VCH;
+        const char* v = row_at(p.v, p.vb, p.vh, p.vn, key0 + 32 * kt + row);
+        st16(lds + row * G::VCH + (chunk ^ G::vswz(row)), ld16(v + chunk * 16));
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int u = 0; u < PU; u++) o = G::score(G::value(lds, 0, u, dt, lane), pu[kt][u], o);
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  return o;
+}
+// Runs use(column, valid) for the columns c0 .. clast of a token, 32 lanes at a
+// time; a lane without one has the first one's.
+template <typename Use>
+__device__ __forceinline__ void for_columns(const Args& p, int token, int c0, int clast, const Use& use) {
+  const int lane = lane_anew() & 31;
+  const int first = token * (int)p.G.d, end = first + (int)p.G.d <= clast ? first + (int)p.G.d : clast + 1;
+  for (int c = first < c0 ? c0 : first; c < end; c += 32) use(c + lane < end ? c + lane : c, c + lane < end);
+}
+// A token's columns c0 .. clast, output dims 32 dt .., of all segments.
+template <typename T, int D, int V>
+__device__ __forceinline__ void walk_token(const Args& p, int r, const Request& rq, int kvh, int token, int dt, int c0, int clast,
+                           uint4* lds) {
+  using G = Geo<T, D, V>;
+  const int half = lane_anew() >> 5;
+  const int32_t pos = rq.n - rq.L + token;
+  const Walk w = walk(p, pos, pos, G::kSeg);
+  for_columns(p, token, c0, clast, [&](int c, bool valid) __attribute__((always_inline)) {
+    float M = kNone, L = 0.f;
+    f32x16 O = {};
+#pragma unroll 1
+    for (int i = 0; i < w.count(); i++) {
+      float m, l, fa, fb;
+      const f32x16 o = token_segment<T, D, V>(p, r, rq, kvh, c, dt, w.unit(i), lds, m, l);
+      fold_base(M, L, m, half_swap_sum(l), fa, fb);
+#pragma unroll
+      for (int e = 0; e < 16; e++) O[e] = __builtin_fmaf(o[e], fb, O[e] * fa);
+    }
+    const int head = kvh * (int)p.G.d + c - token * (int)p.G.d;
+    float e, den;
+    finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
+           p.sinks != nullptr, e, den);
+    const float inv = inverse(den);
+    T* out = out_at<T>(p, r, rq, token, head);
+    if (valid)
+#pragma unroll
+      for (int i = 0; i < 16; i++) out[32 * dt + G::row(i, half)] = result<T>(O[i], e, inv);
+  });
+}
+
 // Split route: a segment's (m, l, o) of NC columns, four steps to a pass, one
 // per wave. What bounds it is reading the cache, which it does 64 KB at a
 // time: a step's values are on their way while its scores are computed, the
@@ -499,7 +627,9 @@ __device__ __forceinline__ T* out_at(const Args& p, int r, const Request& rq, in
 // TB/s); this kernel and its fold take 390, 410 with loads that keep their
 // lines in the caches. (32 loads a wave in flight, keys and values together,
 // were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
-template <typename T, int D, int V, int NC>
+// ONE: no request has more than one token, so that no row is seen by some only
+// (the code for these costs one request of 8192 rows 1.3 us of 18.4, 64 1.7 %).
+template <typename T, int D, int V, int NC, bool ONE>
 __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_kernel(Args p) {
   using G = Geo<T, D, V>;
   constexpr int S = G::kStep, KT = G::KT, PU = G::PU;
@@ -508,6 +638,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
   __shared__ const char* s_row[2][4 * S];
   __shared__ float s_max[4][NC];
   __shared__ float s_sum[4][2 * NC];
+  __shared__ int s_odd[2];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5, cn = col & (NC - 1);
@@ -543,6 +674,9 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
   const Walk w = walk(p, lo, hi, G::kSeg);
   const int parts = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
   if (part0 >= parts) return;
+  const bool several = !ONE && lo != hi;  // tokens, which may see different rows
+  if (several && threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  int turn = 0;
 
   // Column; one without a token takes the first one's query and sees nothing.
   const int cc = c0 + col;
@@ -703,6 +837,14 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
           }
         }
       }
+      if (several) {
+        if (ln == 0) s_odd[~turn & 1] = 0;  // of the last part, of which all know
+        if (!all_seen(p, lo, hi, key0, S)) {
+          uint32_t odd = 0;
+          for (int j = 0; j < VL; j++) odd |= G::odd(s_kv[wave * S * G::MCH + j * 64 + ln]);
+          if (__builtin_amdgcn_ballot_w64((odd & G::kOdd) != 0) != 0) s_odd[turn & 1] = 1;
+        }
+      }
       barrier();  // everyone is done with the values and p
     }
 
@@ -719,6 +861,29 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
           *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
               f32x4{o[x][4 * b], o[x][4 * b + 1], o[x][4 * b + 2], o[x][4 * b + 3]};
       }
+    }
+    if (several) {
+      // Some values that not all tokens see are infinities or NaN: the tokens'
+      // results one by one. (Each wave has 32 rows of the values' place.)
+      if (__builtin_expect_with_probability(__builtin_amdgcn_readfirstlane(s_odd[turn & 1]), 1, 0.0)) {
+        const int t0 = c0 / p.G, tasks = (clast / p.G - t0 + 1) * G::DT;
+        for (int i = wave; i < tasks; i += 4) {
+          const int dt = i % G::DT;
+          for_columns(p, t0 + i / G::DT, c0, clast, [&](int c, bool valid) __attribute__((always_inline)) {
+            const int t = c / p.G;
+            float m, l;
+            const f32x16 y = token_segment<T, D, V>(p, r, rq, kvh, c, dt, w.unit(part), s_kv + wave * 32 * G::VCH, m, l);
+            l = half_swap_sum(l);
+            if (!valid) return;
+            const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + c;
+            if (dt == 0 && half == 0) p.pml[slot] = make_float2(m, l);
+#pragma unroll
+            for (int e = 0; e < 16; e++) p.po[slot * V + 32 * dt + G::row(e, half)] = y[e];
+          });
+        }
+        __syncthreads();
+      }
+      turn++;
     }
   } while ((part += p.gseg.d) < parts);
 }
@@ -845,6 +1010,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
   __shared__ const char* s_row[NB][2][S];
   __shared__ int32_t s_entry[8][64];
   __shared__ uint64_t s_map[8];
+  __shared__ int s_odd;
   __shared__ int s_scan[NW + LW + 3];
   __shared__ float s_ml[2][64 * NW];  // each lane's own M and L
 
@@ -921,7 +1087,6 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
   const int cc = cw + col;
   const bool cv = cc < ncol;
   const int tok = cv ? cc / p.G : 0;
-  const int32_t pos = cv ? p0 + tok : -1;
   const bool whole_tile = cw + 32 <= ncol;
   uint4 q[G::NQ];
   load_query<G>(query_at<T>(p, r, rq, tok, kvh * (int)p.G.d + (cv ? cc - tok * (int)p.G.d : 0)), half, q);
@@ -1004,6 +1169,30 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
     else if (lw == 0) wait_loads_but<(AHEAD - 1) * (LPS + 1)>();
     else wait_loads_but<(AHEAD - 1) * LPS>();
   };
+  // Steps all_b .. all_e - 1 are seen whole by every token. (As are some with
+  // first tokens: a look at those costs little.) `next_look`: the next other one.
+  int all_b = 0, all_e = steps;
+  if (lo != hi) {
+    const int32_t start = p.window ? hi - p.window + 1 : 0, past = lo < 0 ? 0 : (lo + 1) / S;
+    const int skip = (start > 0 ? (start + S - 1) / S : 0) - w.b;
+    all_b = w.a + (skip > 0 ? skip : 0);
+    all_e = w.a + past - w.b;
+    if (all_e < all_b) all_e = all_b;
+  }
+  int next_look = all_b > 0 ? 0 : all_e;
+  // Before the barrier of step j: whether this wave's part of its values, which
+  // some tokens may not see, holds an infinity or NaN.
+  auto look_at_values = [&](int j) __attribute__((always_inline)) {
+    if (j != next_look) return;
+    next_look = j + 1 == all_b ? all_e : j + 1;
+    const uint4* at = s_kv + j % NB * (KU + VU) + KU + 64 * lw + opaque(lane);
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < (VU + NT - 1) / NT; i++)
+      if (VU % NT == 0 || i * NT + 64 * lw < VU) odd |= G::odd(at[i * NT]);
+    if (__builtin_amdgcn_ballot_w64((odd & G::kOdd) != 0) != 0) s_odd = 1;
+  };
+  if (tid == 0) s_odd = 0;
   if (loads && lw == 0) {
     int32_t entry[NB];
 #pragma unroll
@@ -1019,6 +1208,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
     if (loads) {
       for (int j = 0; j < steps; j++) {
         await_step(j);
+        look_at_values(j);
         barrier();
         start_step(j + AHEAD);
         if (lw == 0) put_rows(j + NB, s_entry[(j + NB) & 7][opaque(lane)]);
@@ -1029,7 +1219,10 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
     // LDS addresses are computed anew each step: kept across steps they take
     // the registers that o and O need.
     const int ln = opaque(lane), hf = ln >> 5;
-    if constexpr (LW == 0) await_step(j);
+    if constexpr (LW == 0) {
+      await_step(j);
+      look_at_values(j);
+    }
     barrier();  // step j is there, and everyone is done with step j - 1's buffer
     if constexpr (LW == 0) start_step(j + AHEAD);
     const uint4 *kd = s_kv + j % NB * (KU + VU), *vd = kd + KU;
@@ -1048,8 +1241,9 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
             s[n % KT] = G::score(k, q[n / KT], s[n % KT]);
           });
       if (!full) {
-        const int ps = opaque(pos);  // keeps the bits' computation in this branch
-        G::hide(s, seen_bits(p, ps, key0, mapped) >> (4 * hf));
+        // (The column's position anew: it would take a register.)
+        const int c = cw + (opaque(lane) & 31);
+        G::hide(s, seen_bits(p, c < ncol ? p0 + c / p.G : -1, key0, mapped) >> (4 * hf));
       }
       // A lane's sum of at most kMostSum holds no score that moves the base;
       // else, and at a segment's first step, the largest score decides.
@@ -1122,32 +1316,54 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
 
   // The column anew (kept, it would take registers that the loop needs).
   const int lane2 = opaque(lane), cc2 = cw + (lane2 & 31), half2 = lane2 >> 5;
-  if (cc2 >= ncol) return;
-  const int tok2 = cc2 / p.G, head = kvh * (int)p.G.d + cc2 - tok2 * (int)p.G.d;
-  const float M = s_ml[0][wave * 64 + lane2], L = s_ml[1][wave * 64 + lane2];
-  float e, den;
-  finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
-         p.sinks != nullptr, e, den);
-  const float inv = inverse(den);
-  T* out = out_at<T>(p, r, rq, tok2, head);
+  if (cc2 < ncol) {
+    const int tok2 = cc2 / p.G, head = kvh * (int)p.G.d + cc2 - tok2 * (int)p.G.d;
+    const float M = s_ml[0][wave * 64 + lane2], L = s_ml[1][wave * 64 + lane2];
+    float e, den;
+    finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
+           p.sinks != nullptr, e, den);
+    const float inv = inverse(den);
+    T* out = out_at<T>(p, r, rq, tok2, head);
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++) {
+    for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      T4 y;
+      for (int b = 0; b < 4; b++) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 y;
 #pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, inv);
-      *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half2) = y;
+        for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, inv);
+        *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half2) = y;
+      }
     }
   }
+  // (Set before the last step's barrier, if at all.)
+  // (With no probability: else what follows costs the loop above its registers,
+  // 1 % of its time.)
+  if (__builtin_expect_with_probability(!__builtin_amdgcn_readfirstlane(s_odd), 1, 1.0)) return;
+  __syncthreads();
+  // Waves that have room for 32 rows of values each. (All from the arguments
+  // again: what is kept for this takes registers from the loop.)
+  constexpr int FIT = NB * (KU + VU) / (32 * G::VCH), RW = FIT < NW ? FIT : NW;
+  typedef __attribute__((address_space(4))) const Args KernelArgs;
+  KernelArgs* args = (KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const Args& again = *(const Args*)args;
+  const Request rq2 = request(again, r);
+  const int from = tile * COLS, all = rq2.L * (int)again.G.d, to = (from + COLS < all ? from + COLS : all) - 1;
+  const int t0 = from / again.G, tasks = (to / again.G - t0 + 1) * DT;
+  if (wave < RW)
+#pragma unroll 1
+    for (int i = wave; i < tasks; i += RW)
+      walk_token<T, D, V>(again, r, rq2, kvh, t0 + i / DT, i % DT, from, to, s_kv + wave * 32 * G::VCH);
 }
 
 template <typename T, int D, int V>
 Kernels kernels_of() {
   Kernels k;
-  k.split16 = split_kernel<T, D, V, 16>;
-  k.split32 = split_kernel<T, D, V, 32>;
+  k.split16 = split_kernel<T, D, V, 16, false>;
+  k.split32 = split_kernel<T, D, V, 32, false>;
+  k.split16_one = split_kernel<T, D, V, 16, true>;
+  k.split32_one = split_kernel<T, D, V, 32, true>;
   k.combine = combine_kernel<T, D, V>;
   using G = Geo<T, D, V>;
   k.seg = G::kSeg, k.pass = 4 * G::kStep;

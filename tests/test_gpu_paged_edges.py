@@ -35,3 +35,77 @@ def test_slots_of_entries_that_are_no_pages(cuda):
     k = torch.ones(70, 1, 64, dtype=BF16, device=cuda)
     bi.paged_cache_update(k, k, kc, vc, t.slots)
     assert not bool(kc.any()) and not bool(vc.any())
+
+
+def as_int(x):
+    return x.contiguous().view(torch.int32 if x.dtype == F32 else torch.int16)
+
+
+@pytest.mark.parametrize("D, V", [(64, 64), (96, 96), (128, 128), (192, 128), (192, 192), (256, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("L, H, Hkv", [(6, 8, 2), (40, 8, 8), (500, 12, 2), (300, 3, 1)])
+@pytest.mark.parametrize("window, first", [(None, 0), (130, 3)])
+def test_a_token_is_safe_from_rows_that_only_others_see(cuda, dtype, D, V, L, H, Hkv, window, first):
+    """Infinities and NaN in keys and values that some of a chunk's tokens see,
+    as the window begins and as it ends: the others have the bits that they have
+    without them, those that see one the bits that they have alone."""
+    n, page = 900, 16
+    g = torch.Generator(device=cuda).manual_seed(D + V + L)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
+    k, v, q = rn(1, Hkv, n, D), rn(1, Hkv, n, V), rn(1, H, L, D)
+    run = lambda k, v, lo, hi: bi.window_attention(q[:, :, lo:hi], k[:, :, :n - L + hi],
+                                                   v[:, :, :n - L + hi], window, sink_tokens=first)
+    clean = run(k, v, 0, L)
+    kb, vb = k.clone(), v.clone()
+    inf, nan = float("inf"), float("nan")
+    at = n - L + L // 2  # from this token on
+    vb[:, :, at, 0], vb[:, 0, at, 5], vb[:, :, at, V - 1] = inf, nan, -inf
+    kb[:, :, at + 2, 3] = nan
+    bad = [at, at + 2]
+    if window:
+        early = n - L - window + 1 + L // 3  # up to the token window - 1 behind it
+        vb[:, :, early, 1] = -inf
+        bad.append(early)
+    got = run(kb, vb, 0, L)
+    pos = torch.arange(n - L, n, device=cuda)
+    sees = torch.zeros(L, dtype=torch.bool, device=cuda)
+    for b in bad:
+        sees |= (b <= pos) & ((b > pos - window) if window else True)
+    assert bool(sees.any()) and (bool((~sees).any()) or L == 6)  # 6: each sees one of them, none both
+    free = ~sees
+    assert torch.equal(as_int(got[:, :, free]), as_int(clean[:, :, free]))
+    edge = set(range(min(L, 3))) | {L // 3, L // 3 + 1, L // 2 - 1, L // 2, L // 2 + 1, L // 2 + 2, L - 1}
+    for t in sorted(edge):
+        alone = run(kb, vb, t, t + 1)
+        assert torch.equal(as_int(got[:, :, t:t + 1]), as_int(alone)), t
+        if sees[t]:
+            assert not bool(alone.isfinite().all())
+    # Over pages, beside a single token of the same request.
+    pages = -(-n // page)
+    order = torch.randperm(pages, generator=g, device=cuda)
+    i = torch.arange(n, device=cuda)
+    kc, vc = rn(pages, Hkv, page, D), rn(pages, Hkv, page, V)
+    kc[order[i // page], :, i % page], vc[order[i // page], :, i % page] = kb[0].transpose(0, 1), vb[0].transpose(0, 1)
+    table = order.to(torch.int32)[None].repeat(2, 1)
+    qt = q[0].transpose(0, 1)
+    y = bi.paged_attention(torch.cat([qt, qt[L // 3:L // 3 + 1]]), kc, vc, table, i32([0, L, L + 1], cuda),
+                           i32([n, n - L + L // 3 + 1], cuda), window=window, sink_tokens=first)
+    want = got[0].transpose(0, 1)
+    assert torch.equal(as_int(y[:L]), as_int(want))
+    assert torch.equal(as_int(y[L:]), as_int(want[L // 3:L // 3 + 1]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("window", [None, 1100])
+def test_a_prompt_is_safe_from_its_last_row(cuda, dtype, window):
+    """A prompt of the size that eight waves to a workgroup take, whose last
+    token's values are infinite: only that token's result is."""
+    H, Hkv, n, D = 32, 8, 2200, 128
+    g = torch.Generator(device=cuda).manual_seed(1)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
+    q, k, v = rn(1, H, n, D), rn(1, Hkv, n, D), rn(1, Hkv, n, D)
+    clean = bi.window_attention(q, k, v, window)
+    v[:, :, n - 1] = float("inf")
+    got = bi.window_attention(q, k, v, window)
+    assert torch.equal(as_int(got[:, :, :-1]), as_int(clean[:, :, :-1]))
+    assert bool((got[:, :, -1] == float("inf")).all())
