@@ -109,3 +109,19 @@ def test_a_prompt_is_safe_from_its_last_row(cuda, dtype, window):
     got = bi.window_attention(q, k, v, window)
     assert torch.equal(as_int(got[:, :, :-1]), as_int(clean[:, :, :-1]))
     assert bool((got[:, :, -1] == float("inf")).all())
+
+
+@pytest.mark.parametrize("D, V, H, Hkv, n, L, window, first, sharp", [
+    (256, 256, 16, 1, 471, 471, 428, 0, 3), (256, 256, 40, 1, 700, 64, None, 0, 3),
+    (192, 128, 16, 8, 393, 32, None, 0, 1), (256, 256, 24, 3, 1010, 40, 960, 4, 1)])
+def test_sharp_scores_in_32_bits(cuda, D, V, H, Hkv, n, L, window, first, sharp):
+    """Scores of several hundred: what a weight may be off by is set by the sum
+    of the products' magnitudes, not by the score that is left of it."""
+    g = torch.Generator().manual_seed(n)
+    q = torch.randn(L, H, D, generator=g) * sharp
+    k, v = torch.randn(n, Hkv, D, generator=g), torch.randn(n, Hkv, V, generator=g)
+    heads = lambda x: x.to(cuda).transpose(0, 1)[None]
+    got = bi.window_attention(heads(q), heads(k), heads(v), window, sink_tokens=first, scale=5.0)
+    want, tol = ref.rows(q, k, v, n, window or 0, first, 5.0, None)
+    err = (got[0].transpose(0, 1).double().cpu() - want).abs()
+    assert bool((err <= tol).all()), (err / tol).max()
