@@ -319,7 +319,7 @@ extern "C" int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H,
                                                 int64_t D, int64_t V, int64_t window,
                                                 int64_t sink_tokens, int64_t max_query,
                                                 int64_t max_seq, int dtype) {
-  if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || !bi::elem_size(dtype) ||
+  if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H > 65535 || H % Hkv || !bi::elem_size(dtype) ||
       !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
     return 0;
   const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
@@ -365,7 +365,7 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
 extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t qL,
                                                  int64_t N, int64_t D, int64_t V, int64_t window,
                                                  int64_t sink_tokens, int dtype) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || qL <= 0 || N <= 0 || !bi::elem_size(dtype) ||
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H > 65535 || H % Hkv || qL <= 0 || N <= 0 || !bi::elem_size(dtype) ||
       !dims_built(D, V) || qL > kMost || N > kMost || B > kMost || window < 0 || sink_tokens < 0)
     return 0;
   const Call c = {B, B * qL, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), qL, N, true,

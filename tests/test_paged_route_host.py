@@ -55,3 +55,21 @@ def _few(D, V, dtype, H, Hkv, R, L, N):
     G = H // Hkv
     seg = (64 if max(D, V) * (4 if dtype == F32 else 2) <= 256 else 32) * (4 if dtype == F32 else 8)
     return R * Hkv * max(G, 32) * -(-N // seg) * (V + 2) * 4
+
+
+@pytest.mark.parametrize("heads", [65536, 1 << 40, (1 << 62) + 1])
+def test_head_counts_that_no_call_takes_need_no_workspace(heads):
+    """The same bound as the calls': products of sizes past it passed 64 bits, and
+    a division by one of them ended the process."""
+    L = _lib.lib()
+    assert L.bi_paged_attention_workspace(1 << 24, 1 << 24, heads, heads, 128, 128, 0, 0, 1, 4096, BF16) == 0
+    assert L.bi_window_attention_workspace(1 << 24, heads, heads, 1, 4096, 128, 128, 0, 0, BF16) == 0
+
+
+@pytest.mark.parametrize("R", [1 << 20, 1 << 29])
+@pytest.mark.parametrize("Hkv, G", [(1, 1), (8, 4), (128, 1), (255, 257), (1, 65535), (65535, 1)])
+@pytest.mark.parametrize("max_query, max_seq", [(1, 1 << 40), (64, 1 << 29), (1 << 29, 1 << 29)])
+def test_largest_sizes(R, Hkv, G, max_query, max_seq):
+    w = _lib.lib().bi_paged_attention_workspace(min(R * max_query, 1 << 29), R, Hkv * G, Hkv, 256, 256, 0,
+                                                0, max_query, max_seq, F32)
+    assert 0 <= w <= 1 << 32
