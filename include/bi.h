@@ -260,8 +260,9 @@ int bi_paged_update(const void* k, const void* v, void* k_cache, void* v_cache,
  * rows it does not see. bi_window_attention gives the same bits for the same
  * rows in contiguous memory. (Not bi_sdpa's bits: its chains have no segments.)
  * Rows that a token does not see never reach its output, whatever they hold:
- * not a NaN or infinity either that another token of its request sees (calls
- * that meet one in such a row take longer).
+ * not a NaN or infinity either that another token of its request sees. (Calls
+ * of many tokens per request that meet one in such a row of values take up to a
+ * hundred times as long.)
  * Built for (D, V) in {(64, 64), (96, 96), (128, 128), (192, 128), (192, 192),
  * (256, 256)}.
  */

@@ -34,9 +34,11 @@
 // times an infinity or NaN in it would be NaN for the others. The values of the
 // steps that not all tokens see whole (a prompt's diagonal, a window's ends) are
 // looked at as they pass; where one of them is infinite or NaN, the workgroup
-// computes its tokens once more one by one (token_segment). The look costs 4096
+// computes its tokens once more one by one (a split one by its own loop, a whole
+// one by token_segment). The look costs 4096
 // tokens over 8192 rows 420 -> 425 us, prompts of 8192 tokens under a window of
-// 1024 190 -> 193, of 64 62.7 -> 65.7.
+// 1024 190 -> 193, of 64 62.7 -> 65.7. (With NaN in every value the first takes
+// 58 ms.)
 //
 // Two routes, the same bits:
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment),
@@ -166,6 +168,15 @@ __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
   return key - key / p.page * (int32_t)p.page.d;
 }
 
+
+// The kernel's arguments, read again: for what is needed seldom, so that it is not
+// kept in registers meanwhile.
+__device__ __forceinline__ const Args& args_again() {
+  typedef __attribute__((address_space(4))) const Args KernelArgs;
+  KernelArgs* args = (KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  return *(const Args*)args;
+}
 
 __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+v"(x));
@@ -669,14 +680,14 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
   const int ncol = rq.L * (int)p.G.d;
   if (rq.beyond || ncol > p.split_cols || c0 >= ncol) return;
   const int clast = (c0 + NC < ncol ? c0 + NC : ncol) - 1;
-  const int32_t lo = rq.n - rq.L + c0 / p.G, hi = rq.n - rq.L + clast / p.G;
+  int32_t lo = rq.n - rq.L + c0 / p.G, hi = rq.n - rq.L + clast / p.G;
   // The segment's passes (4 steps each) that some column sees.
   const Walk w = walk(p, lo, hi, G::kSeg);
   const int parts = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
   if (part0 >= parts) return;
   const bool several = !ONE && lo != hi;  // tokens, which may see different rows
   if (several && threadIdx.x < 2) s_odd[threadIdx.x] = 0;
-  int turn = 0;
+  int turn = 0, token = -1;  // token: the one whose results are computed once more
 
   // Column; one without a token takes the first one's query and sees nothing.
   const int cc = c0 + col;
@@ -686,6 +697,11 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
   const int32_t pos = cv ? rq.n - rq.L + tok : -1;
   const char* kh = static_cast<const char*>(p.k) + kvh * p.kh * (int64_t)sizeof(T);
   const char* vh = static_cast<const char*>(p.v) + kvh * p.vh * (int64_t)sizeof(T);
+  // In vector registers: scalar ones are short, and what is left of them decides
+  // how the compiler orders the loads and products of a pass (128 tokens over 8192
+  // rows 107 us, 117 with these and the arguments of the results' store kept
+  // there; 104 without computing tokens once more).
+  if (!ONE) asm volatile("" : "+v"(kh), "+v"(vh));
 
   int part = part0, s0, s1;
   // Row addresses of the wave's step of a segment; a row that no column sees,
@@ -733,11 +749,12 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
   // The grid has p.gseg places for a request's segments: a few are enough
   // where there are many workgroups, and empty ones are not free (64 requests
   // of 250 rows under a bound of 65536 65 us, 128 with a place for each).
-  do {
+  for (;;) {
     s0 = w.unit(part) * PN, s1 = s0 + PN;
-    while (!any_seen(p, lo, hi, s0 * PS, PS)) s0++;
-    while (!any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
-    if (p.window || part != part0) {
+    if (!ONE && token >= 0 && !any_seen(p, lo, hi, s0 * PS, G::kSeg)) s1 = s0;  // one token may see none of it
+    while (s0 < s1 && !any_seen(p, lo, hi, s0 * PS, PS)) s0++;
+    while (s0 < s1 && !any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
+    if (p.window || part != part0 || token >= 0) {
       entry0 = entry_for(s0);
       entry = entry_for(s0 + 1);
     }
@@ -837,7 +854,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
           }
         }
       }
-      if (several) {
+      if (several && token < 0) {
         if (ln == 0) s_odd[~turn & 1] = 0;  // of the last part, of which all know
         if (!all_seen(p, lo, hi, key0, S)) {
           uint32_t odd = 0;
@@ -849,13 +866,14 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
     }
 
     l = half_swap_sum(l);
-    if (cv) {
-      const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + cc;
-      if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
+    const Args& again = ONE ? p : args_again();
+    if (cv && (ONE || token < 0 || (c0 + col) / again.G == token)) {
+      const int64_t slot = (((int64_t)r * again.Hkv.d + kvh) * again.nseg.d + part) * again.ccap.d + cc;
+      if (wave == 0 && half == 0) again.pml[slot] = make_float2(m, l);
 #pragma unroll
       for (int x = 0; x < TW; x++) {
         if (wave + 4 * x >= G::DT) break;
-        float* to = p.po + slot * V + 32 * (wave + 4 * x);
+        float* to = again.po + slot * V + 32 * (wave + 4 * x);
 #pragma unroll
         for (int b = 0; b < 4; b++)
           *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
@@ -863,29 +881,20 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
       }
     }
     if (several) {
-      // Some values that not all tokens see are infinities or NaN: the tokens'
-      // results one by one. (Each wave has 32 rows of the values' place.)
-      if (__builtin_expect_with_probability(__builtin_amdgcn_readfirstlane(s_odd[turn & 1]), 1, 0.0)) {
-        const int t0 = c0 / p.G, tasks = (clast / p.G - t0 + 1) * G::DT;
-        for (int i = wave; i < tasks; i += 4) {
-          const int dt = i % G::DT;
-          for_columns(p, t0 + i / G::DT, c0, clast, [&](int c, bool valid) __attribute__((always_inline)) {
-            const int t = c / p.G;
-            float m, l;
-            const f32x16 y = token_segment<T, D, V>(p, r, rq, kvh, c, dt, w.unit(part), s_kv + wave * 32 * G::VCH, m, l);
-            l = half_swap_sum(l);
-            if (!valid) return;
-            const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + c;
-            if (dt == 0 && half == 0) p.pml[slot] = make_float2(m, l);
-#pragma unroll
-            for (int e = 0; e < 16; e++) p.po[slot * V + 32 * dt + G::row(e, half)] = y[e];
-          });
-        }
-        __syncthreads();
+      // Some values that not all tokens see are infinities or NaN: the segment once
+      // more, token by token; the columns of others are computed as they come and
+      // not stored. (Each pass ends with a barrier.)
+      if (token >= 0 ? token < clast / again.G
+                     : __builtin_expect_with_probability(__builtin_amdgcn_readfirstlane(s_odd[turn & 1]), 1, 0.0)) {
+        token = token < 0 ? c0 / again.G : token + 1;
+        lo = hi = rq.n - rq.L + token;
+        continue;
       }
+      if (token >= 0) lo = rq.n - rq.L + c0 / again.G, hi = rq.n - rq.L + clast / again.G, token = -1;
       turn++;
     }
-  } while ((part += p.gseg.d) < parts);
+    if ((part += again.gseg.d) >= parts) return;
+  }
 }
 
 // Tokens that no kernel computes: 0 where no request owns them, NaN where the
