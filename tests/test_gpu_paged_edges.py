@@ -95,6 +95,57 @@ def test_a_token_is_safe_from_rows_that_only_others_see(cuda, dtype, D, V, L, H,
     assert torch.equal(as_int(y[L:]), as_int(want[L // 3:L // 3 + 1]))
 
 
+@pytest.mark.parametrize("dtype, D", [(BF16, 128), (F16, 64), (BF16, 256), (F32, 96)])
+@pytest.mark.parametrize("border", [512, 1024])
+@pytest.mark.parametrize("window, first", [(None, 0), (40, 0), (12, 2)])
+def test_a_token_is_safe_where_segments_meet(cuda, dtype, D, border, window, first):
+    """Tokens on both sides of a segment's border, so that some see nothing of
+    a segment that others see, with NaN in values before and behind it."""
+    n, L, H, Hkv = border + 11, 24, 6, 3
+    g = torch.Generator(device=cuda).manual_seed(border + D)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
+    q, k, v = rn(1, H, L, D), rn(1, Hkv, n, D), rn(1, Hkv, n, D)
+    nan = float("nan")
+    v[:, 0, border + 4, 7] = nan  # seen by the last seven tokens only
+    v[:, 1, border - 3, D - 1] = nan  # by those from the eleventh on
+    v[:, 2, border - 20, 0] = nan  # by all, but under a window by the first ones only, or none
+    got = bi.window_attention(q, k, v, window, sink_tokens=first)
+    for t in range(L):
+        end = n - L + t + 1
+        alone = bi.window_attention(q[:, :, t:t + 1], k[:, :, :end], v[:, :, :end], window, sink_tokens=first)
+        assert torch.equal(as_int(got[:, :, t:t + 1]), as_int(alone)), t
+    for h, row in enumerate((border + 4, border - 3, border - 20)):
+        pos = torch.arange(n - L, n, device=cuda)
+        sees = (row <= pos) & ((row > pos - window) if window else True)
+        assert torch.equal(got[0, 2 * h:2 * h + 2].isfinite().all(-1), ~sees.expand(2, L))
+
+
+@pytest.mark.parametrize("window", [None, 4400])
+def test_a_token_is_safe_under_a_loose_bound(cuda, window):
+    """256 requests of two tokens under a bound of 65536 rows, whose workgroups
+    take several segments each, with NaN in the last row of some of them."""
+    R, H, Hkv, D, page, W = 256, 16, 8, 64, 16, 300
+    g = torch.Generator(device=cuda).manual_seed(4)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda).to(BF16)
+    k, v, q = rn(Hkv, W * page, D), rn(Hkv, W * page, D), rn(2 * R, H, D)
+    ends = (4601, 2101, 701, 513, 4097, 65)  # kv head h has NaN in the last row of the h-th
+    for h, end in enumerate(ends):
+        v[h, end - 1, h] = float("nan")
+    pages = lambda x: x.view(Hkv, W, page, D).transpose(0, 1).contiguous()
+    lens = [ends[r % 6] if r % 7 else 4800 - r for r in range(R)]
+    table = torch.arange(W, dtype=torch.int32, device=cuda).repeat(R, 1)
+    got = bi.paged_attention(q, pages(k), pages(v), table, i32(range(0, 2 * R + 1, 2), cuda), i32(lens, cuda),
+                             window=window, max_query=2, max_seq=65536)
+    for r in range(0, R, 5):
+        for t in range(2):
+            end = lens[r] - 1 + t
+            alone = bi.window_attention(q[2 * r + t][None, :, None], k[None, :, :end], v[None, :, :end], window)
+            assert torch.equal(as_int(got[2 * r + t]), as_int(alone[0, :, 0])), (r, t)
+            for h, row in enumerate(e - 1 for e in ends):
+                sees = row < end and (window is None or row > end - 1 - window)
+                assert bool(got[2 * r + t, 2 * h:2 * h + 2].isfinite().all()) == (not sees), (r, t, h)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("window", [None, 1100])
 def test_a_prompt_is_safe_from_its_last_row(cuda, dtype, window):
