@@ -36,8 +36,8 @@
 // looked at as they pass; where one of them is infinite or NaN, the workgroup
 // computes its tokens once more one by one (a split one by its own loop, a whole
 // one by token_segment). The look costs 4096
-// tokens over 8192 rows 420 -> 425 us, prompts of 8192 tokens under a window of
-// 1024 190 -> 193, of 64 62.7 -> 65.7. (With NaN in every value the first takes
+// tokens over 8192 rows 427 -> 434 us, prompts of 8192 tokens under a window of
+// 1024 188 -> 191, of 64 62.7 -> 65.7. (With NaN in every value the first takes
 // 58 ms.)
 //
 // Two routes, the same bits:
@@ -635,11 +635,11 @@ __device__ __forceinline__ void walk_token(const Args& p, int r, const Request& 
 // next pass's keys while the values are used, both through the same registers
 // (the table's entries are loaded two passes ahead). The same loads without
 // any computation read 64 requests of 8191 rows in pages of 16 in 350 us (6.1
-// TB/s); this kernel and its fold take 390, 410 with loads that keep their
-// lines in the caches. (32 loads a wave in flight, keys and values together,
+// TB/s); this kernel and its fold take 365 to 390, 5 % more with loads that
+// keep their lines in the caches. (32 loads a wave in flight, keys and values together,
 // were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
 // ONE: no request has more than one token, so that no row is seen by some only
-// (the code for these costs one request of 8192 rows 1.3 us of 18.4, 64 1.7 %).
+// (the code for these costs one request of 8192 rows 1.0 us of 18.7, 64 1.4 %).
 template <typename T, int D, int V, int NC, bool ONE>
 __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_kernel(Args p) {
   using G = Geo<T, D, V>;
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(256, (Geo<T, D, V>::split_per_cu(NC))) split_k
 
   // The grid has p.gseg places for a request's segments: a few are enough
   // where there are many workgroups, and empty ones are not free (64 requests
-  // of 250 rows under a bound of 65536 65 us, 128 with a place for each).
+  // of 250 rows under a bound of 65536 53 us, 128 with a place for each).
   for (;;) {
     s0 = w.unit(part) * PN, s1 = s0 + PN;
     if (!ONE && token >= 0 && !any_seen(p, lo, hi, s0 * PS, G::kSeg)) s1 = s0;  // one token may see none of it

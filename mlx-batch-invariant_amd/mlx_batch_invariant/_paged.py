@@ -18,7 +18,8 @@ lengths. :func:`window_attention` is the same attention over contiguous keys.
 Keys are taken by their position in the request, in segments of a fixed length
 whose results are folded in a fixed order: a token's output has the same bits
 whatever else is in the batch, however many tokens are new, whichever pages
-hold its keys, and for paged and contiguous keys alike. The kernels
+hold its keys, and for paged and contiguous keys alike. Rows that a token does
+not see never reach it, infinities and NaN in them included. The kernels
 (csrc/bi_paged*.hip) have no backward pass.
 """
 
@@ -252,8 +253,10 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
 
     ``window=w`` lets a token at position p see rows j > p - w only, and
     besides them the first ``sink_tokens`` rows. ``sinks`` (H,) is a logit per
-    head that enters its denominator. Rows whose table entry is not a page of
-    the cache are not seen.
+    head that enters its denominator, rounded to q's type. Rows whose table
+    entry is not a page of the cache are not seen. A call of many tokens per
+    request takes far longer where a value that only some of them see is
+    infinite or NaN.
 
     ``max_query`` and ``max_seq`` bound the requests' new tokens and lengths
     (by default T and the table's capacity). The launch is sized by them, so
