@@ -35,10 +35,9 @@
 // steps that not all tokens see whole (a prompt's diagonal, a window's ends) are
 // looked at as they pass; where one of them is infinite or NaN, the workgroup
 // computes its tokens once more one by one (a split one by its own loop, a whole
-// one by token_segment). The look costs 4096
-// tokens over 8192 rows 427 -> 434 us, prompts of 8192 tokens under a window of
-// 1024 188 -> 191, of 64 62.7 -> 65.7. (With NaN in every value the first takes
-// 58 ms.)
+// one by token_segment). The look costs 4096 tokens over 8192 rows 427 -> 434
+// us, prompts of 8192 tokens under a window of 1024 188 -> 191, of 64 62.7 ->
+// 65.7. (With NaN in every value the first takes 58 ms.)
 //
 // Two routes, the same bits:
 //   * split: a workgroup per (request, kv head, up to 32 columns, segment),
@@ -167,7 +166,6 @@ __device__ __forceinline__ int32_t row_of(const Args& p, int32_t key) {
   if (!p.qstart) return key;
   return key - key / p.page * (int32_t)p.page.d;
 }
-
 
 // The kernel's arguments, read again: for what is needed seldom, so that it is not
 // kept in registers meanwhile.
@@ -523,8 +521,9 @@ __device__ __forceinline__ int lane_anew() {
 // Column c's (m, l of its lane half, o of the dims 32 dt ..) over one segment, by
 // one wave whose lanes hold the columns of one token: the arithmetic of the
 // kernels below with zeros for every row that the token does not see, for
-// tokens beside others that see a row of values with an infinity or NaN. (Slow
-// and rare: it keeps little in registers.) `lds`: 32 rows of values.
+// tokens of a whole workgroup beside others that see a row of values with an
+// infinity or NaN. (Slow and rare: it keeps little in registers.) `lds`: 32 rows
+// of values.
 template <typename T, int D, int V>
 __device__ __forceinline__ f32x16 token_segment(const Args& p, int r, const Request& rq, int kvh, int c, int dt,
                                                 int segment, uint4* lds, float& m, float& l) {
@@ -636,8 +635,8 @@ __device__ __forceinline__ void walk_token(const Args& p, int r, const Request& 
 // (the table's entries are loaded two passes ahead). The same loads without
 // any computation read 64 requests of 8191 rows in pages of 16 in 350 us (6.1
 // TB/s); this kernel and its fold take 365 to 390, 5 % more with loads that
-// keep their lines in the caches. (32 loads a wave in flight, keys and values together,
-// were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
+// keep their lines in the caches. (32 loads a wave in flight, keys and values
+// together, were no faster: alone they read 4.7 TB/s, 16 a wave 6.0-6.4.)
 // ONE: no request has more than one token, so that no row is seen by some only
 // (the code for these costs one request of 8192 rows 1.0 us of 18.7, 64 1.4 %).
 template <typename T, int D, int V, int NC, bool ONE>
@@ -1353,10 +1352,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo<T, D, V>::kTwoWaves ? 2 :
   // Waves that have room for 32 rows of values each. (All from the arguments
   // again: what is kept for this takes registers from the loop.)
   constexpr int FIT = NB * (KU + VU) / (32 * G::VCH), RW = FIT < NW ? FIT : NW;
-  typedef __attribute__((address_space(4))) const Args KernelArgs;
-  KernelArgs* args = (KernelArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(args));
-  const Args& again = *(const Args*)args;
+  const Args& again = args_again();
   const Request rq2 = request(again, r);
   const int from = tile * COLS, all = rq2.L * (int)again.G.d, to = (from + COLS < all ? from + COLS : all) - 1;
   const int t0 = from / again.G, tasks = (to / again.G - t0 + 1) * DT;
