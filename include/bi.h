@@ -300,6 +300,80 @@ int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t
                                       int64_t D, int64_t V, int64_t window, int64_t sink_tokens,
                                       int dtype);
 
+/*
+ * bi_paged_update for a cache of 8 bits: a row of one token and head is kept as
+ * whole numbers c in -127 .. 127 and a scale s, its values being c * s.
+ *
+ *   k_cache, v_cache    int8, strides[4..9] as in bi_paged_update
+ *   k_scales, v_scales  (num_pages, Hkv, page_size) float, element strides
+ *                       scale_strides[0..2] and [3..5] (page, head, row)
+ *   keep_scales 0       s = max |x| / 127 is written for every token and head,
+ *                       and c = x / s rounded to the nearest, ties to even. A
+ *                       row of zeros has s = 0; one with an infinity or NaN
+ *                       s = NaN and codes 0, so that it reads as NaN.
+ *   keep_scales 1       the scales are read (not negative; they may lie at
+ *                       strides of 0, one for a page or a head); what passes
+ *                       127 s is cut off, a NaN is 0, as all is where s = 0
+ *
+ * Codes and scale depend on the row alone.
+ */
+int bi_paged_update_q8(const void* k, const void* v, int8_t* k_cache, int8_t* v_cache,
+                       float* k_scales, float* v_scales, const int32_t* slots, int64_t T,
+                       int64_t Hkv, int64_t D, int64_t V, int64_t num_pages, int64_t page_size,
+                       const int64_t* strides, const int64_t* scale_strides, int keep_scales,
+                       int dtype, void* hip_stream);
+
+/*
+ * The way back: rows of a paged cache as tokens. k[t] (T, Hkv, D) and v[t] (T,
+ * Hkv, V) become row slots[t] % page_size of page slots[t] / page_size, zeros
+ * where the slot is negative or not below num_pages * page_size. With scales the
+ * cache is int8 and a value is c * s in 32 bits, rounded once to `dtype`; with
+ * NULL for both it is of `dtype` and copied. Strides as in bi_paged_update_q8.
+ */
+int bi_paged_read(const void* k_cache, const void* v_cache, const float* k_scales,
+                  const float* v_scales, const int32_t* slots, void* k, void* v, int64_t T,
+                  int64_t Hkv, int64_t D, int64_t V, int64_t num_pages, int64_t page_size,
+                  const int64_t* strides, const int64_t* scale_strides, int dtype,
+                  void* hip_stream);
+
+/*
+ * Rotary positions: pair i of every head of token t turns by the angle
+ * positions[t] * inv_freq[i], (x, y) -> scale * (x cos - y sin, x sin + y cos).
+ *
+ *   q (T, H, D), k (T, Hkv, D)   element strides strides[0..1], [2..3] (token,
+ *                head), the last dimension contiguous; H or Hkv may be 0
+ *   q_out, k_out contiguous, not overlapping q and k
+ *   positions    (T) int32, of either sign
+ *   inv_freq     (n) doubles, radians per position
+ *   interleaved  0: pair i is dims offset + i and offset + n + i;
+ *                1: dims offset + 2 i and offset + 2 i + 1
+ * The other dims are copied. Angles are reduced in 64 bits; a token's result
+ * depends on the token alone.
+ */
+int bi_rotary(const void* q, const void* k, void* q_out, void* k_out, const int32_t* positions,
+              const double* inv_freq, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t n,
+              int64_t offset, const int64_t* strides, float scale, int interleaved, int dtype,
+              void* hip_stream);
+
+/*
+ * Log probabilities of given tokens under rows of logits, the rows' entropies,
+ * and their `top` largest logits.
+ *
+ *   logits       (rows, V), rows `stride` elements apart
+ *   tokens       (rows) of token_bytes 4 or 8; one that is not in 0 .. V - 1
+ *                has the log probability NaN
+ *   logprobs     (rows) ln softmax(logits)[token]
+ *   entropy      (rows) -sum p ln p, in nats; -inf logits count for nothing
+ *   top_ids, top_logprobs  (rows, top) in descending order, ties by ascending
+ *                id; top is at most 64 and at most V. A NaN logit counts as the
+ *                largest.
+ * Log probabilities and entropy of a row with a NaN or +inf, or of -inf alone,
+ * are NaN. A row's results depend on the row alone.
+ */
+int bi_token_logprobs(const void* logits, const void* tokens, float* logprobs, float* entropy,
+                      int64_t* top_ids, float* top_logprobs, int64_t rows, int64_t V,
+                      int64_t stride, int64_t top, int token_bytes, int dtype, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,7 +27,8 @@ PAGED_UNITS = sorted(f for f in os.listdir(HERE)
                      if f.startswith("bi_paged_attn_d") and f.endswith(".hip"))
 SOURCES = ["bi_abi.cpp", "bi_gemm.hip", "bi_gemm_f32.hip", "bi_gemm_f16.hip", "bi_gemm_bf16.hip",
            "bi_qgemm_f16.hip", "bi_qgemm_bf16.hip", "bi_sdpa.hip", *SDPA_MFMA_UNITS,
-           "bi_paged.hip", "bi_paged_attn.hip", *PAGED_UNITS]
+           "bi_paged.hip", "bi_paged_q8.hip", "bi_rotary.hip", "bi_logprobs.hip", "bi_paged_attn.hip",
+           *PAGED_UNITS]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -25,10 +25,12 @@ import torch.nn.functional as F
 from ._attention import HEAD_DIMS, scaled_dot_product_attention, supported_head_dims
 from ._attention import _mask_args, _sdpa
 from ._gemm import TILE, addmm, geometries, linear, matmul
-from ._paged import (PAGED_HEAD_DIMS, PageTables, page_tables, paged_attention,
+from ._logprobs import TokenLogprobs, token_logprobs
+from ._paged import (PAGED_HEAD_DIMS, PageTables, page_tables, paged_attention, paged_cache_read,
                      paged_cache_update, window_attention)
 from ._quant import (QUANT_BITS, QuantizedLinear, dequantize, quantize, quantized_linear,
                      quantized_matmul)
+from ._rotary import rotary, rotary_frequencies
 
 __all__ = [
     "matmul",
@@ -43,10 +45,15 @@ __all__ = [
     "QUANT_BITS",
     "page_tables",
     "paged_cache_update",
+    "paged_cache_read",
     "paged_attention",
     "window_attention",
     "PageTables",
     "PAGED_HEAD_DIMS",
+    "rotary",
+    "rotary_frequencies",
+    "token_logprobs",
+    "TokenLogprobs",
     "batch_invariant_mode",
     "is_enabled",
     "TILE",

@@ -49,6 +49,11 @@ SIGNATURES = {
     "bi_window_attention": (_c_int, [_c_vp] * 5 + [_c_i64] * 7 + [_c_i64p, _c_float]
                             + [_c_i64] * 2 + [_c_int, _c_vp, _c_i64, _c_vp]),
     "bi_window_attention_workspace": (_c_i64, [_c_i64] * 9 + [_c_int]),
+    "bi_paged_update_q8": (_c_int, [_c_vp] * 7 + [_c_i64] * 6 + [_c_i64p, _c_i64p, _c_int, _c_int,
+                                                                 _c_vp]),
+    "bi_paged_read": (_c_int, [_c_vp] * 7 + [_c_i64] * 6 + [_c_i64p, _c_i64p, _c_int, _c_vp]),
+    "bi_rotary": (_c_int, [_c_vp] * 6 + [_c_i64] * 6 + [_c_i64p, _c_float, _c_int, _c_int, _c_vp]),
+    "bi_token_logprobs": (_c_int, [_c_vp] * 6 + [_c_i64] * 4 + [_c_int, _c_int, _c_vp]),
     "bi_gemm_num_geometries": (_c_int, []),
     "bi_gemm_geometry_info": (_c_int, [_c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_int),
                                        ctypes.POINTER(_c_int)]),

@@ -5,8 +5,9 @@ fuse the graph around them but never inside (reference
 tests/test_invariance.py:595-640). The same holds here: while torch.compile
 traces, ``bi.*`` calls become the ops ``mlx_bi::gemm``, ``mlx_bi::qgemm`` and
 ``mlx_bi::sdpa`` (and, for the paged cache, ``mlx_bi::page_tables``,
-``mlx_bi::paged_cache_update``, ``mlx_bi::paged_attention`` and
-``mlx_bi::window_attention``), which the compiler treats as opaque nodes (their
+``mlx_bi::paged_cache_update`` (``_q8`` and ``_kept`` with scales),
+``mlx_bi::paged_cache_read``, ``mlx_bi::paged_attention`` (``_q8``) and
+``mlx_bi::window_attention``; ``mlx_bi::rotary`` and ``mlx_bi::token_logprobs``), which the compiler treats as opaque nodes (their
 fake implementations give only output shapes) and which run the HIP kernels
 unchanged. Eager calls skip the dispatcher and launch directly.
 """
@@ -117,3 +118,78 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
 @window_attention.register_fake
 def _window_attention_fake(q, k, v, scale, window, sink_tokens, sinks):
     return q.new_empty((q.shape[0], q.shape[1], q.shape[2], v.shape[-1]))
+
+
+@torch.library.custom_op("mlx_bi::paged_cache_update_q8",
+                         mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
+def paged_cache_update_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                          v_cache: torch.Tensor, slots: torch.Tensor, k_scales: torch.Tensor,
+                          v_scales: torch.Tensor) -> None:
+    from . import _paged
+
+    _paged._update_q8_eager(k, v, k_cache, v_cache, slots, k_scales, v_scales, False)
+
+
+@paged_cache_update_q8.register_fake
+def _paged_cache_update_q8_fake(k, v, k_cache, v_cache, slots, k_scales, v_scales):
+    return None
+
+
+@torch.library.custom_op("mlx_bi::paged_cache_update_kept", mutates_args=("k_cache", "v_cache"))
+def paged_cache_update_kept(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, slots: torch.Tensor, k_scales: torch.Tensor,
+                            v_scales: torch.Tensor) -> None:
+    from . import _paged
+
+    _paged._update_q8_eager(k, v, k_cache, v_cache, slots, k_scales, v_scales, True)
+
+
+@paged_cache_update_kept.register_fake
+def _paged_cache_update_kept_fake(k, v, k_cache, v_cache, slots, k_scales, v_scales):
+    return None
+
+
+@torch.library.custom_op("mlx_bi::paged_cache_read", mutates_args=())
+def paged_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                     k_scales: Optional[torch.Tensor], v_scales: Optional[torch.Tensor],
+                     dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    from . import _paged
+
+    return _paged._read_eager(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+
+
+@paged_cache_read.register_fake
+def _paged_cache_read_fake(k_cache, v_cache, slots, k_scales, v_scales, dtype):
+    T, Hkv = slots.shape[0], k_cache.shape[1]
+    return (k_cache.new_empty((T, Hkv, k_cache.shape[3]), dtype=dtype),
+            k_cache.new_empty((T, Hkv, v_cache.shape[3]), dtype=dtype))
+
+
+@torch.library.custom_op("mlx_bi::rotary", mutates_args=())
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+           interleaved: bool, offset: int, scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    from . import _rotary
+
+    return _rotary._rotary_eager(q, k, positions, inv_freq, interleaved, offset, scale)
+
+
+@rotary.register_fake
+def _rotary_fake(q, k, positions, inv_freq, interleaved, offset, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("mlx_bi::token_logprobs", mutates_args=())
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import _logprobs
+
+    # Outputs of a custom op may not share storage.
+    return tuple(t.clone() for t in _logprobs._logprobs_eager(logits, tokens, top))
+
+
+@token_logprobs.register_fake
+def _token_logprobs_fake(logits, tokens, top):
+    f32 = dict(dtype=torch.float32)
+    return (logits.new_empty(tokens.shape, **f32), logits.new_empty(tokens.shape, **f32),
+            logits.new_empty((*tokens.shape, top), dtype=torch.int64),
+            logits.new_empty((*tokens.shape, top), **f32))

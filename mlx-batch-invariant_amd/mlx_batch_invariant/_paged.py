@@ -21,6 +21,13 @@ whatever else is in the batch, however many tokens are new, whichever pages
 hold its keys, and for paged and contiguous keys alike. Rows that a token does
 not see never reach it, infinities and NaN in them included. The kernels
 (csrc/bi_paged*.hip) have no backward pass.
+
+A cache of 8 bits holds int8 codes, and beside them ``k_scales`` and
+``v_scales`` (num_pages, Hkv, page_size) float32: a row's values are its codes
+times its scale. The same calls take it, with ``k_scales=`` and ``v_scales=``.
+Each token and head has a scale of its own, so that what a token attends to does
+not depend on the tokens written beside or after it.
+:func:`paged_cache_read` gives values back, from a cache of any type.
 """
 
 import collections
@@ -40,6 +47,7 @@ PageTables = collections.namedtuple(
 
 
 _I32 = torch.int32
+_I64x6 = ctypes.c_int64 * 6
 _I64x9 = ctypes.c_int64 * 9
 _I64x10 = ctypes.c_int64 * 10
 
@@ -151,7 +159,19 @@ def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_si
     return slots, positions, start, seq, used.view(())
 
 
-def _cache_shapes(k_cache, v_cache):
+def _no_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("%s has no backward pass: call it under torch.no_grad()" % what)
+
+
+def _scale_strides(name, scales, cache):
+    if scales.dtype != torch.float32 or scales.shape != cache.shape[:3]:
+        raise ValueError("%s must be float32 of shape %s, got %s of shape %s"
+                         % (name, tuple(cache.shape[:3]), scales.dtype, tuple(scales.shape)))
+    return scales.stride()
+
+
+def _cache_shapes(k_cache, v_cache, k_scales=None, v_scales=None):
     """The caches' strides (page, head, row, 1), after their checks."""
     ks, vs = k_cache.shape, v_cache.shape
     if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3]:
@@ -160,7 +180,16 @@ def _cache_shapes(k_cache, v_cache):
     kst, vst = k_cache.stride(), v_cache.stride()
     if kst[3] != 1 or vst[3] != 1:
         raise ValueError("the caches' last dimension must be contiguous")
-    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in _lib.DTYPE_CODES:
+    if k_scales is not None or v_scales is not None or k_cache.dtype is torch.int8:
+        if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8 or k_scales is None \
+                or v_scales is None:
+            raise ValueError("k_scales and v_scales go with int8 caches, and these with both, got "
+                             "caches of %s and %s, %s and %s scales"
+                             % (k_cache.dtype, v_cache.dtype, "no" if k_scales is None else "k",
+                                "no" if v_scales is None else "v"))
+        _scale_strides("k_scales", k_scales, k_cache)
+        _scale_strides("v_scales", v_scales, v_cache)
+    elif k_cache.dtype != v_cache.dtype or k_cache.dtype not in _lib.DTYPE_CODES:
         raise ValueError("caches must share a dtype of float32, float16 or bfloat16, got %s and %s"
                          % (k_cache.dtype, v_cache.dtype))
     if ks[0] * ks[2] >= 2 ** 31:
@@ -169,14 +198,23 @@ def _cache_shapes(k_cache, v_cache):
     return kst, vst
 
 
-def paged_cache_update(k, v, k_cache, v_cache, slots):
+def paged_cache_update(k, v, k_cache, v_cache, slots, *, k_scales=None, v_scales=None,
+                       keep_scales=False):
     """Writes new tokens' keys (T, Hkv, D) and values (T, Hkv, V) into the
     caches, in place: token t goes to row ``slots[t] % page_size`` of page
     ``slots[t] // page_size`` (int32, from :func:`page_tables`). A token whose
     slot is negative or not a row of the cache is not written. The slots that
     are written must be distinct. ``k`` and ``v`` may be strided views, such as
-    slices of a projection's output."""
-    _cache_shapes(k_cache, v_cache)
+    slices of a projection's output.
+
+    Into int8 caches a row goes as codes in -127 .. 127, and its scale, max |x| /
+    127, into ``k_scales`` and ``v_scales`` (num_pages, Hkv, page_size) float32; a
+    code is x / scale rounded to the nearest, ties to even. A row with an
+    infinity or NaN has scale NaN and reads as NaN. With ``keep_scales`` the
+    scales are given (not negative) and not written, and may be expanded views,
+    one for each page or head; values past 127 scales are cut off, NaN is 0.
+    """
+    _cache_shapes(k_cache, v_cache, k_scales, v_scales)
     if k.ndim != 3 or v.ndim != 3 or k.shape[:2] != v.shape[:2]:
         raise ValueError("k and v must be (tokens, Hkv, head dim), got %s and %s"
                          % (tuple(k.shape), tuple(v.shape)))
@@ -185,14 +223,34 @@ def paged_cache_update(k, v, k_cache, v_cache, slots):
         raise ValueError("k %s and v %s do not fit caches %s and %s"
                          % (tuple(k.shape), tuple(v.shape), tuple(k_cache.shape),
                             tuple(v_cache.shape)))
-    if not k.dtype == v.dtype == k_cache.dtype:
-        raise ValueError("k and v must share the caches' dtype %s, got %s and %s"
-                         % (k_cache.dtype, k.dtype, v.dtype))
+    if k_scales is None:
+        if keep_scales:
+            raise ValueError("keep_scales goes with k_scales and v_scales")
+        if not k.dtype == v.dtype == k_cache.dtype:
+            raise ValueError("k and v must share the caches' dtype %s, got %s and %s"
+                             % (k_cache.dtype, k.dtype, v.dtype))
+    else:
+        if k.dtype != v.dtype or k.dtype not in _lib.DTYPE_CODES:
+            raise ValueError("k and v must share a dtype of float32, float16 or bfloat16, got %s "
+                             "and %s" % (k.dtype, v.dtype))
+        if not keep_scales:
+            for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+                if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                    raise ValueError("%s is an expanded view, which keep_scales=True takes: a scale "
+                                     "is written for every token and head" % name)
     _int32("slots", slots, k.shape[0])
     if torch.compiler.is_compiling():
         from . import _ops  # noqa: F401  (registers the ops)
 
-        torch.ops.mlx_bi.paged_cache_update(k, v, k_cache, v_cache, slots)
+        if k_scales is None:
+            torch.ops.mlx_bi.paged_cache_update(k, v, k_cache, v_cache, slots)
+        elif keep_scales:
+            torch.ops.mlx_bi.paged_cache_update_kept(k, v, k_cache, v_cache, slots, k_scales,
+                                                     v_scales)
+        else:
+            torch.ops.mlx_bi.paged_cache_update_q8(k, v, k_cache, v_cache, slots, k_scales, v_scales)
+    elif k_scales is not None:
+        _update_q8_eager(k, v, k_cache, v_cache, slots, k_scales, v_scales, keep_scales)
     else:
         _update_eager(k, v, k_cache, v_cache, slots)
 
@@ -219,6 +277,76 @@ def _update_eager(k, v, k_cache, v_cache, slots):
     _call(dev, "bi_paged_update", _lib.lib().bi_paged_update, k.data_ptr(), v.data_ptr(),
           k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), T, Hkv, D, V, P, page, st,
           _lib.DTYPE_CODES[k.dtype])
+
+
+def _update_q8_eager(k, v, k_cache, v_cache, slots, k_scales, v_scales, keep_scales):
+    dev = k.device
+    _on_one_gpu("paged_cache_update", dev, (v, k_cache, v_cache, slots, k_scales, v_scales))
+    T, Hkv, D = k.shape
+    P, _, page, V = v_cache.shape
+    if not (T and P and Hkv and page and D and V):
+        return
+    kt, kh, one = k.stride()
+    if one != 1:
+        k = k.contiguous()
+        kt, kh, _ = k.stride()
+    vt, vh, one = v.stride()
+    if one != 1:
+        v = v.contiguous()
+        vt, vh, _ = v.stride()
+    slots = slots.contiguous()
+    kp, kg, kr, _ = k_cache.stride()
+    vp, vg, vr, _ = v_cache.stride()
+    st = _I64x10(kt, kh, vt, vh, kp, kg, kr, vp, vg, vr)
+    sst = _I64x6(*k_scales.stride(), *v_scales.stride())
+    _call(dev, "bi_paged_update_q8", _lib.lib().bi_paged_update_q8, k.data_ptr(), v.data_ptr(),
+          k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+          slots.data_ptr(), T, Hkv, D, V, P, page, st, sst, bool(keep_scales),
+          _lib.DTYPE_CODES[k.dtype])
+
+
+def paged_cache_read(k_cache, v_cache, slots, *, k_scales=None, v_scales=None, dtype=None):
+    """The way back of :func:`paged_cache_update`: keys (T, Hkv, D) and values
+    (T, Hkv, V) of the rows ``slots`` (T,) int32, contiguous; zeros for a slot
+    that is negative or not a row of the cache. A slot may stand there more than
+    once. The rows of a request are those of its table: ``block_tables[r, i //
+    page_size] * page_size + i % page_size``.
+
+    From int8 caches with ``k_scales`` and ``v_scales`` a value is code * scale in
+    32 bits, rounded once to ``dtype`` (float32, float16 or bfloat16; by default
+    float32). Other caches are copied, in their own dtype."""
+    _cache_shapes(k_cache, v_cache, k_scales, v_scales)
+    if dtype is None:
+        dtype = torch.float32 if k_scales is not None else k_cache.dtype
+    if dtype not in _lib.DTYPE_CODES or (k_scales is None and dtype != k_cache.dtype):
+        raise ValueError("rows of %s caches cannot be read as %s" % (k_cache.dtype, dtype))
+    _int32("slots", slots, None)
+    args = (k_cache, v_cache, slots, k_scales, v_scales, dtype)
+    if torch.compiler.is_compiling():
+        from . import _ops  # noqa: F401  (registers the ops)
+
+        return tuple(torch.ops.mlx_bi.paged_cache_read(*args))
+    return _read_eager(*args)
+
+
+def _read_eager(k_cache, v_cache, slots, k_scales, v_scales, dtype):
+    dev = k_cache.device
+    _on_one_gpu("paged_cache_read", dev, (v_cache, slots, k_scales, v_scales))
+    P, Hkv, page, D = k_cache.shape
+    T, V = slots.shape[0], v_cache.shape[3]
+    k = torch.empty((T, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty((T, Hkv, V), dtype=dtype, device=dev)
+    if not (T and Hkv and D and V and P and page):
+        return k.zero_(), v.zero_()
+    kp, kg, kr, _ = k_cache.stride()
+    vp, vg, vr, _ = v_cache.stride()
+    st = _I64x10(Hkv * D, D, Hkv * V, V, kp, kg, kr, vp, vg, vr)
+    sst = None if k_scales is None else _I64x6(*k_scales.stride(), *v_scales.stride())
+    slots = slots.contiguous()
+    _call(dev, "bi_paged_read", _lib.lib().bi_paged_read, k_cache.data_ptr(), v_cache.data_ptr(),
+          _at(k_scales), _at(v_scales), slots.data_ptr(), k.data_ptr(), v.data_ptr(), T, Hkv, D, V, P,
+          page, st, sst, _lib.DTYPE_CODES[dtype])
+    return k, v
 
 
 def _attention_options(q, D, V, H, Hkv, scale, window, sink_tokens, sinks):

@@ -1,0 +1,193 @@
+"""Rotary positions, the 8-bit cache and log probabilities without a GPU:
+refusals of the C ABI (before any HIP call) and of the Python layer, and the
+frequencies."""
+
+import math
+
+import pytest
+import torch
+
+import mlx_batch_invariant as bi
+from mlx_batch_invariant import _lib
+
+P = 16  # a pointer that is never followed: validation fails first
+I32 = torch.int32
+
+
+def _err():
+    return _lib.lib().bi_last_error().decode()
+
+
+# --------------------------------------------------------------------- C ABI
+
+
+def test_rotary_abi_refusals():
+    def call(q=P, out=P, pos=P, f=P, T=4, H=2, Hkv=1, D=64, n=32, offset=0, strides=True,
+             dtype=_lib.BF16):
+        st = _lib.i64_array((128, 64, 64, 64)) if strides else None
+        return _lib.lib().bi_rotary(q, P, out, P, pos, f, T, H, Hkv, D, n, offset, st, 1.0, 0, dtype,
+                                    None)
+
+    assert call(dtype=9) == _lib.EINVAL and "dtype" in _err()
+    assert call(T=-1) == _lib.EINVAL and "sizes" in _err()
+    assert call(D=0) == _lib.EINVAL
+    assert call(n=33) == _lib.EINVAL and "fit" in _err()
+    assert call(offset=1) == _lib.EINVAL and "fit" in _err()
+    assert call(n=1 << 62) == _lib.EINVAL and "fit" in _err()
+    assert call(offset=1 << 62) == _lib.EINVAL and "fit" in _err()
+    assert call(q=None) == _lib.EINVAL and "null" in _err()
+    assert call(f=None) == _lib.EINVAL and call(pos=None) == _lib.EINVAL
+    assert call(strides=False) == _lib.EINVAL
+    assert call(q=17) == _lib.EINVAL and "aligned" in _err()
+    assert call(T=1 << 30, H=1 << 20) == _lib.EINVAL and "too large" in _err()
+    assert call(T=0) == _lib.OK and call(H=0, Hkv=0) == _lib.OK
+
+
+def test_update_and_read_abi_refusals():
+    st = _lib.i64_array((128, 64, 128, 64, 2048, 1024, 64, 2048, 1024, 64))
+    sst = _lib.i64_array((32, 16, 1) * 2)
+
+    def update(k=P, ks=P, T=4, Hkv=2, D=64, V=64, pages=3, page=16, dtype=_lib.BF16, st=st, sst=sst):
+        return _lib.lib().bi_paged_update_q8(k, P, P, P, ks, P, P, T, Hkv, D, V, pages, page, st, sst,
+                                             0, dtype, None)
+
+    def read(k=P, kc=P, ks=P, vs=P, T=4, Hkv=2, D=64, V=64, pages=3, page=16, dtype=_lib.BF16, st=st,
+             sst=sst):
+        return _lib.lib().bi_paged_read(kc, P, ks, vs, P, k, P, T, Hkv, D, V, pages, page, st, sst,
+                                        dtype, None)
+
+    for call in (update, read):
+        assert call(dtype=7) == _lib.EINVAL and "dtype" in _err()
+        assert call(Hkv=0) == _lib.EINVAL and "sizes" in _err()
+        assert call(page=0) == _lib.EINVAL
+        assert call(pages=1 << 28) == _lib.EINVAL and "too large" in _err()
+        assert call(T=1 << 30, Hkv=4) == _lib.EINVAL and "too large" in _err()
+        assert call(k=None) == _lib.EINVAL and "null" in _err()
+        assert call(st=None) == _lib.EINVAL and call(sst=None) == _lib.EINVAL
+        assert call(k=17) == _lib.EINVAL and "aligned" in _err()
+        assert call(ks=18) == _lib.EINVAL and "aligned" in _err()
+        assert call(T=0) == _lib.OK
+    assert update(ks=None) == _lib.EINVAL and update(pages=0) == _lib.OK
+    assert read(kc=None) == _lib.EINVAL
+    assert read(vs=None) == _lib.EINVAL and read(ks=None) == _lib.EINVAL
+
+
+def test_logprobs_abi_refusals():
+    def call(x=P, out=P, ids=P, rows=4, V=100, stride=100, top=5, token_bytes=8, dtype=_lib.F16):
+        return _lib.lib().bi_token_logprobs(x, P, out, P, ids, P, rows, V, stride, top, token_bytes,
+                                            dtype, None)
+
+    assert call(dtype=3) == _lib.EINVAL and "dtype" in _err()
+    assert call(V=0) == _lib.EINVAL and call(rows=-1) == _lib.EINVAL and call(stride=-1) == _lib.EINVAL
+    assert call(V=1 << 31) == _lib.EINVAL and "sizes" in _err()
+    assert call(top=65) == _lib.EINVAL and "top" in _err()
+    assert call(V=4) == _lib.EINVAL and "top" in _err()
+    assert call(top=-1) == _lib.EINVAL
+    assert call(token_bytes=2) == _lib.EINVAL and "tokens" in _err()
+    assert call(x=None) == _lib.EINVAL and call(ids=None) == _lib.EINVAL and call(out=None) == _lib.EINVAL
+    assert call(x=17) == _lib.EINVAL and "aligned" in _err()
+    assert call(rows=0) == _lib.OK
+
+
+# -------------------------------------------------------------------- Python
+
+
+def test_rotary_refusals():
+    q, k = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
+    pos, f = torch.zeros(3, dtype=I32), torch.zeros(32, dtype=torch.float64)
+    for bad, words in [((q[0], k, pos, f), "tokens, heads"), ((q, k[:2], pos, f), "tokens, heads"),
+                       ((q, k[..., :32], pos, f), "tokens, heads"), ((q, k.half(), pos, f), "dtype"),
+                       ((q.double(), None, pos, f), "dtype"), ((q, k, pos.long(), f), "int32"),
+                       ((q, k, pos[:2], f), "shape"), ((q, k, pos, f.float()), "float64"),
+                       ((q, k, pos, f[None]), "float64"), ((q, k, pos, torch.cat([f, f])), "fit")]:
+        with pytest.raises(ValueError, match=words):
+            bi.rotary(*bad)
+    with pytest.raises(ValueError, match="fit"):
+        bi.rotary(q, k, pos, f, offset=2)
+    with pytest.raises(ValueError, match="fit"):
+        bi.rotary(q, k, pos, f[:8], offset=-1)
+    with pytest.raises(ValueError, match="GPU"):
+        bi.rotary(q, k, pos, f)
+    with pytest.raises(NotImplementedError, match="backward"):
+        bi.rotary(q.requires_grad_(), k, pos, f)
+
+
+def test_frequencies():
+    f = bi.rotary_frequencies(8, device="cpu")
+    assert f.dtype == torch.float64
+    assert f.tolist() == pytest.approx([1, 0.1, 0.01, 0.001], rel=1e-14)
+    assert bi.rotary_frequencies(8, method="linear", factor=4.0, device="cpu").tolist() == (f / 4).tolist()
+    g = bi.rotary_frequencies(8, method="base", factor=4.0, device="cpu")
+    assert g[0] == 1 and g[3] == pytest.approx(f[3] / 4, rel=1e-14)
+    f = bi.rotary_frequencies(128, base=5e5, device="cpu")
+    g = bi.rotary_frequencies(128, base=5e5, method="parts", factor=8.0, original=8192, low=1.0,
+                              high=4.0, device="cpu")
+    turns = 8192 * f / (2 * math.pi)
+    assert (g[turns > 4] == f[turns > 4]).all()
+    assert torch.allclose(g[turns < 1], f[turns < 1] / 8, rtol=1e-14)
+    mid = (turns > 1) & (turns < 4)
+    assert mid.any() and ((g < f) & (g > f / 8))[mid].all()
+    for kw in (dict(dim=7), dict(dim=0), dict(dim=8, base=0.0), dict(dim=8, factor=0.0),
+               dict(dim=8, method="other"), dict(dim=2, method="base", factor=2.0),
+               dict(dim=8, method="parts", factor=2.0),
+               dict(dim=8, method="parts", factor=2.0, original=10, low=4.0, high=4.0)):
+        with pytest.raises(ValueError):
+            bi.rotary_frequencies(**kw, device="cpu")
+
+
+def q8_cache(pages=4, Hkv=2, page=16, D=64):
+    return (torch.zeros(pages, Hkv, page, D, dtype=torch.int8), torch.zeros(pages, Hkv, page, D, dtype=torch.int8),
+            torch.zeros(pages, Hkv, page), torch.zeros(pages, Hkv, page))
+
+
+def test_scales_and_caches_go_together():
+    kc, vc, ks, vs = q8_cache()
+    x, slots = torch.zeros(3, 2, 64), torch.zeros(3, dtype=I32)
+    update = lambda kc=kc, vc=vc, k=x, v=x, **kw: bi.paged_cache_update(k, v, kc, vc, slots, **kw)
+    read = lambda kc=kc, vc=vc, **kw: bi.paged_cache_read(kc, vc, slots, **kw)
+    for call in (update, read):
+        for kw in (dict(), dict(k_scales=ks), dict(v_scales=vs)):
+            with pytest.raises(ValueError, match="int8 caches"):
+                call(**kw)
+        with pytest.raises(ValueError, match="int8 caches"):
+            call(kc=kc.float(), vc=vc.float(), k_scales=ks, v_scales=vs)
+        with pytest.raises(ValueError, match="int8 caches"):
+            call(vc=vc.float(), k_scales=ks, v_scales=vs)
+        with pytest.raises(ValueError, match="k_scales must"):
+            call(k_scales=ks.half(), v_scales=vs)
+        with pytest.raises(ValueError, match="v_scales must"):
+            call(k_scales=ks, v_scales=vs[:3])
+        with pytest.raises(ValueError, match="GPU"):
+            call(k_scales=ks, v_scales=vs)
+    with pytest.raises(ValueError, match="dtype"):
+        update(k=x.to(torch.int8), v=x.to(torch.int8), k_scales=ks, v_scales=vs)
+    with pytest.raises(ValueError, match="dtype"):
+        update(k=x.half(), k_scales=ks, v_scales=vs)
+    wide = ks[:, :, :1].expand(4, 2, 16)
+    with pytest.raises(ValueError, match="v_scales is an expanded"):
+        update(k_scales=ks, v_scales=wide)
+    with pytest.raises(ValueError, match="GPU"):
+        update(k_scales=wide, v_scales=wide, keep_scales=True)
+    with pytest.raises(ValueError, match="keep_scales"):
+        update(kc=kc.float(), vc=vc.float(), keep_scales=True)
+    with pytest.raises(ValueError, match="read as"):
+        read(k_scales=ks, v_scales=vs, dtype=torch.int8)
+    with pytest.raises(ValueError, match="read as"):
+        read(kc=kc.half(), vc=vc.half(), dtype=torch.float32)
+    with pytest.raises(ValueError, match="int32"):
+        bi.paged_cache_read(kc, vc, slots.long(), k_scales=ks, v_scales=vs)
+
+
+def test_token_logprobs_refusals():
+    x, t = torch.zeros(3, 50), torch.zeros(3, dtype=torch.long)
+    for bad, words in [((x.double(), t), "logits"), ((x, t[:2]), "tokens"), ((x, t.short()), "tokens"),
+                       ((x[0, 0], t[0]), "logits"), ((x[:, :0], t), "vocabulary")]:
+        with pytest.raises(ValueError, match=words):
+            bi.token_logprobs(*bad)
+    for top in (-1, 51, 65):
+        with pytest.raises(ValueError, match="top"):
+            bi.token_logprobs(x, t, top=top)
+    with pytest.raises(ValueError, match="GPU"):
+        bi.token_logprobs(x, t)
+    with pytest.raises(NotImplementedError, match="backward"):
+        bi.token_logprobs(x.requires_grad_(), t)
