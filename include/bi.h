@@ -337,6 +337,38 @@ int bi_paged_read(const void* k_cache, const void* v_cache, const float* k_scale
                   void* hip_stream);
 
 /*
+ * bi_paged_attention over a cache of 8 bits: the same rule, with keys k_cache *
+ * k_scales and values v_cache * v_scales.
+ *
+ *   k_cache, v_cache    int8, strides[2..7] as in bi_paged_attention (pointers
+ *                       and strides are multiples of 16 bytes)
+ *   k_scales, v_scales  (num_pages, Hkv, page_size) float, element strides
+ *                       scale_strides[0..2] and [3..5] (page, head, row; 0 for
+ *                       one a page or a head). A negative key scale gives NaN.
+ *   dtype               of q, sinks and out: BI_F16 or BI_BF16
+ *
+ * Scores are sums of exact products of codes and q in 32 bits times the row's
+ * scale in 32 bits; weights times the row's scale are rounded to bf16 (BI_F16: to
+ * two bf16, 2^-17), products and sums in 32 bits, the denominator the sum of the
+ * weights of 32 bits. A token's bits depend on its own request's rows alone, as
+ * there, and nothing in a row that a token does not see reaches it.
+ */
+int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const int8_t* v_cache,
+                          const float* k_scales, const float* v_scales,
+                          const int32_t* block_tables, const int32_t* query_start,
+                          const int32_t* seq_lens, const void* sinks, void* out, int64_t T,
+                          int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V,
+                          int64_t num_pages, int64_t page_size, int64_t W, const int64_t* strides,
+                          const int64_t* scale_strides, float scale, int64_t window,
+                          int64_t sink_tokens, int64_t max_query, int64_t max_seq, int dtype,
+                          void* workspace, int64_t workspace_bytes, void* hip_stream);
+
+/* Bytes with which bi_paged_attention_q8 runs fastest; 0 if it would use none. */
+int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D,
+                                        int64_t V, int64_t window, int64_t sink_tokens,
+                                        int64_t max_query, int64_t max_seq, int dtype);
+
+/*
  * Rotary positions: pair i of every head of token t turns by the angle
  * positions[t] * inv_freq[i], (x, y) -> scale * (x cos - y sin, x sin + y cos).
  *

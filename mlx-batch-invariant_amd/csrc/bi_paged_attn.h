@@ -49,6 +49,10 @@ struct Args {
   int32_t once;           // keys and values are read by one of these only
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
+  // A cache of 8 bits: its scales and their element strides (page, head, row).
+  const float* ks;
+  const float* vs;
+  int64_t ksb, ksh, ksn, vsb, vsh, vsn;
 };
 
 typedef void (*Kernel)(Args);
@@ -69,7 +73,9 @@ struct Kernels {
 };
 
 #define BI_PAGED_DIM_PAIRS(X) X(64, 64) X(96, 96) X(128, 128) X(192, 128) X(192, 192) X(256, 256)
-#define BI_PAGED_DECLARE(D, V) Kernels kernels_d##D##_v##V(int dtype);
+#define BI_PAGED_DECLARE(D, V)            \
+  Kernels kernels_d##D##_v##V(int dtype); \
+  Kernels kernels8_d##D##_v##V(int dtype);  // a cache of 8 bits; f16 and bf16
 BI_PAGED_DIM_PAIRS(BI_PAGED_DECLARE)
 #undef BI_PAGED_DECLARE
 

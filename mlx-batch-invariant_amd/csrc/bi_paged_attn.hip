@@ -16,8 +16,9 @@ bool dims_built(int64_t D, int64_t V) {
   return false;
 }
 
-Kernels kernels(int64_t D, int64_t V, int dtype) {
-#define BI_CASE(d, v) if (D == d && V == v) return kernels_d##d##_v##v(dtype);
+// `q8`: over a cache of 8 bits.
+Kernels kernels(int64_t D, int64_t V, int dtype, bool q8) {
+#define BI_CASE(d, v) if (D == d && V == v) return q8 ? kernels8_d##d##_v##v(dtype) : kernels_d##d##_v##v(dtype);
   BI_PAGED_DIM_PAIRS(BI_CASE)
 #undef BI_CASE
   return Kernels{};
@@ -30,7 +31,8 @@ constexpr int64_t kMost = (int64_t)1 << 29;
 // A call as the host knows it; `exact`: every request has max_query tokens.
 struct Call {
   int64_t R, tokens, G, Hkv, D, V, window, first, max_query, max_seq;
-  bool exact, f32;
+  bool exact;
+  double bytes;  // of a cached element
 };
 
 // How a call is split: the columns up to which a request is (0: none), columns
@@ -109,7 +111,7 @@ Plan plan(const Call& c, const Kernels& k) {
   const bool cut = c.window && wide < seq;
   const double rows = cut ? wide : seq;
   const double chunk = (double)(c.max_query < c.max_seq ? c.max_query : c.max_seq);
-  const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * (c.f32 ? 4.0 : 2.0) / 5e6;
+  const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * c.bytes / 5e6;
   const double all = (double)c.R * ((cols + 127) / 128), full = (double)c.tokens * c.G / 128.0 + c.R;
   const double tiles = (all < full ? all : full) * c.Hkv / cus;
   const double walked = (cut ? rows + 128.0 / c.G + 64.0 : rows) * k.row_us;
@@ -155,11 +157,11 @@ Plan plan(const Call& c, const Kernels& k) {
 
 int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, int64_t ws_bytes,
            void* stream) {
-  const Kernels k = kernels(D, V, dtype);
+  const Kernels k = kernels(D, V, dtype, p.ks != nullptr);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t most = p.qstart ? p.max_query : p.qL;
   const Call c = {p.R, p.qstart ? p.T : (int64_t)p.R * p.qL, p.G.d, p.Hkv.d, D, V, p.window, p.first,
-                  most, p.qstart ? p.max_seq : p.N, !p.qstart, dtype == BI_F32};
+                  most, p.qstart ? p.max_seq : p.N, !p.qstart, p.ks ? 1.0 : (double)bi::elem_size(dtype)};
   Plan s = plan(c, k);
   if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0, 0};
   hipError_t e;
@@ -262,20 +264,20 @@ void common(Args& p, int64_t H, int64_t Hkv, float scale, int64_t window, int64_
   p.qsign = scale < 0.f ? (dtype == BI_F32 ? 0x80000000u : 0x80008000u) : 0u;
 }
 
-}  // namespace
-
-extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void* v_cache,
-                                  const int32_t* block_tables, const int32_t* query_start,
-                                  const int32_t* seq_lens, const void* sinks, void* out, int64_t T,
-                                  int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V,
-                                  int64_t num_pages, int64_t page_size, int64_t W,
-                                  const int64_t* strides, float scale, int64_t window,
-                                  int64_t sink_tokens, int64_t max_query, int64_t max_seq,
-                                  int dtype, void* workspace, int64_t workspace_bytes,
-                                  void* hip_stream) {
-  const char* who = "bi_paged_attention";
+// What bi_paged_attention and bi_paged_attention_q8 (`scale_strides`) share.
+int paged_attention(const char* who, const void* q, const void* k_cache, const void* v_cache,
+                    const float* k_scales, const float* v_scales, const int32_t* block_tables,
+                    const int32_t* query_start, const int32_t* seq_lens, const void* sinks, void* out,
+                    int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V,
+                    int64_t num_pages, int64_t page_size, int64_t W, const int64_t* strides,
+                    const int64_t* scale_strides, float scale, int64_t window, int64_t sink_tokens,
+                    int64_t max_query, int64_t max_seq, int dtype, bool q8, void* workspace,
+                    int64_t workspace_bytes, void* hip_stream) {
   int rc = check(who, H, Hkv, D, V, scale, window, sink_tokens, dtype);
   if (rc) return rc;
+  if (q8 && dtype == BI_F32)
+    return bi::fail(BI_EUNSUPPORTED, "%s: fp32 queries over a cache of 8 bits are not built (f16 and "
+                    "bf16 are)", who);
   if (T < 0 || R < 0 || num_pages < 0 || page_size <= 0 || W < 0 || max_query < 0 || max_seq < 0 ||
       T > kMost || T * H > INT32_MAX || R > kMost || num_pages > INT32_MAX || page_size > INT32_MAX ||
       W > INT32_MAX)
@@ -284,10 +286,12 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
                     (long long)W);
   if (T == 0) return BI_OK;
   if (!q || !out || !query_start || (R > 0 && !seq_lens) || !strides ||
-      (R > 0 && W > 0 && !block_tables) || (num_pages > 0 && (!k_cache || !v_cache)))
+      (R > 0 && W > 0 && !block_tables) || (num_pages > 0 && (!k_cache || !v_cache)) ||
+      (q8 && (!k_scales || !v_scales || !scale_strides)))
     return bi::fail(BI_EINVAL, "%s: null pointer", who);
   const int esz = bi::elem_size(dtype);
-  if (!aligned16(q, k_cache, v_cache, strides, 8, esz))
+  if (!aligned16(q, nullptr, nullptr, strides, 2, esz) ||
+      !aligned16(nullptr, k_cache, v_cache, strides + 2, 6, q8 ? 1 : esz))
     return bi::fail(BI_EINVAL, "%s: q and caches must be 16-byte aligned, with strides of "
                     "multiples of 16 bytes", who);
   Args p = {};
@@ -312,7 +316,32 @@ extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void
   p.max_query = clamp32(max_query);
   p.max_seq = clamp32(max_seq);
   p.page = make_div(page_size);
+  if (q8) {
+    if (((uintptr_t)k_scales | (uintptr_t)v_scales) % 4)
+      return bi::fail(BI_EINVAL, "%s: scales not aligned to elements", who);
+    p.ks = k_scales;
+    p.vs = v_scales;
+    p.ksb = scale_strides[0], p.ksh = scale_strides[1], p.ksn = scale_strides[2];
+    p.vsb = scale_strides[3], p.vsh = scale_strides[4], p.vsn = scale_strides[5];
+  }
   return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
+}
+
+}  // namespace
+
+extern "C" int bi_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                                  const int32_t* block_tables, const int32_t* query_start,
+                                  const int32_t* seq_lens, const void* sinks, void* out, int64_t T,
+                                  int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V,
+                                  int64_t num_pages, int64_t page_size, int64_t W,
+                                  const int64_t* strides, float scale, int64_t window,
+                                  int64_t sink_tokens, int64_t max_query, int64_t max_seq,
+                                  int dtype, void* workspace, int64_t workspace_bytes,
+                                  void* hip_stream) {
+  return paged_attention("bi_paged_attention", q, k_cache, v_cache, nullptr, nullptr, block_tables,
+                         query_start, seq_lens, sinks, out, T, R, H, Hkv, D, V, num_pages, page_size, W,
+                         strides, nullptr, scale, window, sink_tokens, max_query, max_seq, dtype, false,
+                         workspace, workspace_bytes, hip_stream);
 }
 
 extern "C" int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
@@ -323,8 +352,37 @@ extern "C" int64_t bi_paged_attention_workspace(int64_t T, int64_t R, int64_t H,
       !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
     return 0;
   const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
-                  clamp32(max_seq), false, dtype == BI_F32};
-  return plan(c, kernels(D, V, dtype)).bytes;
+                  clamp32(max_seq), false, (double)bi::elem_size(dtype)};
+  return plan(c, kernels(D, V, dtype, false)).bytes;
+}
+
+extern "C" int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const int8_t* v_cache,
+                                     const float* k_scales, const float* v_scales,
+                                     const int32_t* block_tables, const int32_t* query_start,
+                                     const int32_t* seq_lens, const void* sinks, void* out, int64_t T,
+                                     int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V,
+                                     int64_t num_pages, int64_t page_size, int64_t W,
+                                     const int64_t* strides,
+                                     const int64_t* scale_strides, float scale, int64_t window,
+                                     int64_t sink_tokens, int64_t max_query, int64_t max_seq,
+                                     int dtype, void* workspace, int64_t workspace_bytes,
+                                     void* hip_stream) {
+  return paged_attention("bi_paged_attention_q8", q, k_cache, v_cache, k_scales, v_scales, block_tables,
+                         query_start, seq_lens, sinks, out, T, R, H, Hkv, D, V, num_pages, page_size, W,
+                         strides, scale_strides, scale, window, sink_tokens, max_query, max_seq, dtype,
+                         true, workspace, workspace_bytes, hip_stream);
+}
+
+extern "C" int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
+                                                int64_t D, int64_t V, int64_t window,
+                                                int64_t sink_tokens, int64_t max_query,
+                                                int64_t max_seq, int dtype) {
+  if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H > 65535 || H % Hkv || (dtype != BI_F16 && dtype != BI_BF16) ||
+      !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
+    return 0;
+  const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
+                  clamp32(max_seq), false, 1.0};
+  return plan(c, kernels(D, V, dtype, true)).bytes;
 }
 
 extern "C" int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks,
@@ -369,6 +427,6 @@ extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t H
       !dims_built(D, V) || qL > kMost || N > kMost || B > kMost || window < 0 || sink_tokens < 0)
     return 0;
   const Call c = {B, B * qL, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), qL, N, true,
-                  dtype == BI_F32};
-  return plan(c, kernels(D, V, dtype)).bytes;
+                  (double)bi::elem_size(dtype)};
+  return plan(c, kernels(D, V, dtype, false)).bytes;
 }

@@ -923,9 +923,8 @@ __device__ void fill(const Args& p, int block) {
 // Split route: folds a column's segments; one wave per column. Beside chunks a
 // wave takes every G-th column of a request, most of which have no more (30
 // single tokens beside two chunks 4.8 us, 10.0 with a wave per column).
-template <typename T, int D, int V>
+template <typename T, int D, int V, int SEG>
 __global__ void __launch_bounds__(256) combine_kernel(Args p) {
-  using G = Geo<T, D, V>;
   constexpr int NV = (V + 127) / 128;
   if ((int)blockIdx.x < p.fill_blocks) {
     fill<T, V>(p, blockIdx.x);
@@ -942,7 +941,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Args p) {
   auto fold = [&](int cc) __attribute__((always_inline)) {
     // The columns that shared a workgroup, and with them its segments.
     const int c0 = cc & -p.nc, clast = (c0 + p.nc < ncol ? c0 + p.nc : ncol) - 1;
-    const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, G::kSeg);
+    const Walk w = walk(p, rq.n - rq.L + c0 / p.G, rq.n - rq.L + clast / p.G, SEG);
     const int n = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
     const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
     const int64_t slot = (int64_t)xh * p.nseg.d * p.ccap.d + cc;  // segments ccap apart
@@ -1369,8 +1368,8 @@ Kernels kernels_of() {
   k.split32 = split_kernel<T, D, V, 32, false>;
   k.split16_one = split_kernel<T, D, V, 16, true>;
   k.split32_one = split_kernel<T, D, V, 32, true>;
-  k.combine = combine_kernel<T, D, V>;
   using G = Geo<T, D, V>;
+  k.combine = combine_kernel<T, D, V, G::kSeg>;
   k.seg = G::kSeg, k.pass = 4 * G::kStep;
   k.row_us = G::row_us();
   k.seg16_us = G::seg_us(16), k.seg32_us = G::seg_us(32);

@@ -1,0 +1,4 @@
+// Attention over a paged cache of 8 bits for D = 128, V = 128 (bi_paged_q8_attn_kernel.h).
+#include "bi_paged_q8_attn_kernel.h"
+
+BI_PAGED_Q8_KERNELS(128, 128)

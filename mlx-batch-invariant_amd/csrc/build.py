@@ -22,9 +22,10 @@ LIB = os.path.join(PKG_ROOT, "mlx_batch_invariant", "libbi.so")
 # Attention: one instantiation unit per built head-dim pair (BI_SDPA_DIM_PAIRS).
 SDPA_MFMA_UNITS = sorted(f for f in os.listdir(HERE)
                          if f.startswith("bi_sdpa_mfma_d") and f.endswith(".hip"))
-# Paged and windowed attention: one unit per head-dim pair (BI_PAGED_DIM_PAIRS).
+# Paged and windowed attention: one unit per head-dim pair (BI_PAGED_DIM_PAIRS),
+# and one over a cache of 8 bits.
 PAGED_UNITS = sorted(f for f in os.listdir(HERE)
-                     if f.startswith("bi_paged_attn_d") and f.endswith(".hip"))
+                     if f.startswith(("bi_paged_attn_d", "bi_paged_q8_attn_d")) and f.endswith(".hip"))
 SOURCES = ["bi_abi.cpp", "bi_gemm.hip", "bi_gemm_f32.hip", "bi_gemm_f16.hip", "bi_gemm_bf16.hip",
            "bi_qgemm_f16.hip", "bi_qgemm_bf16.hip", "bi_sdpa.hip", *SDPA_MFMA_UNITS,
            "bi_paged.hip", "bi_paged_q8.hip", "bi_rotary.hip", "bi_logprobs.hip", "bi_paged_attn.hip",

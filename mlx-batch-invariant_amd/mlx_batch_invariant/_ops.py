@@ -193,3 +193,22 @@ def _token_logprobs_fake(logits, tokens, top):
     return (logits.new_empty(tokens.shape, **f32), logits.new_empty(tokens.shape, **f32),
             logits.new_empty((*tokens.shape, top), dtype=torch.int64),
             logits.new_empty((*tokens.shape, top), **f32))
+
+
+@torch.library.custom_op("mlx_bi::paged_attention_q8", mutates_args=())
+def paged_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       block_tables: torch.Tensor, query_start: torch.Tensor,
+                       seq_lens: torch.Tensor, max_query: int, max_seq: int, scale: float,
+                       window: int, sink_tokens: int, sinks: Optional[torch.Tensor],
+                       k_scales: torch.Tensor, v_scales: torch.Tensor) -> torch.Tensor:
+    from . import _paged
+
+    return _paged._paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens,
+                               max_query, max_seq, scale, window, sink_tokens, sinks, k_scales,
+                               v_scales)
+
+
+@paged_attention_q8.register_fake
+def _paged_attention_q8_fake(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_query,
+                             max_seq, scale, window, sink_tokens, sinks, k_scales, v_scales):
+    return q.new_empty((q.shape[0], q.shape[1], v_cache.shape[3]))

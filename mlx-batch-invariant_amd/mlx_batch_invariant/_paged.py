@@ -369,7 +369,8 @@ def _attention_options(q, D, V, H, Hkv, scale, window, sink_tokens, sinks):
 
 
 def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *, max_query=None,
-                    max_seq=None, scale=None, window=None, sink_tokens=0, sinks=None):
+                    max_seq=None, scale=None, window=None, sink_tokens=0, sinks=None, k_scales=None,
+                    v_scales=None):
     """Causal attention of a step's tokens over a paged cache that holds their
     keys and values already.
 
@@ -389,11 +390,21 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     ``max_query`` and ``max_seq`` bound the requests' new tokens and lengths
     (by default T and the table's capacity). The launch is sized by them, so
     tight bounds are faster; a request beyond one gets NaN.
+
+    ``k_scales`` and ``v_scales`` (num_pages, Hkv, page_size) float32 go with
+    int8 caches (:func:`paged_cache_update`); q is then float16 or bfloat16. Any
+    strides will do, 0 for one scale a page or a head. The bits are as
+    independent of the call as without scales, and another's: the products are
+    of codes.
     """
-    _cache_shapes(k_cache, v_cache)
+    _cache_shapes(k_cache, v_cache, k_scales, v_scales)
     if q.ndim != 3:
         raise ValueError("q must be (tokens, H, head dim), got %s" % (tuple(q.shape),))
-    if q.dtype != k_cache.dtype:
+    if k_scales is not None:
+        if q.dtype == torch.float32:
+            raise NotImplementedError("float32 queries over int8 caches are not built (float16 and "
+                                      "bfloat16 are)")
+    elif q.dtype != k_cache.dtype:
         raise ValueError("q must share the caches' dtype %s, got %s" % (k_cache.dtype, q.dtype))
     T, H, D = q.shape
     P, Hkv, page, Dk = k_cache.shape
@@ -416,13 +427,20 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     if torch.compiler.is_compiling():
         from . import _ops  # noqa: F401  (registers the ops)
 
+        if k_scales is not None:
+            return torch.ops.mlx_bi.paged_attention_q8(*args, k_scales, v_scales)
         return torch.ops.mlx_bi.paged_attention(*args)
-    return _paged_eager(*args)
+    return _paged_eager(*args, k_scales, v_scales)
 
 
 @functools.lru_cache(maxsize=1024)
 def _paged_bytes(device, *sizes):
     return _lib.lib().bi_paged_attention_workspace(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_q8_bytes(device, *sizes):
+    return _lib.lib().bi_paged_attention_q8_workspace(*sizes)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -443,14 +461,14 @@ def _workspace(need, device):
 
 
 def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_query, max_seq,
-                 scale, window, sink_tokens, sinks):
+                 scale, window, sink_tokens, sinks, k_scales=None, v_scales=None):
     dev = q.device
     _on_one_gpu("paged_attention", dev, (k_cache, v_cache, block_tables, query_start, seq_lens,
-                                         sinks))
+                                         sinks, k_scales, v_scales))
     kp, kh, kn, _ = k_cache.stride()
     vp, vh, vn, _ = v_cache.stride()
     ka, va = k_cache.data_ptr(), v_cache.data_ptr()
-    if (kp | kh | kn | vp | vh | vn) * q.element_size() % 16 or (ka | va) % 16:
+    if (kp | kh | kn | vp | vh | vn) * k_cache.element_size() % 16 or (ka | va) % 16:
         raise ValueError("the caches must be 16-byte aligned, with strides of multiples of 16 bytes")
     T, H, D = q.shape
     P, Hkv, page, V = v_cache.shape
@@ -463,6 +481,16 @@ def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_q
     qt, qh, _ = q.stride()
     st = _I64x9(qt, qh, kp, kh, kn, vp, vh, vn, _table(block_tables))
     dt = _lib.DTYPE_CODES[q.dtype]
+    if k_scales is not None:
+        need = _paged_q8_bytes(dev, T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt)
+        ws = _workspace(need, dev)
+        sst = _I64x6(*k_scales.stride(), *v_scales.stride())
+        _call(dev, "bi_paged_attention_q8", _lib.lib().bi_paged_attention_q8, q.data_ptr(), ka, va,
+              k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(),
+              query_start.data_ptr(), seq_lens.data_ptr(), _at(sinks), out.data_ptr(), T, R, H, Hkv, D,
+              V, P, page, W, st, sst, scale, window, sink_tokens, max_query, max_seq, dt, _at(ws),
+              0 if ws is None else need)
+        return out
     need = _paged_bytes(dev, T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt)
     ws = _workspace(need, dev)
     _call(dev, "bi_paged_attention", _lib.lib().bi_paged_attention, q.data_ptr(), ka, va,

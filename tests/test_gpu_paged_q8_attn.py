@@ -1,0 +1,457 @@
+"""Attention over an 8-bit paged cache on the GPU against 64 bits, and the bits
+that may not change."""
+
+import numpy as np
+import pytest
+import torch
+
+import mlx_batch_invariant as bi
+from mlx_batch_invariant import _paged
+
+from helpers import bits
+from paged_ref import UNIT, starts
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+NAN, INF = float("nan"), float("inf")
+DIMS = [(64, 64), (96, 96), (128, 128), (192, 128), (192, 192), (256, 256)]
+
+
+def same(a, b):
+    return bool((bits(a) == bits(b)).all())
+
+
+def rows(q, k, v, n, window=0, first=0, scale=None, sinks=None, seen=None):
+    """Attention of the last L of n rows in float64 and its tolerance: q (L, H,
+    D); k = (codes (n, Hkv, D), scales (n, Hkv)), v alike; CPU tensors. `seen`
+    (n,) hides rows."""
+    dtype, (L, H, D), V = q.dtype, q.shape, v[0].shape[2]
+    Hkv = k[0].shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    q = q.double()
+    pos, key = torch.arange(n - L, n)[:, None], torch.arange(n)[None]
+    see = key <= pos
+    if window:
+        see = see & ((key > pos - window) | (key < first))
+    if seen is not None:
+        see = see & seen[None]
+    out = torch.zeros(L, H, V, dtype=torch.float64)
+    tol = torch.zeros(L, H, V, dtype=torch.float64)
+    if n == 0:
+        return out, tol
+    u, e32 = UNIT[dtype], 2.0 ** -24
+    for h in range(H):
+        g = h * Hkv // H
+        some = see.any(0)  # a row hidden from all may hold anything
+        kh = torch.where(some[:, None], k[0][:, g].double() * k[1][:, g].double()[:, None], 0.0)
+        vh = torch.where(some[:, None], v[0][:, g].double() * v[1][:, g].double()[:, None], 0.0)
+        s = q[:, h] @ kh.T * scale
+        mag = (q[:, h].abs() @ kh.abs().T * abs(scale)).masked_fill(~see, 0).amax(1)
+        s = s.masked_fill(~see, -INF)
+        top = s.amax(1)
+        if sinks is not None:
+            top = torch.maximum(top, sinks[h].double())
+        top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+        e = torch.exp(s - top[:, None])
+        den = e.sum(1)
+        if sinks is not None:
+            den = den + torch.exp(sinks[h].double() - top)
+        w = torch.where(den[:, None] > 0, e / den.clamp(min=1e-300)[:, None], 0.0)
+        out[:, h] = w @ vh
+        # A score is off by its fp32 sum (D roundings of at most `mag`, the
+        # products of codes being exact), the row's factor (the scale times log2
+        # e, and that times the row's: 3) and the product and subtraction of the
+        # base (3), and exp2 (2); p by that. A weight's numerator is off by that,
+        # its product with the row's scale and its rounding to the type (f16: of p
+        # times at most 2, below 2^-14 by 2^-25, beside codes times the scale's
+        # power of two, 2^-14 at least, and against a denominator of at least
+        # 2^-4); the denominator sums what was not rounded. Sums over n rows cost
+        # n roundings each and a fold's few, numerator and denominator; the result
+        # is rounded once.
+        delta = (D + 6) * e32 * mag + 2 * e32
+        part = u + 2 * delta + (2 * n + 16) * e32
+        tol[:, h] = 1.01 * u * out[:, h].abs() + 1.01 * part[:, None] * (w @ vh.abs()) + 1e-30
+        if dtype == F16:
+            big = max(float(vh.abs().amax()), 127 * 2.0 ** -14)
+            tol[:, h] += n * 2.0 ** -21 * big + 2.0 ** -25  # the result's own half step
+    return out, tol
+
+
+def draw(n, Hkv, D, V, seed, spread=0.5):
+    """A request's keys and values: ((codes, scales), (codes, scales))."""
+    g = torch.Generator().manual_seed(seed)
+    side = lambda d: ((torch.randn(n, Hkv, d, generator=g) * 40).round().clamp(-127, 127).to(torch.int8),
+                      torch.exp(torch.randn(n, Hkv, generator=g) * spread) / 40)
+    return side(D), side(V)
+
+
+class Cache:
+    """Requests in an 8-bit cache with shuffled pages; what belongs to no row holds
+    codes of 99 and scales of `fill`."""
+
+    def __init__(self, kv, page, device, order="phtd", seed=0, spare=3, fill=NAN, width=None):
+        self.kv, self.page = kv, page
+        seq = [k[0].shape[0] for k, _ in kv]
+        Hkv, D, V = kv[0][0][0].shape[1], kv[0][0][0].shape[2], kv[0][1][0].shape[2]
+        g = torch.Generator().manual_seed(seed)
+        need = [-(-n // page) for n in seq]
+        pages = sum(need) + spare
+        perm = torch.randperm(pages, generator=g).to(torch.int32)
+        table = torch.full((len(seq), max(need + [1]) if width is None else width), -1, dtype=torch.int32)
+        kc = torch.full((pages, page, Hkv, D), 99, dtype=torch.int8)
+        vc = torch.full((pages, page, Hkv, V), 99, dtype=torch.int8)
+        ks, vs = torch.full((pages, page, Hkv), fill), torch.full((pages, page, Hkv), fill)
+        at = 0
+        for r, n in enumerate(seq):
+            table[r, :need[r]] = perm[at:at + need[r]]
+            at += need[r]
+            i = torch.arange(n)
+            p = table[r][i // page].long()
+            (kc[p, i % page], ks[p, i % page]), (vc[p, i % page], vs[p, i % page]) = kv[r]
+        move = (lambda t: t.transpose(1, 2).contiguous().to(device)) if order == "phtd" else \
+            (lambda t: t.to(device).transpose(1, 2))
+        self.k, self.v, self.ks, self.vs = move(kc), move(vc), move(ks), move(vs)
+        self.table = table.to(device)
+        self.lens = torch.tensor(seq, dtype=torch.int32, device=device)
+
+    def __call__(self, q, new, **kw):
+        kw = dict(dict(k_scales=self.ks, v_scales=self.vs), **kw)
+        dev = self.k.device
+        return bi.paged_attention(q.to(dev), self.k, self.v, self.table, starts(new, dev), self.lens, **kw)
+
+
+def check(got, want, tol, what=""):
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), "%s error %g at tolerance %g" % (
+        what, (err - tol).max(), tol.flatten()[(err - tol).argmax()])
+
+
+def queries(T, H, D, dtype, seed):
+    return torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# Requests (length, new tokens): one token, first tokens, lengths around the
+# tiles and segments of the kernels, chunks past a column tile.
+MIXED = [(1, 1), (31, 1), (33, 2), (64, 64), (65, 1), (127, 3), (128, 1), (129, 7), (255, 1), (257, 5),
+         (300, 300), (513, 40), (0, 0), (40, 0), (777, 1), (1030, 9)]
+
+
+@pytest.mark.parametrize("route", ["split", "whole"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D, V, H, Hkv", [(64, 64, 8, 8), (96, 96, 6, 2), (128, 128, 32, 8), (192, 128, 4, 4),
+                                          (192, 192, 3, 1), (256, 256, 16, 2)])
+def test_mixed(cuda, D, V, H, Hkv, dtype, route, monkeypatch):
+    if route == "whole":
+        monkeypatch.setattr(_paged, "_workspace", lambda need, device: None)
+    seq, new = zip(*MIXED)
+    kv = [draw(n, Hkv, D, V, 100 + n) for n in seq]
+    c = Cache(kv, 16, cuda)
+    q = queries(sum(new), H, D, dtype, 1)
+    got = c(q, new)
+    t = 0
+    for r, (n, L) in enumerate(MIXED):
+        check(got[t:t + L], *rows(q[t:t + L], *kv[r], n), "request %d" % r)
+        t += L
+
+
+@pytest.mark.parametrize("window, first, scale, sink", [
+    (1, 0, None, False), (100, 0, None, True), (64, 4, 0.3, False), (257, 300, None, False),
+    (5000, 2, -0.1, True), (40, 65, None, True), (0, 0, None, True)])
+@pytest.mark.parametrize("dtype, page, order", [(BF16, 16, "pthd"), (F16, 40, "phtd"), (BF16, 3, "phtd")])
+def test_windows(cuda, dtype, page, order, window, first, scale, sink):
+    cases = [(1, 1), (100, 100), (400, 33), (600, 1), (900, 4), (1300, 130)]
+    seq, new = zip(*cases)
+    H, Hkv, D = 8, 2, 64
+    kv = [draw(n, Hkv, D, D, n) for n in seq]
+    c = Cache(kv, page, cuda, order)
+    q = queries(sum(new), H, D, dtype, 2)
+    sinks = (queries(1, 1, H, dtype, 3)[0, 0] * 3) if sink else None
+    got = c(q, new, window=window or None, sink_tokens=first, scale=scale,
+            sinks=None if sinks is None else sinks.to(cuda))
+    t = 0
+    for r, (n, L) in enumerate(cases):
+        check(got[t:t + L], *rows(q[t:t + L], *kv[r], n, window, first, scale, sinks), "request %d" % r)
+        t += L
+
+
+def test_many_heads_share_one(cuda):
+    cases = [(300, 1), (70, 3)]
+    seq, new = zip(*cases)
+    kv = [draw(n, 1, 64, 64, n) for n in seq]
+    q = queries(4, 71, 64, BF16, 4)
+    got = Cache(kv, 16, cuda)(q, new)
+    check(got[:1], *rows(q[:1], *kv[0], 300))
+    check(got[1:], *rows(q[1:], *kv[1], 70))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_scores(cuda, dtype):
+    """Scores far from 0, growing and falling along the keys: the running base has
+    to follow them, across segments too."""
+    n, D = 1500, 64
+    for name, ramp in (("up", torch.linspace(-300, 300, n)), ("down", torch.linspace(300, -300, n)),
+                       ("far", torch.full((n,), -5000.0))):
+        (kc, ks), v = draw(n, 2, D, D, 6)
+        kc = (kc.float() * 0.05).round().to(torch.int8)
+        kc[..., 0] = torch.where(ramp >= 0, 100, -100).to(torch.int8)[:, None]
+        ks = (ramp.abs() / 100)[:, None].expand(n, 2).contiguous()
+        q = torch.zeros(3, 2, D, dtype=dtype)
+        q[..., 0] = 8.0
+        got = Cache([((kc, ks), v)], 16, cuda)(q, [3])
+        check(got, *rows(q, (kc, ks), v, n), name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("L", [1, 40, 200])
+def test_scales_of_any_size(cuda, dtype, L):
+    """Zeros, and scales of 2^-60 to 2^60 beside each other in keys (with queries
+    as small) and values."""
+    n, H, Hkv, D = 700, 8, 2, 128
+    (kc, ks), (vc, vs) = draw(n, Hkv, D, D, 8)
+    g = torch.Generator().manual_seed(2)
+    for s in (ks, vs):
+        s[torch.rand(n, Hkv, generator=g) < 0.1] = 0.0
+    if dtype == BF16:
+        vs *= 2.0 ** torch.randint(-60, 61, (n, Hkv), generator=g).float()
+    else:
+        vs *= 2.0 ** torch.randint(-20, 9, (n, Hkv), generator=g).float()
+    q = queries(L, H, D, dtype, 3)
+    got = Cache([((kc, ks), (vc, vs))], 16, cuda)(q, [L])
+    check(got, *rows(q, (kc, ks), (vc, vs), n))
+    ks *= 2.0 ** 40
+    got = Cache([((kc, ks), (vc, vs))], 16, cuda)(q, [L], scale=D ** -0.5 * 2.0 ** -40)
+    check(got, *rows(q, (kc, ks), (vc, vs), n, scale=D ** -0.5 * 2.0 ** -40))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [NAN, INF, -1.0])
+def test_rows_reach_only_tokens_that_see_them(cuda, dtype, bad):
+    """A row whose scales are NaN, infinite or (keys) negative spoils the tokens
+    that see it and leaves the bits of the others, on both routes."""
+    n, L, H, Hkv, D = 900, 200, 8, 2, 128
+    (kc, ks), (vc, vs) = draw(n, Hkv, D, D, 5)
+    q = queries(L, H, D, dtype, 3)
+    base = Cache([((kc, ks), (vc, vs))], 16, cuda)(q, [L])
+    row = n - 77
+    for side in ("k", "v"):
+        if side == "v" and bad == -1.0:
+            continue
+        k2, v2 = ks.clone(), vs.clone()
+        (k2 if side == "k" else v2)[row, 1] = bad
+        c = Cache([((kc, k2), (vc, v2))], 16, cuda)
+        for new in (L, 40):
+            got = c(q[L - new:], [new])
+            b = base[L - new:]
+            hit = torch.zeros(new, H, dtype=torch.bool, device=cuda)
+            hit[max(0, new - 77):, 4:] = True
+            assert same(got[~hit], b[~hit])
+            if side == "k" and bad == INF:  # a score of -inf has weight 0; else NaN
+                hit &= (q[L - new:].double() @ kc[row, 1].double() >= 0).to(cuda)
+                assert bool(hit.any())
+            if not (side == "v" and bad == INF):  # (infinite values give infinities or NaN)
+                assert bool((got.isnan().any(-1) == hit).all())
+            assert bool((~got.isfinite()).any(-1)[hit].all())
+
+
+@pytest.mark.parametrize("per", ["page", "head", "all"])
+def test_scales_of_blocks(cuda, per):
+    """One scale for a page, a head or all, as views of stride 0."""
+    n, H, Hkv, D, page = 300, 8, 4, 64, 32
+    (kc, _), (vc, _) = draw(n, Hkv, D, D, 3)
+    c = Cache([((kc, torch.ones(n, Hkv)), (vc, torch.ones(n, Hkv)))], page, cuda)
+    P = c.k.shape[0]
+    g = torch.Generator().manual_seed(1)
+    at = {"page": (P, Hkv, 1), "head": (1, Hkv, 1), "all": (1, 1, 1)}[per]
+    sk, sv = (torch.exp(torch.randn(at, generator=g) * 0.5).to(cuda) / 40 for _ in range(2))
+    sk, sv = sk.expand(P, Hkv, page), sv.expand(P, Hkv, page)
+    i = torch.arange(n, device=cuda)
+    p = c.table[0].long()[i // page]
+    k, v = (kc, sk[p, :, i % page].cpu()), (vc, sv[p, :, i % page].cpu())
+    for L in (1, 77):
+        q = queries(L, H, D, BF16, L)
+        check(c(q, [L], k_scales=sk, v_scales=sv), *rows(q, k, v, n))
+
+
+# --------------------------------------------------------------------- bits
+
+
+@pytest.mark.parametrize("window, first", [(0, 0), (150, 5)])
+@pytest.mark.parametrize("dtype, D, V, H, Hkv", [(BF16, 128, 128, 32, 8), (F16, 64, 64, 8, 8),
+                                                 (F16, 128, 128, 8, 2), (BF16, 256, 256, 4, 2),
+                                                 (BF16, 96, 96, 16, 1), (F16, 192, 128, 8, 2),
+                                                 (BF16, 192, 192, 4, 4)])
+def test_bits_do_not_depend_on_the_call(cuda, dtype, D, V, H, Hkv, window, first, monkeypatch):
+    """A request of 700 rows whose last 300 tokens are new: as one chunk, in
+    chunks, token by token, between other requests, with and without a
+    workspace, over other pages."""
+    n, L = 700, 300
+    kv = draw(n, Hkv, D, V, D)
+    q = queries(L, H, D, dtype, 7).to(cuda)
+    kw = dict(window=window or None, sink_tokens=first)
+    c = Cache([kv], 16, cuda)
+    base = c(q, [L], **kw)
+    assert same(Cache([kv], 37, cuda, "pthd", seed=2, fill=0.5)(q, [L], **kw), base)
+    # In pieces: the keys behind a piece are in the cache already, unseen.
+    for ws in (True, False):
+        if not ws:
+            monkeypatch.setattr(_paged, "_workspace", lambda need, device: None)
+            assert same(c(q, [L], **kw), base)
+        at = 0
+        for piece in (1, 2, 5, 8, 31, 33, 1, 64, 100, 55):
+            c.lens.fill_(n - L + at + piece)
+            y = c(q[at:at + piece], [piece], **kw)
+            assert same(y, base[at:at + piece]), piece
+            y = c(q[at:at + piece], [piece], max_query=piece, max_seq=n - L + at + piece, **kw)
+            assert same(y, base[at:at + piece]), piece
+            at += piece
+        c.lens.fill_(n)
+    monkeypatch.undo()
+    # Between others, which bring one token, a chunk, nothing.
+    others = [(50, 1), (n, L), (900, 200), (n, 1), (5, 0), (n, 7)]
+    seq, new = zip(*others)
+    m = Cache([kv if s == n else draw(s, Hkv, D, V, s) for s in seq], 16, cuda, seed=3)
+    qm = torch.cat([q[L - k:] if s == n else queries(k, H, D, dtype, s).to(cuda) for s, k in others])
+    y = m(qm, new, **kw)
+    t = 0
+    for s, k in others:
+        if s == n:
+            assert same(y[t:t + k], base[L - k:]), k
+        t += k
+
+
+@pytest.mark.parametrize("D, V", DIMS)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("window", [None, 190, 1100])
+def test_bits_of_every_launch(cuda, dtype, D, V, window):
+    """A prompt, halves of it, chunks and single tokens: the same rows, the same
+    bits, by every kernel."""
+    H, Hkv, n, page = 32, 8, 2200, 64
+    g = torch.Generator(device=cuda).manual_seed(D + V)
+    q = torch.randn(n, H, D, generator=g, device=cuda).to(dtype)
+    k, v = (torch.randn(n, Hkv, d, generator=g, device=cuda) for d in (D, V))
+    P = -(-n // page)
+    table = torch.randperm(P, generator=g, device=cuda).to(torch.int32)[None]
+    kc, vc = (torch.zeros(P, Hkv, page, d, dtype=torch.int8, device=cuda) for d in (D, V))
+    ks, vs = torch.zeros(P, Hkv, page, device=cuda), torch.zeros(P, Hkv, page, device=cuda)
+    i = torch.arange(n, device=cuda)
+    slots = (table[0, i // page] * page + i % page).to(torch.int32)
+    bi.paged_cache_update(k, v, kc, vc, slots, k_scales=ks, v_scales=vs)
+    run = lambda lo, hi: bi.paged_attention(
+        q[lo:hi], kc, vc, table, starts([hi - lo], cuda), torch.tensor([hi], dtype=torch.int32, device=cuda),
+        window=window, sink_tokens=3, k_scales=ks, v_scales=vs)
+    base = run(0, n)
+    for lo, hi in ((0, 1100), (1100, 2200), (700, 1000), (2100, 2200), (2195, 2200), (2000, 2001), (0, 1)):
+        assert same(run(lo, hi), base[lo:hi]), (lo, hi)
+    back, vback = bi.paged_cache_read(kc, vc, slots, k_scales=ks, v_scales=vs)
+    side = lambda c, s, x: ((x / s.transpose(1, 2).flatten(0, 1)[slots.long()][..., None]).round().to(torch.int8).cpu(),
+                            s.transpose(1, 2).flatten(0, 1)[slots.long()].cpu())
+    kk, vv = side(kc, ks, back), side(vc, vs, vback)
+    for lo, hi in ((0, 5), (1500, 1503), (2190, 2200)):
+        check(base[lo:hi], *rows(q[lo:hi].cpu(), (kk[0][:hi], kk[1][:hi]), (vv[0][:hi], vv[1][:hi]), hi,
+                                 window or 0, 3), "rows %d" % lo)
+
+
+# -------------------------------------------------------------------- edges
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_pages_that_are_not_there(cuda, dtype):
+    """Entries below 0, past the cache and past the table hide their rows."""
+    n, page = 600, 16
+    kv = [draw(n, 2, 64, 64, r) for r in (1, 2)]
+    c = Cache(kv, page, cuda)
+    q = queries(41, 4, 64, dtype, 2)
+    seen = torch.ones(n, dtype=torch.bool)
+    for j, bad in ((0, -1), (1, -2 ** 31), (9, c.k.shape[0]), (20, 2 ** 31 - 1), (37, -1)):
+        c.table[:, j] = bad
+        seen[j * page:(j + 1) * page] = False
+    got = c(q, [40, 1])
+    check(got[:40], *rows(q[:40], *kv[0], n, seen=seen))
+    check(got[40:], *rows(q[40:], *kv[1], n, seen=seen))
+    # A table narrower than the sequence; one of no columns, where nothing is seen.
+    seen[10 * page:] = False
+    c.table = c.table[:, :10]
+    check(c(q, [40, 1], max_seq=n)[:40], *rows(q[:40], *kv[0], n, seen=seen))
+    c.table = c.table[:, :0]
+    assert bool((c(q, [40, 1], max_seq=n) == 0).all())
+
+
+def test_tokens_without_a_request_and_bounds(cuda):
+    """Padding tokens are 0, a token before every key is 0, a request beyond a
+    bound is NaN, and none of them touches another."""
+    kv = [draw(s, 2, 64, 64, s) for s in (100, 3, 500)]
+    c = Cache(kv, 16, cuda)
+    q = queries(60, 4, 64, BF16, 2).to(cuda)
+    qs = torch.tensor([5, 15, 20, 50], dtype=torch.int32, device=cuda)
+    run = lambda **kw: bi.paged_attention(q, c.k, c.v, c.table, qs, c.lens, k_scales=c.ks, v_scales=c.vs, **kw)
+    y = run()
+    assert bool((y[:5] == 0).all()) and bool((y[50:] == 0).all())
+    assert bool((y[15:17] == 0).all())  # five tokens of a request of three rows
+    check(y[5:15], *rows(q[5:15].cpu(), *kv[0], 100))
+    check(y[17:20], *rows(q[17:20].cpu(), *kv[1], 3))
+    check(y[20:50], *rows(q[20:50].cpu(), *kv[2], 500))
+    z = run(max_query=29, max_seq=100)
+    assert bool(z[20:50].isnan().all()) and same(z[:20], y[:20]) and same(z[50:], y[50:])
+    none = q[:0]
+    assert bi.paged_attention(none, c.k, c.v, c.table, qs * 0, c.lens, k_scales=c.ks, v_scales=c.vs).shape == (0, 4, 64)
+
+
+def test_far_rows(cuda):
+    """Pages past 2^31 bytes, and scales past 2^31 elements, from the cache's start."""
+    page, Hkv, D, n = 64, 1, 64, 200
+    pages = (1 << 31) // (page * D) + 40
+    kc = torch.empty(pages, Hkv, page, D, dtype=torch.int8, device=cuda)
+    vc = torch.empty(pages, Hkv, page, D, dtype=torch.int8, device=cuda)
+    wide = torch.empty(pages, Hkv, page, 65, device=cuda)  # 8.7 GB
+    ks, vs = wide[..., 0], wide[..., 64]
+    k, v = draw(n, Hkv, D, D, 4)
+    far = torch.tensor([[pages - 1, 3, pages - 7, pages - 20]], dtype=torch.int32, device=cuda)
+    i = torch.arange(n, device=cuda)
+    p = far[0].long()[i // page]
+    for cache, scales, (code, s) in ((kc, ks, k), (vc, vs, v)):
+        cache[p, :, i % page], scales[p, :, i % page] = code.to(cuda), s.to(cuda)
+    for L in (1, 150):
+        q = queries(L, 4, D, BF16, L)
+        got = bi.paged_attention(q.to(cuda), kc, vc, far, starts([L], cuda),
+                                 torch.tensor([n], dtype=torch.int32, device=cuda), k_scales=ks, v_scales=vs)
+        check(got, *rows(q, k, v, n))
+
+
+def test_on_two_streams_and_in_a_graph(cuda):
+    """Two calls at once, each with a workspace of its own; a captured one is
+    replayed with other lengths."""
+    kv = [draw(1500, 2, 128, 128, 1), draw(600, 2, 128, 128, 2)]
+    c = Cache(kv, 16, cuda)
+    q = queries(9, 8, 128, BF16, 2).to(cuda)
+    want = c(q, [1, 8])
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(10):
+        for s in (a, b):
+            with torch.cuda.stream(s):
+                got.append(c(q, [1, 8]))
+    torch.cuda.synchronize()
+    assert all(same(g, want) for g in got)
+    with torch.cuda.stream(a):
+        qs = starts([1, 8], cuda)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=a):
+            y = bi.paged_attention(q, c.k, c.v, c.table, qs, c.lens, max_query=8, k_scales=c.ks, v_scales=c.vs)
+    for lens in ([1500, 600], [3, 9], [700, 8], [1500, 600]):
+        c.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        w = bi.paged_attention(q, c.k, c.v, c.table, qs, c.lens, max_query=8, k_scales=c.ks, v_scales=c.vs)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(y, w), lens
+
+
+def test_compiles(cuda):
+    c = Cache([draw(300, 2, 64, 64, 1)], 16, cuda)
+    q = queries(5, 4, 64, F16, 2).to(cuda)
+    qs = starts([5], cuda)
+    fn = lambda q: bi.paged_attention(q, c.k, c.v, c.table, qs, c.lens, window=70, k_scales=c.ks, v_scales=c.vs)
+    got = torch.compile(fn, fullgraph=True, backend="aot_eager")(q)
+    assert same(got, fn(q))
