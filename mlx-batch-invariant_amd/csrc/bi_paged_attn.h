@@ -49,10 +49,12 @@ struct Args {
   int32_t once;           // keys and values are read by one of these only
   int32_t split_cols;     // requests of at most this many columns are split
   int32_t fill_blocks;    // workgroups that fill tokens no kernel computes
-  // A cache of 8 bits: its scales and their element strides (page, head, row).
+  // A cache of 8 bits: its scales, and byte strides below 2^32 (page, row) and of
+  // the heads; for keys and values those above are not used.
   const float* ks;
   const float* vs;
-  int64_t ksb, ksh, ksn, vsb, vsh, vsn;
+  uint32_t k8b, k8n, v8b, v8n, ksb, ksn, vsb, vsn;
+  int64_t ksh, vsh;
 };
 
 typedef void (*Kernel)(Args);
@@ -65,6 +67,7 @@ struct Kernels {
   Kernel whole4, whole8, whole4_pair;
   int whole4_threads;       // its loading waves among them
   int seg, pass;            // rows per segment and per pass of the split route (four steps)
+  int places = 8192;        // split workgroups with work, about: more take several segments each
   // For the choice of route, in microseconds: what a row costs a whole
   // workgroup, and a full segment the split ones of 16 and 32 columns that a
   // CU runs together, per_cu of them.

@@ -50,7 +50,8 @@ int64_t full_tiles(const Call& c, const Plan& s) {
 }
 
 // A plan that splits requests of up to `most` columns.
-Plan split_up_to(const Call& c, int64_t most, int64_t seg) {
+Plan split_up_to(const Call& c, int64_t most, const Kernels& k) {
+  const int64_t seg = k.seg;
   Plan s;
   const int64_t cols = c.max_query * c.G;
   s.split_cols = most;
@@ -65,9 +66,9 @@ Plan split_up_to(const Call& c, int64_t most, int64_t seg) {
     const int64_t n = (span + seg - 2) / seg + 1 + (c.first + seg - 1) / seg;
     if (n < s.nseg) s.nseg = n;
   }
-  // Places for a request's segments: 8192 workgroups in all, not counting
+  // Places for a request's segments: k.places workgroups in all, not counting
   // columns that no token has.
-  const int64_t places = 8192 / (c.Hkv * full_tiles(c, s));
+  const int64_t places = k.places / (c.Hkv * full_tiles(c, s));
   s.gseg = places < 1 ? 1 : places < s.nseg ? places : s.nseg;
   s.bytes = c.R * c.Hkv * s.ccap * s.nseg * (c.V + 2) * (int64_t)sizeof(float);
   return s;
@@ -142,7 +143,7 @@ Plan plan(const Call& c, const Kernels& k) {
   // Bounds far above the average request: most have a few columns.
   const bool loose = cols > few && c.tokens * c.G <= c.R * (few / 2);
   if (cols <= few || (cols <= 2048 && !loose)) {
-    const Plan s = split_up_to(c, cols > few ? cols : few, k.seg);
+    const Plan s = split_up_to(c, cols > few ? cols : few, k);
     if (fits(c, s) && split(s) < whole) return s;
     if (cols <= few && whole <= split(s)) return none;
   }
@@ -150,8 +151,8 @@ Plan plan(const Call& c, const Kernels& k) {
   // two launches that find nothing, 3 to 4 us each).
   if (c.exact || c.tokens >= c.R * c.max_query) return none;
   // Beside whole chunks; where the results would take too much, single tokens.
-  Plan s = split_up_to(c, few, k.seg);
-  if (!fits(c, s)) s = split_up_to(c, c.G, k.seg);
+  Plan s = split_up_to(c, few, k);
+  if (!fits(c, s)) s = split_up_to(c, c.G, k);
   return fits(c, s) ? s : none;
 }
 
@@ -319,10 +320,18 @@ int paged_attention(const char* who, const void* q, const void* k_cache, const v
   if (q8) {
     if (((uintptr_t)k_scales | (uintptr_t)v_scales) % 4)
       return bi::fail(BI_EINVAL, "%s: scales not aligned to elements", who);
+    // Pages and rows, whose numbers a kernel multiplies row by row, in 32 bits.
+    uint32_t* const to[8] = {&p.k8b, &p.k8n, &p.v8b, &p.v8n, &p.ksb, &p.ksn, &p.vsb, &p.vsn};
+    const int64_t from[8] = {strides[2], strides[4], strides[5], strides[7], scale_strides[0] * 4,
+                             scale_strides[2] * 4, scale_strides[3] * 4, scale_strides[5] * 4};
+    for (int i = 0; i < 8; i++) {
+      if (from[i] < 0 || from[i] > UINT32_MAX)
+        return bi::fail(BI_EUNSUPPORTED, "%s: pages and rows lie less than 4 GiB apart", who);
+      *to[i] = (uint32_t)from[i];
+    }
     p.ks = k_scales;
     p.vs = v_scales;
-    p.ksb = scale_strides[0], p.ksh = scale_strides[1], p.ksn = scale_strides[2];
-    p.vsb = scale_strides[3], p.vsh = scale_strides[4], p.vsn = scale_strides[5];
+    p.ksh = scale_strides[1], p.vsh = scale_strides[4];
   }
   return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
 }

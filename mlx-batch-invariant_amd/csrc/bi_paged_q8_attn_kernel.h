@@ -10,11 +10,11 @@
 // Fixed arithmetic of a column:
 //   * Steps are of 64 rows for all head dims, eight to a segment.
 //   * A code is a whole number, which bf16 and f16 hold exactly: raw_j is a
-//     chain of 32x32x16 products of codes and the query over the head dim. The
-//     lane half h takes the codes of 16-byte chunk 2 c + h in products 2 c and 2
-//     c + 1, eight each.
+//     chain of 16x16x32 products of codes and the query over the head dim. The
+//     lanes' quarter g takes the codes of 16-byte chunk 4 c + g in products 2 c
+//     and 2 c + 1, eight each (what is left of 96 dims: of 8-byte piece 8 + g).
 //   * c_j is rounded once to 32 bits; p_j = 2^(fma(raw_j, c_j, -m)); l sums the p
-//     of 32 bits, in a fixed order per lane half.
+//     of 32 bits, in a fixed order per quarter.
 //   * bf16: the weights p_j * vs_j are rounded to bf16, whose range holds any
 //     scale: half a step of 2^-8 of a weight whose value's code is off by as much
 //     as 2^-8 of the largest. f16: the scale's power of two 2^e, kept to 2^-14 ..
@@ -22,10 +22,18 @@
 //     largest, 2^-14 its smallest normal number), and the weights p_j * (vs_j /
 //     2^e), of p's own size for scales in that range, are rounded to f16. (Scales
 //     past 2^19, of values past 6e7, overflow them.)
-// A row that a column does not see has p and weight 0 by selection, whatever its
-// codes and scales, and codes are finite: so no row's content reaches a token that
-// does not see it, and there is no case of values to look for. A negative scale
-// of keys gives NaN.
+// A row that a column does not see has the raw score -inf, and with it p and
+// weight 0, whatever its codes, which are finite. Its scales are made so too: a row
+// whose scales are infinite or NaN, or negative for keys, gets c_j above 0 and vs_j =
+// 0, and a mark by which the sum, and with it the result, of every column that sees
+// the row is NaN. So no row's content reaches a token that does not see it, and there
+// is no case of values to look for.
+//
+// (Products of 16 columns, not of 32 as in the kernels of the other types: single
+// tokens have 4 or 8, and what a wave spends its time on there is the issue of
+// vector instructions, one in 5 cycles, for conversions, exponentials and
+// addresses. Half the columns are half of these, and half the registers, so that
+// more waves share a SIMD.)
 #pragma once
 
 #include "bi_paged_attn_kernel.h"
@@ -74,60 +82,145 @@ __device__ __forceinline__ uint16_t scale_power(float vs, float& left) {
   return (uint16_t)((e + 15) << 10);
 }
 
+// The largest, and the sum, of a column's four quarters.
+__device__ __forceinline__ float quarters_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_max(__builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 template <typename T, int D_, int V_>
 struct Geo8 {
   static constexpr int D = D_, V = V_;
-  using G = Geo<T, D, V>;
-  static constexpr int kStep = 64, KT = 2, kSegSteps = 8, kSeg = kSegSteps * kStep;
+  static constexpr int kStep = 64, RT = kStep / 16, kSegSteps = 8, kSeg = kSegSteps * kStep;
   static constexpr int CH = D / 16, VCH = V / 16;  // 16-byte chunks of a row of codes
   static constexpr int MCH = CH > VCH ? CH : VCH;
-  static constexpr int NQ = D / 16;                // products of a score
-  static constexpr int DT = V / 32;
-  static constexpr int PU = 2;                     // units of eight weights per tile and lane
+  static constexpr int NQ = D / 32;                // products of a score
+  static constexpr int DT = V / 16;                // tiles of output dims
+  static constexpr int TCH = D / 8, TVCH = V / 8;  // chunks of a row in the type
   static constexpr bool kPower = __is_same(T, _Float16);  // values' codes carry 2^e
-  static constexpr bool kTwoWaves = V + D / 4 <= 160;
-  static constexpr int split_per_cu() { return D + V <= 256 ? 2 : 1; }
+  static constexpr bool kTwoWaves = V + D / 4 <= 160;     // whole route: two waves per SIMD
+  // Whole route: products of a wave's second 16 columns whose query waits in LDS
+  // (128 dims: with all in registers, of which 234 are in use at once, some were
+  // kept in scratch memory).
+  static constexpr int kFarQuery = D == 128 && V == 128 ? NQ : 0;
+  // Split route: workgroups of NC columns that a compute unit's registers hold.
+  static constexpr int split_per_cu(int NC) {
+    return NC == 16 ? (D + V <= 128 ? 4 : D + V <= 256 ? 3 : 2) : (D + V <= 128 ? 3 : D + V <= 320 ? 2 : 1);
+  }
 
   static constexpr double row_us() { return 1e-3 * (kTwoWaves ? 13.0 + 0.04 * (D + V) : 28.0 + 0.08 * (D + V)); }
   static constexpr double seg_us() { return 5.0 + 0.023 * (kSeg * (D + V) / 1024.0); }
 
-  // Codes of keys in LDS (split route): row r's chunk c at chunk c ^ kswz(r). A
-  // read takes one chunk of 16 rows per pass; the exchange spreads them over all
-  // banks.
-  __device__ __forceinline__ static int kswz(int r) {
-    if constexpr (CH % 16 == 0) return r & 15;
-    else if constexpr (CH % 8 == 0) return (r >> 1) & 7;
-    else if constexpr (CH % 4 == 0) return (r >> 2) & 3;
+  __device__ __forceinline__ static f32x4 product(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (kPower)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  // The 16-byte piece (eight dims in the type) that quarter g takes in product n.
+  __device__ __forceinline__ static int piece(int n, int g) {
+    return NQ % 2 && n + 1 == NQ ? 4 * n + g : 2 * (4 * (n >> 1) + g) + (n & 1);
+  }
+
+  // Rows in LDS, of C chunks: row r's chunk c at chunk c ^ swz<C>(r). A read takes
+  // one chunk of 16 rows per pass, which the exchange spreads over all banks.
+  template <int C> __device__ __forceinline__ static uint32_t swz(uint32_t r) {
+    if constexpr (C % 16 == 0) return r & 15;
+    else if constexpr (C % 8 == 0) return (r >> 1) & 7;
+    else if constexpr (C % 4 == 0) return (r >> 2) & 3;
     else return (r >> 3) & 1;
   }
-  // Codes of values: row r at place vplace(r), which puts the eight rows of a
-  // product's lane half side by side, its chunk c at chunk c ^ vswz(place): 32
-  // lanes read 32 bytes of eight rows per pass.
-  __device__ __forceinline__ static int vplace(int r) {
-    return (r & ~12) | ((r >> 1) & 4) | ((r << 1) & 8);
+  // Values of codes: row r at place vplace(r), which puts the eight rows of a
+  // product's quarter (4 g .. and 16 + 4 g ..) side by side.
+  __device__ __forceinline__ static uint32_t vplace(uint32_t r) {
+    return (r & 35) | ((r >> 2) & 4) | ((r << 1) & 24);
   }
-  __device__ __forceinline__ static int vswz(int at) {
-    if constexpr (VCH == 16) return (at & 7) << 1;
-    else if constexpr (VCH == 8) return ((at >> 1) & 3) << 1;
-    else if constexpr (VCH == 12 || VCH == 4) return ((at >> 2) & 1) << 1;
-    else return 0;
+  // Values in the type (whole route): a transposing read takes four rows, of two
+  // quarters 32 bytes of eight rows per pass. (The lowest bit is for the stores.)
+  __device__ __forceinline__ static uint32_t tswz(uint32_t r) {
+    if constexpr (TVCH % 16 == 0) return (r & 7) << 1 | (r & 1);
+    else if constexpr (TVCH % 8 == 0) return ((r >> 1) & 3) << 1 | (r & 1);
+    else return ((r >> 2) & 1) << 1 | (r & 1);
   }
-  // The values' operand of product u of the tile at row0, output dims 32 dt ..;
-  // `power`: 2^e by place.
-  __device__ __forceinline__ static uint4 value(const uint4* v, const uint16_t* power, int row0, int u, int dt,
-                                                int lane) {
-    const int i = lane & 15, at = row0 + 16 * u + 8 * (lane >> 5) + (i >> 1);
-    const int c = 2 * dt + ((lane >> 4) & 1);
-    const char* from = reinterpret_cast<const char*>(v + at * VCH + (c ^ vswz(at))) + 8 * (i & 1);
+  // Row and chunk of the unit that thread `t` of N takes in turn j, rows of C chunks.
+  template <int C, int N> struct Unit {
+    uint32_t row, chunk;
+    __device__ __forceinline__ Unit(int j, uint32_t t) {
+      if constexpr (N % C == 0) row = j * (N / C) + t / C, chunk = t % C;
+      else row = (j * N + t) / C, chunk = j * N + t - row * C;
+    }
+  };
+  // Byte offset in LDS of a unit that lane `t` of a wave stores in turn j. Where
+  // rows are a power of two of chunks, turns differ by constants: places and
+  // exchanges are permutations of the row number's bits.
+  template <int C, typename Place>
+  __device__ __forceinline__ static uint32_t stored(int j, uint32_t t, const Place& place) {
+    if constexpr ((C & (C - 1)) == 0) {
+      const uint32_t at = place(t / C), turn = place(j * (64 / C));
+      return ((at * C + ((t % C) ^ swz<C>(at))) * 16 ^ swz<C>(turn) * 16) + turn * C * 16;
+    } else {
+      const Unit<C, 64> x(j, t);
+      const uint32_t at = place(x.row);
+      return (at * C + (x.chunk ^ swz<C>(at))) * 16;
+    }
+  }
+  __device__ __forceinline__ static uint32_t key_stored(int j, uint32_t t) {
+    return stored<CH>(j, t, [](uint32_t r) { return r; });
+  }
+  __device__ __forceinline__ static uint32_t value_stored(int j, uint32_t t) {
+    return stored<VCH>(j, t, [](uint32_t r) { return vplace(r); });
+  }
+
+  // Products 2 c and 2 c + 1 (one: the last of an odd number) of a tile of 16 rows
+  // of codes, as operands.
+  __device__ __forceinline__ static void keys(const uint4* k, int row0, int c, uint32_t ln, uint4 (&x)[2]) {
+    const uint32_t own = ln & 15, g = ln >> 4;
+    const char* row = reinterpret_cast<const char*>(k) + row0 * CH * 16 + own * CH * 16;
+    if (NQ % 2 && 2 * c + 1 == NQ) {
+      const uint2 w = *reinterpret_cast<const uint2*>(row + ((4 * c + (g >> 1)) ^ swz<CH>(own)) * 16 + 8 * (g & 1));
+      x[0] = codes8<T>(w.x, w.y);
+    } else {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(row + ((4 * c + g) ^ swz<CH>(own)) * 16);
+      x[0] = codes8<T>(w[0], w[1]);
+      x[1] = codes8<T>(w[2], w[3]);
+    }
+  }
+  // The values' operand of product u of a step's codes, output dims 16 dt ..;
+  // `power`: 2^e by place. (The exchange depends on the lane alone.)
+  __device__ __forceinline__ static uint4 value(const uint4* v, const uint16_t* power, int u, int dt, uint32_t ln) {
+    const uint32_t own = 8 * (ln >> 4) + ((ln & 15) >> 1);
+    const char* from = reinterpret_cast<const char*>(v) + ((own * VCH + (dt ^ swz<VCH>(own))) * 16 + 8 * (ln & 1)) +
+                       32 * u * VCH * 16;
     const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)from);
     const uint4 y = codes8<T>((uint32_t)x[0], (uint32_t)x[1]);
     if constexpr (!kPower) return y;
-    else return times(y, *reinterpret_cast<const uint4*>(power + row0 + 16 * u + 8 * (lane >> 5)));
+    else return times(y, *reinterpret_cast<const uint4*>(power + 32 * u + 8 * (ln >> 4)));
   }
-  // A column's query: chunk 4 c + 2 half + j for product 2 c + j.
-  __device__ __forceinline__ static void load_query(const char* q, int half, uint4 (&out)[NQ]) {
+  // The same operands from rows in the type.
+  __device__ __forceinline__ static uint4 key_of_type(const uint4* k, int row0, int n, uint32_t ln) {
+    const uint32_t own = ln & 15;
+    return k[(row0 + own) * TCH + (piece(n, ln >> 4) ^ swz<TCH>(own))];
+  }
+  __device__ __forceinline__ static uint4 value_of_type(const uint4* v, int u, int dt, uint32_t ln) {
+    const uint32_t own = 4 * (ln >> 4) + ((ln & 15) >> 2), part = ln & 3;
+    i16x4 a[2];
 #pragma unroll
-    for (int n = 0; n < NQ; n++) out[n] = ld16(q + (4 * (n >> 1) + 2 * half + (n & 1)) * 16);
+    for (int x = 0; x < 2; x++) {  // (tswz has bits 0 to 2 of the row: rows 16 on have the same)
+      const char* at = reinterpret_cast<const char*>(v + (32 * u + 16 * x + own) * TVCH +
+                                                     ((2 * dt + (part >> 1)) ^ tswz(own))) + 8 * (part & 1);
+      a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
+    }
+    const uint2 lo = __builtin_bit_cast(uint2, a[0]), hi = __builtin_bit_cast(uint2, a[1]);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+
+  __device__ __forceinline__ static void load_query(const char* q, int g, uint4 (&out)[NQ]) {
+#pragma unroll
+    for (int n = 0; n < NQ; n++) out[n] = ld16(q + piece(n, g) * 16);
   }
   __device__ __forceinline__ static void sign_query(const Args& p, uint4 (&q)[NQ]) {
 #pragma unroll
@@ -135,100 +228,145 @@ struct Geo8 {
       q[n] = make_uint4(q[n].x ^ p.qsign, q[n].y ^ p.qsign, q[n].z ^ p.qsign, q[n].w ^ p.qsign);
   }
 
-  // c_j from a row's scale: above 0, so that an unseen row's -inf stays one.
-  __device__ __forceinline__ static float factor(const Args& p, float ks) {
-    return ks >= 0.f ? fmaxf(ks * p.scale2, 1.2e-38f) : NAN;
+  // A row's c_j, above 0 so that an unseen row's -inf stays one, and what its
+  // values' weights are multiplied with; whether it spoils what sees it.
+  __device__ __forceinline__ static bool factors(const Args& p, float ks, float vs, float& c, float& left, uint16_t& power) {
+    c = ks * p.scale2;
+    const bool good = ks >= 0.f && c < INFINITY && fabsf(vs) < INFINITY;
+    c = good ? fmaxf(c, 1.2e-38f) : 1.f;
+    left = good ? vs : 0.f;
+    if constexpr (kPower) power = scale_power(left, left);
+    return !good;
   }
-  // The rows' numbers of a tile's elements 4 b .. 4 b + 3 from LDS.
-  __device__ __forceinline__ static f32x4 rows4(const float* at, int kt, int b, int half) {
-    return *reinterpret_cast<const f32x4*>(at + 32 * kt + 8 * b + 4 * half);
+  // Element i of row tile t is row 16 t + 4 g + i; `seen` is shifted by 4 g.
+  __device__ __forceinline__ static f32x4 rows4(const float* at, int t, int g) {
+    return *reinterpret_cast<const f32x4*>(at + 16 * t + 4 * g);
   }
-  // The largest score; `seen` (shifted by the half's four rows) says which count.
-  template <bool FULL>
-  __device__ __forceinline__ static float top(const f32x16 (&s)[KT], const float* c, int half, uint64_t seen) {
-    float m = -INFINITY;
+  // Scores of unseen rows become -inf.
+  template <int CT> __device__ __forceinline__ static void hide(f32x4 (&s)[RT][CT], const uint64_t (&seen)[CT]) {
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-      const uint32_t w = (uint32_t)(seen >> (32 * kt));
+    for (int t = 0; t < RT; t++)
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const f32x4 f = rows4(c, kt, b, half);
+      for (int k = 0; k < CT; k++) {
+        const uint32_t w = (uint32_t)(seen[k] >> (16 * t));
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float x = s[kt][4 * b + i] * f[i];
-          if (!FULL) x = w & (1u << (8 * b + i)) ? x : -INFINITY;
-          m = __builtin_elementwise_maximum(m, x);
-        }
+        for (int i = 0; i < 4; i++) s[t][k][i] = w & (1u << i) ? s[t][k][i] : -INFINITY;
+      }
+  }
+  // The largest scores of CT column tiles.
+  template <int CT>
+  __device__ __forceinline__ static void top(const f32x4 (&s)[RT][CT], const float* c, int g, float (&m)[CT]) {
+#pragma unroll
+    for (int k = 0; k < CT; k++) m[k] = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const f32x4 f = rows4(c, t, g);
+#pragma unroll
+      for (int k = 0; k < CT; k++) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = s[t][k][i] * f[i];
+        m[k] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m[k], x[0]), x[1]);
+        m[k] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m[k], x[2]), x[3]);
       }
     }
-    return half_swap_max(m);
+#pragma unroll
+    for (int k = 0; k < CT; k++) m[k] = quarters_max(m[k]);
   }
-  // A step's weights in the type, and the lane's sum of p: a chain for eight
-  // rows, then these in pairs. (Eight rows at a time: else the compiler reads
-  // all factors first, into registers that there are not.)
-  template <bool FULL>
-  __device__ __forceinline__ static float weights(const f32x16 (&s)[KT], const float* c, const float* vs,
-                                                  int half, uint64_t seen, float m, uint4 (&u)[KT][PU]) {
-    float sum[KT * PU];
+  // A step's weights in the type, and the lane's sums of p: a chain for the eight
+  // rows of a product, then both. (Four rows at a time: else the compiler reads all
+  // factors first, into registers that there are not.)
+  template <int CT>
+  __device__ __forceinline__ static void weights(const f32x4 (&s)[RT][CT], const float* c, const float* vs, int g,
+                                                 const float (&m)[CT], uint4 (&u)[RT / 2][CT], float (&sum)[CT]) {
 #pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-      const uint32_t w = (uint32_t)(seen >> (32 * kt));
+    for (int j = 0; j < RT / 2; j++) {
+      uint32_t d[CT][4];
+      float l[CT];
 #pragma unroll
-      for (int j = 0; j < PU; j++) {
-        float l = 0.f;
-        uint32_t d[4];
+      for (int b = 0; b < 2; b++) {
+        const int t = 2 * j + b;
+        const f32x4 f = rows4(c, t, g), h = rows4(vs, t, g);
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-          const f32x4 f = rows4(c, kt, 2 * j + b, half), g = rows4(vs, kt, 2 * j + b, half);
-          f32x4 z;
+        for (int k = 0; k < CT; k++) {
+          f32x4 e;
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * j + 4 * b + i], f[i], -m));
-            if (!FULL) e = w & (1u << (16 * j + 8 * b + i)) ? e : 0.f;
-            l = b == 0 && i == 0 ? e : l + e;
-            z[i] = e * g[i];
-            if (!FULL) z[i] = w & (1u << (16 * j + 8 * b + i)) ? z[i] : 0.f;
+            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k][i], f[i], -m[k]));
+            l[k] = b == 0 && i == 0 ? e[i] : l[k] + e[i];
           }
+          f32x4 z;
+#pragma unroll
+          for (int i = 0; i < 4; i++) z[i] = e[i] * h[i];
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const f32x2 two = {z[2 * i], z[2 * i + 1]};
-            if constexpr (kPower) d[2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, f16x2));
-            else d[2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16x2));
+            if constexpr (kPower) d[k][2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, f16x2));
+            else d[k][2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16x2));
           }
         }
-        sum[kt * PU + j] = l;
-        u[kt][j] = make_uint4(d[0], d[1], d[2], d[3]);
         __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int k = 0; k < CT; k++) {
+        u[j][k] = make_uint4(d[k][0], d[k][1], d[k][2], d[k][3]);
+        sum[k] = j == 0 ? l[k] : sum[k] + l[k];
+      }
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+  // Columns that see a row that spoils them.
+  template <int CT> __device__ __forceinline__ static void spoil(const Args& p, const int32_t (&pos)[CT], int32_t key0, uint64_t bad, float (&sum)[CT]) {
+#pragma unroll
+    for (int k = 0; k < CT; k++)
+      if (seen_bits(p, pos[k], key0, bad) != 0) sum[k] = NAN;
   }
 };
 
-// A row's scale, 0 for one without a page; from device memory, as ld16.
-__device__ __forceinline__ float ld_scale(const float* at, bool there) {
+// As feed(), with the operands two products ahead: of half as many registers.
+template <int N, typename Read, typename Use>
+__device__ __forceinline__ void feed2(const Read& read, const Use& use) {
+  static_assert(N % 2 == 0, "pairs");
+  uint4 x[2][2];
+  x[0][0] = read(0), x[0][1] = read(1);
+#pragma unroll
+  for (int n = 0; n < N; n += 2) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (n + 2 < N) x[(n / 2 + 1) & 1][0] = read(n + 2), x[(n / 2 + 1) & 1][1] = read(n + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    use(n, x[(n / 2) & 1][0]);
+    use(n + 1, x[(n / 2) & 1][1]);
+  }
+}
+
+// A row of a page, and its scale from device memory, as ld16; zeros for a row
+// without a page.
+__device__ __forceinline__ const char* row_at(const char* base, int32_t id, uint32_t page, int32_t row, uint32_t step) {
+  const char* at = base + ((uint64_t)(uint32_t)id * page + (uint64_t)(uint32_t)row * step);
+  return id >= 0 ? at : reinterpret_cast<const char*>(g_zero_row);
+}
+__device__ __forceinline__ float ld_scale(const char* at) {
   typedef __attribute__((address_space(1))) const float gfloat;
-  return *(gfloat*)(there ? at : reinterpret_cast<const float*>(g_zero_row));
+  return *(gfloat*)at;
 }
 
 // Split route: a segment's (m, l, o) of NC columns, four steps to a pass, one
 // per wave, as for the other types. Keys and values of the next pass are on their
-// way through registers of their own while a pass is computed.
+// way through registers of their own while a pass is computed, across the ends of
+// the workgroup's segments.
 template <typename T, int D, int V, int NC>
-__global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu())) split8_kernel(Args p) {
+__global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
-  using G = typename G8::G;
-  constexpr int S = G8::kStep, KT = G8::KT, PU = G8::PU;
+  constexpr int S = G8::kStep, RT = G8::RT, CT = NC / 16, NU = RT / 2;
   __shared__ uint4 s_kv[4 * S * G8::MCH];  // a step per wave: its keys, then its values
-  __shared__ uint4 s_p[4 * KT * PU * 2 * NC];
+  __shared__ uint4 s_p[4 * NU * CT * 64];
   __shared__ const char* s_row[2][4 * S];
   __shared__ __attribute__((aligned(16))) float s_c[4 * S], s_vs[4 * S];
   __shared__ __attribute__((aligned(16))) uint16_t s_pow[G8::kPower ? 4 * S : 8];
   __shared__ float s_max[4][NC];
-  __shared__ float s_sum[4][2 * NC];
+  __shared__ float s_sum[4][CT * 64];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, half = lane >> 5, cn = col & (NC - 1);
+  const int col = lane & 15, g = lane >> 4;
   // Workgroup -> kv head, columns, segment of the walk, request.
   const int x = blockIdx.x, xc = x / p.Hkv, kvh = x - xc * (int)p.Hkv.d;
   const int xq = xc / (p.once ? p.slots : p.ctiles);
@@ -252,47 +390,69 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu())) split8_k
   const int parts = w.count() < (int)p.nseg.d ? w.count() : p.nseg.d;
   if (part0 >= parts) return;
 
-  // Column; one without a token takes the first one's query and sees nothing.
-  const int cc = c0 + col;
-  const bool cv = col < NC && cc < ncol;
-  const int cq = cv ? cc : c0;
-  const int tok = cq / p.G, head = kvh * (int)p.G.d + (cq - tok * (int)p.G.d);
-  const int32_t pos = cv ? rq.n - rq.L + tok : -1;
+  // Columns; one without a token takes the first one's query, and nobody its result.
+  bool cv[CT];
+  int32_t pos[CT];
+  const char* qa[CT];
+#pragma unroll
+  for (int k = 0; k < CT; k++) {
+    const int cc = c0 + 16 * k + col;
+    cv[k] = cc < ncol;
+    const int cq = cv[k] ? cc : c0, tok = cq / p.G;
+    pos[k] = cv[k] ? rq.n - rq.L + tok : -1;
+    qa[k] = query_at<T>(p, r, rq, tok, kvh * (int)p.G.d + (cq - tok * (int)p.G.d));
+  }
   const char* kh = static_cast<const char*>(p.k) + kvh * p.kh;
   const char* vh = static_cast<const char*>(p.v) + kvh * p.vh;
-  const float* ksh = p.ks + kvh * p.ksh;
-  const float* vsh = p.vs + kvh * p.vsh;
+  const char* ksh = reinterpret_cast<const char*>(p.ks + kvh * p.ksh);
+  const char* vsh = reinterpret_cast<const char*>(p.vs + kvh * p.vsh);
 
-  int s0, s1;
-  // Row addresses of the wave's step of a segment, and its scales, on their way; a
-  // row that no column sees, or that has no page, is a row of zeros.
-  float ks, vs;
-  auto key_of = [&](int si) __attribute__((always_inline)) { return si * PS + wave * S; };
-  auto entry_for = [&](int si) __attribute__((always_inline)) -> int32_t {
-    return entry_of(p, r, key_of(si) + lane);
+  // A pass of the workgroup's parts of the walk, which it takes one after the
+  // other as one run of passes: pass `si` (counted from the request's first row)
+  // of segment `part`, whose passes that some column sees end before `s1`.
+  struct At {
+    int part, si, s1;
   };
-  auto put_rows = [&](int si, int32_t entry) __attribute__((always_inline)) -> uint64_t {
-    const int32_t key = key_of(si) + lane;
-    const int32_t id = si < s1 && any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry, key) : -1;
-    const int64_t row = row_of(p, key);
-    const char* zero = reinterpret_cast<const char*>(g_zero_row);
-    s_row[0][wave * S + lane] = id >= 0 ? kh + id * p.kb + row * p.kn : zero;
-    s_row[1][wave * S + lane] = id >= 0 ? vh + id * p.vb + row * p.vn : zero;
-    ks = ld_scale(ksh + id * p.ksb + row * p.ksn, id >= 0);
-    vs = ld_scale(vsh + id * p.vsb + row * p.vsn, id >= 0);
+  auto open = [&](At& t) __attribute__((always_inline)) {
+    if (t.part >= parts) return;
+    t.si = w.unit(t.part) * PN, t.s1 = t.si + PN;
+    while (t.si < t.s1 && !any_seen(p, lo, hi, t.si * PS, PS)) t.si++;
+    while (t.si < t.s1 && !any_seen(p, lo, hi, (t.s1 - 1) * PS, PS)) t.s1--;
+  };
+  auto after = [&](At t) __attribute__((always_inline)) -> At {
+    if (t.part < parts && ++t.si >= t.s1) {
+      t.part += p.gseg.d;
+      open(t);
+    }
+    return t;
+  };
+  // Row addresses of the wave's step of a pass, and its scales, on their way; a row
+  // that no column sees, or that has no page, is a row of zeros.
+  float ks, vs;
+  auto entry_for = [&](const At& t) __attribute__((always_inline)) -> int32_t {
+    return entry_of(p, r, t.si * PS + wave * S + lane);
+  };
+  auto put_rows = [&](const At& t, int32_t entry) __attribute__((always_inline)) -> uint64_t {
+    const int32_t key = t.si * PS + wave * S + lane;
+    const int32_t id = t.part < parts && any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry, key) : -1;
+    const int32_t row = row_of(p, key);
+    s_row[0][wave * S + lane] = row_at(kh, id, p.k8b, row, p.k8n);
+    s_row[1][wave * S + lane] = row_at(vh, id, p.v8b, row, p.v8n);
+    ks = ld_scale(row_at(ksh, id, p.ksb, row, p.ksn));
+    vs = ld_scale(row_at(vsh, id, p.vsb, row, p.vsn));
     __builtin_amdgcn_wave_barrier();
     return __builtin_amdgcn_ballot_w64(id >= 0);
   };
   // Rows are loaded whole, consecutive lanes taking consecutive chunks.
   constexpr int KL = S * G8::CH / 64, VL = S * G8::VCH / 64;
-  uint4 xk[KL], xv[VL], q[G8::NQ];
+  uint4 xk[KL], xv[VL], q[CT][G8::NQ];
   auto load_rows = [&](uint4* to, const char* const* rows, auto chunks, auto load) __attribute__((always_inline)) {
     constexpr int C = decltype(chunks)::value;
     const int ln = opaque(lane);
 #pragma unroll
     for (int j = 0; j < S * C / 64; j++) {
-      const uint32_t at = j * 64 + ln, row = at / C;
-      to[j] = load(rows[wave * S + row] + (at - row * C) * 16);
+      const typename G8::template Unit<C, 64> u(j, ln);
+      to[j] = load(rows[wave * S + u.row] + u.chunk * 16);
     }
   };
   auto load_keys = [&]() __attribute__((always_inline)) {
@@ -304,134 +464,159 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu())) split8_k
     else load_rows(xv, s_row[1], std::integral_constant<int, G8::VCH>(), ld16);
   };
 
-  for (int part = part0; part < parts; part += p.gseg.d) {
-    s0 = w.unit(part) * PN, s1 = s0 + PN;
-    while (s0 < s1 && !any_seen(p, lo, hi, s0 * PS, PS)) s0++;
-    while (s0 < s1 && !any_seen(p, lo, hi, (s1 - 1) * PS, PS)) s1--;
-    if (p.window || part != part0) {
-      entry0 = entry_for(s0);
-      entry = entry_for(s0 + 1);
+  // Keys and values of the next pass and the table's entries of the one after it
+  // are on their way while a pass is computed, whichever segments these are of.
+  At at = {part0, 0, 0};
+  open(at);
+  At next = after(at);
+  if (p.window) entry0 = entry_for(at);
+  if (p.window || next.part != part0) entry = entry_for(next);
+#pragma unroll
+  for (int k = 0; k < CT; k++) G8::load_query(qa[k], g, q[k]);
+  uint64_t mapped = put_rows(at, entry0);
+  load_keys();
+  load_values();
+#pragma unroll
+  for (int k = 0; k < CT; k++) G8::sign_query(p, q[k]);
+
+  constexpr int TW = (G8::DT + 3) / 4;  // tiles of output dims per wave
+  float m[CT], l[CT];
+  f32x4 o[TW][CT];
+  auto begin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < CT; k++) {
+      m[k] = kNone, l[k] = 0.f;
+#pragma unroll
+      for (int y = 0; y < TW; y++) o[y][k] = f32x4{};
     }
-    G8::load_query(query_at<T>(p, r, rq, tok, head), half, q);
-    uint64_t mapped = put_rows(s0, entry0);
+  };
+  begin();
+  for (;;) {
+    const int32_t pass0 = at.si * PS, key0 = pass0 + wave * S;
+    const At third = after(next);
+    const int32_t entry2 = entry_for(third);
+    const int lk = opaque(lane);
+    uint4* own = s_kv + wave * S * G8::MCH;
+#pragma unroll
+    for (int j = 0; j < KL; j++)
+      st16(reinterpret_cast<uint4*>(reinterpret_cast<char*>(own) + G8::key_stored(j, lk)), xk[j]);
+    float c, left;
+    uint16_t power = 0;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(G8::factors(p, ks, vs, c, left, power));
+    s_c[wave * S + lk] = c;
+    s_vs[wave * S + lk] = left;
+    if constexpr (G8::kPower) s_pow[wave * S + G8::vplace(lk)] = power;
+    const uint64_t now = mapped;
+    mapped = put_rows(next, entry);
+    entry = entry2;
     load_keys();
-    load_values();
-    G8::sign_query(p, q);
-
-    constexpr int TW = (G8::DT + 3) / 4;  // tiles of output dims per wave
-    float m = kNone, l = 0.f;
-    f32x16 o[TW];
+    __builtin_amdgcn_wave_barrier();
+    // Scores of the wave's step and their largest.
+    f32x4 s[RT][CT];
 #pragma unroll
-    for (int i = 0; i < TW; i++) o[i] = f32x16{};
-    for (int si = s0; si < s1; si++) {
-      const int32_t pass0 = si * PS, key0 = pass0 + wave * S;
-      const int32_t entry2 = entry_for(si + 2);
-      const int lk = opaque(lane);
+    for (int t = 0; t < RT; t++) {
 #pragma unroll
-      for (int j = 0; j < KL; j++) {
-        const uint32_t at = j * 64 + lk, row = at / G8::CH, c = (at - row * G8::CH) ^ G8::kswz(row);
-        st16(s_kv + wave * S * G8::MCH + row * G8::CH + c, xk[j]);
+      for (int k = 0; k < CT; k++) s[t][k] = f32x4{};
+#pragma unroll
+      for (int c = 0; c < (G8::NQ + 1) / 2; c++) {
+        uint4 x[2];
+        G8::keys(own, 16 * t, c, lk, x);
+#pragma unroll
+        for (int n = 2 * c; n < 2 * c + 2 && n < G8::NQ; n++)
+#pragma unroll
+          for (int k = 0; k < CT; k++) s[t][k] = G8::product(x[n & 1], q[k][n], s[t][k]);
       }
-      s_c[wave * S + lk] = G8::factor(p, ks);
-      float left = vs;
-      if constexpr (G8::kPower) s_pow[wave * S + G8::vplace(lk)] = scale_power(vs, left);
-      s_vs[wave * S + lk] = left;
-      const uint64_t now = mapped;
-      mapped = put_rows(si + 1, entry);
-      entry = entry2;
-      load_keys();
-      __builtin_amdgcn_wave_barrier();
-      // Scores of the wave's step and their largest.
-      f32x16 s[KT];
+    }
+    const bool full = now == ~0ull && all_seen(p, lo, hi, key0, S);
+    if (!full) {
+      uint64_t seen[CT];
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++) {
-        f32x16 c = {};
-        const int row = 32 * kt + (lk & 31);
+      for (int k = 0; k < CT; k++) seen[k] = seen_bits(p, pos[k], key0, now) >> (4 * g);
+      G8::template hide<CT>(s, seen);
+    }
+    const float* cs = s_c + wave * S;
+    float top[CT];
+    G8::template top<CT>(s, cs, g, top);
+    if (g == 0)
 #pragma unroll
-        for (int t = 0; t < G8::NQ / 2; t++) {
-          const uint4 k = s_kv[wave * S * G8::MCH + row * G8::CH + ((2 * t + (lk >> 5)) ^ G8::kswz(row))];
-          c = G::score(codes8<T>(k.x, k.y), q[2 * t], c);
-          c = G::score(codes8<T>(k.z, k.w), q[2 * t + 1], c);
-        }
-        s[kt] = c;
-      }
-      const bool full = now == ~0ull && all_seen(p, lo, hi, key0, S) && c0 + NC <= ncol;
-      const uint64_t seen = full ? 0 : seen_bits(p, pos, key0, now) >> (4 * half);
-      const float* cs = s_c + wave * S;
-      const float top = full ? G8::template top<true>(s, cs, half, seen) : G8::template top<false>(s, cs, half, seen);
-      if (lane < NC) s_max[wave][lane] = top;
-      barrier();
+      for (int k = 0; k < CT; k++) s_max[wave][16 * k + col] = top[k];
+    barrier();
 
-      // The bases of the pass's steps; this wave's weights.
-      float base[4], f[4];
+    // The bases of the pass's steps; this wave's weights.
+    float f[CT][4], mw[CT];
+#pragma unroll
+    for (int k = 0; k < CT; k++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        base[i] = next_base(m, s_max[i][cn], 1.f);
-        f[i] = pow2(m - base[i]);
-        m = base[i];
+        const float base = next_base(m[k], s_max[i][16 * k + col], 1.f);
+        f[k][i] = pow2(m[k] - base);
+        m[k] = base;
+        if (i == 0 || i <= wave) mw[k] = base;
       }
-      const float mw = wave == 0 ? base[0] : wave == 1 ? base[1] : wave == 2 ? base[2] : base[3];
-      uint4 pu[KT][PU];
-      const float psum = full ? G8::template weights<true>(s, cs, s_vs + wave * S, half, seen, mw, pu)
-                              : G8::template weights<false>(s, cs, s_vs + wave * S, half, seen, mw, pu);
-      if (col < NC) {
+    uint4 pu[NU][CT];
+    float psum[CT];
+    G8::template weights<CT>(s, cs, s_vs + wave * S, g, mw, pu, psum);
+    if (bad & now) G8::template spoil<CT>(p, pos, key0, bad & now, psum);
+    const int ln = opaque(lane);
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++)
+    for (int k = 0; k < CT; k++) {
 #pragma unroll
-          for (int j = 0; j < PU; j++) s_p[((wave * KT + kt) * PU + j) * 2 * NC + half * NC + col] = pu[kt][j];
-        s_sum[wave][half * NC + col] = psum;
-      }
-      const int ln = opaque(lane);
+      for (int u = 0; u < NU; u++) s_p[((wave * NU + u) * CT + k) * 64 + ln] = pu[u][k];
+      s_sum[wave][64 * k + ln] = psum[k];
+    }
 #pragma unroll
-      for (int j = 0; j < VL; j++) {
-        const uint32_t at = j * 64 + ln, row = at / G8::VCH, place = G8::vplace(row);
-        const int c = (at - row * G8::VCH) ^ G8::vswz(place);
-        st16(s_kv + wave * S * G8::MCH + place * G8::VCH + c, xv[j]);
-      }
-      load_values();
-      barrier();
+    for (int j = 0; j < VL; j++)
+      st16(reinterpret_cast<uint4*>(reinterpret_cast<char*>(own) + G8::value_stored(j, ln)), xv[j]);
+    load_values();
+    barrier();
 
-      // The sum, and the wave's tiles of output dims over the pass's steps.
+    // The sum, and the wave's tiles of output dims over the pass's steps.
 #pragma unroll
-      for (int i = 0; i < 4; i++) l = __builtin_fmaf(l, f[i], s_sum[i][half * NC + cn]);
+    for (int i = 0; i < 4; i++) {
+      if (!any_seen(p, lo, hi, pass0 + i * S, S)) continue;
 #pragma unroll
-      for (int y = 0; y < TW; y++) {
-        const int dt = wave + 4 * y;
-        if (dt >= G8::DT) break;
+      for (int k = 0; k < CT; k++) {
+        if (wave == 0) l[k] = __builtin_fmaf(l[k], f[k][i], s_sum[i][64 * k + ln]);
+        if (__builtin_amdgcn_ballot_w64(f[k][i] != 1.f) != 0)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          if (!any_seen(p, lo, hi, pass0 + i * S, S)) continue;
-          if (__builtin_amdgcn_ballot_w64(f[i] != 1.f) != 0)
+          for (int y = 0; y < TW; y++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[y][e] *= f[i];
+            for (int e = 0; e < 4; e++) o[y][k][e] *= f[k][i];
+      }
 #pragma unroll
-          for (int kt = 0; kt < KT; kt++) {
+      for (int u = 0; u < NU; u++) {
+        uint4 x[CT];
 #pragma unroll
-            for (int j = 0; j < PU; j++) {
-              const uint4 v = G8::value(s_kv + i * S * G8::MCH, s_pow + i * S, 32 * kt, j, dt, ln);
-              const uint4 u = s_p[((i * KT + kt) * PU + j) * 2 * NC + (ln >> 5) * NC + (ln & (NC - 1))];
-              o[y] = G::score(v, u, o[y]);
-            }
-          }
+        for (int k = 0; k < CT; k++) x[k] = s_p[((i * NU + u) * CT + k) * 64 + ln];
+#pragma unroll
+        for (int y = 0; y < TW; y++) {
+          const int dt = wave + 4 * y;
+          if (G8::DT % 4 && dt >= G8::DT) break;
+          const uint4 v = G8::value(s_kv + i * S * G8::MCH, s_pow + i * S, u, dt, ln);
+#pragma unroll
+          for (int k = 0; k < CT; k++) o[y][k] = G8::product(v, x[k], o[y][k]);
         }
       }
-      barrier();  // everyone is done with the values and weights
     }
-
-    l = half_swap_sum(l);
-    if (cv) {
-      const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + part) * p.ccap.d + cc;
-      if (wave == 0 && half == 0) p.pml[slot] = make_float2(m, l);
+    if (next.part != at.part) {  // the segment's last pass
 #pragma unroll
-      for (int y = 0; y < TW; y++) {
-        if (wave + 4 * y >= G8::DT) break;
-        float* to = p.po + slot * V + 32 * (wave + 4 * y);
+      for (int k = 0; k < CT; k++) {
+        const float sum = quarters_sum(l[k]);
+        if (!cv[k]) continue;
+        const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + at.part) * p.ccap.d + c0 + 16 * k + col;
+        if (wave == 0 && g == 0) p.pml[slot] = make_float2(m[k], sum);
 #pragma unroll
-        for (int b = 0; b < 4; b++)
-          *reinterpret_cast<f32x4*>(to + 8 * b + 4 * half) =
-              f32x4{o[y][4 * b], o[y][4 * b + 1], o[y][4 * b + 2], o[y][4 * b + 3]};
+        for (int y = 0; y < TW; y++) {
+          if (wave + 4 * y >= G8::DT) break;
+          *reinterpret_cast<f32x4*>(p.po + slot * V + 16 * (wave + 4 * y) + 4 * g) = o[y][k];
+        }
       }
+      if (next.part >= parts) return;
+      begin();
     }
+    barrier();  // everyone is done with the values and weights
+    at = next;
+    next = third;
   }
 }
 
@@ -443,25 +628,26 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu())) split8_k
 template <typename T, int D, int V, int NW, int LW>
 __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 : 1)) whole8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
-  using G = typename G8::G;
-  constexpr int S = G8::kStep, KT = G8::KT, PU = G8::PU, DT = G8::DT, COLS = 32 * NW;
-  constexpr int KU = S * G::CH, VU = S * G::VCH;  // 16-byte units of a step in LDS
-  constexpr int NT = 64 * (LW ? LW : NW), NB = 2;  // NT: threads that load
+  constexpr int S = G8::kStep, RT = G8::RT, NU = RT / 2, DT = G8::DT, CT = 2, COLS = 32 * NW;
+  constexpr int KU = S * G8::TCH, VU = S * G8::TVCH;  // 16-byte units of a step in LDS
+  constexpr int NLW = LW ? LW : NW, NT = 64 * NLW, NB = 2;  // waves and threads that load
   constexpr int KN = (S * G8::CH + NT - 1) / NT, VN = (S * G8::VCH + NT - 1) / NT;  // loads per thread
   __shared__ uint4 s_kv[NB * (KU + VU)];
-  __shared__ const char* s_row[4][2][S];
-  __shared__ __attribute__((aligned(16))) float s_c[4][S], s_vs[4][S];
-  __shared__ uint16_t s_pow[4][G8::kPower ? S : 1];
-  __shared__ uint64_t s_map[8];
+  constexpr int RING = 2 * NLW;
+  __shared__ const char* s_row[RING][2][S];
+  __shared__ __attribute__((aligned(16))) float s_c[RING][S], s_vs[RING][S];
+  __shared__ uint16_t s_pow[RING][G8::kPower ? S : 1];
+  __shared__ uint64_t s_map[2 * RING], s_bad[RING];
+  __shared__ uint4 s_q[NW][G8::kFarQuery ? G8::kFarQuery : 1][G8::kFarQuery ? 64 : 1];
   __shared__ int s_scan[NW + LW + 3];
-  __shared__ float s_ml[2][64 * NW];  // each lane's own M and L
+  __shared__ float s_ml[CT][2][64 * NW];  // each lane's own M and L
 
   if ((int)blockIdx.x < p.fill_blocks) {
     fill<T, V>(p, blockIdx.x);
     return;
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, half = lane >> 5;
+  const int col = lane & 15;
 
   // Workgroup -> kv head, request, column tile; a request's last tiles first.
   const int x = blockIdx.x - p.fill_blocks;
@@ -517,21 +703,24 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
   const bool loads = LW == 0 || wave >= NW;
   const int lw = LW ? wave - NW : wave;  // which of the loading waves
 
-  const int cc = cw + col;
-  const bool cv = cc < ncol;
-  const int tok = cv ? cc / p.G : 0;
-  const bool whole_tile = cw + 32 <= ncol;
-  uint4 q[G8::NQ];
-  G8::load_query(query_at<T>(p, r, rq, tok, kvh * (int)p.G.d + (cv ? cc - tok * (int)p.G.d : 0)), half, q);
-  G8::sign_query(p, q);
+  uint4 q[CT][G8::NQ];
+#pragma unroll
+  for (int k = 0; k < CT; k++) {
+    const int cc = cw + 16 * k + col, cq = cc < ncol ? cc : 0, tok = cq / p.G;
+    G8::load_query(query_at<T>(p, r, rq, tok, kvh * (int)p.G.d + (cq - tok * (int)p.G.d)), lane >> 4, q[k]);
+    G8::sign_query(p, q[k]);
+    if (k == 1 && wave < NW)
+#pragma unroll
+      for (int n = 0; n < G8::kFarQuery; n++) s_q[wave][n][lane] = q[k][n];
+  }
 
   const Walk w = walk(p, lo, hi, S);
   const int steps = w.count();
 
-  // A step's way into LDS, by the first wave: its rows' addresses from the table's
-  // entries three steps before it is computed, and their scales from registers two
-  // before; then by all, its codes into registers two steps before, and as bf16 or
-  // f16 into LDS one before.
+  // A step's way into LDS: its rows' addresses from the table's entries, 2 NLW steps
+  // before it is computed, and their scales NLW before, both by the loading wave
+  // whose turn it is; then by all, its codes into registers two steps before, and in
+  // the type into LDS one before.
   int32_t entry = 0;
   float ks = 0.f, vs = 0.f;
   auto entry_for = [&](int j) __attribute__((always_inline)) -> int32_t {
@@ -544,21 +733,30 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
     const int ln = opaque(lane);
     const int32_t key = w.unit(j) * S + ln;
     const int32_t id = j < steps && any_seen(a, lo, hi, key, 1) ? page_of(a, r, entry, key) : -1;
-    const int64_t row = row_of(a, key);
-    const char* zero = reinterpret_cast<const char*>(g_zero_row);
-    const char *k = static_cast<const char*>(a.k) + kvh * a.kh, *v = static_cast<const char*>(a.v) + kvh * a.vh;
-    s_row[j & 3][0][ln] = id >= 0 ? k + id * a.kb + row * a.kn : zero;
-    s_row[j & 3][1][ln] = id >= 0 ? v + id * a.vb + row * a.vn : zero;
-    ks = ld_scale(a.ks + kvh * a.ksh + id * a.ksb + row * a.ksn, id >= 0);
-    vs = ld_scale(a.vs + kvh * a.vsh + id * a.vsb + row * a.vsn, id >= 0);
-    s_map[j & 7] = __builtin_amdgcn_ballot_w64(id >= 0);
+    const int32_t row = row_of(a, key);
+    s_row[j % RING][0][ln] = row_at(static_cast<const char*>(a.k) + kvh * a.kh, id, a.k8b, row, a.k8n);
+    s_row[j % RING][1][ln] = row_at(static_cast<const char*>(a.v) + kvh * a.vh, id, a.v8b, row, a.v8n);
+    ks = ld_scale(row_at(reinterpret_cast<const char*>(a.ks + kvh * a.ksh), id, a.ksb, row, a.ksn));
+    vs = ld_scale(row_at(reinterpret_cast<const char*>(a.vs + kvh * a.vsh), id, a.vsb, row, a.vsn));
+    s_map[j % (2 * RING)] = __builtin_amdgcn_ballot_w64(id >= 0);
   };
   auto put_scales = [&](int j) __attribute__((always_inline)) {
     const int ln = opaque(lane);
-    s_c[j & 3][ln] = G8::factor(p, ks);
-    float left = vs;
-    if constexpr (G8::kPower) s_pow[j & 3][ln] = scale_power(vs, left);
-    s_vs[j & 3][ln] = left;
+    float c, left;
+    uint16_t power = 0;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(G8::factors(args_again(), ks, vs, c, left, power));
+    s_c[j % RING][ln] = c;
+    s_vs[j % RING][ln] = left;
+    if constexpr (G8::kPower) s_pow[j % RING][ln] = power;
+    s_bad[j % RING] = bad;
+  };
+  // (Between steps j - 1 and j: everyone is done with the rows of step j + 1 and the
+  // scales of step j - 1, whose places these take.)
+  auto prepare = [&](int j) __attribute__((always_inline)) {
+    if (j % NLW != lw) return;
+    put_scales(j + NLW);
+    put_rows(j + 2 * NLW);
+    entry = entry_for(j + 3 * NLW);
   };
   uint4 xk[KN], xv[VN];
   auto load_codes = [&](uint4* to, const char* const* rows, auto chunks) __attribute__((always_inline)) {
@@ -566,58 +764,63 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
     const int td = opaque(64 * lw + lane);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const uint32_t at = i * NT + td, row = at / C;
-      if (U % NT == 0 || at < U) to[i] = ld16(rows[row] + (at - row * C) * 16);
+      const typename G8::template Unit<C, NT> u(i, td);
+      if (U % NT == 0 || i * NT + td < U) to[i] = ld16(rows[u.row] + u.chunk * 16);
     }
   };
   auto load_step = [&](int j) __attribute__((always_inline)) {
-    load_codes(xk, s_row[j & 3][0], std::integral_constant<int, G8::CH>());
-    load_codes(xv, s_row[j & 3][1], std::integral_constant<int, G8::VCH>());
+    load_codes(xk, s_row[j % RING][0], std::integral_constant<int, G8::CH>());
+    load_codes(xv, s_row[j % RING][1], std::integral_constant<int, G8::VCH>());
   };
   auto put_step = [&](int j) __attribute__((always_inline)) {
     uint4 *kd = s_kv + (j & 1) * (KU + VU), *vd = kd + KU;
     const int td = opaque(64 * lw + lane);
 #pragma unroll
     for (int i = 0; i < KN; i++) {
-      const uint32_t at = i * NT + td, row = at / G8::CH, c = 2 * (at - row * G8::CH);
-      if (S * G8::CH % NT == 0 || at < S * G8::CH) {
-        st16(kd + row * G::CH + (c ^ G::kswz(row)), codes8<T>(xk[i].x, xk[i].y));
-        st16(kd + row * G::CH + ((c + 1) ^ G::kswz(row)), codes8<T>(xk[i].z, xk[i].w));
+      const typename G8::template Unit<G8::CH, NT> u(i, td);
+      const uint32_t row = u.row, c = 2 * u.chunk;
+      if (S * G8::CH % NT == 0 || i * NT + td < S * G8::CH) {
+        st16(kd + row * G8::TCH + (c ^ G8::template swz<G8::TCH>(row)), codes8<T>(xk[i].x, xk[i].y));
+        st16(kd + row * G8::TCH + ((c + 1) ^ G8::template swz<G8::TCH>(row)), codes8<T>(xk[i].z, xk[i].w));
       }
     }
 #pragma unroll
     for (int i = 0; i < VN; i++) {
-      const uint32_t at = i * NT + td, row = at / G8::VCH, c = 2 * (at - row * G8::VCH);
-      if (S * G8::VCH % NT == 0 || at < S * G8::VCH) {
+      const typename G8::template Unit<G8::VCH, NT> u(i, td);
+      const uint32_t row = u.row, c = 2 * u.chunk;
+      if (S * G8::VCH % NT == 0 || i * NT + td < S * G8::VCH) {
         uint4 a = codes8<T>(xv[i].x, xv[i].y), b = codes8<T>(xv[i].z, xv[i].w);
         if constexpr (G8::kPower) {
-          const uint32_t f = s_pow[j & 3][row] * 0x10001u;
+          const uint32_t f = s_pow[j % RING][row] * 0x10001u;
           a = times(a, make_uint4(f, f, f, f)), b = times(b, make_uint4(f, f, f, f));
         }
-        st16(vd + row * G::VCH + (c ^ G::vswz(row)), a);
-        st16(vd + row * G::VCH + ((c + 1) ^ G::vswz(row)), b);
+        st16(vd + row * G8::TVCH + (c ^ G8::tswz(row)), a);
+        st16(vd + row * G8::TVCH + ((c + 1) ^ G8::tswz(row)), b);
       }
     }
   };
 
-  float m = kNone, l = 0.f;
+  float m[CT], l[CT];
   bool fresh = true;  // the segment has no step yet
-  f32x16 O[DT], o[DT];
+  f32x4 O[DT][CT], o[DT][CT];
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++) O[dt] = f32x16{}, o[dt] = f32x16{};
-  if (wave < NW) {
-    s_ml[0][tid] = kNone;
-    s_ml[1][tid] = 0.f;
+  for (int k = 0; k < CT; k++) {
+    m[k] = kNone, l[k] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) O[dt][k] = o[dt][k] = f32x4{};
+    if (wave < NW) {
+      s_ml[k][0][tid] = kNone;
+      s_ml[k][1][tid] = 0.f;
+    }
   }
 
-  if (loads && lw == 0) {
-#pragma unroll
-    for (int j = 0; j < 3; j++) {
-      entry = entry_for(j);
-      put_rows(j);
-      if (j < 2) put_scales(j);
-    }
-    entry = entry_for(3);
+  if (loads) {
+    entry = entry_for(lw);
+    put_rows(lw);
+    put_scales(lw);
+    entry = entry_for(lw + NLW);
+    put_rows(lw + NLW);
+    entry = entry_for(lw + 2 * NLW);
   }
   __syncthreads();
   if (loads) {
@@ -625,78 +828,98 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
     put_step(0);
     load_step(1);
   }
-  auto ahead = [&](int j) __attribute__((always_inline)) {
-    if (lw == 0) {
-      put_scales(j + 2);
-      put_rows(j + 3);
-      entry = entry_for(j + 4);
-    }
-  };
   if constexpr (LW != 0)
     if (loads) {
       for (int j = 0; j < steps; j++) {
         barrier();
         if (j + 1 < steps) put_step(j + 1);
         if (j + 2 < steps) load_step(j + 2);
-        ahead(j);
+        prepare(j);
       }
       return;
     }
   for (int j = 0; j < steps; j++) {
-    const int ln = opaque(lane), hf = ln >> 5;
+    const uint32_t ln = opaque(lane);
+    const int g = ln >> 4;
     barrier();  // step j is there, and everyone is done with step j - 1's buffer
     if constexpr (LW == 0) {
       if (j + 1 < steps) put_step(j + 1);
-      ahead(j);
+      prepare(j);
     }
     const uint4 *kd = s_kv + (j & 1) * (KU + VU), *vd = kd + KU;
     const int32_t unit = w.unit(j), key0 = unit * S;
     const bool mine = any_seen(p, wlo, whi, key0, S);
-    uint4 pu[KT][PU];
+    uint4 pu[NU][CT];
     if (mine) {
-      const uint64_t mapped = uniform(s_map[j & 7]);
-      const bool full = whole_tile && mapped == ~0ull && all_seen(p, wlo, whi, key0, S);
-      f32x16 s[KT];
+      const uint64_t mapped = uniform(s_map[j % (2 * RING)]);
+      const bool full = mapped == ~0ull && all_seen(p, wlo, whi, key0, S);
+      f32x4 s[RT][CT];
 #pragma unroll
-      for (int kt = 0; kt < KT; kt++) s[kt] = f32x16{};
-      feed<KT * G8::NQ>(
-          [&](int n) __attribute__((always_inline)) {
-            const int t = n / KT, row = 32 * (n % KT) + (ln & 31);
-            return kd[row * G::CH + ((4 * (t >> 1) + 2 * hf + (t & 1)) ^ G::kswz(row))];
-          },
-          [&](int n, uint4 k) __attribute__((always_inline)) {
-            s[n % KT] = G::score(k, q[n / KT], s[n % KT]);
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int k = 0; k < CT; k++) s[t][k] = f32x4{};
+      uint4 far[2];
+      auto far_query = [&](int n) __attribute__((always_inline)) { far[n & 1] = s_q[wave][n][ln]; };
+      if (G8::kFarQuery) far_query(0);
+      feed2<RT * G8::NQ>(
+          [&](int n) __attribute__((always_inline)) { return G8::key_of_type(kd, 16 * (n % RT), n / RT, ln); },
+          [&](int n, uint4 x) __attribute__((always_inline)) {
+            const int i = n / RT;
+            if (n % RT == 0 && i + 1 < G8::kFarQuery) far_query(i + 1);
+            s[n % RT][0] = G8::product(x, q[0][i], s[n % RT][0]);
+            s[n % RT][1] = G8::product(x, i < G8::kFarQuery ? far[i & 1] : q[1][i], s[n % RT][1]);
           });
-      uint64_t seen = 0;
+      const uint64_t bad = uniform(s_bad[j % RING]) & mapped;
+      auto positions = [&](int32_t(&pos)[CT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < CT; k++) {
+          const int c = cw + 16 * k + (opaque(lane) & 15);
+          pos[k] = c < ncol ? p0 + c / p.G : -1;
+        }
+      };
       if (!full) {
-        const int c = cw + (opaque(lane) & 31);
-        seen = seen_bits(p, c < ncol ? p0 + c / p.G : -1, key0, mapped) >> (4 * hf);
+        int32_t pos[CT];
+        uint64_t seen[CT];
+        positions(pos);
+#pragma unroll
+        for (int k = 0; k < CT; k++) seen[k] = seen_bits(p, pos[k], key0, mapped) >> (4 * g);
+        G8::template hide<CT>(s, seen);
       }
-      const float *cs = s_c[j & 3], *gs = s_vs[j & 3];
+      const float *cs = s_c[j % RING], *gs = s_vs[j % RING];
       // A lane's sum of at most kMostSum holds no score that moves the base;
       // else, and at a segment's first step, the largest score decides.
-      float psum;
+      float psum[CT];
       bool look = fresh;
       for (;;) {
+        const int h = opaque(g);  // (so that no row's factor is read before the loop, into registers)
         if (look) {
-          const float t = full ? G8::template top<true>(s, cs, hf, seen) : G8::template top<false>(s, cs, hf, seen);
-          const float mn = next_base(m, t, 1.f);
-          if (!fresh && __builtin_amdgcn_ballot_w64(mn != m) != 0) {
-            const float f = pow2(m - mn);
-            l *= f;  // exact, as in the sum's fma(l, f, .)
+          float t[CT];
+          G8::template top<CT>(s, cs, h, t);
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+          for (int k = 0; k < CT; k++) {
+            const float mn = next_base(m[k], t[k], 1.f);
+            if (!fresh && __builtin_amdgcn_ballot_w64(mn != m[k]) != 0) {
+              const float f = pow2(m[k] - mn);
+              l[k] *= f;  // exact, as in the sum's fma(l, f, .)
 #pragma unroll
-              for (int i = 0; i < 16; i++) o[dt][i] *= f;
+              for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[dt][k][i] *= f;
+            }
+            m[k] = mn;
           }
-          m = mn;
         }
-        psum = full ? G8::template weights<true>(s, cs, gs, hf, seen, m, pu)
-                    : G8::template weights<false>(s, cs, gs, hf, seen, m, pu);
-        if (look || __builtin_amdgcn_ballot_w64(psum > kMostSum) == 0) break;
+        G8::template weights<CT>(s, cs, gs, h, m, pu, psum);
+        if (look || __builtin_amdgcn_ballot_w64(psum[0] > kMostSum || psum[1] > kMostSum) == 0) break;
         look = true;
       }
-      l += psum;
+      if (bad) {
+        int32_t pos[CT];
+        positions(pos);
+        G8::template spoil<CT>(p, pos, key0, bad, psum);
+      }
+#pragma unroll
+      for (int k = 0; k < CT; k++) l[k] += psum[k];
       fresh = false;
     }
     // (Not before the scores, whose operands need the registers.)
@@ -704,59 +927,60 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
       if (j + 2 < steps) load_step(j + 2);
     if (mine) {
       // Products of one output tile are a chain: those of the others go between.
-      feed<DT * KT * PU>(
-          [&](int n) __attribute__((always_inline)) {
-            return G::value(vd, n / DT / PU * 32, n / DT % PU, n % DT, ln);
-          },
+      feed<DT * NU>(
+          [&](int n) __attribute__((always_inline)) { return G8::value_of_type(vd, n / DT, n % DT, ln); },
           [&](int n, uint4 v) __attribute__((always_inline)) {
-            o[n % DT] = G::score(v, pu[n / DT / PU][n / DT % PU], o[n % DT]);
+#pragma unroll
+            for (int k = 0; k < CT; k++) o[n % DT][k] = G8::product(v, pu[n / DT][k], o[n % DT][k]);
           });
     }
     // The segment's end: fold it.
     if (j + 1 == steps || w.unit(j + 1) / G8::kSegSteps != unit / G8::kSegSteps) {
       if (!fresh) {
         const int td = opaque(tid);
-        float M = s_ml[0][td], L = s_ml[1][td], fa, fb;
-        fold_base(M, L, m, half_swap_sum(l), fa, fb);
-        s_ml[0][td] = M;
-        s_ml[1][td] = L;
-        if (__builtin_amdgcn_ballot_w64(fa != 1.f) != 0)
 #pragma unroll
-          for (int dt = 0; dt < DT; dt++)
+        for (int k = 0; k < CT; k++) {
+          float M = s_ml[k][0][td], L = s_ml[k][1][td], fa, fb;
+          fold_base(M, L, m[k], quarters_sum(l[k]), fa, fb);
+          s_ml[k][0][td] = M;
+          s_ml[k][1][td] = L;
+          if (__builtin_amdgcn_ballot_w64(fa != 1.f) != 0)
 #pragma unroll
-            for (int i = 0; i < 16; i++) O[dt][i] *= fa;
+            for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
+              for (int i = 0; i < 4; i++) O[dt][k][i] *= fa;
 #pragma unroll
-          for (int i = 0; i < 16; i++) O[dt][i] = __builtin_fmaf(o[dt][i], fb, O[dt][i]);
-          o[dt] = f32x16{};
+          for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) O[dt][k][i] = __builtin_fmaf(o[dt][k][i], fb, O[dt][k][i]);
+            o[dt][k] = f32x4{};
+          }
+          m[k] = kNone;
+          l[k] = 0.f;
         }
-        m = kNone;
-        l = 0.f;
         fresh = true;
       }
     }
   }
 
-  const int lane2 = opaque(lane), cc2 = cw + (lane2 & 31), half2 = lane2 >> 5;
-  if (cc2 < ncol) {
-    const int tok2 = cc2 / p.G, head = kvh * (int)p.G.d + cc2 - tok2 * (int)p.G.d;
-    const float M = s_ml[0][wave * 64 + lane2], L = s_ml[1][wave * 64 + lane2];
+#pragma unroll
+  for (int k = 0; k < CT; k++) {
+    const int lane2 = opaque(lane), cc = cw + 16 * k + (lane2 & 15);
+    if (cc >= ncol) continue;
+    const int tok = cc / p.G, head = kvh * (int)p.G.d + cc - tok * (int)p.G.d;
+    const float M = s_ml[k][0][wave * 64 + lane2], L = s_ml[k][1][wave * 64 + lane2];
     float e, den;
     finish(M, L, p.sinks ? (float)static_cast<const T*>(p.sinks)[head] * 1.4426950408889634f : 0.f,
            p.sinks != nullptr, e, den);
     const float inv = inverse(den);
-    T* out = out_at<T>(p, r, rq, tok2, head);
+    T* out = out_at<T>(p, r, rq, tok, head);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 y;
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        T4 y;
-#pragma unroll
-        for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][4 * b + i], e, inv);
-        *reinterpret_cast<T4*>(out + 32 * dt + 8 * b + 4 * half2) = y;
-      }
+      for (int i = 0; i < 4; i++) y[i] = result<T>(O[dt][k][i], e, inv);
+      *reinterpret_cast<T4*>(out + 16 * dt + 4 * (lane2 >> 4)) = y;
     }
   }
 }
@@ -771,7 +995,7 @@ Kernels kernels8_of() {
   k.seg = G8::kSeg, k.pass = 4 * G8::kStep;
   k.row_us = G8::row_us();
   k.seg16_us = k.seg32_us = G8::seg_us();
-  k.per_cu16 = k.per_cu32 = G8::split_per_cu();
+  k.per_cu16 = G8::split_per_cu(16), k.per_cu32 = G8::split_per_cu(32);
   k.whole4_pair = nullptr;
   if constexpr (G8::kTwoWaves) {
     k.whole4 = whole8_kernel<T, D, V, 4, 4>;
@@ -781,6 +1005,7 @@ Kernels kernels8_of() {
     k.whole8 = nullptr;
   }
   k.whole4_threads = G8::kTwoWaves ? 512 : 256;
+  k.places = 2048;
   return k;
 }
 

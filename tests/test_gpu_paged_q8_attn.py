@@ -226,7 +226,7 @@ def test_scales_of_any_size(cuda, dtype, L):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("bad", [NAN, INF, -1.0])
 def test_rows_reach_only_tokens_that_see_them(cuda, dtype, bad):
-    """A row whose scales are NaN, infinite or (keys) negative spoils the tokens
+    """A row whose scales are NaN, infinite or (keys) negative makes NaN of the tokens
     that see it and leaves the bits of the others, on both routes."""
     n, L, H, Hkv, D = 900, 200, 8, 2, 128
     (kc, ks), (vc, vs) = draw(n, Hkv, D, D, 5)
@@ -245,12 +245,7 @@ def test_rows_reach_only_tokens_that_see_them(cuda, dtype, bad):
             hit = torch.zeros(new, H, dtype=torch.bool, device=cuda)
             hit[max(0, new - 77):, 4:] = True
             assert same(got[~hit], b[~hit])
-            if side == "k" and bad == INF:  # a score of -inf has weight 0; else NaN
-                hit &= (q[L - new:].double() @ kc[row, 1].double() >= 0).to(cuda)
-                assert bool(hit.any())
-            if not (side == "v" and bad == INF):  # (infinite values give infinities or NaN)
-                assert bool((got.isnan().any(-1) == hit).all())
-            assert bool((~got.isfinite()).any(-1)[hit].all())
+            assert bool(got[hit].isnan().all())
 
 
 @pytest.mark.parametrize("per", ["page", "head", "all"])
