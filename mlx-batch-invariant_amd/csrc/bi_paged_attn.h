@@ -55,6 +55,7 @@ struct Args {
   const float* vs;
   uint32_t k8b, k8n, v8b, v8n, ksb, ksn, vsb, vsn;
   int64_t ksh, vsh;
+  Div eight;              // 8 * Hkv where a row's heads are next to each other, else 0
 };
 
 typedef void (*Kernel)(Args);

@@ -183,7 +183,9 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     p.once = ctiles == 1 || most * p.G.d > s.split_cols;
     const Kernel split = most > 1 ? (s.nc == 16 ? k.split16 : k.split32)
                                   : (s.nc == 16 ? k.split16_one : k.split32_one);
-    hipLaunchKernelGGL(split, dim3((unsigned)split_grid(c, s)), dim3(256), 0, st, p);
+    int64_t grid = split_grid(c, s);
+    if (p.eight.d) grid = (grid / p.Hkv.d + 7) / 8 * 8 * p.Hkv.d;
+    hipLaunchKernelGGL(split, dim3((unsigned)grid), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   const bool whole = most * p.G.d > s.split_cols;
@@ -332,6 +334,7 @@ int paged_attention(const char* who, const void* q, const void* k_cache, const v
     p.ks = k_scales;
     p.vs = v_scales;
     p.ksh = scale_strides[1], p.vsh = scale_strides[4];
+    if (Hkv > 1 && D + V <= 256 && strides[3] < strides[4]) p.eight = make_div(8 * Hkv);
   }
   return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
 }

@@ -367,8 +367,19 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  // Workgroup -> kv head, columns, segment of the walk, request.
-  const int x = blockIdx.x, xc = x / p.Hkv, kvh = x - xc * (int)p.Hkv.d;
+  // Workgroup -> kv head, columns, segment of the walk, request. Neighbours in the
+  // grid land on different XCDs: so do neighbouring heads, but for a cache whose
+  // rows hold all heads side by side, which share lines, of scales above all: there
+  // a row's heads go to one XCD (64 requests in a token-major cache, 128 dims 163 ->
+  // 153 us, 64 dims 136 -> 114; in a head-major one it costs 132 -> 136, and with
+  // 256 dims 150 -> 163).
+  const int x = blockIdx.x;
+  int xc = x / p.Hkv, kvh = x - xc * (int)p.Hkv.d;
+  if (p.eight.d) {
+    const int set = x / p.eight, at = x - set * (int)p.eight.d;
+    kvh = at >> 3, xc = 8 * set + (at & 7);
+    if (xc >= (int)(p.slots.d * p.ctiles.d)) return;  // (the grid is rounded up)
+  }
   const int xq = xc / (p.once ? p.slots : p.ctiles);
   const int xr = xc - xq * (int)(p.once ? p.slots : p.ctiles).d;
   const int xs = p.once ? xr : xq, c0 = (p.once ? xq : xr) * NC;
@@ -455,12 +466,14 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
       to[j] = load(rows[wave * S + u.row] + u.chunk * 16);
     }
   };
+  // (Past the caches, but for lines that hold parts of other heads' rows too.)
+  const bool past = p.once && (!p.eight.d || (G8::CH % 8 == 0 && G8::VCH % 8 == 0));
   auto load_keys = [&]() __attribute__((always_inline)) {
-    if (p.once) load_rows(xk, s_row[0], std::integral_constant<int, G8::CH>(), ld16_once);
+    if (past) load_rows(xk, s_row[0], std::integral_constant<int, G8::CH>(), ld16_once);
     else load_rows(xk, s_row[0], std::integral_constant<int, G8::CH>(), ld16);
   };
   auto load_values = [&]() __attribute__((always_inline)) {
-    if (p.once) load_rows(xv, s_row[1], std::integral_constant<int, G8::VCH>(), ld16_once);
+    if (past) load_rows(xv, s_row[1], std::integral_constant<int, G8::VCH>(), ld16_once);
     else load_rows(xv, s_row[1], std::integral_constant<int, G8::VCH>(), ld16);
   };
 
@@ -833,8 +846,8 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
       for (int j = 0; j < steps; j++) {
         barrier();
         if (j + 1 < steps) put_step(j + 1);
+        prepare(j);  // (before the loads that the next step waits for, and with them for its own)
         if (j + 2 < steps) load_step(j + 2);
-        prepare(j);
       }
       return;
     }
