@@ -7,11 +7,11 @@
 // -inf is a token that is ruled out and counts for nothing; a row with a NaN or
 // +inf, and one of -inf alone, is NaN. M, S and U are in 32 bits.
 //
-// The k largest, ties to the lowest id. The threads form 64 groups; the k-th
-// largest of the groups' largest logits bounds the k-th largest logit of all
-// from below. What is not below it, some k to 5 k logits of most rows, is put
-// in order wave by wave, by insertion into a list that the lanes hold, and what
-// the waves' lists hold is counted against each other.
+// The k largest, ties to the lowest id. The threads form 256 groups (64 for up to
+// 16); the k-th largest of the groups' largest logits bounds the k-th largest
+// logit of all from below. What is not below it, k to 1.2 k logits of most rows,
+// is put in order wave by wave, by insertion into a list that the lanes hold, and
+// what the waves' lists hold is counted against each other.
 //
 // A workgroup has a row to itself and keeps it in registers (longer rows than
 // these hold pass by and only the threads with a large logit read theirs once
@@ -53,12 +53,12 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 
 // NT threads of NU units of 16 bytes each; HELD: all of a row is in these.
 template <typename T, int NT, int NU, bool HELD>
-__global__ void __launch_bounds__(NT) logprobs_kernel(LogprobArgs p) {
-  constexpr int U = 16 / sizeof(T), NW = NT / 64, GROUP = NT / 64;
+__global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(LogprobArgs p) {
+  constexpr int U = 16 / sizeof(T), NW = NT / 64, GROUP = NT / 256;
   // (Rows begin at any element: the element's place decides which thread has
   // it, whatever the row's alignment.)
   typedef T Vec __attribute__((ext_vector_type(U), aligned(sizeof(T))));
-  __shared__ float s_group[64];
+  __shared__ float4 s_group[64];
   __shared__ float2 s_sum[NW];
   __shared__ int32_t s_list[NW * kMostTop], s_id[NW * kMostTop];
   __shared__ int s_count;
@@ -114,14 +114,14 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(LogprobArgs p) {
     m = top;
   }
 
-  // The groups' largest, and of them the row's.
+  // The groups' largest, four to a lane, and of them the row's.
   float g = m;
 #pragma unroll
   for (int d = 1; d < GROUP; d <<= 1) g = larger(g, __shfl_xor(g, d));
-  if (lane % GROUP == 0) s_group[tid / GROUP] = g;
+  if (lane % GROUP == 0) reinterpret_cast<float*>(s_group)[tid / GROUP] = g;
   __syncthreads();
-  g = s_group[lane];
-  const int32_t og = order_of(g);
+  const float4 four = s_group[lane];
+  g = larger(larger(four.x, four.y), larger(four.z, four.w));
   float M = g;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) M = larger(M, __shfl_xor(M, d));
@@ -143,42 +143,56 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(LogprobArgs p) {
   if (lane == 0) s_sum[wave] = make_float2(s, ud);
 
   if (p.top) {
-    // The largest number that `top` groups reach: bit by bit.
+    // A number that `top` groups reach, the largest of 16 bits: bit by bit. (With the
+    // other 16, which bf16 has not, a row of fp32 would have a few candidates less.)
+    auto key_of = [](float v) __attribute__((always_inline)) { return (uint32_t)order_of(v) ^ 0x80000000u; };
     uint32_t bound = 0;
-    const uint32_t key = (uint32_t)og ^ 0x80000000u;
+    if (p.top <= 16) {
+      const uint32_t key = key_of(g);
 #pragma unroll
-    for (int b = 31; b >= 0; b--) {
-      const uint32_t t = bound | (1u << b);
-      if (__popcll(__builtin_amdgcn_ballot_w64(key >= t)) >= p.top) bound = t;
+      for (int b = 31; b >= 16; b--) {
+        const uint32_t t = bound | (1u << b);
+        if (__popcll(__builtin_amdgcn_ballot_w64(key >= t)) >= p.top) bound = t;
+      }
+    } else {
+      const uint32_t key[4] = {key_of(four.x), key_of(four.y), key_of(four.z), key_of(four.w)};
+#pragma unroll
+      for (int b = 31; b >= 16; b--) {
+        const uint32_t t = bound | (1u << b);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) n += __popcll(__builtin_amdgcn_ballot_w64(key[i] >= t));
+        if (n >= p.top) bound = t;
+      }
     }
-    const int32_t least = (int32_t)(bound ^ 0x80000000u);
+    // As a logit. (A bound that is NaN, where `top` groups have one, is below none; so is
+    // one between -inf and the smallest number, where fewer groups than `top` have any.)
+    const float least = logit_of((int32_t)(bound ^ 0x80000000u));
     // The wave's list: lane n has the n-th largest so far.
     int32_t lo = INT32_MIN, lid = INT32_MAX;
-    if (__builtin_amdgcn_ballot_w64(order_of(m) >= least) != 0) {
-      const bool mine = order_of(m) >= least;
+    const bool mine = !(m < least);
+    if (__builtin_amdgcn_ballot_w64(mine) != 0) {
       for (int r = 0; r < rounds; r++) {
-        uint32_t bits = 0;
-        static_assert(NU * U <= 32, "a bit for each element");
+        uint64_t bits = 0;
+        static_assert(NU * U <= 64, "a bit for each element");
         const int64_t first = (int64_t)r * NU * NT + tid;
         if (mine) {
 #pragma unroll
           for (int i = 0; i < NU; i++) {
             const Vec v = HELD ? x[i] : load(first + (int64_t)i * NT);
 #pragma unroll
-            for (int j = 0; j < U; j++) {
-              const int64_t at = (first + (int64_t)i * NT) * U + j;
-              if (at < p.V && order_of((float)v[j]) >= least) bits |= 1u << (i * U + j);
-            }
+            for (int j = 0; j < U; j++) bits |= (uint64_t)!((float)v[j] < least) << (i * U + j);
           }
         }
+        const bool one = HELD && __popcll(bits) == 1;  // then it is the thread's largest
         while (__builtin_amdgcn_ballot_w64(bits != 0) != 0) {
           // A candidate of every lane that has one, put in one after the other.
           int32_t o = INT32_MIN, id = INT32_MAX;
           if (bits) {
-            const int b = __builtin_ctz(bits);
+            const int b = __builtin_ctzll(bits);
             bits &= bits - 1;
-            id = (int32_t)((first + (int64_t)(b / U) * NT) * U + b % U);
-            o = order_of((float)row[id]);
+            const int64_t at = (first + (int64_t)(b / U) * NT) * U + b % U;
+            if (at < p.V) id = (int32_t)at, o = order_of(one ? m : (float)row[at]);
           }
           uint64_t todo = __builtin_amdgcn_ballot_w64(id != INT32_MAX);
           while (todo) {
@@ -188,9 +202,11 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(LogprobArgs p) {
             const bool before = lo > co || (lo == co && lid < cid);
             const int at = __popcll(__builtin_amdgcn_ballot_w64(before));
             if (at >= p.top) continue;
-            const int32_t po = __shfl_up(lo, 1), pid = __shfl_up(lid, 1);
-            if (lane == at) lo = co, lid = cid;
-            if (lane > at) lo = po, lid = pid;
+            // The lane before's (shifted through the whole wave).
+            const int32_t po = __builtin_amdgcn_update_dpp(0, lo, 0x138, 0xF, 0xF, false);
+            const int32_t pid = __builtin_amdgcn_update_dpp(0, lid, 0x138, 0xF, 0xF, false);
+            lo = lane > at ? po : lane == at ? co : lo;
+            lid = lane > at ? pid : lane == at ? cid : lid;
           }
         }
       }
@@ -220,13 +236,26 @@ __global__ void __launch_bounds__(NT) logprobs_kernel(LogprobArgs p) {
   }
   if (p.top) {
     const int n = s_count;
-    for (int i = tid; i < n; i += NT) {
-      const int32_t o = s_list[i], id = s_id[i];
-      int rank = 0;
-      for (int j = 0; j < n; j++) rank += s_list[j] > o || (s_list[j] == o && s_id[j] < id);
-      if (rank < p.top) {
-        p.top_ids[r * p.top + rank] = id;
-        p.top_logprobs[r * p.top + rank] = logit_of(o) - M - ln;
+    auto put = [&](int32_t o, int32_t id, int rank) __attribute__((always_inline)) {
+      if (rank >= p.top) return;
+      p.top_ids[r * p.top + rank] = id;
+      p.top_logprobs[r * p.top + rank] = logit_of(o) - M - ln;
+    };
+    if (n <= 64) {  // one wave, its lanes' candidates against each other
+      if (wave != 0) return;
+      const int32_t o = lane < n ? s_list[lane] : INT32_MIN, id = lane < n ? s_id[lane] : INT32_MAX;
+      int rank = lane < n ? 0 : kMostTop;
+      for (int j = 0; j < n; j++) {
+        const int32_t oj = __builtin_amdgcn_readlane(o, j), idj = __builtin_amdgcn_readlane(id, j);
+        rank += oj > o || (oj == o && idj < id);
+      }
+      put(o, id, rank);
+    } else {
+      for (int i = tid; i < n; i += NT) {
+        const int32_t o = s_list[i], id = s_id[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += s_list[j] > o || (s_list[j] == o && s_id[j] < id);
+        put(o, id, rank);
       }
     }
   }
