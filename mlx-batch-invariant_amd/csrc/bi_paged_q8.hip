@@ -51,71 +51,138 @@ template <typename T, int U> struct Vec {
 };
 
 // x / s to the nearest whole number, ties to even, within -127 .. 127.
-__device__ __forceinline__ int8_t code_of(float x, float s) {
+__device__ __forceinline__ float code_of(float x, float s) {
   float n = __builtin_rintf(x / s);
   // The quotient's own rounding may have made a tie of what is none.
   const float r = 2.f * __builtin_fmaf(-n, s, x);
   if (r > s) n += 1.f;
   if (r < -s) n -= 1.f;
   n = fminf(fmaxf(n, -127.f), 127.f);
-  return (int8_t)(int)n;
+  return x == x ? n : 0.f;
+}
+// The codes of U values with scale s above 0, `inv` about 1 / s: n = rint(x * inv)
+// is the nearest whole number to x / s if |x - n s| is below s / 2, which it nearly
+// always is; the fma rounds that difference once, and s / 2 is a number of 32 bits, so
+// the comparison is exact. Else, next to a tie, the wave divides. (With a division for
+// every value 8161 tokens took 25 us; memory would take 10.)
+template <int U>
+__device__ __forceinline__ void codes_of(const float (&x)[U], float s, float inv, bool keep, int8_t (&c)[U]) {
+  float n[U], far = 0.f;
+  bool odd = !(s > 1e-30f && s < 1e37f);
+#pragma unroll
+  for (int i = 0; i < U; i++) {
+    n[i] = __builtin_rintf(x[i] * inv);
+    far = fmaxf(far, fabsf(__builtin_fmaf(-n[i], s, x[i])));
+    if (keep) {
+      odd |= x[i] != x[i];
+      n[i] = fminf(fmaxf(n[i], -127.f), 127.f);
+    }
+  }
+  if (__builtin_amdgcn_ballot_w64(odd || !(2.f * far < s)) != 0)
+#pragma unroll
+    for (int i = 0; i < U; i++) n[i] = code_of(x[i], s);
+#pragma unroll
+  for (int i = 0; i < U; i++) c[i] = (int8_t)(int)n[i];
+}
+
+// The largest of `lanes` neighbouring lanes, a power of two, by moves within a
+// register (a shuffle by way of the LDS takes ten times as long).
+template <int CTRL> __device__ __forceinline__ float max_with(float x) {
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ float row_max(float x, int lanes) {
+  if (lanes > 1) x = max_with<0xB1>(x);   // lane ^ 1
+  if (lanes > 2) x = max_with<0x4E>(x);   // lane ^ 2
+  if (lanes > 4) x = max_with<0x141>(x);  // 7 - lane of eight
+  if (lanes > 8) x = max_with<0x140>(x);  // 15 - lane of sixteen
+  if (lanes > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if (lanes > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return x;
+}
+
+// A row's side, and its token and head, from the thread's place.
+struct Place {
+  int kv, lane;
+  int32_t t, head;
+  bool real;
+};
+__device__ __forceinline__ Place place(const Q8Args& p) {
+  Place x;
+  x.kv = (int)blockIdx.x >= p.side[0].blocks;
+  const Side& w = p.side[x.kv];
+  const uint32_t thread = (blockIdx.x - (x.kv ? p.side[0].blocks : 0)) * kThreads + threadIdx.x;
+  x.lane = threadIdx.x & (w.lanes - 1);
+  const uint32_t id = thread >> w.shift;
+  x.real = id < p.rows;
+  x.t = x.real ? (int32_t)id / p.Hkv : 0;
+  x.head = x.real ? (int32_t)id - x.t * (int32_t)p.Hkv.d : 0;
+  return x;
 }
 
 // One row of a token and head by `lanes` lanes, U elements at a time each (16
-// bytes, or one where rows are not aligned to that). What bounds it is memory.
-template <typename T, int U>
+// bytes, or one where rows are not aligned to that); ONE: each lane has one unit at
+// most. What bounds it is memory, and the chain of a wave, of which there are few
+// rounds: both rows of a token and head by the same lanes took 27 us for 8161 tokens
+// of 4 KB, a row each 21.
+template <typename T, int U, bool ONE>
 __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
   typedef typename Vec<T, U>::type In;
   typedef typename Vec<int8_t, U>::type Out;
-  const int kv = (int)blockIdx.x >= p.side[0].blocks;
-  const Side& w = p.side[kv];
-  const int64_t block = blockIdx.x - (kv ? p.side[0].blocks : 0);
-  const int lane = threadIdx.x & (w.lanes - 1);
-  const int64_t id = (block * kThreads + threadIdx.x) >> w.shift;
-  const bool real = id < p.rows;
-  const int32_t t = real ? (int32_t)id / p.Hkv : 0, head = real ? (int32_t)id - t * (int32_t)p.Hkv.d : 0;
-  const int32_t slot = p.slots[t];
-  const bool write = real && slot >= 0 && slot < p.slots_end;
-  const char* row = w.src + t * w.ts + head * w.hs;
-  const int32_t pg = (write ? slot : 0) / p.page, at = (write ? slot : 0) - pg * (int32_t)p.page.d;
-  float* scale = w.scale + pg * w.sp + head * w.sh + at * w.sr;
-
-  // The first unit stays in registers: for most heads it is the only one.
+  const Place x = place(p);
+  const Side& w = p.side[x.kv];
+  // (The row is loaded before the slot is looked at, so that both are under way together.)
+  const char* row = w.src + x.t * w.ts + x.head * w.hs;
   In first = {};
+  if (x.lane < w.units) first = reinterpret_cast<const In*>(row)[x.lane];
+  const int32_t slot = p.slots[x.t];
   float top = 0.f;
-  bool odd = false;  // an infinity or NaN
-  float s;
-  if (p.keep) {
-    if (lane < w.units) first = reinterpret_cast<const In*>(row)[lane];
-    s = write ? *scale : 0.f;
-  } else {
-    for (int u = lane; u < w.units; u += w.lanes) {
-      const In x = reinterpret_cast<const In*>(row)[u];
-      if (u == lane) first = x;
+  if (!p.keep) {
+    bool odd = false;  // an infinity or NaN
+    auto look = [&](const In& y) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < U; i++) {
-        const float a = fabsf((float)x[i]);
+        const float a = fabsf((float)y[i]);
         odd |= !(a <= FLT_MAX);
         top = fmaxf(top, a);
       }
-    }
-    top = odd ? INFINITY : top;
-    for (int d = 1; d < w.lanes; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    };
+    look(first);
+    if (!ONE)
+      for (int u = x.lane + w.lanes; u < w.units; u += w.lanes) look(reinterpret_cast<const In*>(row)[u]);
+    top = row_max(odd ? INFINITY : top, w.lanes);
+  }
+  if (!x.real || slot < 0 || slot >= p.slots_end) return;
+  const int32_t pg = slot / p.page, at = slot - pg * (int32_t)p.page.d;
+  float* scale = w.scale + pg * w.sp + x.head * w.sh + at * w.sr;
+  float s;
+  if (p.keep) {
+    s = *scale;
+  } else {
     s = top <= FLT_MAX ? top / 127.f : NAN;
-    if (write && lane == 0) *scale = s;
+    if (x.lane == 0) *scale = s;
   }
-  if (!write) return;
-  Out* out = reinterpret_cast<Out*>(w.dst + pg * w.cp + head * w.ch + at * w.cr);
-  for (int u = lane; u < w.units; u += w.lanes) {
-    const In x = u == lane ? first : reinterpret_cast<const In*>(row)[u];
-    Out c;
+  const float inv = 1.f / s;
+  Out* out = reinterpret_cast<Out*>(w.dst + pg * w.cp + x.head * w.ch + at * w.cr);
+  auto put = [&](int u, const In& y) __attribute__((always_inline)) {
+    float v[U];
+    int8_t c[U] = {};
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      const float v = (float)x[i];
-      c[i] = s > 0.f && v == v ? code_of(v, s) : (int8_t)0;
-    }
-    out[u] = c;
-  }
+    for (int i = 0; i < U; i++) v[i] = (float)y[i];
+    if (s > 0.f) codes_of<U>(v, s, inv, p.keep, c);
+    Out z;
+#pragma unroll
+    for (int i = 0; i < U; i++) z[i] = c[i];
+    out[u] = z;
+  };
+  if (x.lane < w.units) put(x.lane, first);
+  if (!ONE)
+    for (int u = x.lane + w.lanes; u < w.units; u += w.lanes) put(u, reinterpret_cast<const In*>(row)[u]);
 }
 
 // The way back: unit by unit, a code's value c * s in 32 bits, rounded once
@@ -124,32 +191,28 @@ template <typename C, typename T, int U>
 __global__ void __launch_bounds__(kThreads) read_kernel(Q8Args p) {
   typedef typename Vec<C, U>::type In;
   typedef typename Vec<T, U>::type Out;
-  const int kv = (int)blockIdx.x >= p.side[0].blocks;
-  const Side& w = p.side[kv];
-  const int64_t block = blockIdx.x - (kv ? p.side[0].blocks : 0);
-  const int lane = threadIdx.x & (w.lanes - 1);
-  const int64_t id = (block * kThreads + threadIdx.x) >> w.shift;
-  if (id >= p.rows) return;
-  const int32_t t = (int32_t)id / p.Hkv, head = (int32_t)id - t * (int32_t)p.Hkv.d;
-  const int32_t slot = p.slots[t];
+  const Place x = place(p);
+  if (!x.real) return;
+  const Side& w = p.side[x.kv];
+  const int32_t slot = p.slots[x.t];
   const bool there = slot >= 0 && slot < p.slots_end;
   const int32_t pg = (there ? slot : 0) / p.page, at = (there ? slot : 0) - pg * (int32_t)p.page.d;
-  const In* row = reinterpret_cast<const In*>(w.src + pg * w.cp + head * w.ch + at * w.cr);
+  const In* row = reinterpret_cast<const In*>(w.src + pg * w.cp + x.head * w.ch + at * w.cr);
   float s = 1.f;
   if constexpr (sizeof(C) == 1)
-    if (there) s = w.scale[pg * w.sp + head * w.sh + at * w.sr];
-  Out* out = reinterpret_cast<Out*>(w.dst + t * w.ts + head * w.hs);
-  for (int u = lane; u < w.units; u += w.lanes) {
-    Out y = {};
+    if (there) s = w.scale[pg * w.sp + x.head * w.sh + at * w.sr];
+  Out* out = reinterpret_cast<Out*>(w.dst + x.t * w.ts + x.head * w.hs);
+  for (int u = x.lane; u < w.units; u += w.lanes) {
+    Out z = {};
     if (there) {
-      const In x = row[u];
+      const In y = row[u];
 #pragma unroll
       for (int i = 0; i < U; i++) {
-        if constexpr (sizeof(C) == 1) y[i] = (T)((float)x[i] * s);
-        else y[i] = x[i];
+        if constexpr (sizeof(C) == 1) z[i] = (T)((float)y[i] * s);
+        else z[i] = y[i];
       }
     }
-    out[u] = y;
+    out[u] = z;
   }
 }
 
@@ -206,15 +269,19 @@ int start(const char* who, Q8Args& p, void (*kernel)(Q8Args), int unit, void* st
     w.shift = shift_for(w.units);
     w.lanes = 1 << w.shift;
     const int64_t blocks = (p.rows * w.lanes + kThreads - 1) / kThreads;
+    if (blocks * kThreads > INT32_MAX) return bi::fail(BI_EINVAL, "%s: sizes too large", who);
     w.blocks = (int32_t)blocks;
     all += blocks;
   }
-  if (all > INT32_MAX) return bi::fail(BI_EINVAL, "%s: sizes too large", who);
   hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? BI_OK : bi::launch_error(e, who);
 }
 
+template <typename T> void (*update_for(bool wide, bool one))(Q8Args) {
+  constexpr int U = 16 / sizeof(T);
+  return !wide ? update_kernel<T, 1, false> : one ? update_kernel<T, U, true> : update_kernel<T, U, false>;
+}
 template <typename C> void (*read_for(int dtype, bool wide))(Q8Args) {
   if constexpr (sizeof(C) == 1) {
     if (dtype == BI_F32) return wide ? read_kernel<C, float, 4> : read_kernel<C, float, 1>;
@@ -254,10 +321,11 @@ extern "C" int bi_paged_update_q8(const void* k, const void* v, int8_t* k_cache,
   p.side[0].scale = k_scales, p.side[1].scale = v_scales;
   p.keep = keep_scales;
   const bool wide = aligned(p, tokens, cache, 16 / esz, esz, 1);
+  const bool one = D * esz <= 1024 && V * esz <= 1024;  // 64 lanes of 16 bytes
   void (*f)(Q8Args);
-  if (dtype == BI_F32) f = wide ? update_kernel<float, 4> : update_kernel<float, 1>;
-  else if (dtype == BI_F16) f = wide ? update_kernel<_Float16, 8> : update_kernel<_Float16, 1>;
-  else f = wide ? update_kernel<__bf16, 8> : update_kernel<__bf16, 1>;
+  if (dtype == BI_F32) f = update_for<float>(wide, one);
+  else if (dtype == BI_F16) f = update_for<_Float16>(wide, one);
+  else f = update_for<__bf16>(wide, one);
   return start(who, p, f, wide ? 16 / esz : 1, hip_stream);
 }
 
