@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
     s = top <= FLT_MAX ? top / 127.f : NAN;
     if (x.lane == 0) *scale = s;
   }
-  const float inv = 1.f / s;
+  const float inv = __builtin_amdgcn_rcpf(s);
   Out* out = reinterpret_cast<Out*>(w.dst + pg * w.cp + x.head * w.ch + at * w.cr);
   auto put = [&](int u, const In& y) __attribute__((always_inline)) {
     float v[U];

@@ -11,6 +11,7 @@ from . import _lib
 from ._paged import _call, _no_grad, _on_one_gpu
 
 MAX_TOP = 64
+_INTS = (torch.int64, torch.int32)
 
 TokenLogprobs = collections.namedtuple("TokenLogprobs",
                                        ("logprobs", "entropy", "top_ids", "top_logprobs"))
@@ -32,16 +33,17 @@ def token_logprobs(logits, tokens, top=0):
     Log probabilities and entropy of a row that holds a NaN or +inf, or nothing
     but -inf, are NaN.
     """
-    if logits.ndim < 1 or logits.dtype not in _lib.DTYPE_CODES:
+    shape = logits.shape
+    if not len(shape) or logits.dtype not in _lib.DTYPE_CODES:
         raise ValueError("logits must be float32, float16 or bfloat16 of one dimension or more, got "
-                         "%s of shape %s" % (logits.dtype, tuple(logits.shape)))
-    if tokens.dtype not in (torch.int64, torch.int32) or tokens.shape != logits.shape[:-1]:
+                         "%s of shape %s" % (logits.dtype, tuple(shape)))
+    if tokens.dtype not in _INTS or tokens.shape != shape[:-1]:
         raise ValueError("tokens must be int64 or int32 of shape %s, got %s of shape %s"
-                         % (tuple(logits.shape[:-1]), tokens.dtype, tuple(tokens.shape)))
-    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
+                         % (tuple(shape[:-1]), tokens.dtype, tuple(tokens.shape)))
+    if not 0 <= top <= MAX_TOP or top > shape[-1]:
         raise ValueError("top must be between 0 and %d and at most the vocabulary of %d, got %r"
-                         % (MAX_TOP, logits.shape[-1], top))
-    if not logits.shape[-1]:
+                         % (MAX_TOP, shape[-1], top))
+    if not shape[-1]:
         raise ValueError("logits of no vocabulary")
     _no_grad("token_logprobs", logits)
     if torch.compiler.is_compiling():
@@ -54,21 +56,20 @@ def token_logprobs(logits, tokens, top=0):
 def _logprobs_eager(logits, tokens, top):
     dev = logits.device
     _on_one_gpu("token_logprobs", dev, (tokens,))
-    lead, V = logits.shape[:-1], logits.shape[-1]
+    lead, V = tokens.shape, logits.shape[-1]
     rows = tokens.numel()
-    # One allocation for what is float.
-    buf = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
-    logprobs, entropy, tops = buf.split_with_sizes((rows, rows, rows * top))
+    f32 = dict(dtype=torch.float32, device=dev)
+    logprobs, entropy = torch.empty(lead, **f32), torch.empty(lead, **f32)
+    tops = torch.empty((*lead, top), **f32)
     ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
     if rows:
         x = logits
-        if x.ndim != 2 or x.stride(1) != 1:
+        if x.ndim != 2 or (x.stride(1) != 1 and V > 1):
             x = x.reshape(rows, V)
             if V > 1 and x.stride(1) != 1:
                 x = x.contiguous()
         tokens = tokens.contiguous()
-        at = buf.data_ptr()
         _call(dev, "bi_token_logprobs", _lib.lib().bi_token_logprobs, x.data_ptr(), tokens.data_ptr(),
-              at, at + 4 * rows, ids.data_ptr(), at + 8 * rows, rows, V, x.stride(0), top,
-              tokens.element_size(), _lib.DTYPE_CODES[x.dtype])
-    return logprobs.view(lead), entropy.view(lead), ids, tops.view(*lead, top)
+              logprobs.data_ptr(), entropy.data_ptr(), ids.data_ptr(), tops.data_ptr(), rows, V,
+              x.stride(0), top, tokens.element_size(), _lib.DTYPE_CODES[x.dtype])
+    return logprobs, entropy, ids, tops

@@ -183,8 +183,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int
                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     from . import _logprobs
 
-    # Outputs of a custom op may not share storage.
-    return tuple(t.clone() for t in _logprobs._logprobs_eager(logits, tokens, top))
+    return _logprobs._logprobs_eager(logits, tokens, top)
 
 
 @token_logprobs.register_fake

@@ -46,7 +46,7 @@ PageTables = collections.namedtuple(
     "PageTables", ("block_tables", "slots", "positions", "query_start", "seq_lens", "pages_used"))
 
 
-_I32 = torch.int32
+_I32, _I8 = torch.int32, torch.int8
 _I64x6 = ctypes.c_int64 * 6
 _I64x9 = ctypes.c_int64 * 9
 _I64x10 = ctypes.c_int64 * 10
@@ -159,16 +159,23 @@ def _page_tables_eager(block_tables, context_lens, new_lens, free_pages, page_si
     return slots, positions, start, seq, used.view(())
 
 
-def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(what, a, b=None):
+    if (a.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("%s has no backward pass: call it under torch.no_grad()" % what)
 
 
-def _scale_strides(name, scales, cache):
-    if scales.dtype != torch.float32 or scales.shape != cache.shape[:3]:
-        raise ValueError("%s must be float32 of shape %s, got %s of shape %s"
-                         % (name, tuple(cache.shape[:3]), scales.dtype, tuple(scales.shape)))
-    return scales.stride()
+def _scale_shapes(rows, k_scales, v_scales, k_cache, v_cache):
+    """The checks of 8-bit caches, whose pages have the shape `rows` (num_pages,
+    Hkv, page_size)."""
+    if k_cache.dtype is not _I8 or v_cache.dtype is not _I8 or k_scales is None or v_scales is None:
+        raise ValueError("k_scales and v_scales go with int8 caches, and these with both, got "
+                         "caches of %s and %s, %s and %s scales"
+                         % (k_cache.dtype, v_cache.dtype, "no" if k_scales is None else "k",
+                            "no" if v_scales is None else "v"))
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t.dtype is not torch.float32 or t.shape != rows:
+            raise ValueError("%s must be float32 of shape %s, got %s of shape %s"
+                             % (name, tuple(rows), t.dtype, tuple(t.shape)))
 
 
 def _cache_shapes(k_cache, v_cache, k_scales=None, v_scales=None):
@@ -180,15 +187,8 @@ def _cache_shapes(k_cache, v_cache, k_scales=None, v_scales=None):
     kst, vst = k_cache.stride(), v_cache.stride()
     if kst[3] != 1 or vst[3] != 1:
         raise ValueError("the caches' last dimension must be contiguous")
-    if k_scales is not None or v_scales is not None or k_cache.dtype is torch.int8:
-        if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8 or k_scales is None \
-                or v_scales is None:
-            raise ValueError("k_scales and v_scales go with int8 caches, and these with both, got "
-                             "caches of %s and %s, %s and %s scales"
-                             % (k_cache.dtype, v_cache.dtype, "no" if k_scales is None else "k",
-                                "no" if v_scales is None else "v"))
-        _scale_strides("k_scales", k_scales, k_cache)
-        _scale_strides("v_scales", v_scales, v_cache)
+    if k_scales is not None or v_scales is not None or k_cache.dtype is _I8:
+        _scale_shapes(ks[:3], k_scales, v_scales, k_cache, v_cache)
     elif k_cache.dtype != v_cache.dtype or k_cache.dtype not in _lib.DTYPE_CODES:
         raise ValueError("caches must share a dtype of float32, float16 or bfloat16, got %s and %s"
                          % (k_cache.dtype, v_cache.dtype))
@@ -235,7 +235,7 @@ def paged_cache_update(k, v, k_cache, v_cache, slots, *, k_scales=None, v_scales
                              "and %s" % (k.dtype, v.dtype))
         if not keep_scales:
             for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-                if any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+                if 0 in t.stride() and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
                     raise ValueError("%s is an expanded view, which keep_scales=True takes: a scale "
                                      "is written for every token and head" % name)
     _int32("slots", slots, k.shape[0])

@@ -71,19 +71,21 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, offset=0, scale=1.0)
     ``q`` and ``k`` may be strided views, such as slices of a projection's
     output.
     """
-    if q.ndim != 3 or (k is not None and (k.ndim != 3 or k.shape[::2] != q.shape[::2])):
+    qs, dt = q.shape, q.dtype
+    ks = qs if k is None else k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("q and k must be (tokens, heads, head dim), got %s and %s"
-                         % (tuple(q.shape), None if k is None else tuple(k.shape)))
-    if q.dtype not in _lib.DTYPE_CODES or (k is not None and k.dtype != q.dtype):
+                         % (tuple(qs), None if k is None else tuple(ks)))
+    if dt not in _lib.DTYPE_CODES or (k is not None and k.dtype is not dt):
         raise ValueError("q and k must share a dtype of float32, float16 or bfloat16, got %s and %s"
-                         % (q.dtype, None if k is None else k.dtype))
-    _int32("positions", positions, q.shape[0])
-    if inv_freq.dtype != torch.float64 or inv_freq.ndim != 1:
+                         % (dt, None if k is None else k.dtype))
+    _int32("positions", positions, qs[0])
+    if inv_freq.dtype is not torch.float64 or inv_freq.ndim != 1:
         raise ValueError("inv_freq must be float64 of one dimension, got %s of shape %s"
                          % (inv_freq.dtype, tuple(inv_freq.shape)))
-    if offset < 0 or offset + 2 * inv_freq.shape[0] > q.shape[2]:
-        raise ValueError("%d pairs from dim %r on do not fit heads of %d"
-                         % (inv_freq.shape[0], offset, q.shape[2]))
+    n = inv_freq.shape[0]
+    if offset < 0 or offset + 2 * n > qs[2]:
+        raise ValueError("%d pairs from dim %r on do not fit heads of %d" % (n, offset, qs[2]))
     _no_grad("rotary", q, k)
     args = (q, k, positions, inv_freq, bool(interleaved), int(offset), float(scale))
     if torch.compiler.is_compiling():
