@@ -344,14 +344,21 @@ int bi_paged_read(const void* k_cache, const void* v_cache, const float* k_scale
  *                       and strides are multiples of 16 bytes)
  *   k_scales, v_scales  (num_pages, Hkv, page_size) float, element strides
  *                       scale_strides[0..2] and [3..5] (page, head, row; 0 for
- *                       one a page or a head). A negative key scale gives NaN.
+ *                       one a page or a head)
  *   dtype               of q, sinks and out: BI_F16 or BI_BF16
  *
+ * Pages and rows (strides[2], [4], [5], [7] and those of the scales) lie less
+ * than 4 GiB apart, none at a negative stride (else BI_EUNSUPPORTED); heads at any
+ * stride, and all at any offset.
+ *
  * Scores are sums of exact products of codes and q in 32 bits times the row's
- * scale in 32 bits; weights times the row's scale are rounded to bf16 (BI_F16: to
- * two bf16, 2^-17), products and sums in 32 bits, the denominator the sum of the
- * weights of 32 bits. A token's bits depend on its own request's rows alone, as
- * there, and nothing in a row that a token does not see reaches it.
+ * scale in 32 bits; weights times the row's scale are rounded to `dtype` (BI_F16:
+ * but for the scale's power of two, which goes with the codes, so that scales from
+ * 2^-14 lose nothing; those of 2^19 and above, of values past 6e7, overflow),
+ * products and sums are of 32 bits, the denominator the sum of the weights of 32
+ * bits. A token that sees a row whose key or value scale is infinite or NaN, or
+ * whose key scale is negative, is NaN. A token's bits depend on its own request's
+ * rows alone, as there, and nothing in a row that a token does not see reaches it.
  */
 int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const int8_t* v_cache,
                           const float* k_scales, const float* v_scales,

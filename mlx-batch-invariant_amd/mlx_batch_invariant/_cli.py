@@ -4,7 +4,8 @@ Mirrors reference mlx_batch_invariant/_cli.py:17-161 (the linear batch sweep,
 the attention query-length sweep, the stock negative control and the exit
 codes), on torch + the HIP kernels, and adds the axes this build promises:
 every row position of a batch, context growth with masked keys past 4096, HIP
-graph capture, and a paged cache (chunks, batches, pages, contiguous keys). Exit status 1 on any variance or if stock torch.matmul
+graph capture, and a paged cache (chunks, batches, pages, contiguous keys), also
+of 8 bits with turned keys. Exit status 1 on any variance or if stock torch.matmul
 comes out invariant everywhere (then the sweep proves nothing); 2 on usage.
 """
 
@@ -12,7 +13,8 @@ import argparse
 import platform
 import sys
 
-from . import __version__, paged_attention, scaled_dot_product_attention, window_attention
+from . import (__version__, paged_attention, paged_cache_update, rotary, rotary_frequencies,
+               scaled_dot_product_attention, token_logprobs, window_attention)
 from ._gemm import linear
 
 _DTYPES = ("bfloat16", "float16", "float32")
@@ -159,6 +161,60 @@ def _paged_case(dtype, gen, device, H, Hkv, D, n, L, window=None, first=0):
     return bad
 
 
+def _paged_q8_case(dtype, gen, device, H, Hkv, D, n, L, window=None, first=0):
+    """The last L tokens of a request of n rows, turned by their positions, over an
+    8-bit paged cache: written at once and token by token, attended to token by
+    token, in a batch and over other pages; and their log probabilities, taking the
+    results as logits, row by row. Returns what differs."""
+    import torch
+
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=device)
+    same = lambda a, b: torch.equal(_bits(a), _bits(b))
+    k, v = (_rn((n, Hkv, D), dtype, gen, device) for _ in range(2))
+    q = _rn((L, H, D), dtype, gen, device)
+    f = rotary_frequencies(D, device=device)
+    at = torch.arange(n, dtype=torch.int32, device=device)
+    bad = []
+    q, turned = rotary(q, None, at[n - L:], f)[0], rotary(k, None, at, f)[0]
+    if not same(rotary(k[n // 2:n // 2 + 1], None, at[n // 2:n // 2 + 1], f)[0], turned[n // 2:n // 2 + 1]):
+        bad.append("rotary")
+    k = turned
+
+    def paged(page, pieces):
+        pages = -(-n // page)
+        table = torch.randperm(pages + 2, generator=gen)[:pages].to(torch.int32).to(device)
+        c = [torch.zeros(pages + 2, Hkv, page, D, dtype=torch.int8, device=device) for _ in range(2)]
+        s = dict((name, torch.zeros(pages + 2, Hkv, page, device=device))
+                 for name in ("k_scales", "v_scales"))
+        slots = table[at.long() // page] * page + at % page
+        for a, b in pieces:
+            paged_cache_update(k[a:b], v[a:b], *c, slots[a:b], **s)
+        return c, s, table[None]
+
+    (kc, vc), s, table = paged(16, [(0, n)])
+    kw = dict(window=window, sink_tokens=first, **s)
+    base = paged_attention(q, kc, vc, table, i32([0, L]), i32([n]), **kw)
+    for a in (0, L // 2, L - 1):
+        if not same(paged_attention(q[a:a + 1], kc, vc, table, i32([0, 1]), i32([n - L + a + 1]), **kw),
+                    base[a:a + 1]):
+            bad.append("token %d" % a)
+    both = paged_attention(torch.cat([q[-3:], q]), kc, vc, torch.cat([table, table]),
+                           i32([0, 3, 3 + L]), i32([n, n]), **kw)
+    if not same(both[3:], base) or not same(both[:3], base[-3:]):
+        bad.append("batch")
+    (k2, v2), s2, t2 = paged(48, [(i, i + 1) for i in range(n)])
+    if not same(paged_attention(q, k2, v2, t2, i32([0, L]), i32([n]), window=window, sink_tokens=first,
+                                **s2), base):
+        bad.append("pages")
+    x = base.reshape(L, H * D)
+    ids = torch.arange(L, device=device) % (H * D)
+    got = token_logprobs(x, ids, top=5)
+    one = token_logprobs(x[L // 2], ids[L // 2], top=5)
+    if not all(torch.equal(a, b[L // 2]) for a, b in zip(one, got)):
+        bad.append("logprobs")
+    return bad
+
+
 def _stock_matmul_variant(batches, gen, device):
     """Stock torch.matmul must be batch-variant somewhere (reference
     _cli.py:121-128 checks fp32 4096x4096; hipBLASLt picks kernels per shape,
@@ -230,6 +286,13 @@ def verify(argv=None):
             bad = _paged_case(dtype, gen, device, H, Hkv, D, n, L, window, first)
             fails += bool(bad)
             print("  %-9s paged    H=%d/%-2d N=%-6d %s%s"
+                  % (name, H, Hkv, n, "ok" if not bad else "VARIANT over %s" % ", ".join(bad),
+                     "" if window is None else " (window %d)" % window))
+            if dtype == torch.float32:
+                continue
+            bad = _paged_q8_case(dtype, gen, device, H, Hkv, D, n, L, window, first)
+            fails += bool(bad)
+            print("  %-9s paged8   H=%d/%-2d N=%-6d %s%s"
                   % (name, H, Hkv, n, "ok" if not bad else "VARIANT over %s" % ", ".join(bad),
                      "" if window is None else " (window %d)" % window))
         if not args.quick:

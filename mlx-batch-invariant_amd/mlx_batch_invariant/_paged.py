@@ -392,10 +392,12 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     tight bounds are faster; a request beyond one gets NaN.
 
     ``k_scales`` and ``v_scales`` (num_pages, Hkv, page_size) float32 go with
-    int8 caches (:func:`paged_cache_update`); q is then float16 or bfloat16. Any
-    strides will do, 0 for one scale a page or a head. The bits are as
-    independent of the call as without scales, and another's: the products are
-    of codes.
+    int8 caches (:func:`paged_cache_update`); q is then float16 or bfloat16.
+    Expanded scales will do, one for a page or a head; pages and rows lie less
+    than 4 GiB apart. The bits are as independent of the call as without scales,
+    but others: the products are of codes, and weights times their row's scale
+    are rounded to q's type. A token is NaN that sees a row whose scale is
+    infinite or NaN, or negative for keys.
     """
     _cache_shapes(k_cache, v_cache, k_scales, v_scales)
     if q.ndim != 3:

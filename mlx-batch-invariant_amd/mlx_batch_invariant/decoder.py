@@ -15,9 +15,14 @@ generator, so the same seed gives the same model.
 
 :class:`PagedCache` and :func:`serve_step` run the same model over a paged cache,
 request by request and chunk by chunk (bi.page_tables, bi.paged_cache_update,
-bi.paged_attention); :func:`generate` decodes greedily on top of them. Under
+bi.paged_attention); :func:`generate` decodes greedily on top of them, and
+:func:`score` gives the log probabilities of given texts' tokens. Under
 ``batch_invariant_mode`` a request's logits have the same bits whatever is
-served beside it and however its prompt is cut into chunks.
+served beside it and however its prompt is cut into chunks: so do the log
+probabilities, those of a generated token and of the same token scored. The
+cache may be of 8 bits (``dtype=torch.int8``), and a configuration with
+``rope_base`` turns queries and keys by their positions (bi.rotary), which the
+reference's model does not.
 """
 
 import math
@@ -37,6 +42,9 @@ class DecoderConfig:
     layers: int = 32
     vocab: int = 32000
     eps: float = 1e-5
+    rope_base: float = 0.0  # 0: no positions
+    rope_dim: int = 0       # dims of a head that turn, from the first; 0: all
+    rope_interleaved: bool = False
 
 
 # random-init Llama-style decoder, 32 layers, hidden 4096,
@@ -59,12 +67,15 @@ class Block(torch.nn.Module):
         self.n1 = torch.nn.RMSNorm(c.hidden, eps=c.eps, device=device, dtype=dtype)
         self.n2 = torch.nn.RMSNorm(c.hidden, eps=c.eps, device=device, dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, turn=None):
         c = self.c
         B, L, _ = x.shape
         y = self.n1(x)
-        q = self.q(y).view(B, L, c.heads, c.head_dim).transpose(1, 2)
-        k = self.k(y).view(B, L, c.kv_heads, c.head_dim).transpose(1, 2)
+        q, k = self.q(y), self.k(y)
+        if turn is not None:
+            q, k = turn(q.view(B * L, c.heads, c.head_dim), k.view(B * L, c.kv_heads, c.head_dim))
+        q = q.view(B, L, c.heads, c.head_dim).transpose(1, 2)
+        k = k.view(B, L, c.kv_heads, c.head_dim).transpose(1, 2)
         v = self.v(y).view(B, L, c.kv_heads, c.head_dim).transpose(1, 2)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=L > 1,
                                            scale=1.0 / math.sqrt(c.head_dim), enable_gqa=True)
@@ -81,12 +92,33 @@ class Decoder(torch.nn.Module):
         self.blocks = torch.nn.ModuleList(Block(c, device, dtype) for _ in range(c.layers))
         self.norm = torch.nn.RMSNorm(c.hidden, eps=c.eps, device=device, dtype=dtype)
         self.head = torch.nn.Linear(c.hidden, c.vocab, bias=False, device=device, dtype=dtype)
+        self.inv_freq = None
+        if c.rope_base:
+            from . import rotary_frequencies
+
+            self.inv_freq = rotary_frequencies(c.rope_dim or c.head_dim, c.rope_base, device=device)
+
+    def turn(self, positions):
+        """What turns queries and keys (tokens, heads, head dim) by `positions`
+        (tokens,); None without positions."""
+        if self.inv_freq is None:
+            return None
+        from . import rotary
+
+        # (No buffer: a cast of the model would round it.)
+        self.inv_freq = self.inv_freq.to(positions.device)
+        return lambda q, k: rotary(q, k, positions, self.inv_freq,
+                                   interleaved=self.c.rope_interleaved)
 
     def forward(self, ids):
         """Logits of the last position of every sequence, (B, vocab)."""
         x = self.embed(ids)
+        B, L = ids.shape
+        turn = None
+        if self.inv_freq is not None:
+            turn = self.turn(torch.arange(L, dtype=torch.int32, device=ids.device).repeat(B))
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x, turn)
         return self.head(self.norm(x[:, -1]))
 
 
@@ -133,7 +165,8 @@ class PagedCache:
     """Keys and values of up to `requests` requests of up to `max_len` tokens in
     pages shared by all, one pool per layer; one table for all layers. The
     lengths are kept on the host too, which sizes every step without asking the
-    GPU."""
+    GPU. With ``dtype=torch.int8`` the pools hold codes of 8 bits, and scales
+    beside them."""
 
     def __init__(self, config, requests, max_len, page_size=64, num_pages=None, device="cuda",
                  dtype=torch.bfloat16):
@@ -144,6 +177,10 @@ class PagedCache:
         shape = (c.layers, self.num_pages, c.kv_heads, page_size, c.head_dim)
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.k_scales = self.v_scales = None
+        if dtype == torch.int8:
+            self.k_scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+            self.v_scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
         self.tables = torch.full((requests, width), -1, dtype=torch.int32, device=device)
         self.free = torch.arange(self.num_pages, dtype=torch.int32, device=device)
         self.used = 0
@@ -171,6 +208,20 @@ class PagedCache:
         self.lens = after
         return t, max(new), max(after)
 
+    def scales(self, layer):
+        """The layer's scales as keyword arguments of the cache's operators."""
+        if self.k_scales is None:
+            return {}
+        return dict(k_scales=self.k_scales[layer], v_scales=self.v_scales[layer])
+
+    def read(self, request, layer, dtype=None):
+        """Keys and values (n, kv_heads, head_dim) of a request's n tokens."""
+        from . import paged_cache_read
+
+        i = torch.arange(self.lens[request], dtype=torch.int32, device=self.tables.device)
+        slots = self.tables[request][(i // self.page_size).long()] * self.page_size + i % self.page_size
+        return paged_cache_read(self.k[layer], self.v[layer], slots, dtype=dtype, **self.scales(layer))
+
     def release(self, request):
         """Ends a request: its pages are free again and its row, empty, is
         another's. Steps that were launched before still read what was there
@@ -182,11 +233,9 @@ class PagedCache:
         self.lens[request] = 0
 
 
-def serve_step(model, cache, ids, new):
-    """One step over `cache`: ids (sum of new,) are the new tokens, new[r] of
-    request r, one request behind the other. Returns the logits of every
-    request's last token, (requests, vocab); those of a request without a new
-    token are its neighbour's and mean nothing."""
+def _serve(model, cache, ids, new):
+    """A step's tokens through the blocks: (hidden states (tokens, hidden) before
+    the last norm, the step's bi.PageTables)."""
     from . import paged_attention, paged_cache_update
 
     c = model.c
@@ -195,35 +244,86 @@ def serve_step(model, cache, ids, new):
     t, most, longest = cache.begin(new)
     x = model.embed(ids)
     T = x.shape[0]
+    turn = model.turn(t.positions)
     for i, blk in enumerate(model.blocks):
         y = blk.n1(x)
+        q = blk.q(y).view(T, c.heads, c.head_dim)
         k = blk.k(y).view(T, c.kv_heads, c.head_dim)
         v = blk.v(y).view(T, c.kv_heads, c.head_dim)
-        paged_cache_update(k, v, cache.k[i], cache.v[i], t.slots)
-        a = paged_attention(blk.q(y).view(T, c.heads, c.head_dim), cache.k[i], cache.v[i],
-                            t.block_tables, t.query_start, t.seq_lens, max_query=most,
-                            max_seq=longest)
+        if turn is not None:
+            q, k = turn(q, k)
+        scales = cache.scales(i)
+        paged_cache_update(k, v, cache.k[i], cache.v[i], t.slots, **scales)
+        a = paged_attention(q, cache.k[i], cache.v[i], t.block_tables, t.query_start, t.seq_lens,
+                            max_query=most, max_seq=longest, **scales)
         x = x + blk.o(a.reshape(T, c.heads * c.head_dim))
         y = blk.n2(x)
         x = x + blk.down(F.silu(blk.gate(y)) * blk.up(y))
+    return x, t
+
+
+def serve_step(model, cache, ids, new):
+    """One step over `cache`: ids (sum of new,) are the new tokens, new[r] of
+    request r, one request behind the other. Returns the logits of every
+    request's last token, (requests, vocab); those of a request without a new
+    token are its neighbour's and mean nothing."""
+    x, t = _serve(model, cache, ids, new)
     last = (t.query_start[1:] - 1).clamp(min=0).long()
     return model.head(model.norm(x[last]))
 
 
-def generate(model, prompts, steps, chunk=None, page_size=64, logits=None):
-    """Greedy continuation of `prompts` (1-d id tensors of any lengths) by
-    `steps` tokens each, (len(prompts), steps). Prompts enter in chunks of up to
-    `chunk` tokens (all of a prompt by default), all requests in one batch. A
-    list passed as `logits` receives every decoded token's (requests, vocab)."""
-    if not prompts or min(p.shape[0] for p in prompts) < 1 or steps < 1:
-        raise ValueError("expected prompts of one token or more and steps >= 1")
+def score(model, texts, top=0, chunk=None, page_size=64, cache_dtype=None):
+    """Log probabilities of every token of `texts` (1-d id tensors of one token
+    or more) but the first, given those before it: a list with a text's
+    bi.TokenLogprobs of n - 1 tokens each, with the `top` likeliest tokens of
+    every place. Texts enter in chunks of up to `chunk` tokens, all in one batch;
+    `cache_dtype` as :func:`generate`'s."""
+    from . import TokenLogprobs, token_logprobs
+
+    left, cache = _enter(model, texts, 0, chunk, page_size, cache_dtype)
+    device = left[0].device
+    texts, at, parts = left, [0] * len(left), [[] for _ in left]
+    with torch.no_grad():
+        while any(a < p.shape[0] for a, p in zip(at, texts)):
+            part = [p[a:] if chunk is None else p[a:a + chunk] for a, p in zip(at, texts)]
+            new = [p.shape[0] for p in part]
+            x, _ = _serve(model, cache, torch.cat(part), new)
+            # The tokens after the part's; behind a text's last there is none.
+            after = [torch.cat([p[a + 1:a + n + 1], p.new_full((1,), -1)])[:n]
+                     for a, n, p in zip(at, new, texts)]
+            got = token_logprobs(model.head(model.norm(x)), torch.cat(after).to(device), top=top)
+            for r, g in enumerate(zip(*(f.split(new) for f in got))):
+                parts[r].append(g)
+            at = [a + n for a, n in zip(at, new)]
+    return [TokenLogprobs(*(torch.cat(f)[:-1] for f in zip(*p))) for p in parts]
+
+
+def _enter(model, prompts, steps, chunk, page_size, cache_dtype):
+    """(the prompts on the model's device, a cache for them and `steps` more)."""
+    if not prompts or min(p.shape[0] for p in prompts) < 1:
+        raise ValueError("expected prompts of one token or more")
     if chunk is not None and chunk < 1:
         raise ValueError("chunk must be >= 1, got %d" % chunk)
     device = next(model.parameters()).device
-    dtype = model.head.weight.dtype
     left = [p.to(device) for p in prompts]
-    cache = PagedCache(model.c, len(left), max(p.shape[0] for p in left) + steps, page_size,
-                       device=device, dtype=dtype)
+    return left, PagedCache(model.c, len(left), max(p.shape[0] for p in left) + steps, page_size,
+                            device=device, dtype=cache_dtype or model.head.weight.dtype)
+
+
+def generate(model, prompts, steps, chunk=None, page_size=64, logits=None, cache_dtype=None,
+             logprobs=None, top=0):
+    """Greedy continuation of `prompts` (1-d id tensors of any lengths) by
+    `steps` tokens each, (len(prompts), steps). Prompts enter in chunks of up to
+    `chunk` tokens (all of a prompt by default), all requests in one batch. A
+    list passed as `logits` receives every decoded token's (requests, vocab), one
+    passed as `logprobs` its bi.TokenLogprobs (requests,) with the `top`
+    likeliest tokens. `cache_dtype` is the cache's, torch.int8 or by default the
+    model's."""
+    from . import token_logprobs
+
+    if not prompts or min(p.shape[0] for p in prompts) < 1 or steps < 1:
+        raise ValueError("expected prompts of one token or more and steps >= 1")
+    left, cache = _enter(model, prompts, steps, chunk, page_size, cache_dtype)
     first = [None] * len(left)
     with torch.no_grad():
         while any(p.shape[0] for p in left):
@@ -238,6 +338,8 @@ def generate(model, prompts, steps, chunk=None, page_size=64, logits=None):
             if logits is not None:
                 logits.append(y)
             out.append(y.argmax(-1))
+            if logprobs is not None:
+                logprobs.append(token_logprobs(y, out[-1], top=top))
             if s + 1 < steps:
                 y = serve_step(model, cache, out[-1], [1] * len(left))
     return torch.stack(out, 1)

@@ -72,6 +72,52 @@ def test_update_and_read_abi_refusals():
     assert read(vs=None) == _lib.EINVAL and read(ks=None) == _lib.EINVAL
 
 
+def test_attention_abi_refusals():
+    D = 64
+    st = (4 * D, D, 2 * 16 * D, 16 * D, D, 2 * 16 * D, 16 * D, D, 3)
+    sst = (32, 16, 1) * 2
+
+    def call(q=P, kc=P, ks=P, table=P, T=4, R=2, H=4, Hkv=2, D=D, V=D, pages=5, page=16, W=3, st=st, sst=sst,
+             dtype=_lib.BF16, window=0):
+        return _lib.lib().bi_paged_attention_q8(
+            q, kc, P, ks, P, table, P, P, None, P, T, R, H, Hkv, D, V, pages, page, W,
+            _lib.i64_array(st) if st else None, _lib.i64_array(sst) if sst else None, 0.125, window, 0, 4, 48,
+            dtype, None, 0, None)
+
+    other = lambda t, i, x: t[:i] + (x,) + t[i + 1:]
+    assert call(dtype=_lib.F32) == _lib.EUNSUPPORTED and "fp32" in _err()
+    assert call(dtype=7) == _lib.EINVAL and "dtype" in _err()
+    assert call(H=5) == _lib.EINVAL and "multiple" in _err()
+    assert call(D=80) == _lib.EUNSUPPORTED and "built" in _err()
+    assert call(window=-1) == _lib.EINVAL
+    assert call(page=0) == _lib.EINVAL and call(R=-1) == _lib.EINVAL and "sizes" in _err()
+    for kw in (dict(q=None), dict(kc=None), dict(ks=None), dict(table=None), dict(st=None), dict(sst=None)):
+        assert call(**kw) == _lib.EINVAL and "null" in _err()
+    assert call(q=24) == _lib.EINVAL and "16-byte" in _err()
+    assert call(kc=24) == _lib.EINVAL and "16-byte" in _err()
+    assert call(st=other(st, 4, 72)) == _lib.EINVAL and "16-byte" in _err()  # 72 codes of 8 bits
+    assert call(ks=18) == _lib.EINVAL and "scales" in _err()
+    for i in (2, 4, 5, 7):  # pages and rows of the caches
+        assert call(st=other(st, i, 1 << 32)) == _lib.EUNSUPPORTED and "4 GiB" in _err()
+        assert call(st=other(st, i, -64)) == _lib.EUNSUPPORTED
+    for i in (0, 2, 3, 5):  # and of the scales
+        assert call(sst=other(sst, i, 1 << 30)) == _lib.EUNSUPPORTED and "4 GiB" in _err()
+        assert call(sst=other(sst, i, -1)) == _lib.EUNSUPPORTED
+    assert call(T=0) == _lib.OK
+
+
+def test_attention_workspace():
+    def ws(T=1, R=1, H=32, Hkv=8, D=128, V=128, window=0, first=0, most=1, longest=8192, dtype=_lib.BF16):
+        return _lib.lib().bi_paged_attention_q8_workspace(T, R, H, Hkv, D, V, window, first, most, longest,
+                                                          dtype)
+
+    # Two sums and a row of V for each column and segment of 512 rows.
+    assert ws() == 32 * 16 * 130 * 4
+    assert ws(dtype=_lib.F16) == ws() and ws(longest=8193) == 32 * 17 * 130 * 4
+    assert ws(T=0) == ws(R=0) == ws(H=0) == ws(longest=0) == ws(most=0) == 0
+    assert ws(dtype=_lib.F32) == ws(D=80) == ws(H=33) == ws(window=-1) == ws(T=1 << 40) == 0
+
+
 def test_logprobs_abi_refusals():
     def call(x=P, out=P, ids=P, rows=4, V=100, stride=100, top=5, token_bytes=8, dtype=_lib.F16):
         return _lib.lib().bi_token_logprobs(x, P, out, P, ids, P, rows, V, stride, top, token_bytes,
@@ -191,3 +237,48 @@ def test_token_logprobs_refusals():
         bi.token_logprobs(x, t)
     with pytest.raises(NotImplementedError, match="backward"):
         bi.token_logprobs(x.requires_grad_(), t)
+
+
+def test_attention_over_codes_refusals():
+    kc, vc, ks, vs = q8_cache()
+    q, start, lens = torch.zeros(3, 4, 64).half(), torch.tensor([0, 3], dtype=I32), torch.tensor([3], dtype=I32)
+    table = torch.zeros(1, 2, dtype=I32)
+
+    def call(q=q, kc=kc, vc=vc, **kw):
+        return bi.paged_attention(q, kc, vc, table, start, lens, **kw)
+
+    for kw in (dict(), dict(k_scales=ks), dict(v_scales=vs)):
+        with pytest.raises(ValueError, match="int8 caches"):
+            call(**kw)
+    for bad in (dict(kc=kc.half(), vc=vc.half()), dict(vc=vc.half())):
+        with pytest.raises(ValueError, match="int8 caches"):
+            call(**bad, k_scales=ks, v_scales=vs)
+    with pytest.raises(ValueError, match="k_scales must"):
+        call(k_scales=ks.half(), v_scales=vs)
+    with pytest.raises(ValueError, match="v_scales must"):
+        call(k_scales=ks, v_scales=vs[:, :1])
+    with pytest.raises(NotImplementedError, match="float32"):
+        call(q=q.float(), k_scales=ks, v_scales=vs)
+    with pytest.raises(ValueError, match="GPU"):
+        call(k_scales=ks, v_scales=vs)
+
+
+def test_scoring_refusals_and_caches():
+    from mlx_batch_invariant import decoder
+
+    c = decoder.DecoderConfig(hidden=64, inter=64, heads=2, kv_heads=1, head_dim=64, layers=2, vocab=16)
+    m = decoder.build(c, device="cpu", dtype=torch.float32)
+    with pytest.raises(ValueError, match="one token"):
+        decoder.score(m, [])
+    with pytest.raises(ValueError, match="one token"):
+        decoder.score(m, [torch.zeros(3, dtype=torch.long), torch.zeros(0, dtype=torch.long)])
+    with pytest.raises(ValueError, match="chunk"):
+        decoder.score(m, [torch.zeros(3, dtype=torch.long)], chunk=0)
+    assert m.inv_freq is None and m.turn(None) is None
+    cache = decoder.PagedCache(c, 2, 50, page_size=16, device="cpu", dtype=torch.int8)
+    assert cache.k.dtype == torch.int8 and cache.k_scales.shape == cache.k.shape[:-1] == (2, 8, 1, 16)
+    assert cache.scales(1)["v_scales"].data_ptr() == cache.v_scales[1].data_ptr()
+    assert decoder.PagedCache(c, 2, 50, device="cpu").scales(0) == {}
+    turned = decoder.Decoder(decoder.DecoderConfig(hidden=64, inter=64, heads=2, kv_heads=1, head_dim=64, layers=1,
+                                                   vocab=16, rope_base=100.0, rope_dim=8), "cpu", torch.float32)
+    assert turned.inv_freq.tolist() == bi.rotary_frequencies(8, 100.0, device="cpu").tolist()
