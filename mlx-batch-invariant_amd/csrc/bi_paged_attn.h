@@ -56,6 +56,8 @@ struct Args {
   uint32_t k8b, k8n, v8b, v8n, ksb, ksn, vsb, vsn;
   int64_t ksh, vsh;
   Div eight;              // 8 * Hkv where a row's heads are next to each other, else 0
+  char* laid;             // steps of (request, kv head), `units` each, as they lie in LDS
+  int32_t units;
 };
 
 typedef void (*Kernel)(Args);
@@ -67,6 +69,11 @@ struct Kernels {
   // CU (the last two where the registers allow two waves per SIMD, else NULL).
   Kernel whole4, whole8, whole4_pair;
   int whole4_threads;       // its loading waves among them
+  // A cache of 8 bits: what writes its rows as they lie in LDS, a step of `step`
+  // rows as step_bytes, and the whole route over these.
+  Kernel lay = nullptr, laid4 = nullptr, laid8 = nullptr;
+  int step = 0, step_bytes = 0;
+  double laid_row_us = 0;
   int seg, pass;            // rows per segment and per pass of the split route (four steps)
   int places = 8192;        // split workgroups with work, about: more take several segments each
   // For the choice of route, in microseconds: what a row costs a whole

@@ -27,6 +27,8 @@ Kernels kernels(int64_t D, int64_t V, int dtype, bool q8) {
 // Tokens, lengths and windows past this are not computed with (positions
 // minus a window stay in 32 bits).
 constexpr int64_t kMost = (int64_t)1 << 29;
+// Workspaces are not larger.
+constexpr int64_t kMostBytes = (int64_t)1 << 32;
 
 // A call as the host knows it; `exact`: every request has max_query tokens.
 struct Call {
@@ -37,9 +39,12 @@ struct Call {
 
 // How a call is split: the columns up to which a request is (0: none), columns
 // kept per request and kv head, columns per workgroup, segments, workgroups for
-// these, and the bytes of the partial results.
+// these, and the bytes of the partial results. Of the others' rows that are laid
+// out (a cache of 8 bits): the steps of a request, and the bytes, 0 for none.
 struct Plan {
-  int64_t split_cols, ccap, nc, nseg, gseg, bytes;
+  int64_t split_cols, ccap, nc, nseg, gseg, bytes, units, laid;
+  int64_t laid_at() const { return (bytes + 15) / 16 * 16; }
+  int64_t workspace() const { return laid ? laid_at() + laid : bytes; }
 };
 
 // Column tiles of all requests that can have a token (one of each request is
@@ -52,7 +57,7 @@ int64_t full_tiles(const Call& c, const Plan& s) {
 // A plan that splits requests of up to `most` columns.
 Plan split_up_to(const Call& c, int64_t most, const Kernels& k) {
   const int64_t seg = k.seg;
-  Plan s;
+  Plan s = {};
   const int64_t cols = c.max_query * c.G;
   s.split_cols = most;
   s.ccap = cols < most ? cols : most;
@@ -77,7 +82,7 @@ int64_t split_grid(const Call& c, const Plan& s) {
   return c.R * c.Hkv * s.gseg * ((s.ccap + s.nc - 1) / s.nc);
 }
 bool fits(const Call& c, const Plan& s) {
-  return s.bytes <= (int64_t)1 << 32 && split_grid(c, s) <= 1 << 23 && c.R * c.Hkv * s.ccap <= 1 << 24;
+  return s.bytes <= kMostBytes && split_grid(c, s) <= 1 << 23 && c.R * c.Hkv * s.ccap <= 1 << 24;
 }
 
 // Requests are split where that is estimated to take less time than to walk
@@ -99,10 +104,12 @@ bool fits(const Call& c, const Plan& s) {
 // 344, 512 513 / 659. fp32, 128/128, 64 requests of 2048 rows 570 / 284, 256
 // tokens over 4096 rows 559 / 368, 512 559 / 670; 256/256, 1000 tokens of a
 // prompt, 8/8 heads 331 / 124. Of 822 sizes timed both ways it picks the one
-// that takes 8 % more or worse four times, 29 % at most. 64 single tokens under a
+// that takes 8 % more or worse four times, 29 % at most; over a cache of 8 bits, of
+// 666 sizes timed each way, with its rows laid out too, 1 % on average, 20 % or worse
+// ten times, mostly over 200 rows. 64 single tokens under a
 // bound of 64 229, with all these columns split 1030.)
 Plan plan(const Call& c, const Kernels& k) {
-  const Plan none = {0, 0, 0, 0, 0, 0};
+  const Plan none = {};
   const int64_t cols = c.max_query * c.G;
   if (c.R <= 0 || cols <= 0 || c.max_seq <= 0) return none;
   const int64_t few = c.G > 32 ? c.G : 32;
@@ -115,10 +122,33 @@ Plan plan(const Call& c, const Kernels& k) {
   const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * c.bytes / 5e6;
   const double all = (double)c.R * ((cols + 127) / 128), full = (double)c.tokens * c.G / 128.0 + c.R;
   const double tiles = (all < full ? all : full) * c.Hkv / cus;
-  const double walked = (cut ? rows + 128.0 / c.G + 64.0 : rows) * k.row_us;
-  const double first = 7.5 + walked, most = tiles * (7.5 + walked * (cut ? 1.0 : 1.0 - 0.5 * chunk / seq));
-  double whole = first > most ? first : most;
-  whole = 2.0 + (whole > 1.1 * read ? whole : 1.1 * read);
+  auto walk_us = [&](double row_us) {
+    const double walked = (cut ? rows + 128.0 / c.G + 64.0 : rows) * row_us;
+    const double first = 7.5 + walked, most = tiles * (7.5 + walked * (cut ? 1.0 : 1.0 - 0.5 * chunk / seq));
+    const double us = first > most ? first : most;
+    return 2.0 + (us > 1.1 * read ? us : 1.1 * read);
+  };
+  double whole = walk_us(k.row_us);
+  // Whether the rows that are walked whole are laid out first: a launch, and their
+  // codes through memory, three bytes for each, at 4 TB/s.
+  Plan lay = none;
+  if (k.lay) {
+    const double requests = (double)c.tokens / (double)c.max_query, part = (double)c.max_query + wide;
+    const double laid = (cut && part < seq ? part : seq) * (requests < 1.0 ? 1.0 : requests < c.R ? requests : c.R);
+    const double us = walk_us(k.laid_row_us) + 4.0 + laid * c.Hkv * (c.D + c.V) * 3.0 / 4e6;
+    lay.units = (c.max_seq + k.step - 1) / k.step;
+    const double bytes = (double)c.R * (double)(c.Hkv * lay.units * k.step_bytes);
+    if (us < whole && bytes <= (double)kMostBytes) {
+      whole = us;
+      lay.laid = (int64_t)bytes;
+    } else {
+      lay = none;
+    }
+  }
+  auto beside = [&](Plan s) {
+    if (cols > s.split_cols && s.bytes + lay.laid <= kMostBytes) s.units = lay.units, s.laid = lay.laid;
+    return s;
+  };
   auto split = [&](const Plan& s) {
     const double busy = (double)full_tiles(c, s) * c.Hkv, n = (double)s.nseg;
     const int per_cu = s.nc == 16 ? k.per_cu16 : k.per_cu32;
@@ -145,15 +175,15 @@ Plan plan(const Call& c, const Kernels& k) {
   if (cols <= few || (cols <= 2048 && !loose)) {
     const Plan s = split_up_to(c, cols > few ? cols : few, k);
     if (fits(c, s) && split(s) < whole) return s;
-    if (cols <= few && whole <= split(s)) return none;
+    if (cols <= few && whole <= split(s)) return lay;
   }
   // All requests have max_query tokens, or what is missing is padding (else
   // two launches that find nothing, 3 to 4 us each).
-  if (c.exact || c.tokens >= c.R * c.max_query) return none;
+  if (c.exact || c.tokens >= c.R * c.max_query) return lay;
   // Beside whole chunks; where the results would take too much, single tokens.
   Plan s = split_up_to(c, few, k);
   if (!fits(c, s)) s = split_up_to(c, c.G, k);
-  return fits(c, s) ? s : none;
+  return fits(c, s) ? beside(s) : lay;
 }
 
 int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, int64_t ws_bytes,
@@ -164,7 +194,8 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
   const Call c = {p.R, p.qstart ? p.T : (int64_t)p.R * p.qL, p.G.d, p.Hkv.d, D, V, p.window, p.first,
                   most, p.qstart ? p.max_seq : p.N, !p.qstart, p.ks ? 1.0 : (double)bi::elem_size(dtype)};
   Plan s = plan(c, k);
-  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{0, 0, 0, 0, 0, 0};
+  if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{};
+  if (ws_bytes < s.workspace()) s.laid = 0;
   hipError_t e;
   if (s.split_cols) {
     p.split_cols = (int32_t)s.split_cols;
@@ -213,7 +244,8 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     const int64_t longest = p.qstart ? p.max_seq : p.N;
     const int64_t seen = (int64_t)p.window + p.first + 63, causal = longest - most / 2;
     const bool far = (p.window && seen < causal ? seen : causal) > 1024;
-    const bool eight = k.whole8 && far && cols / 256 * p.Hkv.d >= cus;
+    const Kernel whole8 = s.laid ? k.laid8 : k.whole8;
+    const bool eight = whole8 && far && cols / 256 * p.Hkv.d >= cus;
     const bool pair = !eight && k.whole4_pair && cols / 128 * p.Hkv.d > cus;
     const int64_t wc = eight ? 256 : 128;
     // Column tiles: every request with tokens may end in a part of one.
@@ -223,8 +255,16 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, 
     const int64_t blocks = tiles * p.Hkv.d + p.fill_blocks;
     if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
     if (blocks == 0) return BI_OK;
-    hipLaunchKernelGGL(eight ? k.whole8 : pair ? k.whole4_pair : k.whole4, dim3((unsigned)blocks),
-                       dim3(eight ? 512 : pair ? 256 : k.whole4_threads), 0, st, p);
+    if (s.laid && whole) {
+      p.laid = static_cast<char*>(ws) + s.laid_at();
+      p.units = (int32_t)s.units;
+      const int64_t all = (int64_t)p.R * p.Hkv.d * s.units, most_groups = 8 * (int64_t)cus;
+      hipLaunchKernelGGL(k.lay, dim3((unsigned)(all < most_groups ? all : most_groups)), dim3(256), 0, st, p);
+      if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+    }
+    const Kernel whole4 = s.laid ? k.laid4 : k.whole4;
+    hipLaunchKernelGGL(eight ? whole8 : pair ? k.whole4_pair : whole4, dim3((unsigned)blocks),
+                       dim3(eight || s.laid ? 512 : pair ? 256 : k.whole4_threads), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
   }
   return BI_OK;
@@ -394,7 +434,7 @@ extern "C" int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t
     return 0;
   const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
                   clamp32(max_seq), false, 1.0};
-  return plan(c, kernels(D, V, dtype, true)).bytes;
+  return plan(c, kernels(D, V, dtype, true)).workspace();
 }
 
 extern "C" int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks,

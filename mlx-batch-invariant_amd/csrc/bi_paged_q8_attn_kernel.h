@@ -107,13 +107,29 @@ struct Geo8 {
   // (128 dims: with all in registers, of which 234 are in use at once, some were
   // kept in scratch memory).
   static constexpr int kFarQuery = D == 128 && V == 128 ? NQ : 0;
+  // Whole route, a step as it lies in LDS: 16-byte units of keys, of values (both in
+  // the type), then c_j, what values are multiplied with, and the masks of the rows
+  // that have a page and that spoil. Laid out in memory the same.
+  static constexpr int KU = kStep * TCH, VU = kStep * TVCH, FU = kStep / 4, IU = KU + VU + 2 * FU + 1;
+  // Steps of them in LDS.
+  static constexpr int kDeep = 3 * IU * 16 <= 150 * 1024 ? 3 : 2;
   // Split route: workgroups of NC columns that a compute unit's registers hold.
   static constexpr int split_per_cu(int NC) {
     return NC == 16 ? (D + V <= 128 ? 4 : D + V <= 256 ? 3 : 2) : (D + V <= 128 ? 3 : D + V <= 320 ? 2 : 1);
   }
 
-  static constexpr double row_us() { return 1e-3 * (kTwoWaves ? 13.0 + 0.04 * (D + V) : 28.0 + 0.08 * (D + V)); }
-  static constexpr double seg_us() { return 5.0 + 0.023 * (kSeg * (D + V) / 1024.0); }
+  // Prices of a row and of a segment (for the choice of route), fitted to the times
+  // of 666 sizes with each route: rows whose chunks are no power of two cost the
+  // whole workgroups, where all waves share the loads, and small splits more.
+  static constexpr bool kPow2 = (CH & (CH - 1)) == 0 && (VCH & (VCH - 1)) == 0;
+  static constexpr double row_us() {
+    return 1e-3 * (kTwoWaves ? 14.0 + 0.047 * (D + V) + (kPow2 ? 0.0 : 10.0) : 24.0 + 0.0725 * (D + V));
+  }
+  static constexpr double laid_row_us() { return 1e-3 * (10.0 + 0.051 * (D + V)); }
+  static constexpr double seg_us(int NC) {
+    if (NC == 32) return 9.2 + 0.0135 * (D + V);
+    return kTwoWaves ? 4.0 + 0.006 * (D + V) + (kPow2 ? 0.0 : 2.0) : 2.0 + 0.026 * (D + V);
+  }
 
   __device__ __forceinline__ static f32x4 product(uint4 a, uint4 b, f32x4 c) {
     if constexpr (kPower)
@@ -276,7 +292,7 @@ struct Geo8 {
   // A step's weights in the type, and the lane's sums of p: a chain for the eight
   // rows of a product, then both. (Four rows at a time: else the compiler reads all
   // factors first, into registers that there are not.)
-  template <int CT>
+  template <int CT, bool ALL = false>
   __device__ __forceinline__ static void weights(const f32x4 (&s)[RT][CT], const float* c, const float* vs, int g,
                                                  const float (&m)[CT], uint4 (&u)[RT / 2][CT], float (&sum)[CT]) {
 #pragma unroll
@@ -305,7 +321,7 @@ struct Geo8 {
             else d[k][2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16x2));
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!ALL) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int k = 0; k < CT; k++) {
@@ -322,22 +338,30 @@ struct Geo8 {
   }
 };
 
-// As feed(), with the operands two products ahead: of half as many registers.
-template <int N, typename Read, typename Use>
-__device__ __forceinline__ void feed2(const Read& read, const Use& use) {
-  static_assert(N % 2 == 0, "pairs");
-  uint4 x[2][2];
-  x[0][0] = read(0), x[0][1] = read(1);
+// As feed(), with the operands A products ahead.
+template <int N, int A, typename Read, typename Use>
+__device__ __forceinline__ void feed_ahead(const Read& read, const Use& use) {
+  static_assert(N % A == 0, "groups");
+  uint4 x[2][A];
 #pragma unroll
-  for (int n = 0; n < N; n += 2) {
+  for (int i = 0; i < A; i++) x[0][i] = read(i);
+#pragma unroll
+  for (int n = 0; n < N; n += A) {
     __builtin_amdgcn_sched_barrier(0);
-    if (n + 2 < N) x[(n / 2 + 1) & 1][0] = read(n + 2), x[(n / 2 + 1) & 1][1] = read(n + 3);
+    if (n + A < N)
+#pragma unroll
+      for (int i = 0; i < A; i++) x[(n / A + 1) & 1][i] = read(n + A + i);
     __builtin_amdgcn_sched_barrier(0);
-    use(n, x[(n / 2) & 1][0]);
-    use(n + 1, x[(n / 2) & 1][1]);
+#pragma unroll
+    for (int i = 0; i < A; i++) use(n + i, x[(n / A) & 1][i]);
   }
 }
 
+__device__ __forceinline__ uint2 ld8(const void* p) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(1))) const u32x2 gvec;
+  return __builtin_bit_cast(uint2, *(gvec*)p);
+}
 // A row of a page, and its scale from device memory, as ld16; zeros for a row
 // without a page.
 __device__ __forceinline__ const char* row_at(const char* base, int32_t id, uint32_t page, int32_t row, uint32_t step) {
@@ -633,25 +657,128 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
   }
 }
 
-// Whole route: NW waves of 32 columns each walk the steps that some column of
-// the workgroup sees. Each step's codes go from device memory to registers a step
-// before they become bf16 or f16 in LDS, each by one lane of the workgroup, and
-// from there to all waves' products. LW waves more do nothing but that (LW = 0:
-// the NW waves themselves).
-template <typename T, int D, int V, int NW, int LW>
-__global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 : 1)) whole8_kernel(Args p) {
+// Lays rows out as the whole route wants them in LDS: a unit of 16 bytes for each 8
+// codes of a row, in the place it has there.
+//
+// What every workgroup of the whole route would do for the rows that it walks, looking
+// up pages and making numbers of codes, is done once, where there is room for the
+// result (4096 tokens over 8192 rows, 64 column tiles to a kv head, 128 dims: 576 ->
+// 484 us; 192 dims 1342 -> 891, 256 1557 -> 992, where four waves of 32 columns gave
+// way to eight of 16 as well). It costs a launch and three bytes of traffic a code:
+// 12 us for these rows, and 8 requests of 64 tokens over 4000 rows would take 166 us
+// for 116, so the host compares. The list of what is to do, steps of requests that are
+// not split, is the same for all workgroups, which take from it in turn.
+template <typename T, int D, int V>
+__global__ void __launch_bounds__(256) lay8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
-  constexpr int S = G8::kStep, RT = G8::RT, NU = RT / 2, DT = G8::DT, CT = 2, COLS = 32 * NW;
-  constexpr int KU = S * G8::TCH, VU = S * G8::TVCH;  // 16-byte units of a step in LDS
-  constexpr int NLW = LW ? LW : NW, NT = 64 * NLW, NB = 2;  // waves and threads that load
+  constexpr int S = G8::kStep;
+  __shared__ const char* s_row[2][S];
+  __shared__ uint16_t s_pow[S];
+  __shared__ int s_end[256], s_scan[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int next = blockIdx.x, before = 0;
+  for (int r0 = 0; r0 < p.R; r0 += 256) {
+    int sum = 0;
+    if (r0 + tid < p.R) {
+      const Request rq = request(p, r0 + tid);
+      if (!rq.beyond && rq.L * (int)p.G.d > p.split_cols)
+        sum = walk(p, rq.n - rq.L, rq.n - 1, S).count() * (int)p.Hkv.d;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(sum, d);
+      if (lane >= d) sum += y;
+    }
+    if (lane == 63) s_scan[wave] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (i < wave) sum += s_scan[i];
+    s_end[tid] = before + sum;
+    __syncthreads();
+    const int end = s_end[255];
+    for (; next < end; next += gridDim.x) {
+      int a = 0;  // requests whose steps all come before
+#pragma unroll
+      for (int d = 128; d; d >>= 1)
+        if (s_end[a + d - 1] <= next) a += d;
+      const int r = r0 + a, at = next - (a ? s_end[a - 1] : before);
+      const int i = at / p.Hkv, kvh = at - i * (int)p.Hkv.d;
+      const Request rq = request(p, r);
+      const int32_t lo = rq.n - rq.L, hi = rq.n - 1;
+      const int unit = walk(p, lo, hi, S).unit(i);
+      char* to = p.laid + ((int64_t)(r * (int)p.Hkv.d + kvh) * p.units + unit) * (G8::IU * 16);
+      if (wave == 0) {
+        const int32_t key = unit * S + lane;
+        const int32_t id = any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry_of(p, r, key), key) : -1;
+        const int32_t row = row_of(p, key);
+        s_row[0][lane] = row_at(static_cast<const char*>(p.k) + kvh * p.kh, id, p.k8b, row, p.k8n);
+        s_row[1][lane] = row_at(static_cast<const char*>(p.v) + kvh * p.vh, id, p.v8b, row, p.v8n);
+        const float ks = ld_scale(row_at(reinterpret_cast<const char*>(p.ks + kvh * p.ksh), id, p.ksb, row, p.ksn));
+        const float vs = ld_scale(row_at(reinterpret_cast<const char*>(p.vs + kvh * p.vsh), id, p.vsb, row, p.vsn));
+        float c, left;
+        uint16_t power = 0;
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(G8::factors(p, ks, vs, c, left, power));
+        const uint64_t mapped = __builtin_amdgcn_ballot_w64(id >= 0);
+        s_pow[lane] = power;
+        float* f = reinterpret_cast<float*>(to + (G8::KU + G8::VU) * 16);
+        f[lane] = c;
+        f[S + lane] = left;
+        if (lane == 0) *reinterpret_cast<ulonglong2*>(f + 2 * S) = make_ulonglong2(mapped, bad);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < G8::KU / 256; j++) {
+        const uint32_t n = j * 256 + tid, row = n / G8::TCH, c = (n % G8::TCH) ^ G8::template swz<G8::TCH>(row);
+        const uint2 w = ld8(s_row[0][row] + c * 8);
+        reinterpret_cast<uint4*>(to)[n] = codes8<T>(w.x, w.y);
+      }
+#pragma unroll
+      for (int j = 0; j < G8::VU / 256; j++) {
+        const uint32_t n = j * 256 + tid, row = n / G8::TVCH, c = (n % G8::TVCH) ^ G8::tswz(row);
+        const uint2 w = ld8(s_row[1][row] + c * 8);
+        uint4 y = codes8<T>(w.x, w.y);
+        if constexpr (G8::kPower) {
+          const uint32_t f = s_pow[row] * 0x10001u;
+          y = times(y, make_uint4(f, f, f, f));
+        }
+        reinterpret_cast<uint4*>(to)[G8::KU + n] = y;
+      }
+      __syncthreads();
+    }
+    before = end;
+    __syncthreads();
+  }
+}
+
+// Whole route: NW waves of 16 CT columns each walk the steps that some column of
+// the workgroup sees. LAID: these lie in memory as they are wanted in LDS, and go there
+// past the registers, two steps ahead where three fit. Else each step's codes go from
+// device memory to registers a step before they become bf16 or f16 in LDS, each by one
+// lane of the workgroup, and from there to all waves' products; LW waves more do
+// nothing but that (LW = 0: the NW waves themselves).
+//
+// What bounds it (laid out, 256 columns, 128 dims, 4096 tokens over 8192 rows): a
+// step's 2.4 us are 6000 cycles, of which each SIMD's two waves have products in 34 %
+// and issue vector instructions in 51 %, the LDS is busy in 25 %; what is left is waits.
+// Operands read further ahead, or half of the waves half a step behind the others,
+// changed nothing.
+template <typename T, int D, int V, int NW, int LW, int CT, bool LAID>
+__global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || NW == 8 ? 2 : 1)) whole8_kernel(Args p) {
+  using G8 = Geo8<T, D, V>;
+  constexpr int S = G8::kStep, RT = G8::RT, NU = RT / 2, DT = G8::DT, WC = 16 * CT, COLS = WC * NW;  // columns of a wave, of all
+  constexpr int kFar = CT == 2 ? G8::kFarQuery : 0;
+  constexpr bool kEasy = CT == 1 && D + V <= 384 && D % 64 == 0 && V % 64 == 0;  // registers are left
+  constexpr int KU = G8::KU, VU = G8::VU, IU = LAID ? G8::IU : KU + VU;
+  constexpr int NLW = LW ? LW : NW, NT = 64 * NLW, NB = LAID ? G8::kDeep : 2;  // waves and threads that load
   constexpr int KN = (S * G8::CH + NT - 1) / NT, VN = (S * G8::VCH + NT - 1) / NT;  // loads per thread
-  __shared__ uint4 s_kv[NB * (KU + VU)];
-  constexpr int RING = 2 * NLW;
+  __shared__ uint4 s_kv[NB * IU];
+  constexpr int RING = LAID ? 1 : 2 * NLW;
   __shared__ const char* s_row[RING][2][S];
   __shared__ __attribute__((aligned(16))) float s_c[RING][S], s_vs[RING][S];
   __shared__ uint16_t s_pow[RING][G8::kPower ? S : 1];
   __shared__ uint64_t s_map[2 * RING], s_bad[RING];
-  __shared__ uint4 s_q[NW][G8::kFarQuery ? G8::kFarQuery : 1][G8::kFarQuery ? 64 : 1];
+  __shared__ uint4 s_q[kFar ? NW : 1][kFar ? kFar : 1][kFar ? 64 : 1];
   __shared__ int s_scan[NW + LW + 3];
   __shared__ float s_ml[CT][2][64 * NW];  // each lane's own M and L
 
@@ -705,12 +832,12 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
-  const int c0 = tile * COLS, cw = c0 + 32 * wave;
+  const int c0 = tile * COLS, cw = c0 + WC * wave;
   const int clast = (c0 + COLS < ncol ? c0 + COLS : ncol) - 1;
   const int32_t p0 = rq.n - rq.L;
   const int32_t lo = p0 + c0 / p.G, hi = p0 + clast / p.G;
   // The wave's own columns; a wave without one only loads.
-  const int wlast = cw + 31 < ncol ? cw + 31 : ncol - 1;
+  const int wlast = cw + WC - 1 < ncol ? cw + WC - 1 : ncol - 1;
   const int32_t wlo = cw < ncol ? p0 + cw / p.G : INT32_MAX / 2, whi = cw < ncol ? p0 + wlast / p.G : -1;
 
   const bool loads = LW == 0 || wave >= NW;
@@ -724,7 +851,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
     G8::sign_query(p, q[k]);
     if (k == 1 && wave < NW)
 #pragma unroll
-      for (int n = 0; n < G8::kFarQuery; n++) s_q[wave][n][lane] = q[k][n];
+      for (int n = 0; n < kFar; n++) s_q[wave][n][lane] = q[k][n];
   }
 
   const Walk w = walk(p, lo, hi, S);
@@ -827,44 +954,74 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
     }
   }
 
-  if (loads) {
-    entry = entry_for(lw);
-    put_rows(lw);
-    put_scales(lw);
-    entry = entry_for(lw + NLW);
-    put_rows(lw + NLW);
-    entry = entry_for(lw + 2 * NLW);
-  }
-  __syncthreads();
-  if (loads) {
-    load_step(0);
-    put_step(0);
-    load_step(1);
-  }
-  if constexpr (LW != 0)
+  // LAID: a step's way into LDS, NB - 1 steps ahead.
+  constexpr int NL = (IU + NT - 1) / NT;
+  const char* laid = LAID ? p.laid + (int64_t)(r * (int)p.Hkv.d + kvh) * p.units * (IU * 16) : nullptr;
+  auto fetch = [&](int j) __attribute__((always_inline)) {
+    const char* from = laid + (uint64_t)(uint32_t)w.unit(j) * (IU * 16);
+    uint4* to = s_kv + j % NB * IU + 64 * wave;
+#pragma unroll
+    for (int i = 0; i < NL; i++)
+      if (i * NT + NT <= IU || i * NT + tid < IU)
+        load_to_lds<16>(from + (i * NT + opaque(tid)) * 16, to + i * NT);
+  };
+
+  if constexpr (LAID) {
+#pragma unroll
+    for (int j = 0; j < NB - 1; j++)
+      if (j < steps) fetch(j);
+  } else {
     if (loads) {
-      for (int j = 0; j < steps; j++) {
-        barrier();
-        if (j + 1 < steps) put_step(j + 1);
-        prepare(j);  // (before the loads that the next step waits for, and with them for its own)
-        if (j + 2 < steps) load_step(j + 2);
-      }
-      return;
+      entry = entry_for(lw);
+      put_rows(lw);
+      put_scales(lw);
+      entry = entry_for(lw + NLW);
+      put_rows(lw + NLW);
+      entry = entry_for(lw + 2 * NLW);
     }
+    __syncthreads();
+    if (loads) {
+      load_step(0);
+      put_step(0);
+      load_step(1);
+    }
+    if constexpr (LW != 0)
+      if (loads) {
+        for (int j = 0; j < steps; j++) {
+          barrier();
+          if (j + 1 < steps) put_step(j + 1);
+          prepare(j);  // (before the loads that the next step waits for, and with them for its own)
+          if (j + 2 < steps) load_step(j + 2);
+        }
+        return;
+      }
+  }
   for (int j = 0; j < steps; j++) {
     const uint32_t ln = opaque(lane);
     const int g = ln >> 4;
+    if constexpr (LAID) {  // (the loads of the NB - 2 steps after it may be on their way still)
+      if (j + NB - 2 < steps) wait_loads_but<(IU / NT) * (NB - 2)>();
+      else wait_loads();
+    }
     barrier();  // step j is there, and everyone is done with step j - 1's buffer
-    if constexpr (LW == 0) {
+    if constexpr (LAID) {
+      if (j + NB - 1 < steps) fetch(j + NB - 1);
+    } else if constexpr (LW == 0) {
       if (j + 1 < steps) put_step(j + 1);
       prepare(j);
     }
-    const uint4 *kd = s_kv + (j & 1) * (KU + VU), *vd = kd + KU;
+    const uint4 *kd = s_kv + j % NB * IU, *vd = kd + KU;
+    const float *cs = s_c[j % RING], *gs = s_vs[j % RING];
+    const uint64_t *maps = &s_map[j % (2 * RING)], *bads = &s_bad[j % RING];
+    if constexpr (LAID) {
+      cs = reinterpret_cast<const float*>(vd + VU), gs = cs + S;
+      maps = reinterpret_cast<const uint64_t*>(gs + S), bads = maps + 1;
+    }
     const int32_t unit = w.unit(j), key0 = unit * S;
     const bool mine = any_seen(p, wlo, whi, key0, S);
     uint4 pu[NU][CT];
     if (mine) {
-      const uint64_t mapped = uniform(s_map[j % (2 * RING)]);
+      const uint64_t mapped = uniform(*maps);
       const bool full = mapped == ~0ull && all_seen(p, wlo, whi, key0, S);
       f32x4 s[RT][CT];
 #pragma unroll
@@ -873,16 +1030,16 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
         for (int k = 0; k < CT; k++) s[t][k] = f32x4{};
       uint4 far[2];
       auto far_query = [&](int n) __attribute__((always_inline)) { far[n & 1] = s_q[wave][n][ln]; };
-      if (G8::kFarQuery) far_query(0);
-      feed2<RT * G8::NQ>(
+      if (kFar) far_query(0);
+      feed_ahead<RT * G8::NQ, kEasy ? 8 : 2>(
           [&](int n) __attribute__((always_inline)) { return G8::key_of_type(kd, 16 * (n % RT), n / RT, ln); },
           [&](int n, uint4 x) __attribute__((always_inline)) {
             const int i = n / RT;
-            if (n % RT == 0 && i + 1 < G8::kFarQuery) far_query(i + 1);
-            s[n % RT][0] = G8::product(x, q[0][i], s[n % RT][0]);
-            s[n % RT][1] = G8::product(x, i < G8::kFarQuery ? far[i & 1] : q[1][i], s[n % RT][1]);
+            if (n % RT == 0 && i + 1 < kFar) far_query(i + 1);
+#pragma unroll
+            for (int k = 0; k < CT; k++) s[n % RT][k] = G8::product(x, k == 1 && i < kFar ? far[i & 1] : q[k][i], s[n % RT][k]);
           });
-      const uint64_t bad = uniform(s_bad[j % RING]) & mapped;
+      const uint64_t bad = uniform(*bads) & mapped;
       auto positions = [&](int32_t(&pos)[CT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < CT; k++) {
@@ -898,7 +1055,6 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
         for (int k = 0; k < CT; k++) seen[k] = seen_bits(p, pos[k], key0, mapped) >> (4 * g);
         G8::template hide<CT>(s, seen);
       }
-      const float *cs = s_c[j % RING], *gs = s_vs[j % RING];
       // A lane's sum of at most kMostSum holds no score that moves the base;
       // else, and at a segment's first step, the largest score decides.
       float psum[CT];
@@ -922,8 +1078,11 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
             m[k] = mn;
           }
         }
-        G8::template weights<CT>(s, cs, gs, h, m, pu, psum);
-        if (look || __builtin_amdgcn_ballot_w64(psum[0] > kMostSum || psum[1] > kMostSum) == 0) break;
+        G8::template weights<CT, kEasy>(s, cs, gs, h, m, pu, psum);
+        bool more = false;
+#pragma unroll
+        for (int k = 0; k < CT; k++) more |= psum[k] > kMostSum;
+        if (look || __builtin_amdgcn_ballot_w64(more) == 0) break;
         look = true;
       }
       if (bad) {
@@ -936,11 +1095,11 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves ? 2 
       fresh = false;
     }
     // (Not before the scores, whose operands need the registers.)
-    if constexpr (LW == 0)
+    if constexpr (LW == 0 && !LAID)
       if (j + 2 < steps) load_step(j + 2);
     if (mine) {
       // Products of one output tile are a chain: those of the others go between.
-      feed<DT * NU>(
+      feed_ahead<DT * NU, kEasy ? 8 : 4>(
           [&](int n) __attribute__((always_inline)) { return G8::value_of_type(vd, n / DT, n % DT, ln); },
           [&](int n, uint4 v) __attribute__((always_inline)) {
 #pragma unroll
@@ -1007,16 +1166,20 @@ Kernels kernels8_of() {
   k.combine = combine_kernel<T, D, V, G8::kSeg>;
   k.seg = G8::kSeg, k.pass = 4 * G8::kStep;
   k.row_us = G8::row_us();
-  k.seg16_us = k.seg32_us = G8::seg_us();
+  k.seg16_us = G8::seg_us(16), k.seg32_us = G8::seg_us(32);
+  k.laid_row_us = G8::laid_row_us();
   k.per_cu16 = G8::split_per_cu(16), k.per_cu32 = G8::split_per_cu(32);
   k.whole4_pair = nullptr;
   if constexpr (G8::kTwoWaves) {
-    k.whole4 = whole8_kernel<T, D, V, 4, 4>;
-    k.whole8 = whole8_kernel<T, D, V, 8, 0>;
+    k.whole4 = whole8_kernel<T, D, V, 4, 4, 2, false>;
+    k.laid8 = whole8_kernel<T, D, V, 8, 0, 2, true>;
   } else {
-    k.whole4 = whole8_kernel<T, D, V, 4, 0>;
-    k.whole8 = nullptr;
+    k.whole4 = whole8_kernel<T, D, V, 4, 0, 2, false>;
   }
+  k.laid4 = whole8_kernel<T, D, V, 8, 0, 1, true>;
+  k.lay = lay8_kernel<T, D, V>;
+  k.step = G8::kStep, k.step_bytes = G8::IU * 16;
+  k.whole8 = nullptr;
   k.whole4_threads = G8::kTwoWaves ? 512 : 256;
   k.places = 2048;
   return k;

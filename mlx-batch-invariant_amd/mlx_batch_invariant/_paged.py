@@ -491,7 +491,7 @@ def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_q
               k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(),
               query_start.data_ptr(), seq_lens.data_ptr(), _at(sinks), out.data_ptr(), T, R, H, Hkv, D,
               V, P, page, W, st, sst, scale, window, sink_tokens, max_query, max_seq, dt, _at(ws),
-              0 if ws is None else need)
+              0 if ws is None else ws.numel())
         return out
     need = _paged_bytes(dev, T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt)
     ws = _workspace(need, dev)

@@ -450,3 +450,109 @@ def test_compiles(cuda):
     fn = lambda q: bi.paged_attention(q, c.k, c.v, c.table, qs, c.lens, window=70, k_scales=c.ks, v_scales=c.vs)
     got = torch.compile(fn, fullgraph=True, backend="aot_eager")(q)
     assert same(got, fn(q))
+
+
+def laid_bytes(R, Hkv, D, V, longest):
+    """Of the rows laid out for the whole route: steps of 64 rows, keys and values
+    of 16 bits, two factors a row and two masks."""
+    return R * Hkv * -(-longest // 64) * (64 * (2 * D + 2 * V) + 512 + 16)
+
+
+# Beside requests of a few tokens and none one of many, with more heads sharing a kv
+# head where the kernel of 256 columns is wanted; under a window too.
+@pytest.mark.parametrize("D, V, H, chunk, seq, window, first", [
+    (64, 64, 8, 600, 2000, 0, 0), (96, 96, 8, 600, 2000, 300, 3), (128, 128, 8, 600, 2000, 0, 0),
+    (192, 128, 8, 600, 2000, 300, 3), (192, 192, 8, 600, 2000, 0, 0), (256, 256, 8, 600, 2000, 300, 3),
+    (64, 64, 32, 2100, 2300, 0, 0), (96, 96, 32, 2100, 2300, 0, 0), (128, 128, 32, 2100, 2300, 0, 0)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_laid_out_give_the_same_bits(cuda, D, V, H, chunk, seq, window, first, dtype, monkeypatch):
+    """With room for its rows laid out, with room for partial results only, and with
+    none: the same bits, pages that are not there and rows of bad scales included."""
+    Hkv, lens, new = 2, [900, seq, 0, 77], [1, chunk, 0, 70]
+    kv = [draw(n, Hkv, D, V, 60 + i) for i, n in enumerate(lens)]
+    kv[1][0][1][5, 1] = INF          # seen by all of the chunk without a window
+    kv[1][1][1][seq - 40, 0] = NAN   # by its last tokens
+    cache = Cache(kv, 13, cuda, order="phtd" if H == 8 else "pthd", width=-(-seq // 13) + 2)
+    cache.table[1, 9] = -1
+    cache.table[1, 60] = 1 << 30
+    q = queries(sum(new), H, D, dtype, 6)
+    most = []
+
+    def limited(limit):
+        def workspace(need, device):
+            most.append(need)
+            n = min(need, limit)
+            return torch.full((n,), 0xff, dtype=torch.uint8, device=device) if n else None
+        monkeypatch.setattr(_paged, "_workspace", workspace)
+        return cache(q, new, window=window or None, sink_tokens=first, max_query=chunk, max_seq=seq)
+
+    full = limited(1 << 40)
+    laid = laid_bytes(4, Hkv, D, V, seq)
+    assert most[0] >= laid, "not laid out"
+    assert same(limited(most[0] - 1), full)
+    assert same(limited(most[0] - laid), full) and same(limited(0), full)
+    # Its first tokens' neighbours, and tokens that see no bad row, are numbers.
+    assert bool(torch.isfinite(full[0]).all()) and bool(torch.isfinite(full[chunk + 1:]).all())
+    bad = torch.isnan(full[1:chunk + 1]).any(-1)  # (token, head)
+    pos = torch.arange(seq - chunk, seq)
+    half = H // 2
+    want = torch.zeros(chunk, H, dtype=torch.bool)
+    want[:, :half] = (pos >= seq - 40)[:, None]
+    want[:, half:] = ((pos < 5 + window) if window else pos >= 5)[:, None]
+    if window and first > 5:
+        want[:, half:] = True
+    assert bool((bad.cpu() == want).all())
+
+
+def test_rows_laid_out_are_accurate(cuda):
+    n, L = 2000, 600
+    kv = [draw(n, 2, 128, 128, 3)]
+    q = queries(L, 8, 128, BF16, 4)
+    got = Cache(kv, 16, cuda)(q, [L])
+    want, tol = rows(q, *kv[0], n)
+    check(got, want, tol)
+
+
+def test_many_requests_laid_out(cuda, monkeypatch):
+    """More requests than a workgroup has threads, some without tokens, some whole and
+    some split, and one past the bounds."""
+    R, D, Hkv = 301, 256, 1
+    lens = [(37 * r) % 250 + 6 for r in range(R)]
+    new = [0 if r % 7 == 3 else 1 if r % 5 == 1 else min(lens[r], 128) for r in range(R)]
+    lens[300], new[300] = 260, 1
+    kv = [draw(n, Hkv, D, D, r) for r, n in enumerate(lens)]
+    cache = Cache(kv, 16, cuda)
+    q = queries(sum(new), 8, D, BF16, 5)
+    seen = []
+
+    def workspace(need, device):
+        seen.append(need)
+        return torch.empty(need, dtype=torch.uint8, device=device)
+
+    monkeypatch.setattr(_paged, "_workspace", workspace)
+    a = cache(q, new, max_query=128, max_seq=256)
+    assert seen[0] >= laid_bytes(R, Hkv, D, D, 256)
+    monkeypatch.setattr(_paged, "_workspace", lambda need, device: None)
+    assert same(a, cache(q, new, max_query=128, max_seq=256))
+    assert bool(torch.isnan(a[-1]).all()) and bool(torch.isfinite(a[:-1]).all())
+
+
+def test_laid_out_in_a_graph(cuda):
+    """The rows are laid out anew in each replay."""
+    n, L = 1500, 500
+    kv = [draw(n, 2, 192, 192, 8)]
+    cache = Cache(kv, 16, cuda)
+    q = queries(L, 8, 192, BF16, 9).to(cuda)
+    cache(q, [L])
+    start = starts([L], cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bi.paged_attention(q, cache.k, cache.v, cache.table, start, cache.lens, k_scales=cache.ks,
+                                 v_scales=cache.vs)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, cache(q, [L]))
+        cache.k.neg_()
+        cache.vs.mul_(1.5)
+        q.copy_(q.roll(1, 0))

@@ -114,6 +114,12 @@ def test_attention_workspace():
     # Two sums and a row of V for each column and segment of 512 rows.
     assert ws() == 32 * 16 * 130 * 4
     assert ws(dtype=_lib.F16) == ws() and ws(longest=8193) == 32 * 17 * 130 * 4
+    # Rows laid out for those who walk them whole; not where they would take too much.
+    step = 64 * 4 * 128 + 512 + 16
+    assert ws(T=4096, most=4096) == 8 * 128 * step
+    for R in (1 << 10, 1 << 20, 1 << 29):
+        for Hkv in (1, 32):
+            assert 0 <= ws(T=1 << 25, R=R, H=32, Hkv=Hkv, most=1 << 25, longest=1 << 29) <= 1 << 32
     assert ws(T=0) == ws(R=0) == ws(H=0) == ws(longest=0) == ws(most=0) == 0
     assert ws(dtype=_lib.F32) == ws(D=80) == ws(H=33) == ws(window=-1) == ws(T=1 << 40) == 0
 
