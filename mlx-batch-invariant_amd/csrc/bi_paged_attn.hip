@@ -186,13 +186,13 @@ Plan plan(const Call& c, const Kernels& k) {
   return fits(c, s) ? beside(s) : lay;
 }
 
-int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, void* ws, int64_t ws_bytes,
+int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, void* ws, int64_t ws_bytes,
            void* stream) {
-  const Kernels k = kernels(D, V, dtype, p.ks != nullptr);
+  const Kernels k = kernels(D, V, dtype, q8);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t most = p.qstart ? p.max_query : p.qL;
   const Call c = {p.R, p.qstart ? p.T : (int64_t)p.R * p.qL, p.G.d, p.Hkv.d, D, V, p.window, p.first,
-                  most, p.qstart ? p.max_seq : p.N, !p.qstart, p.ks ? 1.0 : (double)bi::elem_size(dtype)};
+                  most, p.qstart ? p.max_seq : p.N, !p.qstart, q8 ? 1.0 : (double)bi::elem_size(dtype)};
   Plan s = plan(c, k);
   if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{};
   if (ws_bytes < s.workspace()) s.laid = 0;
@@ -330,7 +330,7 @@ int paged_attention(const char* who, const void* q, const void* k_cache, const v
   if (T == 0) return BI_OK;
   if (!q || !out || !query_start || (R > 0 && !seq_lens) || !strides ||
       (R > 0 && W > 0 && !block_tables) || (num_pages > 0 && (!k_cache || !v_cache)) ||
-      (q8 && (!k_scales || !v_scales || !scale_strides)))
+      (q8 && (!scale_strides || (num_pages > 0 && (!k_scales || !v_scales)))))
     return bi::fail(BI_EINVAL, "%s: null pointer", who);
   const int esz = bi::elem_size(dtype);
   if (!aligned16(q, nullptr, nullptr, strides, 2, esz) ||
@@ -376,7 +376,7 @@ int paged_attention(const char* who, const void* q, const void* k_cache, const v
     p.ksh = scale_strides[1], p.vsh = scale_strides[4];
     if (Hkv > 1 && D + V <= 256 && strides[3] < strides[4]) p.eight = make_div(8 * Hkv);
   }
-  return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
+  return launch(who, p, D, V, dtype, q8, workspace, workspace_bytes, hip_stream);
 }
 
 }  // namespace
@@ -469,7 +469,7 @@ extern "C" int bi_window_attention(const void* q, const void* k, const void* v, 
   p.R = (int32_t)B;
   p.qL = (int32_t)qL;
   p.N = (int32_t)N;
-  return launch(who, p, D, V, dtype, workspace, workspace_bytes, hip_stream);
+  return launch(who, p, D, V, dtype, false, workspace, workspace_bytes, hip_stream);
 }
 
 extern "C" int64_t bi_window_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t qL,

@@ -125,7 +125,7 @@ extern "C" int bi_rotary(const void* q, const void* k, void* q_out, void* k_out,
       H > (1 << 20) || Hkv > (1 << 20) || T > INT32_MAX)
     return bi::fail(BI_EINVAL, "%s: bad sizes T=%lld H=%lld Hkv=%lld D=%lld", who, (long long)T,
                     (long long)H, (long long)Hkv, (long long)D);
-  if (n > D / 2 || offset + 2 * n > D)
+  if (n > D / 2 || offset > D - 2 * n)
     return bi::fail(BI_EINVAL, "%s: %lld pairs from dim %lld on do not fit a head of %lld", who,
                     (long long)n, (long long)offset, (long long)D);
   if (T == 0 || H + Hkv == 0) return BI_OK;

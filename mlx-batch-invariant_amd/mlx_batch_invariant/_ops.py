@@ -7,7 +7,8 @@ traces, ``bi.*`` calls become the ops ``mlx_bi::gemm``, ``mlx_bi::qgemm`` and
 ``mlx_bi::sdpa`` (and, for the paged cache, ``mlx_bi::page_tables``,
 ``mlx_bi::paged_cache_update`` (``_q8`` and ``_kept`` with scales),
 ``mlx_bi::paged_cache_read``, ``mlx_bi::paged_attention`` (``_q8``) and
-``mlx_bi::window_attention``; ``mlx_bi::rotary`` and ``mlx_bi::token_logprobs``), which the compiler treats as opaque nodes (their
+``mlx_bi::window_attention``; ``mlx_bi::rotary`` and ``mlx_bi::token_logprobs``), which
+the compiler treats as opaque nodes (their
 fake implementations give only output shapes) and which run the HIP kernels
 unchanged. Eager calls skip the dispatcher and launch directly.
 """

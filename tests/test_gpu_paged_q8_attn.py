@@ -556,3 +556,16 @@ def test_laid_out_in_a_graph(cuda):
         cache.k.neg_()
         cache.vs.mul_(1.5)
         q.copy_(q.roll(1, 0))
+
+
+def test_a_cache_without_pages(cuda):
+    """Nothing is seen: zeros, by one token and by many."""
+    empty = torch.empty(0, 2, 16, 64, dtype=torch.int8, device=cuda)
+    scales = torch.empty(0, 2, 16, device=cuda)
+    table = torch.full((1, 40), -1, dtype=torch.int32, device=cuda)
+    lens = torch.tensor([600], dtype=torch.int32, device=cuda)
+    for L in (1, 600):
+        q = queries(L, 4, 64, BF16, 1).to(cuda)
+        for t in (table, table.new_full((1, 40), 3)):
+            out = bi.paged_attention(q, empty, empty, t, starts([L], cuda), lens, k_scales=scales, v_scales=scales)
+            assert out.shape == (L, 4, 64) and bool((out == 0).all())

@@ -35,6 +35,7 @@ def test_rotary_abi_refusals():
     assert call(offset=1) == _lib.EINVAL and "fit" in _err()
     assert call(n=1 << 62) == _lib.EINVAL and "fit" in _err()
     assert call(offset=1 << 62) == _lib.EINVAL and "fit" in _err()
+    assert call(offset=(1 << 63) - 1) == _lib.EINVAL and "fit" in _err()
     assert call(q=None) == _lib.EINVAL and "null" in _err()
     assert call(f=None) == _lib.EINVAL and call(pos=None) == _lib.EINVAL
     assert call(strides=False) == _lib.EINVAL
