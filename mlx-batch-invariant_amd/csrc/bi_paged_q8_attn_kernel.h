@@ -43,6 +43,7 @@ namespace {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 
 // Four codes as two dwords of bf16 or f16.
 template <typename T> __device__ __forceinline__ uint2 codes4(uint32_t w) {
@@ -110,7 +111,8 @@ struct Geo8 {
   // Whole route, a step as it lies in LDS: 16-byte units of keys, of values (both in
   // the type), then c_j, what values are multiplied with, and the masks of the rows
   // that have a page and that spoil. Laid out in memory the same.
-  static constexpr int KU = kStep * TCH, VU = kStep * TVCH, FU = kStep / 4, IU = KU + VU + 2 * FU + 1;
+  static constexpr int KU = kStep * TCH, VU = kStep * TVCH, FU = kStep / 4;
+  static constexpr int IU = (KU + VU + 2 * FU + 1 + 31) / 32 * 32;  // (whole rows: LDS addresses are multiples of these)
   // Steps of them in LDS.
   static constexpr int kDeep = 3 * IU * 16 <= 150 * 1024 ? 3 : 2;
   // Split route: workgroups of NC columns that a compute unit's registers hold.
@@ -216,20 +218,43 @@ struct Geo8 {
     if constexpr (!kPower) return y;
     else return times(y, *reinterpret_cast<const uint4*>(power + 32 * u + 8 * (ln >> 4)));
   }
-  // The same operands from rows in the type.
-  __device__ __forceinline__ static uint4 key_of_type(const uint4* k, int row0, int n, uint32_t ln) {
-    const uint32_t own = ln & 15;
-    return k[(row0 + own) * TCH + (piece(n, ln >> 4) ^ swz<TCH>(own))];
+  // The same operands from rows in the type, at LDS addresses that are multiples of a
+  // row. Where rows are a power of two long, what product or output tile it is turns
+  // bits of the lane's address that its row has not: one instruction each.
+  struct OfType {
+    uint32_t at;   // the lane's address, of product or tile 0
+    uint32_t own;  // the lane's row and part
+    __device__ __forceinline__ static uint32_t lds(const uint4* p) { return (uint32_t)(uintptr_t)(lds_void*)const_cast<uint4*>(p); }
+  };
+  __device__ __forceinline__ static OfType keys_of_type(const uint4* k, uint32_t ln) {
+    const uint32_t own = ln & 15, g = ln >> 4;
+    if constexpr ((TCH & (TCH - 1)) == 0) return {OfType::lds(k) + own * TCH * 16 + ((2 * g) ^ swz<TCH>(own)) * 16, 0};
+    else return {OfType::lds(k) + own * TCH * 16, ln};
   }
-  __device__ __forceinline__ static uint4 value_of_type(const uint4* v, int u, int dt, uint32_t ln) {
+  __device__ __forceinline__ static uint4 key_of_type(const OfType& k, int row0, int n) {
+    uint32_t at;
+    if constexpr ((TCH & (TCH - 1)) == 0) at = k.at ^ (uint32_t)((n & 1) + 8 * (n >> 1)) * 16;
+    else at = k.at + (piece(n, k.own >> 4) ^ swz<TCH>(k.own & 15)) * 16;
+    return __builtin_bit_cast(uint4, *(lds_u32x4*)(uintptr_t)(at + row0 * TCH * 16));
+  }
+  __device__ __forceinline__ static OfType values_of_type(const uint4* v, uint32_t ln) {
     const uint32_t own = 4 * (ln >> 4) + ((ln & 15) >> 2), part = ln & 3;
+    const uint32_t at = OfType::lds(v) + own * TVCH * 16 + 8 * (part & 1);
+    if constexpr ((TVCH & (TVCH - 1)) == 0) return {at + ((part >> 1) ^ tswz(own)) * 16, 0};
+    else return {at, ln};
+  }
+  __device__ __forceinline__ static uint4 value_of_type(const OfType& v, int u, int dt) {
+    uint32_t at;
+    if constexpr ((TVCH & (TVCH - 1)) == 0) {
+      at = v.at ^ (uint32_t)dt * 32;
+    } else {
+      const uint32_t own = 4 * (v.own >> 4) + ((v.own & 15) >> 2);
+      at = v.at + ((2 * dt + ((v.own & 3) >> 1)) ^ tswz(own)) * 16;
+    }
     i16x4 a[2];
 #pragma unroll
-    for (int x = 0; x < 2; x++) {  // (tswz has bits 0 to 2 of the row: rows 16 on have the same)
-      const char* at = reinterpret_cast<const char*>(v + (32 * u + 16 * x + own) * TVCH +
-                                                     ((2 * dt + (part >> 1)) ^ tswz(own))) + 8 * (part & 1);
-      a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at);
-    }
+    for (int x = 0; x < 2; x++)  // (tswz has bits 0 to 2 of the row: rows 16 on have the same)
+      a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + (32 * u + 16 * x) * TVCH * 16));
     const uint2 lo = __builtin_bit_cast(uint2, a[0]), hi = __builtin_bit_cast(uint2, a[1]);
     return make_uint4(lo.x, lo.y, hi.x, hi.y);
   }
@@ -772,7 +797,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
   constexpr int KU = G8::KU, VU = G8::VU, IU = LAID ? G8::IU : KU + VU;
   constexpr int NLW = LW ? LW : NW, NT = 64 * NLW, NB = LAID ? G8::kDeep : 2;  // waves and threads that load
   constexpr int KN = (S * G8::CH + NT - 1) / NT, VN = (S * G8::VCH + NT - 1) / NT;  // loads per thread
-  __shared__ uint4 s_kv[NB * IU];
+  __shared__ __attribute__((aligned(512))) uint4 s_kv[NB * IU];
   constexpr int RING = LAID ? 1 : 2 * NLW;
   __shared__ const char* s_row[RING][2][S];
   __shared__ __attribute__((aligned(16))) float s_c[RING][S], s_vs[RING][S];
@@ -955,14 +980,14 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
   }
 
   // LAID: a step's way into LDS, NB - 1 steps ahead.
-  constexpr int NL = (IU + NT - 1) / NT;
+  constexpr int MU = KU + VU + 2 * G8::FU + 1, NL = (MU + NT - 1) / NT;  // units that are wanted
   const char* laid = LAID ? p.laid + (int64_t)(r * (int)p.Hkv.d + kvh) * p.units * (IU * 16) : nullptr;
   auto fetch = [&](int j) __attribute__((always_inline)) {
     const char* from = laid + (uint64_t)(uint32_t)w.unit(j) * (IU * 16);
     uint4* to = s_kv + j % NB * IU + 64 * wave;
 #pragma unroll
     for (int i = 0; i < NL; i++)
-      if (i * NT + NT <= IU || i * NT + tid < IU)
+      if (i * NT + NT <= MU || i * NT + tid < MU)
         load_to_lds<16>(from + (i * NT + opaque(tid)) * 16, to + i * NT);
   };
 
@@ -1000,7 +1025,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
     const uint32_t ln = opaque(lane);
     const int g = ln >> 4;
     if constexpr (LAID) {  // (the loads of the NB - 2 steps after it may be on their way still)
-      if (j + NB - 2 < steps) wait_loads_but<(IU / NT) * (NB - 2)>();
+      if (j + NB - 2 < steps) wait_loads_but<(MU / NT) * (NB - 2)>();
       else wait_loads();
     }
     barrier();  // step j is there, and everyone is done with step j - 1's buffer
@@ -1031,8 +1056,9 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
       uint4 far[2];
       auto far_query = [&](int n) __attribute__((always_inline)) { far[n & 1] = s_q[wave][n][ln]; };
       if (kFar) far_query(0);
+      const auto keys = G8::keys_of_type(kd, ln);
       feed_ahead<RT * G8::NQ, kEasy ? 8 : 2>(
-          [&](int n) __attribute__((always_inline)) { return G8::key_of_type(kd, 16 * (n % RT), n / RT, ln); },
+          [&](int n) __attribute__((always_inline)) { return G8::key_of_type(keys, 16 * (n % RT), n / RT); },
           [&](int n, uint4 x) __attribute__((always_inline)) {
             const int i = n / RT;
             if (n % RT == 0 && i + 1 < kFar) far_query(i + 1);
@@ -1099,8 +1125,9 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
       if (j + 2 < steps) load_step(j + 2);
     if (mine) {
       // Products of one output tile are a chain: those of the others go between.
+      const auto values = G8::values_of_type(vd, ln);
       feed_ahead<DT * NU, kEasy ? 8 : 4>(
-          [&](int n) __attribute__((always_inline)) { return G8::value_of_type(vd, n / DT, n % DT, ln); },
+          [&](int n) __attribute__((always_inline)) { return G8::value_of_type(values, n / DT, n % DT); },
           [&](int n, uint4 v) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < CT; k++) o[n % DT][k] = G8::product(v, pu[n / DT][k], o[n % DT][k]);

@@ -454,8 +454,8 @@ def test_compiles(cuda):
 
 def laid_bytes(R, Hkv, D, V, longest):
     """Of the rows laid out for the whole route: steps of 64 rows, keys and values
-    of 16 bits, two factors a row and two masks."""
-    return R * Hkv * -(-longest // 64) * (64 * (2 * D + 2 * V) + 512 + 16)
+    of 16 bits, two factors a row and two masks, in whole 512 bytes."""
+    return R * Hkv * -(-longest // 64) * (-(-(64 * (2 * D + 2 * V) + 512 + 16) // 512) * 512)
 
 
 # Beside requests of a few tokens and none one of many, with more heads sharing a kv

@@ -116,7 +116,7 @@ def test_attention_workspace():
     assert ws() == 32 * 16 * 130 * 4
     assert ws(dtype=_lib.F16) == ws() and ws(longest=8193) == 32 * 17 * 130 * 4
     # Rows laid out for those who walk them whole; not where they would take too much.
-    step = 64 * 4 * 128 + 512 + 16
+    step = -(-(64 * 4 * 128 + 512 + 16) // 512) * 512
     assert ws(T=4096, most=4096) == 8 * 128 * step
     for R in (1 << 10, 1 << 20, 1 << 29):
         for Hkv in (1, 32):
