@@ -106,6 +106,17 @@ __device__ __forceinline__ float row_max(float x, int lanes) {
   return x;
 }
 
+// n * stride: one multiplication of 32 bits by 32, and where a stride is past them
+// (which all lanes know) the rest. (For the write, half of whose instructions were
+// addresses and the search for the largest: 8161 tokens 19.8 -> 17.9 us with both
+// mended; the read, bound by memory, gains nothing.)
+__device__ __forceinline__ int64_t times(int32_t n, int64_t stride) {
+  uint64_t x = (uint64_t)(uint32_t)n * (uint32_t)stride;
+  const uint32_t high = (uint32_t)((uint64_t)stride >> 32);
+  if (high) x += (uint64_t)((uint32_t)n * high) << 32;
+  return (int64_t)x;
+}
+
 // A row's side, and its token and head, from the thread's place.
 struct Place {
   int kv, lane;
@@ -125,11 +136,35 @@ __device__ __forceinline__ Place place(const Q8Args& p) {
   return x;
 }
 
+// The largest magnitude of U values, infinity where one is infinite or NaN: as whole
+// numbers, without their sign, magnitudes have the order of their values, and those
+// are above all. Of 16 bits two at a time.
+template <typename T, int U> __device__ __forceinline__ float largest(const typename Vec<T, U>::type& y) {
+  if constexpr (sizeof(T) == 4 || U == 1) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const float a = fabsf((float)y[i]);
+      top = fmaxf(top, a <= FLT_MAX ? a : INFINITY);
+    }
+    return top;
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t Words __attribute__((ext_vector_type(U / 2)));
+    const Words w = __builtin_bit_cast(Words, y);
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < U / 2; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+    const float a = (float)__builtin_bit_cast(T, m.x > m.y ? m.x : m.y);
+    return a <= FLT_MAX ? a : INFINITY;
+  }
+}
+
 // One row of a token and head by `lanes` lanes, U elements at a time each (16
 // bytes, or one where rows are not aligned to that); ONE: each lane has one unit at
 // most. What bounds it is memory, and the chain of a wave, of which there are few
 // rounds: both rows of a token and head by the same lanes took 27 us for 8161 tokens
-// of 4 KB, a row each 21.
+// of 4 KB, a row each 21 (17.9 now).
 template <typename T, int U, bool ONE>
 __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
   typedef typename Vec<T, U>::type In;
@@ -137,29 +172,21 @@ __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
   const Place x = place(p);
   const Side& w = p.side[x.kv];
   // (The row is loaded before the slot is looked at, so that both are under way together.)
-  const char* row = w.src + x.t * w.ts + x.head * w.hs;
+  const char* row = w.src + times(x.t, w.ts) + times(x.head, w.hs);
   In first = {};
   if (x.lane < w.units) first = reinterpret_cast<const In*>(row)[x.lane];
   const int32_t slot = p.slots[x.t];
   float top = 0.f;
   if (!p.keep) {
-    bool odd = false;  // an infinity or NaN
-    auto look = [&](const In& y) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < U; i++) {
-        const float a = fabsf((float)y[i]);
-        odd |= !(a <= FLT_MAX);
-        top = fmaxf(top, a);
-      }
-    };
+    auto look = [&](const In& y) __attribute__((always_inline)) { top = fmaxf(top, largest<T, U>(y)); };
     look(first);
     if (!ONE)
       for (int u = x.lane + w.lanes; u < w.units; u += w.lanes) look(reinterpret_cast<const In*>(row)[u]);
-    top = row_max(odd ? INFINITY : top, w.lanes);
+    top = row_max(top, w.lanes);
   }
   if (!x.real || slot < 0 || slot >= p.slots_end) return;
   const int32_t pg = slot / p.page, at = slot - pg * (int32_t)p.page.d;
-  float* scale = w.scale + pg * w.sp + x.head * w.sh + at * w.sr;
+  float* scale = w.scale + times(pg, w.sp) + times(x.head, w.sh) + times(at, w.sr);
   float s;
   if (p.keep) {
     s = *scale;
@@ -168,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
     if (x.lane == 0) *scale = s;
   }
   const float inv = __builtin_amdgcn_rcpf(s);
-  Out* out = reinterpret_cast<Out*>(w.dst + pg * w.cp + x.head * w.ch + at * w.cr);
+  Out* out = reinterpret_cast<Out*>(w.dst + times(pg, w.cp) + times(x.head, w.ch) + times(at, w.cr));
   auto put = [&](int u, const In& y) __attribute__((always_inline)) {
     float v[U];
     int8_t c[U] = {};
