@@ -251,3 +251,29 @@ def test_nothing_to_do(cuda):
     empty = p.k[:0], p.v[:0]
     k, v = bi.paged_cache_read(*empty, p.slots, k_scales=p.ks[:0], v_scales=p.vs[:0])
     assert k.shape == (4, 2, 64) and not k.any() and not v.any()
+
+
+def test_strides_past_4_gib(cuda):
+    """Pages, rows of scales and tokens that lie 5 GiB apart."""
+    far = 5 << 30
+    pool = torch.zeros(far + (1 << 20), dtype=torch.int8, device=cuda)
+    k, v = (pool[at:].as_strided((2, 2, 4, 32), (far, 128, 32, 1)) for at in (0, 4096))
+    scales = torch.zeros((far >> 2) + (1 << 16), device=cuda)
+    ks, vs = (scales[at:].as_strided((2, 2, 4), (far >> 2, 4, 1)) for at in (0, 4096))
+    x = torch.randn(5, 2, 32, generator=torch.Generator().manual_seed(1)).to(BF16).to(cuda)
+    tokens = torch.zeros((far >> 1) + (1 << 16), dtype=BF16, device=cuda).as_strided((2, 2, 32), (far >> 1, 32, 1))
+    tokens.copy_(x[:2])
+    slots = torch.tensor([6, 1], dtype=torch.int32, device=cuda)
+    bi.paged_cache_update(tokens, tokens, k, v, slots, k_scales=ks, v_scales=vs)
+    codes, s = codes_of(x[:2].cpu())
+    for c, cs in ((k, ks), (v, vs)):
+        for t, (page, row) in enumerate(((1, 2), (0, 1))):
+            assert same(c[page, :, row].cpu().float(), codes[t].float()) and same(cs[page, :, row].cpu(), s[t])
+    for got in bi.paged_cache_read(k, v, slots, k_scales=ks, v_scales=vs):
+        assert same(got.cpu(), codes.float() * s[..., None])
+    with pytest.raises(NotImplementedError, match="4 GiB"):
+        one = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+        bi.paged_attention(torch.zeros(1, 2, 64, dtype=BF16, device=cuda),
+                           pool.as_strided((2, 2, 4, 64), (far, 256, 64, 1)),
+                           pool.as_strided((2, 2, 4, 64), (far, 256, 64, 1)), slots[None], one, one[1:],
+                           k_scales=ks, v_scales=vs)
