@@ -8,8 +8,8 @@
 // +inf, and one of -inf alone, is NaN. M, S and U are in 32 bits.
 //
 // The k largest, ties to the lowest id. The threads form 256 groups (64 for up to
-// 16); the k-th largest of the groups' largest logits bounds the k-th largest
-// logit of all from below. What is not below it, k to 1.2 k logits of most rows,
+// 32); the k-th largest of the groups' largest logits bounds the k-th largest
+// logit of all from below. What is not below it, k to 1.4 k logits of most rows,
 // is put in order wave by wave, by insertion into a list that the lanes hold, and
 // what the waves' lists hold is counted against each other.
 //
@@ -51,6 +51,22 @@ __device__ __forceinline__ float logit_of(int32_t o) {
 }
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// A wave's value of all lanes, by moves within a register: op is the same of (a, b)
+// and (b, a), so all lanes have the same bits.
+template <int CTRL> __device__ __forceinline__ float moved(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+template <typename Op> __device__ __forceinline__ float of_wave(float x, const Op& op) {
+  x = op(x, moved<0xB1>(x));   // lane ^ 1
+  x = op(x, moved<0x4E>(x));   // lane ^ 2
+  x = op(x, moved<0x141>(x));  // 7 - lane of eight
+  x = op(x, moved<0x140>(x));  // 15 - lane of sixteen
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
 // NT threads of NU units of 16 bytes each; HELD: all of a row is in these.
 template <typename T, int NT, int NU, bool HELD>
 __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(LogprobArgs p) {
@@ -82,6 +98,7 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
   const int rounds = HELD ? 1 : (int)((units + NT * NU - 1) / (NT * NU));
 
   Vec x[NU];
+  float unit[NU];  // the largest of each (HELD)
   float m = -INFINITY, s = 0.f, ud = 0.f;
   auto add = [&](const Vec& v, float base) __attribute__((always_inline)) {
 #pragma unroll
@@ -97,9 +114,12 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
     for (int i = 0; i < NU; i++) x[i] = load(((int64_t)r * NU + i) * NT + tid);
     float top = m;
 #pragma unroll
-    for (int i = 0; i < NU; i++)
+    for (int i = 0; i < NU; i++) {
+      unit[i] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < U; j++) top = larger(top, (float)x[i][j]);
+      for (int j = 0; j < U; j++) unit[i] = larger(unit[i], (float)x[i][j]);
+      top = larger(top, unit[i]);
+    }
     if constexpr (!HELD) {
       // The thread's own base moves to its largest so far.
       const float d = m - top, f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
@@ -116,15 +136,13 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
 
   // The groups' largest, four to a lane, and of them the row's.
   float g = m;
-#pragma unroll
-  for (int d = 1; d < GROUP; d <<= 1) g = larger(g, __shfl_xor(g, d));
+  static_assert(GROUP == 1 || GROUP == 4, "lanes of a group");
+  if constexpr (GROUP == 4) g = larger(g, moved<0xB1>(g)), g = larger(g, moved<0x4E>(g));
   if (lane % GROUP == 0) reinterpret_cast<float*>(s_group)[tid / GROUP] = g;
   __syncthreads();
   const float4 four = s_group[lane];
   g = larger(larger(four.x, four.y), larger(four.z, four.w));
-  float M = g;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) M = larger(M, __shfl_xor(M, d));
+  const float M = of_wave(g, larger);
 
   if constexpr (HELD) {
 #pragma unroll
@@ -135,11 +153,9 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
     s *= f;
     if (M == -INFINITY) s = NAN;
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    s += __shfl_xor(s, d);
-    ud += __shfl_xor(ud, d);
-  }
+  const auto plus = [](float a, float b) __attribute__((always_inline)) { return a + b; };
+  s = of_wave(s, plus);
+  ud = of_wave(ud, plus);
   if (lane == 0) s_sum[wave] = make_float2(s, ud);
 
   if (p.top) {
@@ -147,7 +163,7 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
     // other 16, which bf16 has not, a row of fp32 would have a few candidates less.)
     auto key_of = [](float v) __attribute__((always_inline)) { return (uint32_t)order_of(v) ^ 0x80000000u; };
     uint32_t bound = 0;
-    if (p.top <= 16) {
+    if (p.top <= 32) {
       const uint32_t key = key_of(g);
 #pragma unroll
       for (int b = 31; b >= 16; b--) {
@@ -176,13 +192,12 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
         uint64_t bits = 0;
         static_assert(NU * U <= 64, "a bit for each element");
         const int64_t first = (int64_t)r * NU * NT + tid;
-        if (mine) {
 #pragma unroll
-          for (int i = 0; i < NU; i++) {
-            const Vec v = HELD ? x[i] : load(first + (int64_t)i * NT);
+        for (int i = 0; i < NU; i++) {  // (most units have no candidate in any lane)
+          if (!(HELD ? !(unit[i] < least) : mine)) continue;
+          const Vec v = HELD ? x[i] : load(first + (int64_t)i * NT);
 #pragma unroll
-            for (int j = 0; j < U; j++) bits |= (uint64_t)!((float)v[j] < least) << (i * U + j);
-          }
+          for (int j = 0; j < U; j++) bits |= (uint64_t)!((float)v[j] < least) << (i * U + j);
         }
         const bool one = HELD && __popcll(bits) == 1;  // then it is the thread's largest
         while (__builtin_amdgcn_ballot_w64(bits != 0) != 0) {
@@ -220,6 +235,9 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
   }
   __syncthreads();
 
+  // What is left is one wave's, but for more candidates than it has lanes.
+  const int n = p.top ? s_count : 0;
+  if (n <= 64 && wave != 0) return;
   float S = 0.f, UD = 0.f;
 #pragma unroll
   for (int w = 0; w < NW; w++) {
@@ -235,14 +253,12 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
     p.entropy[r] = ln - UD / S;
   }
   if (p.top) {
-    const int n = s_count;
     auto put = [&](int32_t o, int32_t id, int rank) __attribute__((always_inline)) {
       if (rank >= p.top) return;
       p.top_ids[r * p.top + rank] = id;
       p.top_logprobs[r * p.top + rank] = logit_of(o) - M - ln;
     };
     if (n <= 64) {  // one wave, its lanes' candidates against each other
-      if (wave != 0) return;
       const int32_t o = lane < n ? s_list[lane] : INT32_MIN, id = lane < n ? s_id[lane] : INT32_MAX;
       int rank = lane < n ? 0 : kMostTop;
       for (int j = 0; j < n; j++) {
