@@ -218,39 +218,33 @@ struct Geo8 {
     if constexpr (!kPower) return y;
     else return times(y, *reinterpret_cast<const uint4*>(power + 32 * u + 8 * (ln >> 4)));
   }
-  // The same operands from rows in the type, at LDS addresses that are multiples of a
-  // row. Where rows are a power of two long, what product or output tile it is turns
-  // bits of the lane's address that its row has not: one instruction each.
+  // The same operands from rows in the type. Which product or output tile it is turns
+  // bits of the lane's chunk, which are bits of its address where rows are a power of
+  // two long and the LDS address is a multiple of one: an instruction for each operand.
   struct OfType {
-    uint32_t at;   // the lane's address, of product or tile 0
-    uint32_t own;  // the lane's row and part
+    uint32_t row, chunk;  // LDS address of the lane's row, and its chunk's place in it, in bytes
+    template <int C> __device__ __forceinline__ uint32_t at(uint32_t turn) const {
+      if constexpr ((C & (C - 1)) == 0) return (row + chunk) ^ turn;
+      else return row + (chunk ^ turn);
+    }
     __device__ __forceinline__ static uint32_t lds(const uint4* p) { return (uint32_t)(uintptr_t)(lds_void*)const_cast<uint4*>(p); }
   };
   __device__ __forceinline__ static OfType keys_of_type(const uint4* k, uint32_t ln) {
     const uint32_t own = ln & 15, g = ln >> 4;
-    if constexpr ((TCH & (TCH - 1)) == 0) return {OfType::lds(k) + own * TCH * 16 + ((2 * g) ^ swz<TCH>(own)) * 16, 0};
-    else return {OfType::lds(k) + own * TCH * 16, ln};
+    return {OfType::lds(k) + own * TCH * 16, ((2 * g) ^ swz<TCH>(own)) * 16};
   }
-  __device__ __forceinline__ static uint4 key_of_type(const OfType& k, int row0, int n) {
+  __device__ __forceinline__ static uint4 key_of_type(const OfType& k, int row0, int n, uint32_t ln) {
     uint32_t at;
-    if constexpr ((TCH & (TCH - 1)) == 0) at = k.at ^ (uint32_t)((n & 1) + 8 * (n >> 1)) * 16;
-    else at = k.at + (piece(n, k.own >> 4) ^ swz<TCH>(k.own & 15)) * 16;
+    if (NQ % 2 && n + 1 == NQ) at = k.row + (piece(n, ln >> 4) ^ swz<TCH>(ln & 15)) * 16;
+    else at = k.template at<TCH>(piece(n, 0) * 16);
     return __builtin_bit_cast(uint4, *(lds_u32x4*)(uintptr_t)(at + row0 * TCH * 16));
   }
   __device__ __forceinline__ static OfType values_of_type(const uint4* v, uint32_t ln) {
     const uint32_t own = 4 * (ln >> 4) + ((ln & 15) >> 2), part = ln & 3;
-    const uint32_t at = OfType::lds(v) + own * TVCH * 16 + 8 * (part & 1);
-    if constexpr ((TVCH & (TVCH - 1)) == 0) return {at + ((part >> 1) ^ tswz(own)) * 16, 0};
-    else return {at, ln};
+    return {OfType::lds(v) + own * TVCH * 16, ((part >> 1) ^ tswz(own)) * 16 + 8 * (part & 1)};
   }
   __device__ __forceinline__ static uint4 value_of_type(const OfType& v, int u, int dt) {
-    uint32_t at;
-    if constexpr ((TVCH & (TVCH - 1)) == 0) {
-      at = v.at ^ (uint32_t)dt * 32;
-    } else {
-      const uint32_t own = 4 * (v.own >> 4) + ((v.own & 15) >> 2);
-      at = v.at + ((2 * dt + ((v.own & 3) >> 1)) ^ tswz(own)) * 16;
-    }
+    const uint32_t at = v.template at<TVCH>(dt * 32);
     i16x4 a[2];
 #pragma unroll
     for (int x = 0; x < 2; x++)  // (tswz has bits 0 to 2 of the row: rows 16 on have the same)
@@ -1058,7 +1052,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
       if (kFar) far_query(0);
       const auto keys = G8::keys_of_type(kd, ln);
       feed_ahead<RT * G8::NQ, kEasy ? 8 : 2>(
-          [&](int n) __attribute__((always_inline)) { return G8::key_of_type(keys, 16 * (n % RT), n / RT); },
+          [&](int n) __attribute__((always_inline)) { return G8::key_of_type(keys, 16 * (n % RT), n / RT, ln); },
           [&](int n, uint4 x) __attribute__((always_inline)) {
             const int i = n / RT;
             if (n % RT == 0 && i + 1 < kFar) far_query(i + 1);
