@@ -73,7 +73,7 @@ struct Kernels {
   // rows as step_bytes, and the whole route over these.
   Kernel lay = nullptr, laid4 = nullptr, laid8 = nullptr;
   int step = 0, step_bytes = 0;
-  double laid_row_us = 0;
+  double laid_row_us = 0, laid_tile_us = 0;  // and a workgroup's beginning and end
   int seg, pass;            // rows per segment and per pass of the split route (four steps)
   int places = 8192;        // split workgroups with work, about: more take several segments each
   // For the choice of route, in microseconds: what a row costs a whole

@@ -106,7 +106,7 @@ bool fits(const Call& c, const Plan& s) {
 // prompt, 8/8 heads 331 / 124. Of 822 sizes timed both ways it picks the one
 // that takes 8 % more or worse four times, 29 % at most; over a cache of 8 bits, of
 // 666 sizes timed each way, with its rows laid out too, 1 % on average, 20 % or worse
-// ten times, mostly over 200 rows. 64 single tokens under a
+// seven times, mostly over 200 rows. 64 single tokens under a
 // bound of 64 229, with all these columns split 1030.)
 Plan plan(const Call& c, const Kernels& k) {
   const Plan none = {};
@@ -122,20 +122,20 @@ Plan plan(const Call& c, const Kernels& k) {
   const double read = (double)c.R * rows * c.Hkv * (c.D + c.V) * c.bytes / 5e6;
   const double all = (double)c.R * ((cols + 127) / 128), full = (double)c.tokens * c.G / 128.0 + c.R;
   const double tiles = (all < full ? all : full) * c.Hkv / cus;
-  auto walk_us = [&](double row_us) {
+  auto walk_us = [&](double row_us, double tile_us) {
     const double walked = (cut ? rows + 128.0 / c.G + 64.0 : rows) * row_us;
-    const double first = 7.5 + walked, most = tiles * (7.5 + walked * (cut ? 1.0 : 1.0 - 0.5 * chunk / seq));
+    const double first = 7.5 + walked, most = tiles * (tile_us + walked * (cut ? 1.0 : 1.0 - 0.5 * chunk / seq));
     const double us = first > most ? first : most;
     return 2.0 + (us > 1.1 * read ? us : 1.1 * read);
   };
-  double whole = walk_us(k.row_us);
+  double whole = walk_us(k.row_us, 7.5);
   // Whether the rows that are walked whole are laid out first: a launch, and their
   // codes through memory, three bytes for each, at 4 TB/s.
   Plan lay = none;
   if (k.lay) {
     const double requests = (double)c.tokens / (double)c.max_query, part = (double)c.max_query + wide;
     const double laid = (cut && part < seq ? part : seq) * (requests < 1.0 ? 1.0 : requests < c.R ? requests : c.R);
-    const double us = walk_us(k.laid_row_us) + 4.0 + laid * c.Hkv * (c.D + c.V) * 3.0 / 4e6;
+    const double us = walk_us(k.laid_row_us, k.laid_tile_us) + 4.0 + laid * c.Hkv * (c.D + c.V) * 3.0 / 4e6;
     lay.units = (c.max_seq + k.step - 1) / k.step;
     const double bytes = (double)c.R * (double)(c.Hkv * lay.units * k.step_bytes);
     if (us < whole && bytes <= (double)kMostBytes) {

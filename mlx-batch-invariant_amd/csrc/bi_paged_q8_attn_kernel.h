@@ -128,6 +128,8 @@ struct Geo8 {
     return 1e-3 * (kTwoWaves ? 14.0 + 0.047 * (D + V) + (kPow2 ? 0.0 : 10.0) : 24.0 + 0.0725 * (D + V));
   }
   static constexpr double laid_row_us() { return 1e-3 * (10.0 + 0.051 * (D + V)); }
+  // (One workgroup's ends are beside another's rows where a compute unit has two.)
+  static constexpr double laid_tile_us() { return D + V <= 192 ? 3.0 : 7.5; }
   static constexpr double seg_us(int NC) {
     if (NC == 32) return 9.2 + 0.0135 * (D + V);
     return kTwoWaves ? 4.0 + 0.006 * (D + V) + (kPow2 ? 0.0 : 2.0) : 2.0 + 0.026 * (D + V);
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
 // What every workgroup of the whole route would do for the rows that it walks, looking
 // up pages and making numbers of codes, is done once, where there is room for the
 // result (4096 tokens over 8192 rows, 64 column tiles to a kv head, 128 dims: 576 ->
-// 484 us; 192 dims 1342 -> 891, 256 1557 -> 992, where four waves of 32 columns gave
+// 480 us; 192 dims 1342 -> 887, 256 1557 -> 912, where four waves of 32 columns gave
 // way to eight of 16 as well). It costs a launch and three bytes of traffic a code:
 // 12 us for these rows, and 8 requests of 64 tokens over 4000 rows would take 166 us
 // for 116, so the host compares. The list of what is to do, steps of requests that are
@@ -778,10 +780,10 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
 // nothing but that (LW = 0: the NW waves themselves).
 //
 // What bounds it (laid out, 256 columns, 128 dims, 4096 tokens over 8192 rows): a
-// step's 2.4 us are 6000 cycles, of which each SIMD's two waves have products in 34 %
-// and issue vector instructions in 51 %, the LDS is busy in 25 %; what is left is waits.
+// step's 2.4 us are 6000 cycles, of which each SIMD's two waves have products in 35 %
+// and issue vector instructions in 47 %, the LDS is busy in 25 %; what is left is waits.
 // Operands read further ahead, or half of the waves half a step behind the others,
-// changed nothing.
+// changed nothing; 16 waves of 16 columns, four a SIMD, took 531 us for 485.
 template <typename T, int D, int V, int NW, int LW, int CT, bool LAID>
 __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || NW == 8 ? 2 : 1)) whole8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
@@ -1188,7 +1190,7 @@ Kernels kernels8_of() {
   k.seg = G8::kSeg, k.pass = 4 * G8::kStep;
   k.row_us = G8::row_us();
   k.seg16_us = G8::seg_us(16), k.seg32_us = G8::seg_us(32);
-  k.laid_row_us = G8::laid_row_us();
+  k.laid_row_us = G8::laid_row_us(), k.laid_tile_us = G8::laid_tile_us();
   k.per_cu16 = G8::split_per_cu(16), k.per_cu32 = G8::split_per_cu(32);
   k.whole4_pair = nullptr;
   if constexpr (G8::kTwoWaves) {
