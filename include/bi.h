@@ -357,7 +357,8 @@ int bi_paged_read(const void* k_cache, const void* v_cache, const float* k_scale
  * 2^-14 lose nothing; those of 2^19 and above, of values past 6e7, overflow),
  * products and sums are of 32 bits, the denominator the sum of the weights of 32
  * bits. A token that sees a row whose key or value scale is infinite or NaN, or
- * whose key scale is negative, is NaN. A token's bits depend on its own request's
+ * whose key scale is negative, is NaN, and so is one whose largest score times log2
+ * e is 2^30 or more from 0 within some 512 rows. A token's bits depend on its own request's
  * rows alone, as there, and nothing in a row that a token does not see reaches it.
  */
 int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const int8_t* v_cache,

@@ -93,6 +93,13 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// A segment's sum, NaN where its base is so far from 0 that a score's own rounding,
+// which the base has and the exponent has not, is beyond what an exponential holds
+// (from 2^31 on it may be 128).
+__device__ __forceinline__ float within(float m, float l) {
+  return fabsf(m) < 1073741824.f || m == kNone ? l : NAN;
+}
+
 template <typename T, int D_, int V_>
 struct Geo8 {
   static constexpr int D = D_, V = V_;
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
     if (next.part != at.part) {  // the segment's last pass
 #pragma unroll
       for (int k = 0; k < CT; k++) {
-        const float sum = quarters_sum(l[k]);
+        const float sum = within(m[k], quarters_sum(l[k]));
         if (!cv[k]) continue;
         const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + at.part) * p.ccap.d + c0 + 16 * k + col;
         if (wave == 0 && g == 0) p.pml[slot] = make_float2(m[k], sum);
@@ -1136,7 +1143,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
 #pragma unroll
         for (int k = 0; k < CT; k++) {
           float M = s_ml[k][0][td], L = s_ml[k][1][td], fa, fb;
-          fold_base(M, L, m[k], quarters_sum(l[k]), fa, fb);
+          fold_base(M, L, m[k], within(m[k], quarters_sum(l[k])), fa, fb);
           s_ml[k][0][td] = M;
           s_ml[k][1][td] = L;
           if (__builtin_amdgcn_ballot_w64(fa != 1.f) != 0)

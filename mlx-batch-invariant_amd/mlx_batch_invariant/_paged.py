@@ -397,7 +397,7 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     than 4 GiB apart. The bits are as independent of the call as without scales,
     but others: the products are of codes, and weights times their row's scale
     are rounded to q's type. A token is NaN that sees a row whose scale is
-    infinite or NaN, or negative for keys.
+    infinite or NaN, or negative for keys, or whose scores pass 2^29.
     """
     _cache_shapes(k_cache, v_cache, k_scales, v_scales)
     if q.ndim != 3:

@@ -569,3 +569,55 @@ def test_a_cache_without_pages(cuda):
         for t in (table, table.new_full((1, 40), 3)):
             out = bi.paged_attention(q, empty, empty, t, starts([L], cuda), lens, k_scales=scales, v_scales=scales)
             assert out.shape == (L, 4, 64) and bool((out == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_laid_out_rows_of_any_scale_sinks_and_more_tokens_than_rows(cuda, dtype, monkeypatch):
+    """A chunk of more tokens than its request has rows, whose first see nothing; scales
+    over many powers of two; logit sinks and a negative scale: as without a workspace."""
+    kv = [draw(300, 2, 192, 128, 21, spread=6.0), draw(1400, 2, 192, 128, 22, spread=6.0)]
+    new = [520, 520]
+    cache = Cache(kv, 16, cuda)
+    q = queries(sum(new), 8, 192, dtype, 23)
+    sinks = torch.randn(8, generator=torch.Generator().manual_seed(2)).to(dtype).to(cuda)
+    seen = []
+
+    def workspace(need, device):
+        seen.append(need)
+        return torch.full((need,), 0xff, dtype=torch.uint8, device=device)
+
+    for kw in (dict(), dict(sinks=sinks), dict(scale=-0.07), dict(sinks=sinks, scale=-0.07, window=200)):
+        kw = dict(kw, max_query=520, max_seq=1400)
+        monkeypatch.setattr(_paged, "_workspace", workspace)
+        a = cache(q, new, **kw)
+        assert seen[-1] >= laid_bytes(2, 2, 192, 128, 1400), kw
+        monkeypatch.setattr(_paged, "_workspace", lambda need, device: None)
+        assert same(a, cache(q, new, **kw)), kw
+        assert bool((a[:220] == 0).all())
+        # Without a sink a token's weights sum to 1, and the largest value of what it sees
+        # is above bf16's smallest number. (With one they may all be below it: scores here
+        # reach far below any sink. f16's smallest number is above the smallest scales.)
+        if dtype == BF16 and "sinks" not in kw:
+            assert bool((a[220:] != 0).any(-1).all())
+
+
+@pytest.mark.parametrize("L", [1, 40])
+def test_scores_as_far_as_they_go(cuda, L):
+    """Of one row alone the result is its value, however large the score, or NaN."""
+    D = 64
+    kc = torch.zeros(L, 1, D, dtype=torch.int8)
+    kc[:, :, 0] = 100
+    (vc, vs) = draw(L, 1, D, D, 3)[1]
+    vc = vc[:1].expand(L, 1, D).contiguous()
+    vs = vs[:1].expand(L, 1).contiguous()
+    value = (vc[0, 0].double() * vs[0, 0].double())
+    for power, sign in ((8, 1), (20, 1), (20, -1), (27, 1), (27, -1), (31, 1), (31, -1), (60, 1)):
+        ks = torch.full((L, 1), 2.0 ** (power - 3) / 100)
+        q = torch.zeros(L, 4, D, dtype=BF16)
+        q[..., 0] = 8.0 * sign
+        got = Cache([((kc, ks), (vc, vs))], 16, cuda)(q, [L], scale=1.0)
+        if power > 29:
+            assert bool(torch.isnan(got).all()), (power, sign)
+        else:  # (p's, the weight's and the result's rounding, and equal rows' sum)
+            tol = value.abs() * (2 * UNIT[BF16] + 2.0 ** -20)
+            assert bool(((got.double().cpu() - value).abs() <= tol).all()), (power, sign)
