@@ -354,12 +354,14 @@ int bi_paged_read(const void* k_cache, const void* v_cache, const float* k_scale
  * Scores are sums of exact products of codes and q in 32 bits times the row's
  * scale in 32 bits; weights times the row's scale are rounded to `dtype` (BI_F16:
  * but for the scale's power of two, which goes with the codes, so that scales from
- * 2^-14 lose nothing; those of 2^19 and above, of values past 6e7, overflow),
- * products and sums are of 32 bits, the denominator the sum of the weights of 32
- * bits. A token that sees a row whose key or value scale is infinite or NaN, or
- * whose key scale is negative, is NaN, and so is one whose largest score times log2
- * e is 2^30 or more from 0 within some 512 rows. A token's bits depend on its own request's
- * rows alone, as there, and nothing in a row that a token does not see reaches it.
+ * 2^-14 lose nothing; those of 2^19 and above, of values past 6e7, overflow, and
+ * beside scores past 2^26 those of 2^13), products and sums are of 32 bits, the
+ * denominator the sum of the weights of 32 bits. A token that sees a row whose key
+ * or value scale is infinite or NaN, or whose key scale is negative, is NaN, and so
+ * is one whose largest score times log2 e is 2^30 (BI_F16: 2^28) or more from 0
+ * within some 512 rows; a score below the range of 32 bits is -inf, and its row not
+ * seen. A token's bits depend on its own request's rows alone, as there, and nothing
+ * in a row that a token does not see reaches it.
  */
 int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const int8_t* v_cache,
                           const float* k_scales, const float* v_scales,

@@ -94,10 +94,13 @@ __device__ __forceinline__ float quarters_sum(float x) {
 }
 
 // A segment's sum, NaN where its base is so far from 0 that a score's own rounding,
-// which the base has and the exponent has not, is beyond what an exponential holds
-// (from 2^31 on it may be 128).
-__device__ __forceinline__ float within(float m, float l) {
-  return fabsf(m) < 1073741824.f || m == kNone ? l : NAN;
+// which the base has and the exponent has not, is beyond what a weight holds. Half a
+// step of a score is 64 from 2^30 on, with which an exponential may leave bf16's range
+// (at twice that it is 2^128), and 16 from 2^28 on, with which it leaves f16's
+// (below, p is at most 2^12 and the largest at least 2^-8).
+template <typename T> __device__ __forceinline__ float within(float m, float l) {
+  constexpr float kFar = __is_same(T, _Float16) ? 268435456.f : 1073741824.f;
+  return fabsf(m) < kFar || m == kNone ? l : NAN;
 }
 
 template <typename T, int D_, int V_>
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
     if (next.part != at.part) {  // the segment's last pass
 #pragma unroll
       for (int k = 0; k < CT; k++) {
-        const float sum = within(m[k], quarters_sum(l[k]));
+        const float sum = within<T>(m[k], quarters_sum(l[k]));
         if (!cv[k]) continue;
         const int64_t slot = (((int64_t)r * p.Hkv.d + kvh) * p.nseg.d + at.part) * p.ccap.d + c0 + 16 * k + col;
         if (wave == 0 && g == 0) p.pml[slot] = make_float2(m[k], sum);
@@ -1143,7 +1146,7 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
 #pragma unroll
         for (int k = 0; k < CT; k++) {
           float M = s_ml[k][0][td], L = s_ml[k][1][td], fa, fb;
-          fold_base(M, L, m[k], within(m[k], quarters_sum(l[k])), fa, fb);
+          fold_base(M, L, m[k], within<T>(m[k], quarters_sum(l[k])), fa, fb);
           s_ml[k][0][td] = M;
           s_ml[k][1][td] = L;
           if (__builtin_amdgcn_ballot_w64(fa != 1.f) != 0)

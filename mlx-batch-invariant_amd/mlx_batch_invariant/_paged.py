@@ -397,7 +397,9 @@ def paged_attention(q, k_cache, v_cache, block_tables, query_start, seq_lens, *,
     than 4 GiB apart. The bits are as independent of the call as without scales,
     but others: the products are of codes, and weights times their row's scale
     are rounded to q's type. A token is NaN that sees a row whose scale is
-    infinite or NaN, or negative for keys, or whose scores pass 2^29.
+    infinite or NaN, or negative for keys, or whose largest score among some 512
+    rows is 1.86e8 (float16) or 7.44e8 (bfloat16) or more from 0: 2^28 or 2^30
+    times ln 2.
     """
     _cache_shapes(k_cache, v_cache, k_scales, v_scales)
     if q.ndim != 3:

@@ -621,3 +621,82 @@ def test_scores_as_far_as_they_go(cuda, L):
         else:  # (p's, the weight's and the result's rounding, and equal rows' sum)
             tol = value.abs() * (2 * UNIT[BF16] + 2.0 ** -20)
             assert bool(((got.double().cpu() - value).abs() <= tol).all()), (power, sign)
+
+
+@pytest.mark.parametrize("dtype, bound", [(F16, 2.0 ** 28), (BF16, 2.0 ** 30)])
+@pytest.mark.parametrize("L", [1, 40])
+def test_scores_up_to_the_bound_of_their_type(cuda, dtype, bound, L):
+    """Requests of equal rows, whose result is the row's value: for scales of any bits,
+    whose scores round up and down, it is that below the bound (of scores times log2 e),
+    and NaN past it."""
+    D, R = 64, 64
+    (vc, vs) = draw(1, 1, D, D, 3)[1]
+    value = vc[0, 0].double() * vs[0, 0].double()
+    g = torch.Generator().manual_seed(L)
+    q = torch.zeros(L * R, 4, D, dtype=dtype)
+    q[..., 0] = 8.0
+    # p's exponent is off by half a step of the score, which the denominator shares; p
+    # itself by 2 units of 32 bits, a weight by its rounding (f16: of 2^-8 at least, by
+    # 2^-25 at most where it is subnormal), the result by its own; sums of L.
+    tol = value.abs() * (2.05 * UNIT[dtype] + 2.0 ** -17 + 2.0 ** -20) + (2.0 ** -25 if dtype == F16 else 0.0)
+    for power in range(20, 31):
+        s = 2.0 ** power * (1 + torch.rand(R, generator=g))  # scores times log2 e
+        keep = (s < bound * 0.999) | (s > bound * 1.001)
+        for sign in (1, -1):
+            kv = []
+            for r in range(R):
+                kc = torch.zeros(L, 1, D, dtype=torch.int8)
+                kc[:, :, 0] = 100 * sign
+                ks = torch.full((L, 1), float(s[r] / 800 / 1.4426950408889634))
+                kv.append(((kc, ks), (vc.expand(L, 1, D).contiguous(), vs.expand(L, 1).contiguous())))
+            got = Cache(kv, 16, cuda)(q, [L] * R, scale=1.0).double().cpu().view(R, L, 4, D)
+            for r in range(R):
+                if not keep[r]:
+                    continue
+                if s[r] > bound:
+                    assert bool(got[r].isnan().all()), (float(s[r]), sign)
+                else:
+                    assert bool(((got[r] - value).abs() <= tol).all()), (float(s[r]), sign)
+
+
+@pytest.mark.parametrize("L", [1, 40])
+def test_scores_past_the_range_of_32_bits(cuda, L):
+    """Below it a row is not seen; above it the token is NaN."""
+    D = 64
+    _, v = draw(L, 1, D, D, 3)
+    ks = torch.full((L, 1), 2.0 ** 127 / 1.4426950408889634)
+    q = torch.zeros(L, 4, D, dtype=BF16)
+    q[..., 0] = 8.0
+    for sign in (1, -1):
+        kc = torch.zeros(L, 1, D, dtype=torch.int8)
+        kc[:, :, 0] = 100 * sign
+        got = Cache([((kc, ks), v)], 16, cuda)(q, [L], scale=1.0)
+        assert bool((got.isnan() if sign > 0 else got == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D, V", [(64, 64), (192, 128)])
+def test_bits_of_far_scores(cuda, dtype, D, V, monkeypatch):
+    """Scores of 2^22 to 2^28, a few steps of 32 bits apart: split, whole and whole over
+    rows laid out, the same bits."""
+    n, H, Hkv = 700, 8, 2
+    g = torch.Generator().manual_seed(1)
+    q = torch.zeros(600, H, D, dtype=dtype)
+    q[..., 0] = 8.0
+    q = q.to(cuda)
+    for power in range(22, 28):
+        for sign in (1, -1):
+            c = 2.0 ** power * (1 + torch.rand(1, Hkv, generator=g)) / 800
+            c = c * (1 + torch.randint(-3, 1, (n, Hkv), generator=g) * 2.0 ** -23)
+            c[torch.rand(n, Hkv, generator=g) < 0.01] *= 1 + 2.0 ** -23 * sign
+            kc = torch.zeros(n, Hkv, D, dtype=torch.int8)
+            kc[..., 0] = 100 * sign
+            cache = Cache([((kc, c / 1.4426950408889634), draw(n, Hkv, D, V, power)[1])], 16, cuda)
+            base = cache(q, [600], scale=1.0)
+            one = cache(q[:1], [1], scale=1.0)
+            assert bool(base.isfinite().all())
+            assert same(base[-1:], one), (power, sign)
+            with monkeypatch.context() as m:
+                m.setattr(_paged, "_workspace", lambda need, device: None)
+                assert same(cache(q, [600], scale=1.0), base), (power, sign)
+                assert same(cache(q[:1], [1], scale=1.0), one), (power, sign)
