@@ -56,8 +56,12 @@ struct Args {
   uint32_t k8b, k8n, v8b, v8n, ksb, ksn, vsb, vsn;
   int64_t ksh, vsh;
   Div eight;              // 8 * Hkv where a row's heads are next to each other, else 0
-  char* laid;             // steps of (request, kv head), `units` each, as they lie in LDS
-  int32_t units;
+  // Steps of (request, kv head) as they lie in LDS, `room` in all: `units` to each, or,
+  // with `laid_at`, what a request walks from step laid_at[r] on, where it is not
+  // negative (then there was no room).
+  char* laid;
+  int32_t* laid_at;
+  int32_t units, room;
 };
 
 typedef void (*Kernel)(Args);

@@ -29,6 +29,9 @@ Kernels kernels(int64_t D, int64_t V, int dtype, bool q8) {
 constexpr int64_t kMost = (int64_t)1 << 29;
 // Workspaces are not larger.
 constexpr int64_t kMostBytes = (int64_t)1 << 32;
+// Rows that are laid out have a place for every row that a request may have where that
+// takes no more than this; else for as many as are expected, or as fit in this.
+constexpr int64_t kLaidBytes = (int64_t)1 << 27;
 
 // A call as the host knows it; `exact`: every request has max_query tokens.
 struct Call {
@@ -40,12 +43,15 @@ struct Call {
 // How a call is split: the columns up to which a request is (0: none), columns
 // kept per request and kv head, columns per workgroup, segments, workgroups for
 // these, and the bytes of the partial results. Of the others' rows that are laid
-// out (a cache of 8 bits): the steps of a request, and the bytes, 0 for none.
+// out (a cache of 8 bits): the steps of a request, those that one walks at most,
+// places for all (0: `units` for each), and the bytes, 0 for none.
 struct Plan {
-  int64_t split_cols, ccap, nc, nseg, gseg, bytes, units, laid;
+  int64_t split_cols, ccap, nc, nseg, gseg, bytes, units, walked, room, laid;
   int64_t laid_at() const { return (bytes + 15) / 16 * 16; }
   int64_t workspace() const { return laid ? laid_at() + laid : bytes; }
 };
+// Bytes of a note for each request where its steps are.
+int64_t notes(int64_t R) { return (4 * R + 511) / 512 * 512; }
 
 // Column tiles of all requests that can have a token (one of each request is
 // not full).
@@ -137,7 +143,17 @@ Plan plan(const Call& c, const Kernels& k) {
     const double laid = (cut && part < seq ? part : seq) * (requests < 1.0 ? 1.0 : requests < c.R ? requests : c.R);
     const double us = walk_us(k.laid_row_us, k.laid_tile_us) + 4.0 + laid * c.Hkv * (c.D + c.V) * 3.0 / 4e6;
     lay.units = (c.max_seq + k.step - 1) / k.step;
-    const double bytes = (double)c.R * (double)(c.Hkv * lay.units * k.step_bytes);
+    double bytes = (double)c.R * (double)(c.Hkv * lay.units * k.step_bytes);
+    if (bytes > (double)kLaidBytes) {
+      // As if the tokens were of requests with max_query each: 64 requests of up to 8192
+      // rows, of which one brings a chunk, would have places for all of theirs in 2.2 GB.
+      const int64_t most = (c.max_query + c.window + c.first) / k.step + 4;  // (a window's ends, the first tokens')
+      lay.walked = c.window && most < lay.units ? most : lay.units;
+      const int64_t n = c.tokens / c.max_query + (c.tokens % c.max_query != 0), each = c.Hkv * lay.walked;
+      const double least = (double)(kLaidBytes / k.step_bytes), some = (double)(n < c.R ? n : c.R) * (double)each;
+      const double room = some > least ? some : least, some_bytes = room * k.step_bytes + (double)notes(c.R);
+      if (some_bytes < bytes) bytes = some_bytes, lay.room = bytes <= (double)kMostBytes ? (int64_t)room : 0;
+    }
     if (us < whole && bytes <= (double)kMostBytes) {
       whole = us;
       lay.laid = (int64_t)bytes;
@@ -146,7 +162,8 @@ Plan plan(const Call& c, const Kernels& k) {
     }
   }
   auto beside = [&](Plan s) {
-    if (cols > s.split_cols && s.bytes + lay.laid <= kMostBytes) s.units = lay.units, s.laid = lay.laid;
+    if (cols > s.split_cols && s.bytes + lay.laid <= kMostBytes)
+      s.units = lay.units, s.walked = lay.walked, s.room = lay.room, s.laid = lay.laid;
     return s;
   };
   auto split = [&](const Plan& s) {
@@ -258,14 +275,29 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
     if (s.laid && whole) {
       p.laid = static_cast<char*>(ws) + s.laid_at();
       p.units = (int32_t)s.units;
-      const int64_t all = (int64_t)p.R * p.Hkv.d * s.units, most_groups = 8 * (int64_t)cus;
-      hipLaunchKernelGGL(k.lay, dim3((unsigned)(all < most_groups ? all : most_groups)), dim3(256), 0, st, p);
+      p.room = (int32_t)(s.room ? s.room : (int64_t)p.R * p.Hkv.d * s.units);
+      if (s.room) {
+        p.laid_at = reinterpret_cast<int32_t*>(p.laid);
+        p.laid += notes(p.R);
+      }
+      const int64_t most_groups = 8 * (int64_t)cus;
+      hipLaunchKernelGGL(k.lay, dim3((unsigned)(p.room < most_groups ? p.room : most_groups)), dim3(256), 0, st, p);
       if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
     }
     const Kernel whole4 = s.laid ? k.laid4 : k.whole4;
     hipLaunchKernelGGL(eight ? whole8 : pair ? k.whole4_pair : whole4, dim3((unsigned)blocks),
                        dim3(eight || s.laid ? 512 : pair ? 256 : k.whole4_threads), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+    // Requests for whose rows there may be no room, each of which has more than
+    // split_cols columns (a launch that finds nothing takes some 4 us).
+    const int64_t least = s.split_cols / p.G.d + 1, n = p.T / least < p.R ? p.T / least : p.R;
+    if (p.laid_at && n * p.Hkv.d * s.walked > s.room) {
+      p.fill_blocks = 0;
+      const int64_t rest = (cols / 128 + (p.T < p.R ? p.T : p.R)) * p.Hkv.d;
+      if (rest > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
+      hipLaunchKernelGGL(k.whole4, dim3((unsigned)rest), dim3(k.whole4_threads), 0, st, p);
+      if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
+    }
   }
   return BI_OK;
 }

@@ -388,6 +388,11 @@ __device__ __forceinline__ void feed_ahead(const Read& read, const Use& use) {
   }
 }
 
+// barrier(), N instruction words behind a multiple of the 32 bytes that are fetched at a
+// time (behind s_nop 0).
+template <int N> __device__ __forceinline__ void barrier_at() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\t.p2align 5\n\t.fill %0, 4, 0xbf800000\n\ts_barrier" ::"i"(N) : "memory");
+}
 __device__ __forceinline__ uint2 ld8(const void* p) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   typedef __attribute__((address_space(1))) const u32x2 gvec;
@@ -698,7 +703,9 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
 // way to eight of 16 as well). It costs a launch and three bytes of traffic a code:
 // 12 us for these rows, and 8 requests of 64 tokens over 4000 rows would take 166 us
 // for 116, so the host compares. The list of what is to do, steps of requests that are
-// not split, is the same for all workgroups, which take from it in turn.
+// not split, is the same for all workgroups, which take from it in turn. Where not
+// every step of every request can have a place, requests have theirs one behind the
+// other, as far as there is room, and the first workgroup notes where.
 template <typename T, int D, int V>
 __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
@@ -710,11 +717,16 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
   int next = blockIdx.x, before = 0;
   for (int r0 = 0; r0 < p.R; r0 += 256) {
     int sum = 0;
+    bool whole = false;
     if (r0 + tid < p.R) {
       const Request rq = request(p, r0 + tid);
-      if (!rq.beyond && rq.L * (int)p.G.d > p.split_cols)
-        sum = walk(p, rq.n - rq.L, rq.n - 1, S).count() * (int)p.Hkv.d;
+      whole = !rq.beyond && rq.L * (int)p.G.d > p.split_cols;
+      if (whole) {
+        const int n = walk(p, rq.n - rq.L, rq.n - 1, S).count();
+        sum = n > p.room / p.Hkv ? p.room + 1 : n * (int)p.Hkv.d;
+      }
     }
+    const int own = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int y = __shfl_up(sum, d);
@@ -726,6 +738,8 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
     for (int i = 0; i < 4; i++)
       if (i < wave) sum += s_scan[i];
     s_end[tid] = before + sum;
+    if (p.laid_at && blockIdx.x == 0 && r0 + tid < p.R)
+      p.laid_at[r0 + tid] = whole && before + sum <= p.room ? before + sum - own : -1;
     __syncthreads();
     const int end = s_end[255];
     for (; next < end; next += gridDim.x) {
@@ -733,12 +747,15 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
 #pragma unroll
       for (int d = 128; d; d >>= 1)
         if (s_end[a + d - 1] <= next) a += d;
-      const int r = r0 + a, at = next - (a ? s_end[a - 1] : before);
+      if (s_end[a] > p.room) break;
+      const int r = r0 + a, start = a ? s_end[a - 1] : before, at = next - start;
       const int i = at / p.Hkv, kvh = at - i * (int)p.Hkv.d;
       const Request rq = request(p, r);
       const int32_t lo = rq.n - rq.L, hi = rq.n - 1;
-      const int unit = walk(p, lo, hi, S).unit(i);
-      char* to = p.laid + ((int64_t)(r * (int)p.Hkv.d + kvh) * p.units + unit) * (G8::IU * 16);
+      const Walk w = walk(p, lo, hi, S);
+      const int unit = w.unit(i);
+      const int to_step = p.laid_at ? start + kvh * w.count() + i : (r * (int)p.Hkv.d + kvh) * p.units + unit;
+      char* to = p.laid + (int64_t)to_step * (G8::IU * 16);
       if (wave == 0) {
         const int32_t key = unit * S + lane;
         const int32_t id = any_seen(p, lo, hi, key, 1) ? page_of(p, r, entry_of(p, r, key), key) : -1;
@@ -777,7 +794,7 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
       }
       __syncthreads();
     }
-    before = end;
+    before = end <= p.room ? end : p.room + 1;
     __syncthreads();
   }
 }
@@ -861,6 +878,8 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
   tile = s_scan[NW + LW + 1];
   r = __builtin_amdgcn_readfirstlane(r);
   tile = __builtin_amdgcn_readfirstlane(tile);
+  // (With rows laid out as far as there is room: the others' by a launch of their own.)
+  if (p.laid_at && (p.laid_at[r] >= 0) != LAID) return;
   const Request rq = request(p, r);
   const int ncol = rq.L * (int)p.G.d;
   const int c0 = tile * COLS, cw = c0 + WC * wave;
@@ -987,9 +1006,19 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
 
   // LAID: a step's way into LDS, NB - 1 steps ahead.
   constexpr int MU = KU + VU + 2 * G8::FU + 1, NL = (MU + NT - 1) / NT;  // units that are wanted
-  const char* laid = LAID ? p.laid + (int64_t)(r * (int)p.Hkv.d + kvh) * p.units * (IU * 16) : nullptr;
+  const char* laid = nullptr;
+  Walk place = w;
+  if constexpr (LAID) {
+    int start = (r * (int)p.Hkv.d + kvh) * p.units;
+    if (p.laid_at) {  // (only what the request walks has a place)
+      const Walk all = walk(p, p0, rq.n - 1, S);
+      start = p.laid_at[r] + kvh * all.count();
+      place.b -= all.b - all.a;
+    }
+    laid = p.laid + (int64_t)start * (IU * 16);
+  }
   auto fetch = [&](int j) __attribute__((always_inline)) {
-    const char* from = laid + (uint64_t)(uint32_t)w.unit(j) * (IU * 16);
+    const char* from = laid + (uint64_t)(uint32_t)place.unit(j) * (IU * 16);
     uint4* to = s_kv + j % NB * IU + 64 * wave;
 #pragma unroll
     for (int i = 0; i < NL; i++)
@@ -1027,6 +1056,13 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
         return;
       }
   }
+  // (Where the loop's instructions lie within the 32 bytes that are fetched at a time: the
+  // same ones take, 128 dims, by the place of the step's barrier 221 to 230 us laid out in
+  // 128 columns, for 512 tokens over 8192 rows, in 256 463 to 475, for 4096, and not laid
+  // out 407 to 421, for 4 requests of 512. In 256 columns instructions that do nothing
+  // cost as much within the loop: there they are before it. 64 and 256 dims gain nothing.)
+  constexpr bool kPlaced = D == 128 && V == 128;
+  if constexpr (kPlaced && LAID && CT == 2) asm volatile(".p2align 5\n\t.fill 2, 4, 0xbf800000");
   for (int j = 0; j < steps; j++) {
     const uint32_t ln = opaque(lane);
     const int g = ln >> 4;
@@ -1034,7 +1070,9 @@ __global__ void __launch_bounds__(64 * (NW + LW), (Geo8<T, D, V>::kTwoWaves || N
       if (j + NB - 2 < steps) wait_loads_but<(MU / NT) * (NB - 2)>();
       else wait_loads();
     }
-    barrier();  // step j is there, and everyone is done with step j - 1's buffer
+    // Step j is there, and everyone is done with step j - 1's buffer.
+    if constexpr (kPlaced && !(LAID && CT == 2)) barrier_at<LAID ? 0 : 3>();
+    else barrier();
     if constexpr (LAID) {
       if (j + NB - 1 < steps) fetch(j + NB - 1);
     } else if constexpr (LW == 0) {

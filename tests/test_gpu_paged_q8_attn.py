@@ -700,3 +700,52 @@ def test_bits_of_far_scores(cuda, dtype, D, V, monkeypatch):
                 m.setattr(_paged, "_workspace", lambda need, device: None)
                 assert same(cache(q, [600], scale=1.0), base), (power, sign)
                 assert same(cache(q[:1], [1], scale=1.0), one), (power, sign)
+
+
+@pytest.mark.parametrize("D, V, seq, window, first", [(256, 256, 2200, 0, 0), (64, 64, 8192, 0, 0),
+                                                      (128, 128, 8192, 2500, 3), (192, 128, 4000, 0, 0)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_more_rows_than_there_is_room_for(cuda, D, V, seq, window, first, dtype, monkeypatch):
+    """64 requests, most with more tokens than are split, one with a chunk: laid out as
+    far as there is room, the others as without, and the bits of a call without any."""
+    R, H, Hkv, page = 64, 16, 4, 64
+    g = torch.Generator(device=cuda).manual_seed(D + window)
+    width = -(-seq // page)
+    codes = lambda d: torch.randint(-127, 128, (R * width, Hkv, page, d), generator=g, device=cuda, dtype=torch.int8)
+    scales = lambda: torch.exp(torch.randn(R * width, Hkv, page, generator=g, device=cuda)) / 40
+    kc, vc, ks, vs = codes(D), codes(V), scales() / 10, scales()
+    table = torch.randperm(R * width, generator=g, device=cuda).to(torch.int32).view(R, width)
+    table[3, 5] = -1
+    new = [1 if r % 5 == 0 else 0 if r % 7 == 3 else 600 if r == 11 else 20 for r in range(R)]
+    lens = [seq - 37 * (r % 9) if r % 4 else 500 + 30 * r for r in range(R)]
+    lens[2] = 7  # fewer rows than tokens: some see nothing
+    seqs = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    q = torch.randn(sum(new), H, D, generator=g, device=cuda).to(dtype)
+    most = []
+
+    def limited(limit, **kw):
+        def workspace(need, device):
+            most.append(need)
+            n = min(need, limit)
+            return torch.full((n,), 0xff, dtype=torch.uint8, device=device) if n else None
+        monkeypatch.setattr(_paged, "_workspace", workspace)
+        return bi.paged_attention(q, kc, vc, table, starts(new, cuda), seqs, k_scales=ks, v_scales=vs, max_query=600,
+                                  max_seq=seq, window=window or None, sink_tokens=first, **kw)
+
+    full = limited(1 << 40)
+    beyond = torch.cat([torch.full((n,), lens[r] > seq) for r, n in enumerate(new)])  # (of 2200 rows one is)
+    assert bool((full.isnan().cpu() == beyond[:, None, None]).all())
+    laid = laid_bytes(1, 1, D, V, 64)
+    nseg = -(-seq // 512)
+    if window:
+        nseg = min(nseg, (window + 15 // 4 + 1 + 510) // 512 + 1 + 1)  # (ends, and the first rows)
+    room = most[0] - R * Hkv * 32 * nseg * (V + 2) * 4
+    assert (1 << 27) - laid < room <= (1 << 27) + 512, (most[0], room)
+    assert same(limited(0), full) and same(limited(most[0] - 1), full)
+    # Rows beyond a bound, and a request alone in its place.
+    bound = limited(1 << 40)
+    assert same(bound, full)
+    t = sum(new[:11])
+    one = bi.paged_attention(q[t:t + 600], kc, vc, table[11:12], starts([600], cuda), seqs[11:12], k_scales=ks,
+                             v_scales=vs, window=window or None, sink_tokens=first)
+    assert same(one, full[t:t + 600])

@@ -289,3 +289,19 @@ def test_scoring_refusals_and_caches():
     turned = decoder.Decoder(decoder.DecoderConfig(hidden=64, inter=64, heads=2, kv_heads=1, head_dim=64, layers=1,
                                                    vocab=16, rope_base=100.0, rope_dim=8), "cpu", torch.float32)
     assert turned.inv_freq.tolist() == bi.rotary_frequencies(8, 100.0, device="cpu").tolist()
+
+
+def test_attention_workspace_of_one_chunk_among_many():
+    """Rows laid out where one of 64 requests of up to 8192 rows brings a chunk: no more
+    than 128 MiB beside the partial results, not a place for every row of all."""
+    step = -(-(64 * 4 * 128 + 512 + 16) // 512) * 512
+    ws = lambda T, R, most, longest=8192, window=0: _lib.lib().bi_paged_attention_q8_workspace(
+        T, R, 32, 8, 128, 128, window, 0, most, longest, _lib.BF16)
+    part = lambda R: R * 8 * 32 * 16 * 130 * 4  # 32 columns, 16 segments
+    assert part(64) < ws(1063, 64, 1000) <= part(64) + (1 << 27) + 512
+    # Requests that all bring a chunk have places for what they walk.
+    n = ws(64 * 1000, 64, 1000)
+    assert n == 64 * 8 * 128 * step
+    n = ws(64 * 1000, 64, 1000, window=1000)
+    assert 64 * 8 * 34 * step <= n <= 64 * 8 * 36 * step
+    assert ws(4 * 1000, 4, 1000) == 4 * 8 * 128 * step  # within 128 MiB and more: as many as there are
