@@ -378,6 +378,13 @@ int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t H, int64_t
                                         int64_t V, int64_t window, int64_t sink_tokens,
                                         int64_t max_query, int64_t max_seq, int dtype);
 
+/* Of these, the bytes without which single tokens are computed as slowly as chunks
+ * (the rest holds rows laid out); 0 if there are none. */
+int64_t bi_paged_attention_q8_least_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
+                                              int64_t D, int64_t V, int64_t window,
+                                              int64_t sink_tokens, int64_t max_query,
+                                              int64_t max_seq, int dtype);
+
 /*
  * Rotary positions: pair i of every head of token t turns by the angle
  * positions[t] * inv_freq[i], (x, y) -> scale * (x cos - y sin, x sin + y cos).

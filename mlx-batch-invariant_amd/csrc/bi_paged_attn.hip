@@ -457,16 +457,32 @@ extern "C" int bi_paged_attention_q8(const void* q, const int8_t* k_cache, const
                          true, workspace, workspace_bytes, hip_stream);
 }
 
-extern "C" int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
-                                                int64_t D, int64_t V, int64_t window,
-                                                int64_t sink_tokens, int64_t max_query,
-                                                int64_t max_seq, int dtype) {
+namespace {
+
+Plan q8_plan(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t V, int64_t window,
+             int64_t sink_tokens, int64_t max_query, int64_t max_seq, int dtype) {
   if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || H > 65535 || H % Hkv || (dtype != BI_F16 && dtype != BI_BF16) ||
       !dims_built(D, V) || T > kMost || R > kMost || window < 0 || sink_tokens < 0)
-    return 0;
+    return Plan{};
   const Call c = {R, T, H / Hkv, Hkv, D, V, clamp32(window), clamp32(sink_tokens), clamp32(max_query),
                   clamp32(max_seq), false, 1.0};
-  return plan(c, kernels(D, V, dtype, true)).workspace();
+  return plan(c, kernels(D, V, dtype, true));
+}
+
+}  // namespace
+
+extern "C" int64_t bi_paged_attention_q8_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
+                                                   int64_t D, int64_t V, int64_t window,
+                                                   int64_t sink_tokens, int64_t max_query,
+                                                   int64_t max_seq, int dtype) {
+  return q8_plan(T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dtype).workspace();
+}
+
+extern "C" int64_t bi_paged_attention_q8_least_workspace(int64_t T, int64_t R, int64_t H, int64_t Hkv,
+                                                         int64_t D, int64_t V, int64_t window,
+                                                         int64_t sink_tokens, int64_t max_query,
+                                                         int64_t max_seq, int dtype) {
+  return q8_plan(T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dtype).bytes;
 }
 
 extern "C" int bi_window_attention(const void* q, const void* k, const void* v, const void* sinks,

@@ -55,6 +55,7 @@ SIGNATURES = {
     "bi_paged_attention_q8": (_c_int, [_c_vp] * 10 + [_c_i64] * 9 + [_c_i64p, _c_i64p, _c_float]
                               + [_c_i64] * 4 + [_c_int, _c_vp, _c_i64, _c_vp]),
     "bi_paged_attention_q8_workspace": (_c_i64, [_c_i64] * 10 + [_c_int]),
+    "bi_paged_attention_q8_least_workspace": (_c_i64, [_c_i64] * 10 + [_c_int]),
     "bi_rotary": (_c_int, [_c_vp] * 6 + [_c_i64] * 6 + [_c_i64p, _c_float, _c_int, _c_int, _c_vp]),
     "bi_token_logprobs": (_c_int, [_c_vp] * 6 + [_c_i64] * 4 + [_c_int, _c_int, _c_vp]),
     "bi_gemm_num_geometries": (_c_int, []),

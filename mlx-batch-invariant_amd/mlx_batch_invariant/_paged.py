@@ -486,8 +486,12 @@ def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_q
     st = _I64x9(qt, qh, kp, kh, kn, vp, vh, vn, _table(block_tables))
     dt = _lib.DTYPE_CODES[q.dtype]
     if k_scales is not None:
-        need = _paged_q8_bytes(dev, T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt)
+        sizes = T, R, H, Hkv, D, V, window, sink_tokens, max_query, max_seq, dt
+        need = _paged_q8_bytes(dev, *sizes)
         ws = _workspace(need, dev)
+        if need and ws is None:  # the partial results alone, where rows were to be laid out
+            least = _lib.lib().bi_paged_attention_q8_least_workspace(*sizes)
+            ws = _workspace(least, dev) if least < need else None
         sst = _I64x6(*k_scales.stride(), *v_scales.stride())
         _call(dev, "bi_paged_attention_q8", _lib.lib().bi_paged_attention_q8, q.data_ptr(), ka, va,
               k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(),

@@ -749,3 +749,29 @@ def test_more_rows_than_there_is_room_for(cuda, D, V, seq, window, first, dtype,
     one = bi.paged_attention(q[t:t + 600], kc, vc, table[11:12], starts([600], cuda), seqs[11:12], k_scales=ks,
                              v_scales=vs, window=window or None, sink_tokens=first)
     assert same(one, full[t:t + 600])
+
+
+def test_partial_results_without_memory_for_rows_laid_out(cuda, monkeypatch):
+    """Where the workspace cannot be had, what of it single tokens need is asked for."""
+    lens, new = [3000, 900, 2500, 40], [1, 1, 900, 1]
+    kv = [draw(n, 2, 128, 128, 30 + i) for i, n in enumerate(lens)]
+    cache = Cache(kv, 16, cuda)
+    q = queries(sum(new), 8, 128, BF16, 6)
+    run = lambda: cache(q, new, max_query=900, max_seq=3000)
+    full, asked, real = run(), [], _paged._workspace
+
+    def scarce(need, device):
+        asked.append(need)
+        return real(need, device) if len(asked) > 1 else None
+
+    monkeypatch.setattr(_paged, "_workspace", scarce)
+    assert same(run(), full)
+    part = 4 * 2 * 32 * -(-3000 // 512) * 130 * 4  # 32 columns of each request
+    assert asked == [part + laid_bytes(4, 2, 128, 128, 3000), part]
+    asked.clear()
+
+    def none(need, device):
+        asked.append(need)
+
+    monkeypatch.setattr(_paged, "_workspace", none)
+    assert same(run(), full) and len(asked) == 2

@@ -305,3 +305,15 @@ def test_attention_workspace_of_one_chunk_among_many():
     n = ws(64 * 1000, 64, 1000, window=1000)
     assert 64 * 8 * 34 * step <= n <= 64 * 8 * 36 * step
     assert ws(4 * 1000, 4, 1000) == 4 * 8 * 128 * step  # within 128 MiB and more: as many as there are
+
+
+def test_attention_least_workspace():
+    """The partial results alone, and nothing where there are none."""
+    def ws(T, R, most, least=True, **kw):
+        f = _lib.lib().bi_paged_attention_q8_least_workspace if least else _lib.lib().bi_paged_attention_q8_workspace
+        return f(T, R, 32, 8, 128, 128, 0, 0, most, 8192, kw.get("dtype", _lib.F16))
+
+    assert ws(1063, 64, 1000) == 64 * 8 * 32 * 16 * 130 * 4 < ws(1063, 64, 1000, False)
+    assert ws(64, 64, 1) == ws(64, 64, 1, False) > 0
+    assert ws(4096, 1, 4096) == 0 < ws(4096, 1, 4096, False)
+    assert ws(4096, 1, 4096, dtype=_lib.F32) == ws(0, 1, 1) == 0
