@@ -504,7 +504,7 @@ def _paged_eager(q, k_cache, v_cache, block_tables, query_start, seq_lens, max_q
     _call(dev, "bi_paged_attention", _lib.lib().bi_paged_attention, q.data_ptr(), ka, va,
           block_tables.data_ptr(), query_start.data_ptr(), seq_lens.data_ptr(), _at(sinks),
           out.data_ptr(), T, R, H, Hkv, D, V, P, page, W, st, scale, window, sink_tokens,
-          max_query, max_seq, dt, _at(ws), 0 if ws is None else need)
+          max_query, max_seq, dt, _at(ws), 0 if ws is None else ws.numel())
     return out
 
 
@@ -549,5 +549,5 @@ def _window_eager(q, k, v, scale, window, sink_tokens, sinks):
     ws = _workspace(need, dev)
     _call(dev, "bi_window_attention", _lib.lib().bi_window_attention, q.data_ptr(), k.data_ptr(),
           v.data_ptr(), _at(sinks), out.data_ptr(), B, H, Hkv, qL, N, D, V, st, scale, window,
-          sink_tokens, dt, _at(ws), 0 if ws is None else need)
+          sink_tokens, dt, _at(ws), 0 if ws is None else ws.numel())
     return out

@@ -176,3 +176,27 @@ def test_sharp_scores_in_32_bits(cuda, D, V, H, Hkv, n, L, window, first, sharp)
     want, tol = ref.rows(q, k, v, n, window or 0, first, 5.0, None)
     err = (got[0].transpose(0, 1).double().cpu() - want).abs()
     assert bool((err <= tol).all()), (err / tol).max()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_smaller_workspace_gives_the_same_bits(cuda, dtype, monkeypatch):
+    """Paged and windowed attention with fewer bytes than they ask for, and with none."""
+    from mlx_batch_invariant import _paged
+
+    g = torch.Generator(device=cuda).manual_seed(4)
+    k, v = (torch.randn(1, 2, 3000, 64, generator=g, device=cuda).to(dtype) for _ in range(2))
+    q = torch.randn(3, 8, 64, generator=g, device=cuda).to(dtype)
+    table = torch.arange(30, dtype=torch.int32, device=cuda)[None]
+    pages = [t.view(2, 30, 100, 64).transpose(0, 1).contiguous() for t in (k, v)]
+    paged = lambda: bi.paged_attention(q, *pages, table, i32([0, 3], cuda), i32([3000], cuda))
+    whole = lambda: bi.window_attention(q.transpose(0, 1)[None], k, v, None)
+    want, asked = (paged(), whole()), []
+    for part in (lambda n: n - 1, lambda n: n // 2, lambda n: 0):
+        def workspace(need, device):
+            asked.append(need)
+            return torch.empty(part(need), dtype=torch.uint8, device=device)
+
+        monkeypatch.setattr(_paged, "_workspace", workspace)
+        assert bool((as_int(paged()) == as_int(want[0])).all())
+        assert bool((as_int(whole()) == as_int(want[1])).all())
+    assert min(asked) > 0

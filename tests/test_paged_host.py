@@ -200,3 +200,27 @@ def test_decoder_cache_refusals():
                                   ([torch.zeros(2).long()], 0, None), ([torch.zeros(2).long()], 1, 0)):
         with pytest.raises(ValueError):
             decoder.generate(None, prompts, steps, chunk)
+
+
+def test_the_library_is_told_the_workspace_that_there_is(monkeypatch):
+    """A workspace of fewer bytes than were asked for is passed on as what it is."""
+    from mlx_batch_invariant import _paged
+
+    calls = []
+    monkeypatch.setattr(_paged, "_on_one_gpu", lambda *a: None)
+    monkeypatch.setattr(_paged, "_call", lambda dev, what, fn, *args: calls.append((what, args[-2:])))
+    monkeypatch.setattr(_paged, "_workspace", lambda need, device: torch.empty(need // 2, dtype=torch.uint8))
+    q, lens = torch.zeros(1, 4, 64, dtype=torch.float16), torch.tensor([5000], dtype=torch.int32)
+    start, table = torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, 320, dtype=torch.int32)
+    kc, codes = torch.zeros(4, 2, 16, 64).half(), torch.zeros(4, 2, 16, 64, dtype=torch.int8)
+    scales = torch.zeros(4, 2, 16)
+    bi.paged_attention(q, kc, kc, table, start, lens)
+    bi.paged_attention(q, codes, codes, table, start, lens, k_scales=scales, v_scales=scales)
+    k = torch.zeros(1, 2, 5000, 64).half()
+    bi.window_attention(q.view(1, 4, 1, 64), k, k, None)
+    ask = _lib.lib()
+    sizes = (1, 1, 4, 2, 64, 64, 0, 0, 1, 5120, _lib.F16)
+    need = (ask.bi_paged_attention_workspace(*sizes), ask.bi_paged_attention_q8_workspace(*sizes),
+            ask.bi_window_attention_workspace(1, 4, 2, 1, 5000, 64, 64, 0, 0, _lib.F16))
+    assert min(need) > 0
+    assert [b for _, (_, b) in calls] == [n // 2 for n in need], [w for w, _ in calls]
