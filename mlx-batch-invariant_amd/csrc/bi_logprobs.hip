@@ -277,15 +277,27 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 8 : 6) logprobs_kernel(Logpro
   }
 }
 
-template <typename T> int start(const LogprobArgs& p, int64_t rows, hipStream_t st) {
+// Rows of a launch: its threads are counted in 32 bits, and of those that pass them it
+// starts the rest of a division by 2^32, without an error.
+constexpr int64_t kMostRows = 1 << 21;
+
+template <typename T> int start(LogprobArgs p, int64_t rows, hipStream_t st) {
   constexpr int U = 16 / sizeof(T), NU = 32 / U;
-  const dim3 grid((unsigned)rows);
-  // By the row's length alone, so that its bits are the same in every call.
-  if (p.V <= 256 * 32) hipLaunchKernelGGL((logprobs_kernel<T, 256, NU, true>), grid, dim3(256), 0, st, p);
-  else if (p.V <= 1024 * 32) hipLaunchKernelGGL((logprobs_kernel<T, 1024, NU, true>), grid, dim3(1024), 0, st, p);
-  else hipLaunchKernelGGL((logprobs_kernel<T, 1024, NU, false>), grid, dim3(1024), 0, st, p);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? BI_OK : bi::launch_error(e, "bi_token_logprobs launch");
+  for (;;) {
+    const int64_t n = rows < kMostRows ? rows : kMostRows;
+    const dim3 grid((unsigned)n);
+    // By the row's length alone, so that its bits are the same in every call.
+    if (p.V <= 256 * 32) hipLaunchKernelGGL((logprobs_kernel<T, 256, NU, true>), grid, dim3(256), 0, st, p);
+    else if (p.V <= 1024 * 32) hipLaunchKernelGGL((logprobs_kernel<T, 1024, NU, true>), grid, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((logprobs_kernel<T, 1024, NU, false>), grid, dim3(1024), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return bi::launch_error(e, "bi_token_logprobs launch");
+    if ((rows -= n) == 0) return BI_OK;
+    p.logits = static_cast<const T*>(p.logits) + n * p.stride;
+    p.tokens = static_cast<const char*>(p.tokens) + n * (p.wide_tokens ? 8 : 4);
+    p.logprobs += n, p.entropy += n;
+    if (p.top) p.top_ids += n * p.top, p.top_logprobs += n * p.top;
+  }
 }
 
 }  // namespace

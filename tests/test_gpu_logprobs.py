@@ -179,3 +179,27 @@ def test_compiles(cuda):
     got = torch.compile(fn, fullgraph=True, backend="aot_eager")(x, t)
     for a, b in zip(got, fn(x, t)):
         assert bool((bits(a) == bits(b)).all())
+
+
+@pytest.mark.parametrize("rows, V", [((1 << 24) + 3, 2), ((1 << 22) + 3, 8193)])
+def test_more_rows_than_one_launch_takes(cuda, rows, V):
+    """Rows of 256 and of 1024 threads, 2^32 and more in all; the same row at a stride of 0."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(1, V, generator=g).to(BF16).to(cuda)
+    t = torch.arange(rows, device=cuda) % V
+    top = 1
+    got = bi.token_logprobs(x.expand(rows, V), t, top=top)
+    one = bi.token_logprobs(x.expand(V, V), t[:V], top=top)
+    check(one, x.expand(V, V), t[:V], top)
+    assert bool((got.logprobs.view(torch.int32) == one.logprobs[t].view(torch.int32)).all())
+    assert bool((got.entropy == one.entropy[0]).all())
+    assert bool((got.top_ids == one.top_ids[0]).all()) and bool((got.top_logprobs == one.top_logprobs[0]).all())
+    # Rows of their own on both sides of a launch's end.
+    if V == 2:
+        y = torch.randn(rows, V, generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).to(F16)
+        got = bi.token_logprobs(y, t, top=2)
+        for a in (0, (1 << 21) - 40, (1 << 22) - 3, rows - 70):
+            part = slice(a, a + 70)
+            for z, w in zip(got, bi.token_logprobs(y[part], t[part], top=2)):
+                assert bool((z[part] == w).all())
+        check(got, y, t, 2)
