@@ -314,7 +314,7 @@ int launch(const void* a, const void* b, const void* bias, void* out, int64_t M,
   if (G.pl && !(v.a && v.b))
     return bi::fail(BI_EUNSUPPORTED, "bi_gemm: geometry %d takes 16-byte aligned operands only", g);
   const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-  if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "bi_gemm: too many tiles");
+  if (bi::grid_too_large(blocks, 64 * G.waves)) return bi::fail(BI_EINVAL, "bi_gemm: too many tiles");
   KernelFn fn = select_kernel(dtype, trans_b, g, !(v.a && v.b));
   if (!fn) return bi::fail(BI_EUNSUPPORTED, "bi_gemm: geometry %d not built for this dtype", g);
   if (start || stop)
@@ -503,7 +503,7 @@ int qlaunch_decode(const void* x, const void* w, const void* scales, const void*
   p.qz = biases;
   p.qgroup_shift = group_shift(group_size);
   const int64_t blocks = ceil_div(N, 16);
-  if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "bi_qgemm: too many tiles");
+  if (bi::grid_too_large(blocks, 64 * bi_gemm_dev::kQDecodeWaves)) return bi::fail(BI_EINVAL, "bi_qgemm: too many tiles");
   KernelFn fn = dtype == BI_F16 ? bi_qdecode_kernel_f16(group_size, (int)M, bits)
                                 : bi_qdecode_kernel_bf16(group_size, (int)M, bits);
   if (!fn) return bi::fail(BI_EUNSUPPORTED, "bi_qgemm: decode footprint not built");
@@ -542,7 +542,7 @@ int qlaunch(const void* x, const void* w, const void* scales, const void* biases
   p.qz = biases;
   p.qgroup_shift = group_shift(group_size);
   const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-  if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "bi_qgemm: too many tiles");
+  if (bi::grid_too_large(blocks, 64 * G.waves)) return bi::fail(BI_EINVAL, "bi_qgemm: too many tiles");
   KernelFn fn = select_qkernel(dtype, g, bits, group_size);
   if (!fn) return bi::fail(BI_EUNSUPPORTED, "bi_qgemm: geometry %d not built", g);
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(64 * G.waves), 0,

@@ -213,6 +213,40 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
   Plan s = plan(c, k);
   if (!ws || (uintptr_t)ws % 16 || ws_bytes < s.bytes) s = Plan{};
   if (ws_bytes < s.workspace()) s.laid = 0;
+  // What is walked whole.
+  const bool whole = most * p.G.d > s.split_cols;
+  // Eight waves share their keys' and values' loads and addresses where that
+  // leaves a workgroup for every compute unit and the walk is long (4096
+  // tokens over 8192 keys 476 us, 510 with two workgroups of four; 4096 alone
+  // 174 and 189). Over a short one a second workgroup, which starts while the
+  // first works, gains more: 2048 tokens alone 76 us with eight, 71 with
+  // twice four; 8192 under a window of 64 73 and 63, of 512 135 and 131, of
+  // 1024 197 and 201. With fewer columns four waves fill more (two chunks of
+  // 511 tokens beside 30 decodes 161 us, 175 with eight), two workgroups to a
+  // compute unit where there are more than these.
+  const int64_t cols = p.qstart ? (int64_t)p.T * p.G.d : (int64_t)p.R * p.qL * p.G.d;
+  const int cus = bi::device_cus();
+  // Rows that a tile walks, on average: 64 tokens see 63 more than the window.
+  const int64_t longest = p.qstart ? p.max_seq : p.N;
+  const int64_t seen = (int64_t)p.window + p.first + 63, causal = longest - most / 2;
+  const bool far = (p.window && seen < causal ? seen : causal) > 1024;
+  const Kernel whole8 = s.laid ? k.laid8 : k.whole8, whole4 = s.laid ? k.laid4 : k.whole4;
+  const bool eight = whole8 && far && cols / 256 * p.Hkv.d >= cus;
+  const bool pair = !eight && k.whole4_pair && cols / 128 * p.Hkv.d > cus;
+  const int64_t wc = eight ? 256 : 128, threads = eight || s.laid ? 512 : pair ? 256 : k.whole4_threads;
+  // Column tiles: every request with tokens may end in a part of one.
+  const int64_t requests = p.T < p.R ? p.T : p.R;
+  const int64_t tiles = !whole ? 0 : p.qstart ? cols / wc + requests
+                                              : (int64_t)p.R * (((int64_t)p.qL * p.G.d + wc - 1) / wc);
+  const int32_t fill = p.qstart && !s.split_cols ? 16 : 0;
+  const int64_t blocks = tiles * p.Hkv.d + fill;
+  // Of rows laid out, requests for which there may be no room, each of which has more
+  // than split_cols columns (a launch that finds nothing takes some 4 us).
+  const int64_t least = s.split_cols / p.G.d + 1, n = p.T / least < p.R ? p.T / least : p.R;
+  const bool more = whole && s.laid && s.room && n * p.Hkv.d * s.walked > s.room;
+  const int64_t rest = more ? (cols / 128 + requests) * p.Hkv.d : 0;
+  if (bi::grid_too_large(blocks, threads) || bi::grid_too_large(rest, k.whole4_threads))
+    return bi::fail(BI_EINVAL, "%s: grid too large", who);
   hipError_t e;
   if (s.split_cols) {
     p.split_cols = (int32_t)s.split_cols;
@@ -235,43 +269,14 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
     if (p.eight.d) grid = (grid / p.Hkv.d + 7) / 8 * 8 * p.Hkv.d;
     hipLaunchKernelGGL(split, dim3((unsigned)grid), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
-  }
-  const bool whole = most * p.G.d > s.split_cols;
-  p.fill_blocks = p.qstart ? 16 : 0;
-  if (s.split_cols) {
-    const int64_t cols = (int64_t)p.R * p.Hkv.d * p.cstep.d;
-    hipLaunchKernelGGL(k.combine, dim3((unsigned)((cols + 3) / 4 + p.fill_blocks)), dim3(256), 0,
+    p.fill_blocks = p.qstart ? 16 : 0;
+    const int64_t waves = (int64_t)p.R * p.Hkv.d * p.cstep.d;
+    hipLaunchKernelGGL(k.combine, dim3((unsigned)((waves + 3) / 4 + p.fill_blocks)), dim3(256), 0,
                        st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
-    p.fill_blocks = 0;
   }
-  if (whole || p.fill_blocks) {
-    // Eight waves share their keys' and values' loads and addresses where that
-    // leaves a workgroup for every compute unit and the walk is long (4096
-    // tokens over 8192 keys 476 us, 510 with two workgroups of four; 4096 alone
-    // 174 and 189). Over a short one a second workgroup, which starts while the
-    // first works, gains more: 2048 tokens alone 76 us with eight, 71 with
-    // twice four; 8192 under a window of 64 73 and 63, of 512 135 and 131, of
-    // 1024 197 and 201. With fewer columns four waves fill more (two chunks of
-    // 511 tokens beside 30 decodes 161 us, 175 with eight), two workgroups to a
-    // compute unit where there are more than these.
-    const int64_t cols = p.qstart ? (int64_t)p.T * p.G.d : (int64_t)p.R * p.qL * p.G.d;
-    const int cus = bi::device_cus();
-    // Rows that a tile walks, on average: 64 tokens see 63 more than the window.
-    const int64_t longest = p.qstart ? p.max_seq : p.N;
-    const int64_t seen = (int64_t)p.window + p.first + 63, causal = longest - most / 2;
-    const bool far = (p.window && seen < causal ? seen : causal) > 1024;
-    const Kernel whole8 = s.laid ? k.laid8 : k.whole8;
-    const bool eight = whole8 && far && cols / 256 * p.Hkv.d >= cus;
-    const bool pair = !eight && k.whole4_pair && cols / 128 * p.Hkv.d > cus;
-    const int64_t wc = eight ? 256 : 128;
-    // Column tiles: every request with tokens may end in a part of one.
-    int64_t tiles = p.qstart ? cols / wc + (p.T < p.R ? p.T : p.R)
-                             : (int64_t)p.R * (((int64_t)p.qL * p.G.d + wc - 1) / wc);
-    if (!whole) tiles = 0;
-    const int64_t blocks = tiles * p.Hkv.d + p.fill_blocks;
-    if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
-    if (blocks == 0) return BI_OK;
+  p.fill_blocks = fill;
+  if (blocks) {
     if (s.laid && whole) {
       p.laid = static_cast<char*>(ws) + s.laid_at();
       p.units = (int32_t)s.units;
@@ -284,17 +289,11 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
       hipLaunchKernelGGL(k.lay, dim3((unsigned)(p.room < most_groups ? p.room : most_groups)), dim3(256), 0, st, p);
       if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
     }
-    const Kernel whole4 = s.laid ? k.laid4 : k.whole4;
     hipLaunchKernelGGL(eight ? whole8 : pair ? k.whole4_pair : whole4, dim3((unsigned)blocks),
-                       dim3(eight || s.laid ? 512 : pair ? 256 : k.whole4_threads), 0, st, p);
+                       dim3((unsigned)threads), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
-    // Requests for whose rows there may be no room, each of which has more than
-    // split_cols columns (a launch that finds nothing takes some 4 us).
-    const int64_t least = s.split_cols / p.G.d + 1, n = p.T / least < p.R ? p.T / least : p.R;
-    if (p.laid_at && n * p.Hkv.d * s.walked > s.room) {
+    if (more) {
       p.fill_blocks = 0;
-      const int64_t rest = (cols / 128 + (p.T < p.R ? p.T : p.R)) * p.Hkv.d;
-      if (rest > INT32_MAX) return bi::fail(BI_EINVAL, "%s: grid too large", who);
       hipLaunchKernelGGL(k.whole4, dim3((unsigned)rest), dim3(k.whole4_threads), 0, st, p);
       if ((e = hipGetLastError()) != hipSuccess) return bi::launch_error(e, who);
     }

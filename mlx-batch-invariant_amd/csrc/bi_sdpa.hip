@@ -608,7 +608,7 @@ int sdpa_run(const void* q, const void* k, const void* v, const void* mask,
     if (!ws || (uintptr_t)ws % 16 || ws_bytes < sc.bytes)
       return bi::fail(BI_EINVAL, "bi_sdpa: the workspace needs %lld bytes, 16-byte aligned",
                       (long long)sc.bytes);
-    if (sc.blocks > INT32_MAX) return bi::fail(BI_EINVAL, "bi_sdpa: grid too large");
+    if (bi::grid_too_large(sc.blocks, kThreads)) return bi::fail(BI_EINVAL, "bi_sdpa: grid too large");
     if (shape == SDPA_ROWS) shape = SDPA_TILE;  // built for one column tile
     p.sc = static_cast<float*>(ws);
     p.nsc = sc.nsc;
@@ -636,12 +636,12 @@ int sdpa_run(const void* q, const void* k, const void* v, const void* mask,
     const int64_t ncol = (H / Hkv) * qL;
     blocks = B * Hkv * ((ncol + columns - 1) / columns) * splits;
   }
-  if (blocks > INT32_MAX) return bi::fail(BI_EINVAL, "bi_sdpa: grid too large");
   if (!fn)
     return bi::fail(BI_EINVAL, "bi_sdpa: launch shape %d is not built for this mask", shape);
   const int threads = dtype == BI_F32 || p.sc
                           ? kThreads
                           : sdpa_shape_threads(D, V, shape, mask_mode == BI_MASK_ARRAY);
+  if (bi::grid_too_large(blocks, threads)) return bi::fail(BI_EINVAL, "bi_sdpa: grid too large");
   hipError_t e;
   if (p.sc) {
     const SdpaKernelFn sfn = mfma_kernel(D, V, dtype, false, sc.tiles, SDPA_SCORES);
