@@ -160,13 +160,14 @@ extern "C" int bi_rotary(const void* q, const void* k, void* q_out, void* k_out,
   // operations for each sine and cosine), but fewer where that leaves the GPU
   // short of threads.
   int64_t per = 8;
+  if (T > (INT32_MAX - kThreads) / (items * ((H + Hkv + per - 1) / per)))
+    return bi::fail(BI_EINVAL, "%s: sizes too large", who);
   while (per > 1 && T * items * ((H + Hkv + per - 1) / per) < 256 * 1024) per /= 2;
   const int64_t groups = (H + Hkv + per - 1) / per;
   p.per = (int32_t)per;
   p.items = bi::make_div(items);
   p.groups = bi::make_div(groups);
   p.threads = T * groups * items;
-  if (p.threads > INT32_MAX - kThreads) return bi::fail(BI_EINVAL, "%s: sizes too large", who);
   const Kernel f = dtype == BI_F32 ? pick<float>(wide, interleaved)
                    : dtype == BI_F16 ? pick<_Float16>(wide, interleaved)
                                      : pick<__bf16>(wide, interleaved);

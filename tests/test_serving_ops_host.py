@@ -317,3 +317,14 @@ def test_attention_least_workspace():
     assert ws(64, 64, 1) == ws(64, 64, 1, False) > 0
     assert ws(4096, 1, 4096) == 0 < ws(4096, 1, 4096, False)
     assert ws(4096, 1, 4096, dtype=_lib.F32) == ws(0, 1, 1) == 0
+
+
+def test_rotary_of_more_than_64_bits_is_refused():
+    """Sizes within their bounds whose product passes 2^63."""
+    st = _lib.i64_array((1, 1, 1, 1))
+    most = 1 << 20
+    for T, H, Hkv, D, n in ((2 ** 31 - 1, most, most, most, 0), (2 ** 31 - 1, most, most, most, most // 2),
+                            (1 << 30, most // 2, most // 2, most // 2, 3), (2 ** 31 - 1, most, most, most // 4, 0),
+                            (1 << 26, most, 0, most, 0), (2 ** 31 - 1, 1, 0, 16, 8)):
+        rc = _lib.lib().bi_rotary(P, P, P, P, P, P, T, H, Hkv, D, n, 0, st, 1.0, 0, _lib.F32, None)
+        assert rc == _lib.EINVAL and "too large" in _err(), (T, H, Hkv, D, n)
