@@ -185,6 +185,8 @@ def _cache_shapes(k_cache, v_cache, k_scales=None, v_scales=None):
         raise ValueError("caches must be (num_pages, Hkv, page_size, head dim), got %s and %s"
                          % (tuple(ks), tuple(vs)))
     kst, vst = k_cache.stride(), v_cache.stride()
+    if (ks[3] == 0) != (vs[3] == 0):
+        raise ValueError("keys and values must both have a head dim, got %d and %d" % (ks[3], vs[3]))
     if kst[3] != 1 or vst[3] != 1:
         raise ValueError("the caches' last dimension must be contiguous")
     if k_scales is not None or v_scales is not None or k_cache.dtype is _I8:

@@ -328,3 +328,18 @@ def test_rotary_of_more_than_64_bits_is_refused():
                             (1 << 26, most, 0, most, 0), (2 ** 31 - 1, 1, 0, 16, 8)):
         rc = _lib.lib().bi_rotary(P, P, P, P, P, P, T, H, Hkv, D, n, 0, st, 1.0, 0, _lib.F32, None)
         assert rc == _lib.EINVAL and "too large" in _err(), (T, H, Hkv, D, n)
+
+
+@pytest.mark.parametrize("D, V", [(64, 0), (0, 64)])
+def test_caches_of_one_side_are_refused(D, V):
+    """Keys without values, or values without keys: nothing was written, and zeros read."""
+    x = lambda d: torch.zeros(3, 2, d).half()
+    slots = torch.zeros(3, dtype=I32)
+    caches = torch.zeros(4, 2, 16, D).half(), torch.zeros(4, 2, 16, V).half()
+    codes = tuple(c.to(torch.int8) for c in caches)
+    scales = dict(k_scales=torch.zeros(4, 2, 16), v_scales=torch.zeros(4, 2, 16))
+    for call in (lambda: bi.paged_cache_update(x(D), x(V), *caches, slots),
+                 lambda: bi.paged_cache_update(x(D), x(V), *codes, slots, **scales),
+                 lambda: bi.paged_cache_read(*caches, slots), lambda: bi.paged_cache_read(*codes, slots, **scales)):
+        with pytest.raises(ValueError, match="head dim"):
+            call()
