@@ -203,3 +203,33 @@ def test_more_rows_than_one_launch_takes(cuda, rows, V):
             for z, w in zip(got, bi.token_logprobs(y[part], t[part], top=2)):
                 assert bool((z[part] == w).all())
         check(got, y, t, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_time_of_rows_with_few_allowed_tokens(cuda, dtype):
+    """Three allowed tokens, or equal logits: not tens of times what a row takes whose
+    logits differ (3 to 4 times; 40 where every candidate was looked at alone)."""
+    x = (torch.randn(3, 131072, generator=torch.Generator().manual_seed(1)) * 2.5).to(dtype).to(cuda)
+    few = torch.full_like(x, -math.inf)
+    few[:, [1, 70000, 131065]] = x[:, [1, 70000, 131065]]
+    t = torch.ones(3, dtype=torch.long, device=cuda)
+
+    def time(x):
+        bi.token_logprobs(x, t, top=5)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(10):
+                bi.token_logprobs(x, t, top=5)
+        best = math.inf
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    base = time(x)
+    for y in (few, torch.zeros_like(x)):
+        assert time(y) < 15 * base
