@@ -164,7 +164,7 @@ struct UpdateArgs {
 
 // A copy: a thread moves one U-sized unit of one head's key or value row of one
 // token. (What bounds it is how many loads are in flight as the launch ramps
-// up: 8161 tokens of 4 KB took 16.6 us, 25 with two tokens a thread and 26.5
+// up: 8177 tokens of 4 KB took 16.6 us, 25 with two tokens a thread and 26.5
 // with four; a plain copy of as many bytes 11.1.)
 template <typename U>
 __global__ void __launch_bounds__(kThreads) paged_update_kernel(UpdateArgs p) {

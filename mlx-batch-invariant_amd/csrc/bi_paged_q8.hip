@@ -64,7 +64,7 @@ __device__ __forceinline__ float code_of(float x, float s) {
 // is the nearest whole number to x / s if |x - n s| is below s / 2, which it nearly
 // always is; the fma rounds that difference once, and s / 2 is a number of 32 bits, so
 // the comparison is exact. Else, next to a tie, the wave divides. (With a division for
-// every value 8161 tokens took 25 us; memory would take 10.)
+// every value 8177 tokens took 25 us; memory would take 10.)
 template <int U>
 __device__ __forceinline__ void codes_of(const float (&x)[U], float s, float inv, bool keep, int8_t (&c)[U]) {
   float n[U], far = 0.f;
@@ -108,7 +108,7 @@ __device__ __forceinline__ float row_max(float x, int lanes) {
 
 // n * stride: one multiplication of 32 bits by 32, and where a stride is past them
 // (which all lanes know) the rest. (For the write, half of whose instructions were
-// addresses and the search for the largest: 8161 tokens 19.8 -> 17.9 us with both
+// addresses and the search for the largest: 8177 tokens 19.8 -> 17.9 us with both
 // mended; the read, bound by memory, gains nothing.)
 __device__ __forceinline__ int64_t times(int32_t n, int64_t stride) {
   uint64_t x = (uint64_t)(uint32_t)n * (uint32_t)stride;
@@ -163,7 +163,7 @@ template <typename T, int U> __device__ __forceinline__ float largest(const type
 // One row of a token and head by `lanes` lanes, U elements at a time each (16
 // bytes, or one where rows are not aligned to that); ONE: each lane has one unit at
 // most. What bounds it is memory, and the chain of a wave, of which there are few
-// rounds: both rows of a token and head by the same lanes took 27 us for 8161 tokens
+// rounds: both rows of a token and head by the same lanes took 27 us for 8177 tokens
 // of 4 KB, a row each 21 (17.9 now).
 template <typename T, int U, bool ONE>
 __global__ void __launch_bounds__(kThreads) update_kernel(Q8Args p) {
