@@ -775,3 +775,49 @@ def test_partial_results_without_memory_for_rows_laid_out(cuda, monkeypatch):
 
     monkeypatch.setattr(_paged, "_workspace", none)
     assert same(run(), full) and len(asked) == 2
+
+
+def test_places_of_rows_in_a_graph_and_on_two_streams(cuda):
+    """Requests take their places anew in each replay, as their lengths are then."""
+    R, H, Hkv, D, page, seq = 64, 8, 4, 128, 64, 4096
+    g = torch.Generator(device=cuda).manual_seed(2)
+    width = seq // page
+    kc, vc = (torch.randint(-127, 128, (R * width, Hkv, page, D), generator=g, device=cuda, dtype=torch.int8)
+              for _ in range(2))
+    ks, vs = (torch.rand(R * width, Hkv, page, generator=g, device=cuda) / 100 for _ in range(2))
+    table = torch.randperm(R * width, generator=g, device=cuda).to(torch.int32).view(R, width)
+    q = torch.randn(64 * 20 + 580, H, D, generator=g, device=cuda).to(BF16)
+    qs, lens = (torch.zeros(n, dtype=torch.int32, device=cuda) for n in (R + 1, R))
+
+    def run():
+        return bi.paged_attention(q, kc, vc, table, qs, lens, max_query=600, max_seq=seq, k_scales=ks, v_scales=vs)
+
+    def fill(new, length):
+        qs.copy_(starts(new, cuda))
+        lens.copy_(torch.tensor([length(r) for r in range(R)], dtype=torch.int32))
+
+    steps = [([20] * 63 + [600], lambda r: seq), ([600] + [20] * 63, lambda r: 30 + 60 * r),
+             ([1] * 63 + [600], lambda r: seq - r), ([20] * 64, lambda r: seq - 64 * r),
+             ([0] * 60 + [465] * 4, lambda r: seq)]
+    sizes = (q.shape[0], R, H, Hkv, D, D, 0, 0, 600, seq, 2)
+    need = _paged._lib.lib().bi_paged_attention_q8_workspace(*sizes)
+    least = _paged._lib.lib().bi_paged_attention_q8_least_workspace(*sizes)
+    assert (1 << 27) - laid_bytes(1, 1, D, D, 64) < need - least <= (1 << 27) + 512
+    fill(*steps[0])
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for step in (*steps, *steps[::-1]):
+        fill(*step)
+        want = run()
+        torch.cuda.synchronize()
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want) and all(same(x, want) for x in got)
