@@ -33,7 +33,7 @@ enum bi_dtype { BI_F32 = 0, BI_F16 = 1, BI_BF16 = 2 };
 
 enum bi_status {
   BI_OK = 0,
-  BI_EINVAL = -1,       /* bad argument: null pointer, negative size, bad mode */
+  BI_EINVAL = -1,       /* bad argument: null pointer, negative size, bad mode, a launch past 2^32 threads */
   BI_EUNSUPPORTED = -2, /* valid but not built: e.g. an attention head dim */
   BI_ELAUNCH = -3       /* the HIP launch itself failed */
 };
