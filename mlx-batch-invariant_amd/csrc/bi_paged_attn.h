@@ -62,6 +62,7 @@ struct Args {
   char* laid;
   int32_t* laid_at;
   int32_t units, room;
+  int32_t laid_cols;      // of requests of more columns
 };
 
 typedef void (*Kernel)(Args);

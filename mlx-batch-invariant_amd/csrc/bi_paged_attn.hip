@@ -240,10 +240,11 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
                                               : (int64_t)p.R * (((int64_t)p.qL * p.G.d + wc - 1) / wc);
   const int32_t fill = p.qstart && !s.split_cols ? 16 : 0;
   const int64_t blocks = tiles * p.Hkv.d + fill;
-  // Of rows laid out, requests for which there may be no room, each of which has more
-  // than split_cols columns (a launch that finds nothing takes some 4 us).
+  // Beside rows laid out, requests that are not: of one column tile, or for which there
+  // may be no room, each of which has more than split_cols columns (a launch that finds
+  // nothing takes some 4 us).
   const int64_t least = s.split_cols / p.G.d + 1, n = p.T / least < p.R ? p.T / least : p.R;
-  const bool more = whole && s.laid && s.room && n * p.Hkv.d * s.walked > s.room;
+  const bool more = whole && s.laid && s.room && (s.split_cols < 128 || n * p.Hkv.d * s.walked > s.room);
   const int64_t rest = more ? (cols / 128 + requests) * p.Hkv.d : 0;
   if (bi::grid_too_large(blocks, threads) || bi::grid_too_large(rest, k.whole4_threads))
     return bi::fail(BI_EINVAL, "%s: grid too large", who);
@@ -281,7 +282,9 @@ int launch(const char* who, Args& p, int64_t D, int64_t V, int dtype, bool q8, v
       p.laid = static_cast<char*>(ws) + s.laid_at();
       p.units = (int32_t)s.units;
       p.room = (int32_t)(s.room ? s.room : (int64_t)p.R * p.Hkv.d * s.units);
+      p.laid_cols = p.split_cols;
       if (s.room) {
+        if (p.laid_cols < 128) p.laid_cols = 128;
         p.laid_at = reinterpret_cast<int32_t*>(p.laid);
         p.laid += notes(p.R);
       }

@@ -705,7 +705,8 @@ __global__ void __launch_bounds__(256, (Geo8<T, D, V>::split_per_cu(NC))) split8
 // for 116, so the host compares. The list of what is to do, steps of requests that are
 // not split, is the same for all workgroups, which take from it in turn. Where not
 // every step of every request can have a place, requests have theirs one behind the
-// other, as far as there is room, and the first workgroup notes where.
+// other, as far as there is room, and the first workgroup notes where; then those of one
+// column tile, whose rows would be read once more for nothing, get none.
 template <typename T, int D, int V>
 __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
   using G8 = Geo8<T, D, V>;
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(256) lay8_kernel(Args p) {
     bool whole = false;
     if (r0 + tid < p.R) {
       const Request rq = request(p, r0 + tid);
-      whole = !rq.beyond && rq.L * (int)p.G.d > p.split_cols;
+      whole = !rq.beyond && rq.L * (int)p.G.d > p.laid_cols;
       if (whole) {
         const int n = walk(p, rq.n - rq.L, rq.n - 1, S).count();
         sum = n > p.room / p.Hkv ? p.room + 1 : n * (int)p.Hkv.d;

@@ -704,10 +704,12 @@ def test_bits_of_far_scores(cuda, dtype, D, V, monkeypatch):
 
 @pytest.mark.parametrize("D, V, seq, window, first", [(256, 256, 2200, 0, 0), (64, 64, 8192, 0, 0),
                                                       (128, 128, 8192, 2500, 3), (192, 128, 4000, 0, 0)])
+@pytest.mark.parametrize("few", [20, 40])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_more_rows_than_there_is_room_for(cuda, D, V, seq, window, first, dtype, monkeypatch):
+def test_more_rows_than_there_is_room_for(cuda, D, V, seq, window, first, dtype, few, monkeypatch):
     """64 requests, most with more tokens than are split, one with a chunk: laid out as
-    far as there is room, the others as without, and the bits of a call without any."""
+    far as there is room (but for 20 tokens, one column tile), the others as without, and
+    the bits of a call without any."""
     R, H, Hkv, page = 64, 16, 4, 64
     g = torch.Generator(device=cuda).manual_seed(D + window)
     width = -(-seq // page)
@@ -716,7 +718,7 @@ def test_more_rows_than_there_is_room_for(cuda, D, V, seq, window, first, dtype,
     kc, vc, ks, vs = codes(D), codes(V), scales() / 10, scales()
     table = torch.randperm(R * width, generator=g, device=cuda).to(torch.int32).view(R, width)
     table[3, 5] = -1
-    new = [1 if r % 5 == 0 else 0 if r % 7 == 3 else 600 if r == 11 else 20 for r in range(R)]
+    new = [1 if r % 5 == 0 else 0 if r % 7 == 3 else 600 if r == 11 else few for r in range(R)]
     lens = [seq - 37 * (r % 9) if r % 4 else 500 + 30 * r for r in range(R)]
     lens[2] = 7  # fewer rows than tokens: some see nothing
     seqs = torch.tensor(lens, dtype=torch.int32, device=cuda)
@@ -796,7 +798,7 @@ def test_places_of_rows_in_a_graph_and_on_two_streams(cuda):
         qs.copy_(starts(new, cuda))
         lens.copy_(torch.tensor([length(r) for r in range(R)], dtype=torch.int32))
 
-    steps = [([20] * 63 + [600], lambda r: seq), ([600] + [20] * 63, lambda r: 30 + 60 * r),
+    steps = [([20] * 63 + [600], lambda r: seq), ([40] * 31 + [0] * 32 + [600], lambda r: seq), ([600] + [20] * 63, lambda r: 30 + 60 * r),
              ([1] * 63 + [600], lambda r: seq - r), ([20] * 64, lambda r: seq - 64 * r),
              ([0] * 60 + [465] * 4, lambda r: seq)]
     sizes = (q.shape[0], R, H, Hkv, D, D, 0, 0, 600, seq, 2)
